@@ -19,7 +19,8 @@
  *   K cache     [kv_heads, cap, head_dim]   (f32 or f16 bits)
  *   V cache     [kv_heads, head_dim, cap]   (transposed, f32 or f16 bits)
  *   tiled f16   (new) one buffer per layer, [kv_heads][blocks of 32 positions],
- *               each block K then V in MFMA fragment order (kvlayout.h)
+ *               each block K then V in MFMA fragment order (kvlayout.h); with
+ *               slots, one such cache after the other
  *   Q8_0 cache  (new; no reference counterpart) for `slots` sequences, tiled the
  *               same way: [slots][kv_heads][blocks], each block K codes, V
  *               codes, K scales, V scales; element = f16 scale * int8 code, one
@@ -316,6 +317,108 @@ int llmtie_rope_cache_q8(void* stream, float* q, size_t q_len, size_t q_off, con
                          size_t k_off, const float* v, size_t v_len, size_t v_off, const float* freq_div,
                          size_t heads, size_t kv_heads, size_t head_dim, float theta, size_t pos, int8_t* cache,
                          size_t cache_len, size_t slots, size_t slot, size_t cap);
+
+/* ------------------------------------------- attention over key ranges (new)
+ *
+ * No counterpart in the reference. Prompts and batched single tokens over a
+ * tiled f16 cache of `slots` sequences ([slots][kv_heads][blocks of 32
+ * positions]: llmtie_t16_cache_len halves each, one after the other), in which
+ * every query row sees keys of its own, with
+ *
+ *   score of key j = c * tanh(scale * q.k_j / c) - slope[head] * |i - j|
+ *
+ * where softcap c = 0 stands for no cap, slopes NULL (else [heads] f32, device)
+ * for no bias, and i and j are cache positions: a row's own and the key's. The
+ * scale is positive, the cap zero or positive, both finite. A row that sees no key gets
+ * zeros. Keys that a row does not see contribute nothing to it, whatever they hold. */
+
+/* Which keys the rows of a packed prompt see: made once for all layers. Row r
+ * (of `rows`) is at cache position i = past + r. starts (device, starts_len =
+ * documents + 1, never decreasing) holds each document's first row and the row
+ * behind the last; row r of document d, which covers positions s = past +
+ * starts[d] up to e = past + starts[d + 1] (at most past + rows), sees
+ *   j < table[r]                                      and
+ *   table[rows + r] <= j < table[2 * rows + r]:
+ *   table[r]            = min(shared, causal ? i + 1 : past + rows): leading positions that every row
+ *                         sees (a shared prompt, what a sliding window leaves behind)
+ *   table[rows + r]     = s, or i - window + 1 where a window is given (nonzero) and that is more
+ *   table[2 * rows + r] = causal ? i + 1 : e (at most i + window), and at least min(s + prefix[d], e) where
+ *                         prefix is given (device, one a document): rows that their document's all see.
+ * starts NULL is one document from cache position 0 (s = 0, e = past + rows;
+ * prefix then has one entry). Rows of no document see nothing (zeros). pos, if not NULL, gets the
+ * rows' rotary positions i - s. Attention clamps the ranges to the keys the cache holds. */
+int llmtie_key_ranges(void* stream, const int32_t* starts, size_t starts_len, const int32_t* prefix, size_t prefix_len,
+                      size_t rows, size_t past, int causal, size_t window, size_t shared, int32_t* table,
+                      size_t table_len, int32_t* pos, size_t pos_len);
+
+/* Attention of tq query rows (f16, row r at q[q_off + r * q_stride ..], as
+ * llmtie_rope_rows and llmtie_t16_rope_store leave them) over slot `slot`, which
+ * holds past + tq keys; table as above, of exactly these rows. out = [tq,
+ * heads*head_dim] f16. max_keys bounds the keys a row sees and is used for the
+ * plan alone (0: past + tq). ws: a workspace of
+ * llmtie_flash_attn_ranges_workspace floats, 16-byte aligned, for launches of
+ * few rows over many keys, which are then cut into runs of keys and merged by a
+ * second launch (0 floats: not cut; NULL: never cut). It is written and read on
+ * `stream` by this call alone; concurrent calls need one each. cache and out
+ * are 16-byte aligned. */
+size_t llmtie_flash_attn_ranges_workspace(size_t tq, size_t max_keys, size_t heads, size_t kv_heads, size_t head_dim);
+int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, size_t q_off, size_t q_stride,
+                                 const uint16_t* cache, size_t cache_len, size_t slots, size_t slot,
+                                 const int32_t* table, size_t table_len, size_t max_keys, uint16_t* out,
+                                 size_t out_len, size_t tq, size_t past, size_t heads, size_t kv_heads,
+                                 size_t head_dim, size_t cap, float scale, float softcap, const float* slopes,
+                                 size_t slopes_len, float* ws, size_t ws_len);
+
+/* One token of each of nseq sequences: sequence s attends with row q[q_off + s *
+ * q_stride ..] (f32, magnitudes up to 65504: it is read as the sum of two f16) the
+ * first tk_dev[s] positions of slot slot_dev[s] (slot_dev NULL: slot s), of
+ * those the first `shared` ones and the ones from max(lo_dev[s], tk_dev[s] -
+ * window) on (lo_dev NULL: 0; window 0: none). Its own position is tk_dev[s] -
+ * 1. The three arrays are on the device and may change between replays of a
+ * captured call. Lengths are clamped to cap; max_tk plans the launch for the
+ * lengths to come (longer ones are attended too, less evenly spread) and decides
+ * with it how keys are divided: results under two bounds agree to rounding. A
+ * sequence whose slot is out of range gets a NaN row, one that sees no key
+ * zeros. GQA groups up to 16. out = [nseq, heads*head_dim] f32, 16-byte aligned
+ * as the cache is. */
+int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                                  const uint16_t* cache, size_t cache_len, size_t slots, const int32_t* tk_dev,
+                                  const int32_t* slot_dev, const int32_t* lo_dev, size_t nseq, size_t max_tk,
+                                  size_t window, size_t shared, size_t heads, size_t kv_heads, size_t head_dim,
+                                  size_t cap, float scale, float softcap, const float* slopes, size_t slopes_len,
+                                  llmtie_decode_scratch* scratch, float* out, size_t out_len);
+
+/* --------------------------------------- rotary positions by row (new)
+ *
+ * Row r at position pos[r] (device int32), the first rot_dim dims of each head
+ * (even, 0 to head_dim; the others are copied) rotated in pairs of halves (d, d
+ * + rot_dim / 2) or, `interleaved`, (2d, 2d + 1), by the angle pos * theta^(-2d /
+ * rot_dim) / freq_div[d] (freq_div NULL: 1; rot_dim / 2 floats, device), the
+ * rotated values times mscale. Angles are formed in f64 (llmtie_rope's are the
+ * reference's f32 ones). */
+
+/* t rows of `heads` heads from x[off + r * stride ..] into out[out_off + r *
+ * out_stride ..], f32 or (out_f16) f16. out may be x itself (the same rows, f32)
+ * or apart from them. pos NULL: positions first + r. head_dim even, at most 1024. */
+int llmtie_rope_rows(void* stream, const float* x, size_t x_len, size_t off, size_t stride, void* out, size_t out_len,
+                     size_t out_off, size_t out_stride, int out_f16, const int32_t* pos, size_t pos_len, size_t first,
+                     const float* freq_div, size_t div_len, size_t t, size_t heads, size_t head_dim, size_t rot_dim,
+                     float theta, float mscale, int interleaved);
+
+/* q rotated into q_out (as llmtie_rope_rows; q NULL: none), k rotated and v
+ * stored as f16 at position index[r] of slot slot[r] of a tiled f16 cache of
+ * `slots` slots: the tokens of a batch of sequences, or a prompt's rows, in one
+ * launch. pos, slot and index are device arrays of index_len >= rows entries. A
+ * row whose slot or index is out of range stores nothing (its q is rotated);
+ * no two rows of a call may name the same place. The projections may be one
+ * stacked buffer. */
+int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
+                          size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
+                          size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
+                          size_t v_stride, const int32_t* pos, const int32_t* slot, const int32_t* index,
+                          size_t index_len, const float* freq_div, size_t div_len, size_t rows, size_t heads,
+                          size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
+                          int interleaved, uint16_t* cache, size_t cache_len, size_t slots, size_t cap);
 
 #ifdef __cplusplus
 }

@@ -12,7 +12,7 @@ __version__ = "0.1.0"
 def __getattr__(name):
     # The torch-facing host mirror is imported lazily so that building the
     # library does not need torch.
-    if name in ("Gpu", "DecodeScratch", "Q8", "KvCacheQ8", "gpu"):
+    if name in ("Gpu", "DecodeScratch", "Q8", "KvCacheQ8", "TiledCache16", "KeyRanges", "rope_scaling", "gpu"):
         from . import gpu as _g
         return _g if name == "gpu" else getattr(_g, name)
     raise AttributeError(name)

@@ -63,6 +63,15 @@ SIGNATURES = {
     "llmtie_q8_cache_bytes": (SZ, [SZ, SZ, SZ, SZ]),
     "llmtie_kv_q8_append": (I, [P, P, SZ, SZ, P, SZ, SZ, P, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ]),
     "llmtie_rope_cache_q8": (I, [P, P, SZ, SZ, P, SZ, SZ, P, SZ, SZ, P, SZ, SZ, SZ, F, SZ, P, SZ, SZ, SZ, SZ]),
+    "llmtie_key_ranges": (I, [P, P, SZ, P, SZ, SZ, SZ, I, SZ, SZ, P, SZ, P, SZ]),
+    "llmtie_flash_attn_ranges_workspace": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "llmtie_flash_attn_ranges_t16": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, SZ, SZ, P, SZ, SZ, SZ, SZ, SZ, SZ, SZ, F,
+                                         F, P, SZ, P, SZ]),
+    "llmtie_attn_decode_ranges_t16": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, P, P, P, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, F, F,
+                                          P, SZ, P, P, SZ]),
+    "llmtie_rope_rows": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, I, P, SZ, SZ, P, SZ, SZ, SZ, SZ, SZ, F, F, I]),
+    "llmtie_t16_rope_store": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, I, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, P, P, SZ, P, SZ,
+                                  SZ, SZ, SZ, SZ, SZ, F, F, I, P, SZ, SZ, SZ]),
 }
 
 _lib = None

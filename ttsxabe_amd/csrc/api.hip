@@ -19,6 +19,8 @@
 #include "kvlayout.h"
 #include "kvcache.h"
 #include "prefill.h"
+#include "ranges.h"
+#include "rotary.h"
 
 using namespace llmtie;
 
@@ -1125,6 +1127,317 @@ int llmtie_flash_attn_t16(void* stream, const float* q, size_t q_len, const uint
                           size_t head_dim, size_t cap, float scale, int causal) {
     return llmtie_flash_attn_t16_ws(stream, q, q_len, cache, cache_len, out, out_len, tq, past, heads, kv_heads,
                                     head_dim, cap, scale, causal, nullptr, 0);
+}
+
+}  // extern "C"
+
+// ------------------------------------- key ranges and rotary positions by row
+
+namespace {
+
+int refuse(const char* what) { return fail(LLMTIE_INVALID_ARGUMENT, 0, 0, 0, 0, "%s", what); }
+bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
+// Elements that `rows` rows of `n`, `stride` apart, reach from `off`.
+size_t reach(size_t off, size_t rows, size_t stride, size_t n) {
+    return rows == 0 ? off : sadd(off, sadd(smul(rows - 1, stride), n));
+}
+// Workgroups of 256 threads that a launch (fewer than 2^32 threads) holds.
+constexpr size_t MAX_WGS = ((size_t)1 << 24) - 1;
+
+// What the score arguments must be. (The kernels keep running maxima of raw
+// products, so the scale is positive.)
+int score_checks(float scale, float softcap, const float* slopes, size_t slopes_len, size_t heads) {
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse("a score scale that is not positive");
+    if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return refuse("a score cap that is neither 0 nor positive");
+    if (slopes && slopes_len < heads) return overrun_slice(heads, slopes_len);
+    return LLMTIE_OK;
+}
+
+// Runs that a prompt's row blocks are cut into (1: whole) when they are few and
+// their keys many.
+size_t plan_range_splits(size_t tq, size_t keys, size_t heads, size_t kv_heads) {
+    const size_t group = heads / kv_heads;
+    const size_t gb = group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
+    const size_t pb = 16 * (4 / gb), items = (tq + pb - 1) / pb * (heads / gb);
+    const size_t cus = (size_t)compute_units(), tiles = (keys + 63) / 64;
+    if (items >= cus || tiles <= 8) return 1;
+    return std::max<size_t>(1, std::min<size_t>(std::min<size_t>(32, tiles / 4), 2 * cus / items));
+}
+
+int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows, size_t heads, size_t pos_len,
+                  bool has_pos, size_t first, bool has_div, size_t div_len) {
+    if (hd % 2 != 0 || hd == 0) return fail(LLMTIE_ODD_HEAD_DIM, hd, 0, 0, 0, "a rotary head of odd width %zu", hd);
+    if (rot % 2 != 0) return fail(LLMTIE_ODD_HEAD_DIM, rot, 0, 0, 0, "a rotary head of odd width %zu", rot);
+    if (rot > hd) return overrun_slice(rot, hd);
+    if (hd > 1024) return refuse("a rotary head wider than 1024");
+    if (!(theta > 0.0f) || !std::isfinite(theta) || !std::isfinite(mscale))
+        return refuse("a rotary base that is not positive, or a multiplier that is not finite");
+    if (int r = over_int(rows, smul(heads, hd), sadd(first, rows))) return r;
+    if (has_pos && pos_len < rows) return overrun_slice(rows, pos_len);
+    if (has_div && div_len < rot / 2) return overrun_slice(rot / 2, div_len);
+    return LLMTIE_OK;
+}
+
+// Whether the rotated rows may be written: over the source itself, or apart from it.
+bool overlap(const void* a, size_t an, const void* b, size_t bn) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + bn && y < x + an;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmtie_key_ranges(void* stream, const int32_t* starts, size_t starts_len, const int32_t* prefix, size_t prefix_len,
+                      size_t rows, size_t past, int causal, size_t window, size_t shared, int32_t* table,
+                      size_t table_len, int32_t* pos, size_t pos_len) {
+    if (int r = over_int(sadd(past, rows), starts_len)) return r;
+    if (starts && starts_len == 0) return overrun_slice(1, 0);
+    const size_t docs = starts ? starts_len - 1 : 1;
+    if (prefix && prefix_len < docs) return overrun_slice(docs, prefix_len);
+    if (smul(rows, 3) > table_len) return overrun_slice(smul(rows, 3), table_len);
+    if (pos && pos_len < rows) return overrun_slice(rows, pos_len);
+    if (rows == 0) return ok();
+    if (!table) return invalid("a buffer");
+    KeyRangeArgs a{};
+    a.starts = starts;
+    a.prefix = prefix;
+    a.table = table;
+    a.pos = pos;
+    a.docs = (int)docs;
+    a.rows = (int)rows;
+    a.past = (int)past;
+    a.causal = causal ? 1 : 0;
+    a.window = (int)std::min(window, IMAX);  // wider than any position: no window's effect
+    a.shared = (int)std::min(shared, IMAX);
+    return launched("key_ranges", launch_key_ranges(a, S(stream)));
+}
+
+int llmtie_rope_rows(void* stream, const float* x, size_t x_len, size_t off, size_t stride, void* out, size_t out_len,
+                     size_t out_off, size_t out_stride, int out_f16, const int32_t* pos, size_t pos_len, size_t first,
+                     const float* freq_div, size_t div_len, size_t t, size_t heads, size_t head_dim, size_t rot_dim,
+                     float theta, float mscale, int interleaved) {
+    if (int r = rotary_checks(head_dim, rot_dim, theta, mscale, t, heads, pos_len, pos != nullptr, first,
+                              freq_div != nullptr, div_len))
+        return r;
+    const size_t n = smul(heads, head_dim);
+    if (t > 1 && (stride < n || out_stride < n)) return overrun_slice(n, std::min(stride, out_stride));
+    if (reach(off, t, stride, n) > x_len) return overrun_slice(reach(off, t, stride, n), x_len);
+    if (reach(out_off, t, out_stride, n) > out_len) return overrun_slice(reach(out_off, t, out_stride, n), out_len);
+    if (t == 0 || n == 0) return ok();
+    if (!x || !out) return invalid("a buffer");
+    const size_t es = out_f16 ? 2 : 4;
+    const char* o = static_cast<char*>(out) + out_off * es;
+    const bool same = !out_f16 && o == reinterpret_cast<const char*>(x + off) && (stride == out_stride || t == 1);
+    if (!same && overlap(x + off, reach(0, t, stride, n) * 4, o, reach(0, t, out_stride, n) * es))
+        return refuse("rotated rows that overlap their source but are not its own");
+    RotaryArgs a{};
+    a.q = x + off;
+    a.qo = const_cast<char*>(o);
+    a.pos = pos;
+    a.first = (int)first;
+    a.div = freq_div;
+    a.q_stride = t > 1 ? (long)stride : 0;
+    a.qo_stride = t > 1 ? (long)out_stride : 0;
+    a.rows = (int)t;
+    a.heads = (int)heads;
+    a.hd = (int)head_dim;
+    a.rot = (int)rot_dim;
+    a.interleaved = interleaved ? 1 : 0;
+    a.qo_f16 = out_f16 ? 1 : 0;
+    a.mscale = mscale;
+    a.log2_theta = std::log2((double)theta);
+    return launched("rope_rows", launch_rotary(a, false, S(stream)));
+}
+
+int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
+                          size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
+                          size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
+                          size_t v_stride, const int32_t* pos, const int32_t* slot, const int32_t* index,
+                          size_t index_len, const float* freq_div, size_t div_len, size_t rows, size_t heads,
+                          size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
+                          int interleaved, uint16_t* cache, size_t cache_len, size_t slots, size_t cap) {
+    if (!(head_dim == 64 || head_dim == 128) || kv_heads == 0) return unsupported(head_dim, heads, kv_heads);
+    if (int r = rotary_checks(head_dim, rot_dim, theta, mscale, rows, std::max(heads, kv_heads), index_len, true, 0,
+                              freq_div != nullptr, div_len))
+        return r;
+    if (int r = over_int(cap, slots, kv_heads)) return r;
+    const size_t need = smul(slots, llmtie_t16_cache_len(kv_heads, head_dim, cap));
+    if (cache_len < need) return overrun_slice(need, cache_len);
+    const size_t n = smul(heads, head_dim), nk = smul(kv_heads, head_dim);
+    const size_t es = q_out_f16 ? 2 : 4;
+    if (q) {
+        if (rows > 1 && (q_stride < n || q_out_stride < n)) return overrun_slice(n, std::min(q_stride, q_out_stride));
+        if (reach(q_off, rows, q_stride, n) > q_len) return overrun_slice(reach(q_off, rows, q_stride, n), q_len);
+        if (reach(q_out_off, rows, q_out_stride, n) > q_out_len)
+            return overrun_slice(reach(q_out_off, rows, q_out_stride, n), q_out_len);
+    }
+    if (rows > 1 && (k_stride < nk || v_stride < nk)) return overrun_slice(nk, std::min(k_stride, v_stride));
+    if (reach(k_off, rows, k_stride, nk) > k_len) return overrun_slice(reach(k_off, rows, k_stride, nk), k_len);
+    if (reach(v_off, rows, v_stride, nk) > v_len) return overrun_slice(reach(v_off, rows, v_stride, nk), v_len);
+    if (rows == 0) return ok();
+    if (!k || !v || !pos || !slot || !index || !cache || (q && !q_out)) return invalid("a buffer");
+    if (off16(cache)) return refuse("a cache off 16 bytes");
+    RotaryArgs a{};
+    if (q && heads) {
+        const char* o = static_cast<char*>(q_out) + q_out_off * es;
+        const size_t on = reach(0, rows, q_out_stride, n) * es;
+        const bool same =
+            !q_out_f16 && o == reinterpret_cast<const char*>(q + q_off) && (q_stride == q_out_stride || rows == 1);
+        if (!same && (overlap(q + q_off, reach(0, rows, q_stride, n) * 4, o, on) ||
+                      overlap(k + k_off, reach(0, rows, k_stride, nk) * 4, o, on) ||
+                      overlap(v + v_off, reach(0, rows, v_stride, nk) * 4, o, on)))
+            return refuse("rotated queries that overlap a source but are not their own");
+        a.q = q + q_off;
+        a.qo = const_cast<char*>(o);
+    }
+    a.k = k + k_off;
+    a.v = v + v_off;
+    a.pos = pos;
+    a.slot = slot;
+    a.index = index;
+    a.div = freq_div;
+    a.cache = cache;
+    a.q_stride = rows > 1 ? (long)q_stride : 0;
+    a.qo_stride = rows > 1 ? (long)q_out_stride : 0;
+    a.k_stride = rows > 1 ? (long)k_stride : 0;
+    a.v_stride = rows > 1 ? (long)v_stride : 0;
+    a.rows = (int)rows;
+    a.heads = (int)heads;
+    a.kv = (int)kv_heads;
+    a.hd = (int)head_dim;
+    a.rot = (int)rot_dim;
+    a.interleaved = interleaved ? 1 : 0;
+    a.qo_f16 = q_out_f16 ? 1 : 0;
+    a.slots = (int)slots;
+    a.cap = (int)cap;
+    a.mscale = mscale;
+    a.log2_theta = std::log2((double)theta);
+    return launched("t16_rope_store", launch_rotary(a, true, S(stream)));
+}
+
+size_t llmtie_flash_attn_ranges_workspace(size_t tq, size_t max_keys, size_t heads, size_t kv_heads, size_t head_dim) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || tq == 0 || tq > IMAX || max_keys > IMAX) return 0;
+    const size_t splits = plan_range_splits(tq, max_keys, heads, kv_heads);
+    return splits > 1 ? smul(smul(splits, tq, heads), head_dim + 2) : 0;
+}
+
+int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, size_t q_off, size_t q_stride,
+                                 const uint16_t* cache, size_t cache_len, size_t slots, size_t slot,
+                                 const int32_t* table, size_t table_len, size_t max_keys, uint16_t* out,
+                                 size_t out_len, size_t tq, size_t past, size_t heads, size_t kv_heads,
+                                 size_t head_dim, size_t cap, float scale, float softcap, const float* slopes,
+                                 size_t slopes_len, float* ws, size_t ws_len) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads)) return unsupported(head_dim, heads, kv_heads);
+    if (int r = score_checks(scale, softcap, slopes, slopes_len, heads)) return r;
+    if (sadd(past, tq) > cap) return overrun_cache(sadd(past, tq), cap);
+    if (int r = over_int(smul(heads, head_dim), sadd(cap, 128), slots)) return r;
+    if (slot >= slots) return overrun_slice(sadd(slot, 1), slots);
+    const size_t one = llmtie_t16_cache_len(kv_heads, head_dim, cap);
+    if (cache_len < smul(slots, one)) return overrun_slice(smul(slots, one), cache_len);
+    const size_t n = smul(heads, head_dim), nq = smul(tq, n);
+    if (nq > (size_t)1 << 40) return overrun_slice(nq, (size_t)1 << 40);
+    if (tq > 1 && q_stride < n) return overrun_slice(n, q_stride);
+    if (reach(q_off, tq, q_stride, n) > q_len) return overrun_slice(reach(q_off, tq, q_stride, n), q_len);
+    if (out_len < nq) return overrun_slice(nq, out_len);
+    if (table_len < smul(tq, 3)) return overrun_slice(smul(tq, 3), table_len);
+    if (table_len != smul(tq, 3)) return refuse("a row table of another row count");
+    if (tq == 0) return ok();
+    if (!q || !cache || !table || !out) return invalid("a buffer");
+    if (off16(cache) || off16(out)) return refuse("a cache or a context off 16 bytes");
+    const size_t group = heads / kv_heads;
+    const int gb = group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
+    const size_t keys = std::min(max_keys ? max_keys : IMAX, past + tq);
+    const size_t splits = ws ? plan_range_splits(tq, keys, heads, kv_heads) : 1;
+    if (splits > 1) {
+        const size_t need = smul(smul(splits, tq, heads), head_dim + 2);
+        if (ws_len < need) return overrun_slice(need, ws_len);
+        if (off16(ws)) return refuse("a workspace off 16 bytes");
+    }
+    const int nqt = splits > 1 ? 1 : pick_nqt(tq, heads, gb);
+    const size_t items = smul((tq + 16 * nqt * (4 / gb) - 1) / (16 * nqt * (4 / gb)), heads / gb, splits);
+    if (items > MAX_WGS) return overrun_slice(items, MAX_WGS);
+    RangesArgs a{};
+    a.q = q + q_off;
+    a.cache = cache + slot * one;
+    a.out = out;
+    a.first = table;
+    a.lo = table + tq;
+    a.hi = table + 2 * tq;
+    a.slopes = slopes;
+    a.q_stride = tq > 1 ? (long)q_stride : 0;
+    a.tq = (int)tq;
+    a.past = (int)past;
+    a.heads = (int)heads;
+    a.kv_heads = (int)kv_heads;
+    a.cap = (int)cap;
+    a.scale = scale;
+    a.softcap = softcap;
+    a.gb = gb;
+    a.splits = (int)splits;
+    a.ws = ws;
+    a.qal = !off16(a.q) && a.q_stride % 8 == 0;
+    return launched("flash_attn_ranges", launch_ranges((int)head_dim, nqt, false, a, S(stream)));
+}
+
+int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                                  const uint16_t* cache, size_t cache_len, size_t slots, const int32_t* tk_dev,
+                                  const int32_t* slot_dev, const int32_t* lo_dev, size_t nseq, size_t max_tk,
+                                  size_t window, size_t shared, size_t heads, size_t kv_heads, size_t head_dim,
+                                  size_t cap, float scale, float softcap, const float* slopes, size_t slopes_len,
+                                  llmtie_decode_scratch* scratch, float* out, size_t out_len) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16)
+        return unsupported(head_dim, heads, kv_heads);
+    if (int r = score_checks(scale, softcap, slopes, slopes_len, heads)) return r;
+    if (max_tk == 0 || max_tk > cap) return overrun_cache(max_tk, cap);
+    if (int r = over_int(smul(heads, head_dim), sadd(cap, 128), slots, nseq)) return r;
+    const size_t need = smul(slots, llmtie_t16_cache_len(kv_heads, head_dim, cap));
+    if (cache_len < need) return overrun_slice(need, cache_len);
+    const size_t n = smul(heads, head_dim);
+    if (nseq > 1 && q_stride < n) return overrun_slice(n, q_stride);
+    if (reach(q_off, nseq, q_stride, n) > q_len) return overrun_slice(reach(q_off, nseq, q_stride, n), q_len);
+    if (out_len < smul(nseq, n)) return overrun_slice(smul(nseq, n), out_len);
+    if (!slot_dev && nseq > slots) return overrun_slice(nseq, slots);
+    if (nseq == 0) return ok();
+    if (!q || !cache || !tk_dev || !out) return invalid("a buffer");
+    if (!scratch) return invalid("scratch");
+    if (off16(cache) || off16(out)) return refuse("a cache or a context off 16 bytes");
+    if (int r = llmtie_decode_scratch_status(scratch)) return r;
+    const size_t group = heads / kv_heads, units = smul(nseq, kv_heads);
+    const size_t keys = window ? std::min(max_tk, sadd(window, shared)) : max_tk;
+    const size_t blocks = (keys + 31) / 32;
+    const size_t span = 8;
+    const size_t most = std::min<size_t>(DECODE_MAX_SPLITS, DECODE_MAX_SPLIT_ROWS / group);
+    const size_t splits = std::max<size_t>(
+        1, std::min(std::min((blocks + span - 1) / span, most), (1024 + units - 1) / units));
+    if (smul(units, splits) > MAX_WGS) return overrun_slice(smul(units, splits), MAX_WGS);
+    const size_t parts = smul(units, splits, n / kv_heads);
+    const size_t floats = splits > 1 ? sadd(parts, smul(units, splits, 2 * group)) : 0;
+    if (int r = ensure_scratch(scratch, floats, smul(units, CTR_STRIDE), S(stream))) return r;
+    RangesDecodeArgs a{};
+    a.q = q + q_off;
+    a.cache = cache;
+    a.out = out;
+    a.tk = tk_dev;
+    a.slot = slot_dev;
+    a.lo = lo_dev;
+    a.slopes = slopes;
+    a.part = scratch->part;
+    a.ml_off = (long)parts;
+    a.ctr = scratch->ctr;
+    a.q_stride = nseq > 1 ? (long)q_stride : 0;
+    a.nseq = (int)nseq;
+    a.slots = (int)slots;
+    a.cap = (int)cap;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)group;
+    a.window = (int)std::min(window, IMAX);
+    a.shared = (int)std::min(shared, IMAX);
+    a.splits = (int)splits;
+    a.span = (int)span;
+    a.scale = scale;
+    a.softcap = softcap;
+    return launched("attn_decode_ranges", launch_ranges_decode((int)head_dim, a, S(stream)));
 }
 
 }  // extern "C"

@@ -14,6 +14,7 @@ without a HIP device raises.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from dataclasses import dataclass
 
 import torch
@@ -26,7 +27,7 @@ __all__ = [
     "SplitHeadLost",
     "DecodeScratch",
     "Q8", "KvCacheQ8",
-    "TiledCache16", "Gpu",
+    "TiledCache16", "KeyRanges", "rope_scaling", "Gpu",
 ]
 
 
@@ -207,13 +208,67 @@ class KvCacheQ8:
 
 class TiledCache16:
     """A tiled f16 KV cache for one layer: K and V of every kv head in one
-    buffer, 32-position blocks in MFMA fragment order."""
+    buffer, 32-position blocks in MFMA fragment order; `slots` sequences' one
+    after the other (the operators without slots take the first)."""
 
-    def __init__(self, kv_heads: int, head_dim: int, cap: int, device="cuda", zero=True):
-        self.kv_heads, self.head_dim, self.cap = kv_heads, head_dim, cap
-        n = _lib.lib().llmtie_t16_cache_len(kv_heads, head_dim, cap)
+    def __init__(self, kv_heads: int, head_dim: int, cap: int, device="cuda", zero=True, slots: int = 1):
+        self.kv_heads, self.head_dim, self.cap, self.slots = kv_heads, head_dim, cap, slots
+        n = slots * _lib.lib().llmtie_t16_cache_len(kv_heads, head_dim, cap)
         alloc = torch.zeros if zero else torch.empty
         self.data = alloc(n, dtype=torch.float16, device=device)
+
+    @classmethod
+    def of(cls, data, kv_heads: int, head_dim: int, cap: int, slots: int = 1):
+        """A cache over memory that the caller holds."""
+        self = cls.__new__(cls)
+        self.kv_heads, self.head_dim, self.cap, self.slots, self.data = kv_heads, head_dim, cap, slots, data
+        return self
+
+
+@dataclass
+class KeyRanges:
+    """Which keys each row of a prompt sees: `table` int32 [3, rows] (row r sees
+    keys j < table[0, r] and table[1, r] <= j < table[2, r]), `pos` int32 [rows]
+    its rotary positions, `max_keys` a bound of the keys a row sees (0: unknown)."""
+
+    table: torch.Tensor
+    pos: torch.Tensor | None = None
+    max_keys: int = 0
+
+
+def rope_scaling(rot_dim: int, theta: float, kind: str = "none", factor: float = 1.0, original: int = 8192,
+                 beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda"):
+    """(freq_div, theta, mscale) of a rotary extended to `factor` times its
+    `original` positions, for rope_rows and t16_rope_store.
+
+    linear: every frequency is divided by the factor. ntk: the base grows to
+    theta * factor^(rot / (rot - 2)), which divides the slowest frequency by the
+    factor and leaves the fastest. yarn: frequencies that turn more than
+    beta_fast times within `original` positions stay, those that turn less than
+    beta_slow times are divided by the factor, a ramp over the dims between
+    blends the two, and the rotated values are multiplied by 1 + ln(factor) / 10."""
+    if kind not in ("none", "linear", "ntk", "yarn"):
+        raise InvalidArgument(f"unknown rotary scaling {kind!r}")
+    if rot_dim % 2 or rot_dim < 0:
+        raise OddHeadDim(f"a rotary head of odd width {rot_dim}", (rot_dim,))
+    if not (factor >= 1.0 and theta > 0.0 and original > 0 and beta_fast > beta_slow > 0.0):
+        raise InvalidArgument("a rotary scaling wants factor >= 1, theta, original > 0 and beta_fast > beta_slow > 0")
+    n = rot_dim // 2
+    if kind == "none" or factor == 1.0 or n == 0:
+        return None, theta, 1.0
+    if kind == "ntk":
+        return None, theta * factor ** (rot_dim / (rot_dim - 2)) if rot_dim > 2 else theta, 1.0
+    if kind == "linear":
+        return torch.full((n,), factor, dtype=torch.float32, device=device), theta, 1.0
+    # The dim whose frequency turns b times within `original` positions.
+    def at(b):
+        return n * math.log(original / (b * 2.0 * math.pi)) / math.log(theta)
+    first = max(math.floor(at(beta_fast)), 0)
+    last = min(math.ceil(at(beta_slow)), rot_dim - 1)
+    i = torch.arange(n, dtype=torch.float64)
+    ramp = ((i - first) / max(last - first, 1e-3)).clamp(0.0, 1.0)  # 0: kept, 1: divided
+    div = 1.0 / ((1.0 - ramp) + ramp / factor)
+    return div.to(device=device, dtype=torch.float32), theta, 1.0 + 0.1 * math.log(factor)
 
 
 class Gpu:
@@ -504,3 +559,123 @@ class Gpu:
                                             v_off, _p(freq_div), heads, cache.kv_heads, cache.head_dim,
                                             theta, pos, _p(cache.data), _n(cache.data), cache.slots, slot,
                                             cache.cap))
+
+    # ------------------------------- key ranges and rotary positions by row
+
+    def _run(self, fn, *args):
+        """A call whose launches go to this Gpu's device, whichever is current."""
+        if torch._C._cuda_getDevice() == self.device.index:
+            _check(fn(self._stream(), *args))
+        else:
+            with torch.cuda.device(self.device):
+                _check(fn(self._stream(), *args))
+
+    def _here(self, *tensors):
+        """Checks of (tensor, dtypes, name): as _need, and on this Gpu's device."""
+        for t, dtypes, what in tensors:
+            _need(t, dtypes, what)
+            if t is not None and t.device != self.device:
+                raise InvalidArgument(f"{what} is on {t.device}, not on {self.device}")
+
+    def key_ranges(self, rows, past=0, starts=None, prefix=None, causal=True, window=0, shared=0) -> KeyRanges:
+        """Which keys each of `rows` rows behind `past` positions sees (new; see
+        llmtie_key_ranges): documents from `starts` (int32, one more than there
+        are), `prefix` leading rows of each that its rows all see, a `window`,
+        `shared` leading positions that every row sees."""
+        self._here((starts, _I32, "starts"), (prefix, _I32, "prefix"))
+        if min(rows, past, window, shared) < 0:
+            raise InvalidArgument("a negative count")
+        buf = torch.empty(4 * max(rows, 1), dtype=torch.int32, device=self.device)
+        table, pos = buf[: 3 * rows].view(3, rows), buf[3 * rows: 4 * rows]
+        self._run(self._L.llmtie_key_ranges, _p(starts), _n(starts), _p(prefix), _n(prefix), rows, past,
+                  int(bool(causal)), window, shared, _p(table), _n(table), _p(pos), _n(pos))
+        most = past + rows
+        if causal and window and prefix is None:
+            most = min(most, window + shared)
+        return KeyRanges(table, pos, most)
+
+    def rope_rows(self, x, off, stride, pos, freq_div, t, heads, head_dim, rot_dim, theta, mscale=1.0,
+                  interleaved=False, out=None, out_off=0, out_stride=None):
+        """Rotary positions by row (new): t rows of `heads` heads at x[off + r *
+        stride ..], row r at pos[r] (int32 tensor; an int: pos + r), into `out`
+        (f32 or f16; default in place)."""
+        first = 0 if isinstance(pos, torch.Tensor) else int(pos)
+        posd = pos if isinstance(pos, torch.Tensor) else None
+        if out is None:
+            out, out_off, out_stride = x, off, stride
+        self._here((x, _F32, "x"), (posd, _I32, "pos"), (freq_div, _F32, "freq_div"), (out, _F32 + _H16, "out"))
+        if min(off, stride, first, t, heads, head_dim, rot_dim, out_off) < 0:
+            raise InvalidArgument("a negative count")
+        self._run(self._L.llmtie_rope_rows, _p(x), _n(x), off, stride, _p(out), _n(out), out_off,
+                  heads * head_dim if out_stride is None else out_stride, int(out.dtype != torch.float32), _p(posd),
+                  _n(posd), first, _p(freq_div), _n(freq_div), t, heads, head_dim, rot_dim, theta, mscale,
+                  int(bool(interleaved)))
+
+    def t16_rope_store(self, q, q_off, k, k_off, v, v_off, stride, pos, slot, index, freq_div, rows, heads, rot_dim,
+                       theta, mscale, interleaved, cache: TiledCache16, q_out=None, q_out_off=0, q_out_stride=None):
+        """The rotation of q and k with the store of k and v (new): row r of the
+        projections (`stride` apart, one stacked tensor or three) to position
+        index[r] of slot slot[r] of a tiled cache; q (None: none) into q_out (f32
+        or f16; default in place)."""
+        if q is not None and q_out is None:
+            q_out, q_out_off, q_out_stride = q, q_off, stride
+        self._here((q, _F32, "q"), (k, _F32, "k"), (v, _F32, "v"), (pos, _I32, "pos"), (slot, _I32, "slot"),
+                   (index, _I32, "index"), (freq_div, _F32, "freq_div"), (q_out, _F32 + _H16, "q_out"),
+                   (cache.data, _H16, "cache"))
+        if min(q_off, k_off, v_off, stride, rows, heads, rot_dim, q_out_off) < 0:
+            raise InvalidArgument("a negative count")
+        n = min(_n(pos), _n(slot), _n(index))
+        if n < rows:
+            raise SliceOverrun(f"reading to {rows} in a buffer of {n}", (rows, n))
+        self._run(self._L.llmtie_t16_rope_store, _p(q), _n(q), q_off, stride, _p(q_out), _n(q_out), q_out_off,
+                  heads * cache.head_dim if q_out_stride is None else q_out_stride,
+                  int(q_out is not None and q_out.dtype != torch.float32), _p(k), _n(k), k_off, stride, _p(v), _n(v),
+                  v_off, stride, _p(pos), _p(slot), _p(index), n, _p(freq_div), _n(freq_div), rows, heads,
+                  cache.kv_heads, cache.head_dim, rot_dim, theta, mscale, int(bool(interleaved)), _p(cache.data),
+                  _n(cache.data), cache.slots, cache.cap)
+
+    def flash_attn_ranges(self, q, q_off, q_stride, cache: TiledCache16, slot, ranges: KeyRanges, tq, past, heads,
+                          scale, softcap=0.0, slopes=None):
+        """Attention of tq rows (f16) over their key ranges of a slot of a tiled
+        cache (new), scores capped (`softcap`) or biased by distance (`slopes`,
+        one a head). Returns the f16 context [tq * heads * head_dim]."""
+        self._here((q, _H16, "q"), (cache.data, _H16, "cache"), (ranges.table, _I32, "ranges"),
+                   (slopes, _F32, "slopes"))
+        if min(q_off, q_stride, slot, tq, past, heads, ranges.max_keys) < 0:
+            raise InvalidArgument("a negative count")
+        n = tq * heads * cache.head_dim
+        out = torch.empty(max(n, 1), dtype=torch.float16, device=self.device)
+        ws, keys = None, min(ranges.max_keys or past + tq, past + tq)
+        if keys > 512:  # fewer are never cut
+            floats = self._L.llmtie_flash_attn_ranges_workspace(tq, keys, heads, cache.kv_heads, cache.head_dim)
+            if floats:
+                try:
+                    ws = torch.empty(floats, dtype=torch.float32, device=self.device)
+                except torch.OutOfMemoryError:
+                    pass  # whole, it needs nothing beside its output
+        self._run(self._L.llmtie_flash_attn_ranges_t16, _p(q), _n(q), q_off, q_stride, _p(cache.data), _n(cache.data),
+                  cache.slots, slot, _p(ranges.table), _n(ranges.table), ranges.max_keys, _p(out), n, tq, past, heads,
+                  cache.kv_heads, cache.head_dim, cache.cap, scale, softcap, _p(slopes), _n(slopes), _p(ws), _n(ws))
+        return out[:n]
+
+    def attn_decode_ranges(self, q, q_off, q_stride, cache: TiledCache16, tk_dev, slot_dev, max_tk, heads, scale,
+                           scratch, lo_dev=None, window=0, shared=0, softcap=0.0, slopes=None, out=None):
+        """One token of each of len(tk_dev) sequences over their slots of a tiled
+        cache (new): the first `shared` positions and those from max(lo_dev, tk
+        - window) on, scores as in flash_attn_ranges. Returns the f32 context."""
+        self._here((q, _F32, "q"), (cache.data, _H16, "cache"), (tk_dev, _I32, "tk"), (slot_dev, _I32, "slot"),
+                   (lo_dev, _I32, "lo"), (slopes, _F32, "slopes"), (out, _F32, "out"))
+        if min(q_off, q_stride, max_tk, heads, window, shared) < 0:
+            raise InvalidArgument("a negative count")
+        nseq = tk_dev.numel()
+        for t in (slot_dev, lo_dev):
+            if t is not None and t.numel() < nseq:
+                raise SliceOverrun(f"reading to {nseq} in a buffer of {t.numel()}", (nseq, t.numel()))
+        n = nseq * heads * cache.head_dim
+        if out is None:
+            out = torch.empty(max(n, 1), dtype=torch.float32, device=self.device)
+        self._run(self._L.llmtie_attn_decode_ranges_t16, _p(q), _n(q), q_off, q_stride, _p(cache.data),
+                  _n(cache.data), cache.slots, _p(tk_dev), _p(slot_dev), _p(lo_dev), nseq, max_tk, window, shared,
+                  heads, cache.kv_heads, cache.head_dim, cache.cap, scale, softcap, _p(slopes), _n(slopes),
+                  scratch.handle, _p(out), _n(out))
+        return out[:n]
