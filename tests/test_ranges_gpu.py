@@ -276,6 +276,43 @@ def test_decode_random(gpu, seed):
     close(got, want, tol, (args, lo))
 
 
+@pytest.mark.parametrize("c", [
+    # Batches whose bound is long: every workgroup an equal run of all their blocks, across heads.
+    ([4096, 1, 700, 0, 2999, 33, 64, 1500, 4000], (32, 8, 128), 0, 0, 50.0, False),
+    ([5] * 9, (32, 8, 128), 0, 0, 0.0, False),
+    ([4096] * 9, (16, 8, 128), 0, 0, 0.0, True),
+    ([3000, 0, 2000, 17, 4096, 4095, 4090, 2, 1000], (8, 8, 64), 2500, 100, 30.0, True),
+    ([4096 - 50 * i for i in range(70)], (4, 1, 64), 0, 0, 0.0, False),  # more than 64 sequences
+    ([0] * 64 + [4096, 100], (16, 1, 64), 0, 0, 0.0, False),
+], ids=lambda c: f"{len(c[0])}-{c[1]}")
+def test_decode_of_long_batches(gpu, c):
+    lens, shape, window, shared, softcap, bias = c
+    n = len(lens)
+    slots = list(range(n)) if n < 20 else [i % 8 for i in range(n)]
+    if n >= 20:  # sequences that share slots
+        got, want, tol = decode_shared(gpu, lens, shape, slots, *(f16(s, 8, shape[1], 4096, shape[2]) for s in (1, 2)))
+    else:
+        got, want, tol = decode(gpu, lens, 4096, shape, window, shared, softcap, bias, slots=slots, max_tk=4096)
+    close(got, want, tol)
+
+
+def decode_shared(gpu, lens, shape, slots, k, v):
+    """Sequences of several lengths over the same slots."""
+    from ttsxabe_amd.gpu import DecodeScratch
+    heads, kv, hd = shape
+    n = len(lens)
+    q = torch.randn(n, heads, hd, generator=torch.Generator().manual_seed(5))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    got = gpu.attn_decode_ranges(q.cuda().view(-1), 0, heads * hd, cache_of(k, v), i32(lens), i32(slots), 4096, heads, 0.1,
+                                 DecodeScratch())
+    want, tol = (torch.zeros(n, heads, hd, dtype=torch.float64) for _ in range(2))
+    for i, (s, t) in enumerate(zip(slots, lens)):
+        if t:
+            want[i:i + 1], tol[i:i + 1] = ref.attend(q[i:i + 1], k[s, :, :t], v[s, :, :t], torch.ones(1, t, dtype=torch.bool),
+                                                     torch.tensor([t - 1]), 0.1, decode=True)
+    return got, want, tol
+
+
 def test_decode_padding_and_shared_slots(gpu):
     """A slot out of range is a NaN row; sequences may share a slot; a length past cap is cut to it."""
     got, want, tol = decode(gpu, [20, 30, 25, 25], 40, (8, 2, 128), 0, 0, 0.0, False, slots=[-1, 9, 2, 2])

@@ -1144,6 +1144,11 @@ size_t reach(size_t off, size_t rows, size_t stride, size_t n) {
 // Workgroups of 256 threads that a launch (fewer than 2^32 threads) holds.
 constexpr size_t MAX_WGS = ((size_t)1 << 24) - 1;
 
+// Batched decode over key ranges: blocks of a head kept in one workgroup, and the
+// bytes (half of the 256 MB Infinity Cache) past which a launch streams.
+constexpr int RD_WHOLE = 20;
+constexpr size_t RD_STREAM_BYTES = (size_t)128 << 20;
+
 // What the score arguments must be. (The kernels keep running maxima of raw
 // products, so the scale is positive.)
 int score_checks(float scale, float softcap, const float* slopes, size_t slopes_len, size_t heads) {
@@ -1406,10 +1411,24 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     const size_t group = heads / kv_heads, units = smul(nseq, kv_heads);
     const size_t keys = window ? std::min(max_tk, sadd(window, shared)) : max_tk;
     const size_t blocks = (keys + 31) / 32;
-    const size_t span = 8;
+    // Runs of a head: as many as bring the launch to one workgroup a compute
+    // unit, of four blocks (one a wave) or more; a head of up to RD_WHOLE blocks is
+    // one run (a merge costs ~3 us). Us, whole / cut: 1 sequence of 32/8/128, 14
+    // blocks 6.8 / 7.5, 18 7.5 / 7.5, 28 8.9 / 7.5; of 20/20/64, 18 5.9 / 7.2, 28
+    // 7.0 / 7.3; 16 sequences of 32/8/128, 18 blocks 12.2 / 12.9, 28 16.0 / 15.7.
+    // Twice the workgroups: 1 sequence of 4001 10.0 / 10.0; 4 of 200-6000 15.4 / 15.0;
+    // 16 of 50-600 12.8 / 10.9; 8 of 2000 over 8 heads of 64, 11.9 / 11.3.
+    // Past half the Infinity Cache a launch streams: what it reads cannot be
+    // kept until it is read again, and loads that do not try read faster (32
+    // sequences of 256-8192, 113 / 101 us; 4 of 200-6000, which fit, 15.2 / 16.6).
+    // Two workgroups a compute unit then even out the lengths: 32 of 256-8192, 101
+    // / 108; 32 of 4096, 88 / 85.
+    const size_t span = 4;
     const size_t most = std::min<size_t>(DECODE_MAX_SPLITS, DECODE_MAX_SPLIT_ROWS / group);
-    const size_t splits = std::max<size_t>(
-        1, std::min(std::min((blocks + span - 1) / span, most), (1024 + units - 1) / units));
+    const bool streams = smul(smul(units, blocks), 128, head_dim) > RD_STREAM_BYTES;
+    const size_t target = (size_t)compute_units() * (streams ? 2 : 1);
+    const size_t splits =
+        std::max<size_t>(1, std::min(std::min((blocks + span - 1) / span, most), (target + units - 1) / units));
     if (smul(units, splits) > MAX_WGS) return overrun_slice(smul(units, splits), MAX_WGS);
     const size_t parts = smul(units, splits, n / kv_heads);
     const size_t floats = splits > 1 ? sadd(parts, smul(units, splits, 2 * group)) : 0;
@@ -1435,6 +1454,8 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     a.shared = (int)std::min(shared, IMAX);
     a.splits = (int)splits;
     a.span = (int)span;
+    a.whole = RD_WHOLE;
+    a.stream = streams ? 1 : 0;
     a.scale = scale;
     a.softcap = softcap;
     return launched("attn_decode_ranges", launch_ranges_decode((int)head_dim, a, S(stream)));

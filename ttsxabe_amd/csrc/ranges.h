@@ -53,6 +53,8 @@ struct RangesDecodeArgs {
     long q_stride;
     int nseq, slots, cap, kv_heads, group, window, shared;
     int splits, span;       // workgroups of a head at most; blocks of 32 keys each takes at least
+    int whole;              // a head of up to so many blocks is one workgroup's
+    int stream;             // more bytes than are worth keeping in the Infinity Cache
     float scale, softcap;
 };
 hipError_t launch_ranges_decode(int hd, const RangesDecodeArgs& a, hipStream_t st);

@@ -645,13 +645,13 @@ hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStrea
 // block's 16 loads a lane are in flight while one is computed.
 //
 // The lengths are on the device, so the launch has `splits` runs a head for any
-// of them; each takes an equal share of its head's blocks, at least `span`, and
-// runs past them end at once. A head of several runs leaves (m, l, O) of each
-// with coherent stores, counts its arrivals, and the last one merges them in
-// order (the results do not depend on which that is).
+// of them; a head is cut into even ones, of `span` blocks or more, and those
+// past them end at once. A head of several runs leaves (m, l, O) of each with
+// coherent stores, counts its arrivals, and the last one merges them in order
+// (the results do not depend on which that is).
 constexpr int RD_MAX_ROWS = 1024;  // splits * group at most
 
-template <int HD, int MODE>
+template <int HD, int MODE, int AUX>
 __global__ __launch_bounds__(RT, 2) void ranges_decode_kernel(RangesDecodeArgs a) {
     constexpr int NS = HD / 32, NT = HD / 16, OP = HD + 4;  // a wave's O rows in LDS, padded
     struct Block {
@@ -685,27 +685,30 @@ __global__ __launch_bounds__(RT, 2) void ranges_decode_kernel(RangesDecodeArgs a
             for (int e = tid; e < n; e += RT) out[e] = live ? 0.0f : __builtin_nanf("");
         return;
     }
-    const int share = max(a.span, (nb + a.splits - 1) / a.splits);
-    const int runs = (nb + share - 1) / share;
+    // Its head in even runs.
+    const int runs = nb <= a.whole ? 1 : min(a.splits, (nb + a.span - 1) / a.span);
     if (sp >= runs) return;
-    const int end = min(nb, (sp + 1) * share);
+    const int share = (nb + runs - 1) / runs, begin = sp * share, end = min(nb, begin + share);
 
-    const half8* base = reinterpret_cast<const half8*>(a.cache) +
-                        ((size_t)slot * a.kv_heads + kh) * tiled_nblk(a.cap) * (8 * HD);
+    const char* base = reinterpret_cast<const char*>(a.cache) +
+                       ((size_t)slot * a.kv_heads + kh) * tiled_nblk(a.cap) * (128 * HD);
     auto block = [&](int i) { return i < na ? i : b0 + i - na; };
+    // Unconditional, so that each wait counts its own loads; past the run's end
+    // the resource holds no bytes and nothing is read.
     auto load = [&](Block& x, int i) __attribute__((always_inline)) {
-        const half8* p = base + (size_t)block(min(i, end - 1)) * (8 * HD) + lane;
+        const Region r = region(base + (size_t)block(i) * (128 * HD), i < end ? 128 * HD : 0);
 #pragma unroll
-        for (int j = 0; j < 2 * NS; ++j) x.k[j] = p[64 * j];
+        for (int j = 0; j < 2 * NS; ++j)
+            x.k[j] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(r.r, 16 * lane + 1024 * j, 0, AUX));
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x.v[j] = p[64 * (2 * NS + j)];
+        for (int j = 0; j < NT; ++j)
+            x.v[j] = __builtin_bit_cast(
+                half8, __builtin_amdgcn_raw_buffer_load_b128(r.r, 16 * lane + 1024 * (2 * NS + j), 0, AUX));
     };
-    int i = sp * share + wave;
+    int i = begin + wave;
     Block x0, x1;
-    if (i < end) {
-        load(x0, i);
-        load(x1, i + RW);
-    }
+    load(x0, i);
+    load(x1, i + RW);
     half8 qh[NS], ql[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) qh[s] = ql[s] = zero_h8();
@@ -933,7 +936,9 @@ hipError_t launch_ranges_decode(int hd, const RangesDecodeArgs& a, hipStream_t s
     const int mode = (a.softcap > 0.0f ? SM_CAP : 0) | (a.slopes ? SM_BIAS : 0);
 #define RD(HD, M)                                                                         \
     if (hd == HD && mode == M) {                                                          \
-        hipLaunchKernelGGL((ranges_decode_kernel<HD, M>), grid, dim3(RT), 0, st, a);      \
+        if (a.stream)                                                                     \
+            hipLaunchKernelGGL((ranges_decode_kernel<HD, M, AUX_STREAM>), grid, dim3(RT), 0, st, a); \
+        else hipLaunchKernelGGL((ranges_decode_kernel<HD, M, 0>), grid, dim3(RT), 0, st, a); \
         return hipGetLastError();                                                         \
     }
     RD(64, 0) RD(64, 1) RD(64, 2) RD(64, 3) RD(128, 0) RD(128, 1) RD(128, 2) RD(128, 3)
