@@ -1360,6 +1360,8 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
         if (off16(ws)) return refuse("a workspace off 16 bytes");
     }
     const int nqt = splits > 1 ? 1 : pick_nqt(tq, heads, gb);
+    const size_t ppi = smul((tq + 64 * (4 / gb) - 1) / (64 * (4 / gb)), heads / gb);
+    const bool pp = splits == 1 && ppi >= (getenv("XP") ? atoi(getenv("XP")) : 1024);
     const size_t items = smul((tq + 16 * nqt * (4 / gb) - 1) / (16 * nqt * (4 / gb)), heads / gb, splits);
     if (items > MAX_WGS) return overrun_slice(items, MAX_WGS);
     RangesArgs a{};
@@ -1382,7 +1384,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
     a.splits = (int)splits;
     a.ws = ws;
     a.qal = !off16(a.q) && a.q_stride % 8 == 0;
-    return launched("flash_attn_ranges", launch_ranges((int)head_dim, nqt, false, a, S(stream)));
+    return launched("flash_attn_ranges", launch_ranges((int)head_dim, nqt, pp, a, S(stream)));
 }
 
 int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,

@@ -123,12 +123,12 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7c00
 // never leaves registers.
 template <int HD, int MODE, int NQT>
 struct RangeTile {
-    static constexpr int NS = HD / 32, NT = HD / 16, KF = 4 * NS, VF = 2 * NT, FH = 64 * 8;
+    static constexpr int NS = HD / 32, NT = HD / 16, KF = 4 * NS, VF = 2 * NT, FH = 64 * 8, QPW = 16 * NQT;
     half8 qb[NQT][NS];
     floatx4 o[NT][NQT];
     float m[NQT], l[NQT];
-    int f[NQT], lo[NQT], hi[NQT];
-    float pos[NQT];  // SM_BIAS: the rows' positions
+    const int* rg;   // the wave's rows' ranges in LDS: first, lo, hi, QPW each
+    int pos0, last;  // SM_BIAS: the wave's first row's position, and the prompt's last
     floatx4 sc[2][2][NQT];
     half8 pb[2][NQT];
     float sl2;       // scale * log2(e)
@@ -142,10 +142,14 @@ struct RangeTile {
     __device__ __forceinline__ static uint64_t below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
     // Which of the tile's keys the rows see, one bit a key (a compare a score
     // kept 175 scalar registers of masks, and spilled).
+    __device__ __forceinline__ uint64_t tile_of(int u, int kv0) const {
+        const int* p = rg + 16 * u + (lane & 15);
+        return below(p[0] - kv0) | (below(p[2 * QPW] - kv0) & ~below(p[QPW] - kv0));
+    }
     __device__ __forceinline__ void look(int kv0) {
 #pragma unroll
         for (int u = 0; u < NQT; ++u) {
-            const uint64_t b = below(f[u] - kv0) | (below(hi[u] - kv0) & ~below(lo[u] - kv0));
+            const uint64_t b = tile_of(u, kv0);
             seen[u] = (uint32_t)(b >> (8 * grp)) & 0xffu;
             seen[u] |= ((uint32_t)(b >> 32 >> (8 * grp)) & 0xffu) << 8;
         }
@@ -155,26 +159,37 @@ struct RangeTile {
         return (uint32_t)__builtin_amdgcn_sbfe((int)seen[u], 8 * hf + e, 1);
     }
 
-    __device__ __forceinline__ void start(const RangesArgs& a, int p0, int h, int lane_) {
+    // The queries and ranges of the wave's rows from p0 on; the bounds of what
+    // they see. `mem`: 3 * QPW ints of LDS.
+    __device__ __forceinline__ Bounds start(const RangesArgs& a, int p0, int h, int lane_, int* mem) {
         lane = lane_;
         grp = lane >> 4;
+        rg = mem;
         const int col = lane & 15, ktot = a.past + a.tq;
+        pos0 = a.past + p0;
+        last = ktot - 1;
         sl2 = a.scale * LLMTIE_LOG2E;
         if constexpr ((MODE & SM_CAP) != 0) {
             kc = 2.0f * sl2 / a.softcap;
             c2 = a.softcap * LLMTIE_LOG2E;
         }
         if constexpr ((MODE & SM_BIAS) != 0) slope2 = a.slopes[h] * LLMTIE_LOG2E;
+        Bounds b{0x7fffffff, 0, 0x7fffffff, 0, 0x7fffffff, 0};
 #pragma unroll
         for (int u = 0; u < NQT; ++u) {
             const int r = min(p0 + 16 * u + col, a.tq - 1);
             // Clamped to the keys the cache holds; a range that holds none is
             // moved past every key, so that bounds over rows pass it by.
-            f[u] = max(0, min(a.first[r], ktot));
-            lo[u] = max(0, a.lo[r]);
-            hi[u] = min(a.hi[r], ktot);
-            if (lo[u] >= hi[u]) lo[u] = 0x7fffffff, hi[u] = 0;
-            if constexpr ((MODE & SM_BIAS) != 0) pos[u] = (float)(a.past + r);
+            const int f = max(0, min(a.first[r], ktot));
+            int lo = max(0, a.lo[r]), hi = min(a.hi[r], ktot);
+            if (lo >= hi) lo = 0x7fffffff, hi = 0;
+            if (grp == 0) {
+                int* p = mem + 16 * u + col;
+                p[0] = f, p[QPW] = lo, p[2 * QPW] = hi;
+            }
+            b.f0 = min(b.f0, f), b.f1 = max(b.f1, f);
+            b.l0 = min(b.l0, lo), b.l1 = max(b.l1, lo);
+            b.h0 = min(b.h0, hi), b.h1 = max(b.h1, hi);
             m[u] = RG_NOREF;
             l[u] = 0.0f;
             const uint16_t* q = a.q + (size_t)r * a.q_stride + (size_t)h * HD + 8 * grp;
@@ -192,19 +207,6 @@ struct RangeTile {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int u = 0; u < NQT; ++u) o[t][u] = zero_f4();
-    }
-
-    __device__ __forceinline__ Bounds bounds() const {
-        Bounds b{0x7fffffff, 0, 0x7fffffff, 0, 0x7fffffff, 0};
-#pragma unroll
-        for (int u = 0; u < NQT; ++u) {
-            b.f0 = min(b.f0, f[u]);
-            b.f1 = max(b.f1, f[u]);
-            b.l0 = min(b.l0, lo[u]);
-            b.l1 = max(b.l1, lo[u]);
-            b.h0 = min(b.h0, hi[u]);
-            b.h1 = max(b.h1, hi[u]);
-        }
         b.f0 = __builtin_amdgcn_readfirstlane(row_min(b.f0));
         b.f1 = __builtin_amdgcn_readfirstlane(row_max(b.f1));
         b.l0 = __builtin_amdgcn_readfirstlane(row_min(b.l0));
@@ -258,30 +260,47 @@ struct RangeTile {
     // inside f16, and the tile's max is taken on the rare tiles that move m.
     // P is rounded to f16 for the product (2^-11 of each weight, as the f16
     // context's own rounding); l sums the unrounded values at f32.
-    template <bool MASK>
-    __device__ __forceinline__ void softmax(int kv0) {
-        if constexpr (MASK) look(kv0);
+    // (One copy of it: a masked and an unmasked one spilled 320 registers.)
+    __device__ __forceinline__ void softmax(int kv0, bool whole) {
+        if constexpr (MODE != 0) {
+#pragma unroll
+            for (int u = 0; u < NQT; ++u) {
+                const float pos = (float)min(pos0 + 16 * u + (lane & 15), last);  // SM_BIAS
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int T = 0; T < 2; ++T)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            float s = sc[hf][T][u][r];
+                            if constexpr ((MODE & SM_CAP) != 0)
+                                s = __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(ex2(kc * s) + 1.0f), c2);
+                            else s *= sl2;
+                            if constexpr ((MODE & SM_BIAS) != 0) {
+                                const int key = kv0 + 32 * hf + 8 * grp + 4 * T + r;
+                                s = __builtin_fmaf(-slope2, fabsf(pos - (float)key), s);
+                            }
+                            sc[hf][T][u][r] = s;
+                        }
+            }
+        }
+        if (!whole) {
+            look(kv0);
+#pragma unroll
+            for (int u = 0; u < NQT; ++u)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int T = 0; T < 2; ++T)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const uint32_t on = sees(u, hf, 4 * T + r);
+                            sc[hf][T][u][r] =
+                                __uint_as_float((__float_as_uint(sc[hf][T][u][r]) & on) | (0xff800000u & ~on));
+                        }
+        }
 #pragma unroll
         for (int u = 0; u < NQT; ++u) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                for (int T = 0; T < 2; ++T)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int key = kv0 + 32 * hf + 8 * grp + 4 * T + r;
-                        float s = sc[hf][T][u][r];
-                        if constexpr ((MODE & SM_CAP) != 0)
-                            s = __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(ex2(kc * s) + 1.0f), c2);
-                        else if constexpr (MODE != 0) s *= sl2;
-                        if constexpr ((MODE & SM_BIAS) != 0)
-                            s = __builtin_fmaf(-slope2, fabsf(pos[u] - (float)key), s);
-                        if constexpr (MASK) {
-                            const uint32_t on = sees(u, hf, 4 * T + r);
-                            s = __uint_as_float((__float_as_uint(s) & on) | (0xff800000u & ~on));
-                        }
-                        sc[hf][T][u][r] = s;
-                    }
             auto form = [&]() __attribute__((always_inline)) {
                 float ps = 0.0f;
 #pragma unroll
@@ -336,20 +355,72 @@ struct RangeTile {
     // The values that screen() took out of the tile: a row whose keys hold one
     // gets what a sum with it is.
     __device__ __forceinline__ void specials(const uint4* sp, int kv0) {
+        uint64_t b[NQT];
 #pragma unroll
-        for (int u = 0; u < NQT; ++u) {
-            const uint64_t b = below(f[u] - kv0) | (below(hi[u] - kv0) & ~below(lo[u] - kv0));
-            const uint32_t b0 = (uint32_t)b, b1 = (uint32_t)(b >> 32);
+        for (int u = 0; u < NQT; ++u) b[u] = tile_of(u, kv0);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint4 w = sp[16 * t + 4 * grp + i];
+            for (int i = 0; i < 4; ++i) {
+                __builtin_amdgcn_sched_barrier(0);  // one dim's masks in registers at a time
+                const uint4 w = sp[16 * t + 4 * grp + i];
+#pragma unroll
+                for (int u = 0; u < NQT; ++u) {
+                    const uint32_t b0 = (uint32_t)b[u], b1 = (uint32_t)(b[u] >> 32);
                     // Any common bit: +inf or -inf, else 0 (NaN is in both masks).
                     o[t][u][i] += __uint_as_float(min((w.x & b0) | (w.y & b1), 1u) * 0x7f800000u);
                     o[t][u][i] -= __uint_as_float(min((w.z & b0) | (w.w & b1), 1u) * 0x7f800000u);
                 }
-        }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// Whether some value of a tile is not finite, as this wave's share of a look by
+// all W waves of the workgroup shows.
+template <int HD, int W>
+__device__ __forceinline__ bool odd_values(const half_t* vt, int tid) {
+    const uint4* v = reinterpret_cast<const uint4*>(vt);
+    uint32_t x = 0;
+#pragma unroll
+    for (int k = 0; k < 2 * (HD / 16) / W; ++k) {
+        const uint4 y = v[tid + W * 64 * k];
+        x |= not_finite(y.x) | not_finite(y.y) | not_finite(y.z) | not_finite(y.w);
+    }
+    return __any(x != 0);
+}
+
+// The bounds of all W waves' rows (a barrier).
+template <int W>
+__device__ __forceinline__ Bounds together(const Bounds& mine, int (*wb)[6], int wave, int lane) {
+    if (lane == 0) {
+        wb[wave][0] = mine.f0, wb[wave][1] = mine.f1, wb[wave][2] = mine.l0;
+        wb[wave][3] = mine.l1, wb[wave][4] = mine.h0, wb[wave][5] = mine.h1;
+    }
+    __syncthreads();
+    Bounds b = mine;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        b.f0 = min(b.f0, wb[w][0]), b.f1 = max(b.f1, wb[w][1]), b.l0 = min(b.l0, wb[w][2]);
+        b.l1 = max(b.l1, wb[w][3]), b.h0 = min(b.h0, wb[w][4]), b.h1 = max(b.h1, wb[w][5]);
+    }
+    b.f0 = __builtin_amdgcn_readfirstlane(b.f0), b.f1 = __builtin_amdgcn_readfirstlane(b.f1);
+    b.l0 = __builtin_amdgcn_readfirstlane(b.l0), b.l1 = __builtin_amdgcn_readfirstlane(b.l1);
+    b.h0 = __builtin_amdgcn_readfirstlane(b.h0), b.h1 = __builtin_amdgcn_readfirstlane(b.h1);
+    return b;
+}
+
+// The 64-key tiles that hold a key some row sees: na of the leading keys, then
+// those from tb on.
+struct Tiles {
+    int na, tb, n;
+    __device__ __forceinline__ explicit Tiles(const Bounds& b) {
+        na = (b.f1 + KT - 1) / KT;
+        tb = max(na, b.l0 / KT);
+        n = na + max(0, (b.h1 + KT - 1) / KT - tb);
+    }
+    __device__ __forceinline__ int key0(int i) const {
+        return __builtin_amdgcn_readfirstlane(KT * (i < na ? i : tb + i - na));
     }
 };
 
@@ -467,6 +538,7 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
     using Tile = RangeTile<HD, MODE, NQT>;
     constexpr int FH = Tile::FH, KF = Tile::KF, VF = Tile::VF, QPW = 16 * NQT;
     __shared__ __attribute__((aligned(16))) half_t tbuf[2][(KF + VF) * FH];
+    __shared__ int wrg[RW][3 * QPW];
     __shared__ int wb[RW][6];
     __shared__ int wbad[RW];
     __shared__ uint4 sp_[HD];
@@ -484,31 +556,15 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
     const RangeLoad<HD, RW> issue(a, kh, lane, wave);
 
     Tile t;
-    t.start(a, p0, h, lane);
-    const Bounds mine = t.bounds();
-    if (lane == 0) {
-        wb[wave][0] = mine.f0, wb[wave][1] = mine.f1, wb[wave][2] = mine.l0;
-        wb[wave][3] = mine.l1, wb[wave][4] = mine.h0, wb[wave][5] = mine.h1;
-    }
-    __syncthreads();
-    Bounds all = mine;
-#pragma unroll
-    for (int w = 0; w < RW; ++w) {
-        all.f0 = min(all.f0, wb[w][0]), all.f1 = max(all.f1, wb[w][1]), all.l0 = min(all.l0, wb[w][2]);
-        all.l1 = max(all.l1, wb[w][3]), all.h0 = min(all.h0, wb[w][4]), all.h1 = max(all.h1, wb[w][5]);
-    }
-    // Tiles: na of the leading keys, then those from tb on.
-    const int na = (all.f1 + KT - 1) / KT;
-    const int tb = max(na, all.l0 / KT);
-    const int nt = na + max(0, (all.h1 + KT - 1) / KT - tb);
-    int i0 = 0, i1 = nt;
+    const Bounds mine = t.start(a, p0, h, lane, wrg[wave]);
+    const Bounds all = together<RW>(mine, wb, wave, lane);
+    const Tiles tiles(all);
+    int i0 = 0, i1 = tiles.n;
     if constexpr (SPLIT) {
-        i0 = (int)((long)nt * sp / a.splits);
-        i1 = (int)((long)nt * (sp + 1) / a.splits);
+        i0 = __builtin_amdgcn_readfirstlane((int)((long)tiles.n * sp / a.splits));
+        i1 = __builtin_amdgcn_readfirstlane((int)((long)tiles.n * (sp + 1) / a.splits));
     }
-    i0 = __builtin_amdgcn_readfirstlane(i0);
-    i1 = __builtin_amdgcn_readfirstlane(i1);
-    auto key0 = [&](int i) { return __builtin_amdgcn_readfirstlane(KT * (i < na ? i : tb + i - na)); };
+    auto key0 = [&](int i) { return tiles.key0(i); };
 
     if (i0 < i1) issue(key0(i0), tbuf[0]);
     for (int i = i0; i < i1; ++i) {
@@ -520,14 +576,7 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
         bool bad = false;
         if (!all.whole(kv0)) {
             // Some row does not see some key: are all its values finite?
-            const uint4* v = reinterpret_cast<const uint4*>(cur + KF * FH);
-            uint32_t x = 0;
-#pragma unroll
-            for (int k = 0; k < VF * 64 / RT; ++k) {
-                const uint4 y = v[tid + RT * k];
-                x |= not_finite(y.x) | not_finite(y.y) | not_finite(y.z) | not_finite(y.w);
-            }
-            const bool any = __any(x != 0);
+            const bool any = odd_values<HD, RW>(cur + KF * FH, tid);
             if (lane == 0) wbad[wave] = any;
             __syncthreads();
             bad = (wbad[0] | wbad[1] | wbad[2] | wbad[3]) != 0;
@@ -540,8 +589,7 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
         }
         if (!mine.touches(kv0)) continue;
         t.scores(cur);
-        if (mine.whole(kv0)) t.template softmax<false>(kv0);
-        else t.template softmax<true>(kv0);
+        t.softmax(kv0, mine.whole(kv0));
         t.values(cur);
         if (bad) t.specials(sp_, kv0);
     }
@@ -553,6 +601,95 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
         const float lt = sum4grp(t.l[u]);
         if constexpr (SPLIT) store_part<HD, NQT>(t.o, u, t.m[u], lt, lane, a, sp, p0 + 16 * u, h);
         else store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
+    }
+}
+
+// Long prompts: eight waves in two groups of four that share each tile; waves w
+// and w + 4 share a SIMD. In the period between two barriers the first group
+// computes O += V^T P^T of tile q - 1, S of tile q and its softmax, the second
+// the softmax of tile q - 1, then the same products, so that one wave's softmax
+// (with the instructions of cap and bias) issues beside the other's MFMAs. Tiles rotate
+// through three buffers: period q reads K of tile q and V of tile q - 1, tile q +
+// 1 is issued at its start and waited for at its end. The arithmetic of a row is
+// ranges_kernel's, in the same order.
+constexpr int PPW = 8;
+
+template <int HD, int MODE>
+__global__ __launch_bounds__(PPW * LLMTIE_WAVE, 1) void ranges_pp_kernel(RangesArgs a) {
+    constexpr int NQT = 2;
+    using Tile = RangeTile<HD, MODE, NQT>;
+    constexpr int FH = Tile::FH, KF = Tile::KF, VF = Tile::VF, QPW = 16 * NQT;
+    __shared__ __attribute__((aligned(16))) half_t tbuf[3][(KF + VF) * FH];
+    __shared__ int wrg[PPW][3 * QPW];
+    __shared__ int wb[PPW][6];
+    __shared__ int wbad[2][PPW];
+    __shared__ uint4 sp_[HD];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool second = wave >= 4;
+    const int wl = wave & 3, gb = a.gb, gpr = QPW * (4 / gb), group = a.heads / a.kv_heads;
+    const int item = a.xcd ? (int)(blockIdx.x % 8) * a.grid8 + (int)(blockIdx.x / 8) : (int)blockIdx.x;
+    const int gy = item / a.nrb, bx = a.nrb - 1 - item % a.nrb;
+    const int h = gy * gb + wl % gb, kh = gy * gb / group;
+    const int p0 = bx * 2 * gpr + (second ? gpr : 0) + (wl / gb) * QPW;
+    const RangeLoad<HD, PPW> issue(a, kh, lane, wave);
+    Tile t;
+    const Bounds mine = t.start(a, p0, h, lane, wrg[wave]);
+    const Bounds all = together<PPW>(mine, wb, wave, lane);
+    const Tiles tiles(all);
+    const int n = tiles.n;
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < n) issue(tiles.key0(j), tbuf[j]);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    bool bad = false;  // tile q - 1 had values that are not finite
+    auto open = [&](int q) __attribute__((always_inline)) {
+        if (q >= 2 && q + 1 < n) issue(tiles.key0(q + 1), tbuf[(q + 1) % 3]);
+        bad = false;
+        if (q >= 1 && q <= n && !all.whole(tiles.key0(q - 1))) {
+            int x = 0;
+#pragma unroll
+            for (int w = 0; w < PPW; ++w) x |= wbad[(q + 1) & 1][w];
+            bad = __builtin_amdgcn_readfirstlane(x) != 0;
+            if (bad) {
+                screen_clear<HD, PPW>(sp_, tid);
+                __syncthreads();
+                screen<HD, PPW>(tbuf[(q + 2) % 3] + KF * FH, sp_, tid);
+                __syncthreads();
+            }
+        }
+        if (q < n && !all.whole(tiles.key0(q))) {
+            const bool any = odd_values<HD, PPW>(tbuf[q % 3] + KF * FH, tid);
+            if (lane == 0) wbad[q & 1][wave] = any;
+        }
+    };
+    auto turn = [&](int q) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(0);  // the tile issued at the start of this period
+        __syncthreads();
+        open(q);
+    };
+    open(0);
+    bool done = false;
+    for (int q = 0; q <= n; ++q) {
+        if (done) {
+            t.values(tbuf[(q + 2) % 3]);
+            if (bad) t.specials(sp_, tiles.key0(q - 1));
+        }
+        const int kv0 = tiles.key0(q);
+        done = q < n && mine.touches(kv0);
+        if (done) t.scores(tbuf[q % 3]);
+        // One barrier a period, behind the scores or behind the softmax: the
+        // waves' instructions are the same, half a period apart.
+        if (second) turn(q + 1);
+        if (done) t.softmax(kv0, mine.whole(kv0));
+        if (!second) turn(q + 1);
+    }
+    half_t* R = tbuf[0] + wave * 16 * HD;
+    static_assert(PPW * 16 * HD <= (KF + VF) * FH, "the waves' regions fit one buffer");
+#pragma unroll
+    for (int u = 0; u < NQT; ++u) {
+        const float lt = sum4grp(t.l[u]);
+        store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
     }
 }
 
@@ -606,13 +743,18 @@ __global__ __launch_bounds__(RT) void ranges_merge_kernel(const float* ws, uint1
 
 hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStream_t st) {
     RangesArgs b = a;
-    const int pb = 16 * nqt * (RW / a.gb);
+    const int pb = pp ? 64 * (4 / a.gb) : 16 * nqt * (RW / a.gb);
     b.nrb = (a.tq + pb - 1) / pb;
     const unsigned items = (unsigned)b.nrb * (unsigned)(a.heads / a.gb) * (unsigned)a.splits;
     b.xcd = items % 8 == 0;
     b.grid8 = (int)(items / 8);
     const int mode = (a.softcap > 0.0f ? SM_CAP : 0) | (a.slopes ? SM_BIAS : 0);
     const long rows = (long)a.tq * a.heads;
+#define RP(HD, M)                                                                                                \
+    if (hd == HD && mode == M && pp) {                                                                           \
+        hipLaunchKernelGGL((ranges_pp_kernel<HD, M>), dim3(items), dim3(PPW * LLMTIE_WAVE), 0, st, b);           \
+        return hipGetLastError();                                                                                \
+    }
 #define RL(HD, M, N)                                                                                             \
     if (hd == HD && mode == M && nqt == N && a.splits == 1) {                                                    \
         hipLaunchKernelGGL((ranges_kernel<HD, M, N, false>), dim3(items), dim3(RT), 0, st, b);                   \
@@ -625,11 +767,12 @@ hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStrea
                            dim3(RT), 0, st, a.ws, a.out, rows, a.splits);                                        \
         return hipGetLastError();                                                                                \
     }
-#define RM(HD, M) RL(HD, M, 1) RL(HD, M, 2) RS(HD, M)
+#define RM(HD, M) RP(HD, M) RL(HD, M, 1) RL(HD, M, 2) RS(HD, M)
     RM(64, 0) RM(64, 1) RM(64, 2) RM(64, 3) RM(128, 0) RM(128, 1) RM(128, 2) RM(128, 3)
 #undef RM
 #undef RS
 #undef RL
+#undef RP
     return hipErrorInvalidValue;
 }
 
