@@ -11,7 +11,8 @@ h = 2^-11 of f16):
              d_j = u (hd + 8) scale sum|q k| + 16 u c + 8 u (|s_j| + bias_j)
            which moves p_j by the factor 1 +- d_j, and the sum of all by their mean;
   weights  p_j rounded for the product: h (prompts) or 2^-22 (decode) of each, and
-           half a step of f16's smallest, 2^-25 of the largest weight;
+           half a step of f16's smallest, 2^-25 of the largest weight; the prompts'
+           normaliser is the sum of the rounded ones, as far off as its terms;
   sums     f32 sums over n keys: n u of sum p|v|, and as much of the normaliser;
   output   h (f16) or u (f32) of the value, and f16's 2^-25.
 """
@@ -109,6 +110,8 @@ def attend(q, k, v, seen, at, scale, softcap=0.0, slopes=None, decode=False):
         w = 2.0 ** -22 if decode else H
         off = (p * (w + d + 2 * n * U)) @ vh.abs() + 2.0 ** -25 * (seen / total) @ vh.abs()
         off = off + y.abs() * ((p * d).sum(-1, keepdim=True) + 2 * n * U + 4 * U)
+        if not decode:
+            off = off + y.abs() * (H + 2.0 ** -25 * n / total)
         off = 1.02 * off + y.abs() * (U if decode else H) + (0.0 if decode else 2.0 ** -25)
         out[:, h], tol[:, h] = y, off
     return out, tol

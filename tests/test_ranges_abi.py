@@ -103,7 +103,7 @@ def test_prompts():
     assert prompt(past=509) == 3 and prompt(past=W - 2) == 3
     for scale in (0.0, -1.0, math.nan, math.inf):
         assert prompt(scale=scale) == 10
-    for cap in (-1.0, math.nan, math.inf):
+    for cap in (-1.0, 1e-4, 2e3, math.nan, math.inf):
         assert prompt(softcap=cap) == 10
     assert prompt(slopes=X, slopes_len=31) == 4
     assert prompt(slot=1) == 4 and prompt(slots=0) == 4

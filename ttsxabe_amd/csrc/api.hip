@@ -1152,8 +1152,9 @@ constexpr size_t RD_STREAM_BYTES = (size_t)128 << 20;
 // What the score arguments must be. (The kernels keep running maxima of raw
 // products, so the scale is positive.)
 int score_checks(float scale, float softcap, const float* slopes, size_t slopes_len, size_t heads) {
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return refuse("a score scale that is not positive");
-    if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return refuse("a score cap that is neither 0 nor positive");
+    if (!(scale >= 1e-30f) || !(scale <= 1e30f)) return refuse("a score scale that is not in 1e-30 to 1e30");
+    if (softcap != 0.0f && !(softcap >= 1e-3f && softcap <= 1e3f))
+        return refuse("a score cap that is neither 0 nor in 0.001 to 1000");
     if (slopes && slopes_len < heads) return overrun_slice(heads, slopes_len);
     return LLMTIE_OK;
 }

@@ -79,6 +79,8 @@ hipError_t launch_key_ranges(const KeyRangeArgs& a, hipStream_t st) {
 
 // ------------------------------------------------------------------- scores
 
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+
 // What a launch does to its scores.
 constexpr int SM_CAP = 1, SM_BIAS = 2;
 
@@ -126,16 +128,18 @@ struct RangeTile {
     static constexpr int NS = HD / 32, NT = HD / 16, KF = 4 * NS, VF = 2 * NT, FH = 64 * 8, QPW = 16 * NQT;
     half8 qb[NQT][NS];
     floatx4 o[NT][NQT];
-    float m[NQT], l[NQT];
+    floatx4 l[NQT];  // the sum of the weights, in each element
+    float m[NQT];
     const int* rg;   // the wave's rows' ranges in LDS: first, lo, hi, QPW each
     int pos0, last;  // SM_BIAS: the wave's first row's position, and the prompt's last
     floatx4 sc[2][2][NQT];
     half8 pb[2][NQT];
-    float sl2;       // scale * log2(e)
-    float kc, c2;    // SM_CAP: tanh(scale s / c) c log2(e) = c2 - 2 c2 / (2^(kc s) + 1)
+    float mul, add;  // a logit (log2 units) is mul * (what logits() leaves) + add + the bias
+    float kc;        // SM_CAP: 2 log2(e) scale / c
     float slope2;    // SM_BIAS: slope * log2(e)
     int grp, lane;
 
+    uint32_t up[NQT], dn[NQT];  // values that are not finite (specials)
     uint32_t seen[NQT];  // the masked tile's keys that row col sees, of this lane's: bit 8 half + e
 
     // Bits 0 .. n - 1 of 64.
@@ -168,10 +172,12 @@ struct RangeTile {
         const int col = lane & 15, ktot = a.past + a.tq;
         pos0 = a.past + p0;
         last = ktot - 1;
-        sl2 = a.scale * LLMTIE_LOG2E;
+        mul = a.scale * LLMTIE_LOG2E;
+        add = 0.0f;
         if constexpr ((MODE & SM_CAP) != 0) {
-            kc = 2.0f * sl2 / a.softcap;
-            c2 = a.softcap * LLMTIE_LOG2E;
+            kc = 2.0f * LLMTIE_LOG2E * (a.scale / a.softcap);
+            add = a.softcap * LLMTIE_LOG2E;
+            mul = -2.0f * add;
         }
         if constexpr ((MODE & SM_BIAS) != 0) slope2 = a.slopes[h] * LLMTIE_LOG2E;
         Bounds b{0x7fffffff, 0, 0x7fffffff, 0, 0x7fffffff, 0};
@@ -191,7 +197,8 @@ struct RangeTile {
             b.l0 = min(b.l0, lo), b.l1 = max(b.l1, lo);
             b.h0 = min(b.h0, hi), b.h1 = max(b.h1, hi);
             m[u] = RG_NOREF;
-            l[u] = 0.0f;
+            l[u] = zero_f4();
+            up[u] = dn[u] = 0;
             const uint16_t* q = a.q + (size_t)r * a.q_stride + (size_t)h * HD + 8 * grp;
             if (a.qal) {
 #pragma unroll
@@ -253,38 +260,47 @@ struct RangeTile {
         pipeline<4 * NS>();
     }
 
-    // The online softmax of the tile in log2 units. P = 2^(s - m) is formed
-    // against the row's reference max m, which moves only when a lane's sum
-    // passes 2^15 (a key ~15 above m, the first seen key, or a NaN): O and l
-    // carry the same factor, so O / l does not depend on where m sits, P stays
-    // inside f16, and the tile's max is taken on the rare tiles that move m.
-    // P is rounded to f16 for the product (2^-11 of each weight, as the f16
-    // context's own rounding); l sums the unrounded values at f32.
-    // (One copy of it: a masked and an unmasked one spilled 320 registers.)
-    __device__ __forceinline__ void softmax(int kv0, bool whole) {
-        if constexpr (MODE != 0) {
+    // The scores in place as what a multiply-add makes a logit of: as they are,
+    // or with a cap 1 / (1 + 2^(kc s)), of which the tanh is 1 less twice:
+    //   c tanh(x) = c - 2 c / (1 + e^2x),   x = scale s / c;
+    // and an infinity for a key not seen. A wave issues an instruction in 4 to 7
+    // clocks, whatever it is: four a score here and three in softmax(), which
+    // the cap needs instead of three, set the time of a capped prompt. (A
+    // cubic in x^2 for scores under half the cap, no transcendentals but 9.5
+    // instructions: 8192 rows of 32/8/128 661 us.)
+    __device__ __forceinline__ void logits(int kv0, bool whole) {
+        if constexpr ((MODE & SM_CAP) != 0) {
 #pragma unroll
-            for (int u = 0; u < NQT; ++u) {
-                const float pos = (float)min(pos0 + 16 * u + (lane & 15), last);  // SM_BIAS
+            for (int u = 0; u < NQT; ++u)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                     for (int T = 0; T < 2; ++T)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float s = sc[hf][T][u][r];
-                            if constexpr ((MODE & SM_CAP) != 0)
-                                s = __builtin_fmaf(-2.0f * c2, __builtin_amdgcn_rcpf(ex2(kc * s) + 1.0f), c2);
-                            else s *= sl2;
-                            if constexpr ((MODE & SM_BIAS) != 0) {
-                                const int key = kv0 + 32 * hf + 8 * grp + 4 * T + r;
-                                s = __builtin_fmaf(-slope2, fabsf(pos - (float)key), s);
-                            }
-                            sc[hf][T][u][r] = s;
-                        }
+                        for (int r = 0; r < 4; ++r)
+                            sc[hf][T][u][r] = __builtin_amdgcn_rcpf(ex2(kc * sc[hf][T][u][r]) + 1.0f);
+        }
+        if constexpr ((MODE & SM_BIAS) != 0) {
+            if (mixed(kv0)) {
+                // softmax() takes the keys as behind their rows: for those
+                // ahead of them, twice their distance.
+                const float k2 = 2.0f * slope2 / mul;
+#pragma unroll
+                for (int u = 0; u < NQT; ++u) {
+                    const float d0 = (float)min(pos0 + 16 * u + (lane & 15), last) - (float)(kv0 + 8 * grp);
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                        for (int T = 0; T < 2; ++T)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                sc[hf][T][u][r] = __builtin_fmaf(k2, fminf(d0 - (float)(32 * hf + 4 * T + r), 0.0f),
+                                                                 sc[hf][T][u][r]);
+                }
             }
         }
         if (!whole) {
+            constexpr uint32_t OUT = (MODE & SM_CAP) != 0 ? 0x7f800000u : 0xff800000u;  // mul times it: -inf
             look(kv0);
 #pragma unroll
             for (int u = 0; u < NQT; ++u)
@@ -295,46 +311,74 @@ struct RangeTile {
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const uint32_t on = sees(u, hf, 4 * T + r);
-                            sc[hf][T][u][r] =
-                                __uint_as_float((__float_as_uint(sc[hf][T][u][r]) & on) | (0xff800000u & ~on));
+                            sc[hf][T][u][r] = __uint_as_float((__float_as_uint(sc[hf][T][u][r]) & on) | (OUT & ~on));
                         }
         }
+    }
+    // SM_BIAS: whether the tile has keys behind some rows and ahead of others,
+    // and on which side of the rows its keys lie if not (those of a mixed tile: behind).
+    __device__ __forceinline__ bool mixed(int kv0) const { return kv0 + KT - 1 > pos0 && kv0 < pos0 + QPW - 1; }
+    __device__ __forceinline__ float side(int kv0) const { return kv0 >= pos0 + QPW - 1 ? -slope2 : slope2; }
+
+    // The online softmax of the tile in log2 units. P = 2^(s - m) is formed
+    // against the row's reference max m, which moves only when a weight passes
+    // 2^15 (a key 15 above m, or the first one seen): O and l carry the same
+    // factor, so O / l does not depend on where m sits, P stays inside f16, and
+    // the tile's max is taken on the rare tiles that move m. P is rounded to f16
+    // for the product (2^-11 of each weight, as the f16 context's own rounding);
+    // l is the sum of the rounded weights at f32, by the matrix unit (a product
+    // with ones in values()): 16 additions a row and lane less, beside a
+    // packed maximum that watches for 2^15.
+    // (One copy of it: a masked and an unmasked one spilled 320 registers.)
+    __device__ __forceinline__ void softmax(int kv0, bool whole) {
+        logits(kv0, whole);
 #pragma unroll
         for (int u = 0; u < NQT; ++u) {
+            float sl = 0.0f, at = add;
+            if constexpr ((MODE & SM_BIAS) != 0) {
+                sl = side(kv0);
+                at += sl * (float)(kv0 + 8 * grp - min(pos0 + 16 * u + (lane & 15), last));
+            }
+            // The logit of the lane's key c of the tile, with `off` for what the keys share.
+            auto logit = [&](float s, int c, float off) __attribute__((always_inline)) {
+                if constexpr ((MODE & SM_BIAS) != 0) off = __builtin_fmaf(sl, (float)c, off);
+                return __builtin_fmaf(s, mul, off);
+            };
             auto form = [&]() __attribute__((always_inline)) {
-                float ps = 0.0f;
+                const float off = at - m[u];
+                half2_t top;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                     for (int T = 0; T < 2; ++T)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const float s = sc[hf][T][u][r];
-                            const float e = ex2(MODE ? s - m[u] : __builtin_fmaf(s, sl2, -m[u]));
-                            ps += e;
-                            pb[hf][u][4 * T + r] = to_h(e);
+                        for (int r = 0; r < 4; r += 2) {
+                            half2_t p;
+                            p[0] = to_h(ex2(logit(sc[hf][T][u][r], 32 * hf + 4 * T + r, off)));
+                            p[1] = to_h(ex2(logit(sc[hf][T][u][r + 1], 32 * hf + 4 * T + r + 1, off)));
+                            pb[hf][u][4 * T + r] = p[0];
+                            pb[hf][u][4 * T + r + 1] = p[1];
+                            top = hf | T | r ? __builtin_elementwise_max(top, p) : p;
                         }
-                return ps;
+                return fmaxf((float)top[0], (float)top[1]);
             };
-            float ps = form();
-            if (__any(!(ps <= 32768.0f))) {
+            if (__any(!(form() <= 32768.0f))) {
                 float mx = ninf();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                     for (int T = 0; T < 2; ++T)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, sc[hf][T][u][r]);
-                mx = max4grp(mx);
-                const float mn = fmaxf(m[u], MODE ? mx : mx * sl2);
+                        for (int r = 0; r < 4; ++r)
+                            mx = fmaxf(mx, logit(sc[hf][T][u][r], 32 * hf + 4 * T + r, at));
+                const float mn = fmaxf(m[u], max4grp(mx));
                 const float fac = ex2(m[u] - mn);
                 m[u] = mn;
                 l[u] *= fac;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) o[t][u] *= fac;
-                ps = form();
+                form();
             }
-            l[u] += ps;
         }
     }
 
@@ -349,30 +393,49 @@ struct RangeTile {
 #pragma unroll
                 for (int u = 0; u < NQT; ++u) o[t][u] = mfma16(af, pb[hf][u], o[t][u]);
             }
+        half8 ones;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ones[j] = (half_t)1.0f;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int u = 0; u < NQT; ++u) l[u] = mfma16(ones, pb[hf][u], l[u]);
         pipeline<2 * NT>();
     }
 
-    // The values that screen() took out of the tile: a row whose keys hold one
-    // gets what a sum with it is.
+    // The values that screen() took out of the tile: whether a key that a row
+    // sees held one, a bit a dim of this lane's (4 t + i), for +inf or NaN and
+    // for -inf or NaN. (Adding them to O here had the loop keep it in two places.)
     __device__ __forceinline__ void specials(const uint4* sp, int kv0) {
         uint64_t b[NQT];
 #pragma unroll
         for (int u = 0; u < NQT; ++u) b[u] = tile_of(u, kv0);
+#pragma nounroll
+        for (int d = 0; d < 4 * NT; ++d) {
+            const uint4 w = sp[16 * (d >> 2) + 4 * grp + (d & 3)];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                __builtin_amdgcn_sched_barrier(0);  // one dim's masks in registers at a time
-                const uint4 w = sp[16 * t + 4 * grp + i];
-#pragma unroll
-                for (int u = 0; u < NQT; ++u) {
-                    const uint32_t b0 = (uint32_t)b[u], b1 = (uint32_t)(b[u] >> 32);
-                    // Any common bit: +inf or -inf, else 0 (NaN is in both masks).
-                    o[t][u][i] += __uint_as_float(min((w.x & b0) | (w.y & b1), 1u) * 0x7f800000u);
-                    o[t][u][i] -= __uint_as_float(min((w.z & b0) | (w.w & b1), 1u) * 0x7f800000u);
-                }
+            for (int u = 0; u < NQT; ++u) {
+                const uint32_t b0 = (uint32_t)b[u], b1 = (uint32_t)(b[u] >> 32);
+                up[u] |= min((w.x & b0) | (w.y & b1), 1u) << d;
+                dn[u] |= min((w.z & b0) | (w.w & b1), 1u) << d;
             }
-        __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // What a sum with them is: +inf, -inf, or NaN with both.
+    __device__ __forceinline__ void close() {
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < NQT; ++u) any |= up[u] | dn[u];
+        if (!__any(any != 0)) return;
+#pragma unroll
+        for (int u = 0; u < NQT; ++u)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[t][u][i] += __uint_as_float((up[u] >> (4 * t + i) & 1u) * 0x7f800000u);
+                    o[t][u][i] -= __uint_as_float((dn[u] >> (4 * t + i) & 1u) * 0x7f800000u);
+                }
     }
 };
 
@@ -411,7 +474,9 @@ __device__ __forceinline__ Bounds together(const Bounds& mine, int (*wb)[6], int
 }
 
 // The 64-key tiles that hold a key some row sees: na of the leading keys, then
-// those from tb on.
+// those from tb on; walked from the last to the first. (With a bias by distance
+// the near keys weigh most: from the first to the last, nearly every tile of a
+// steep head raised the row's max and was formed twice.)
 struct Tiles {
     int na, tb, n;
     __device__ __forceinline__ explicit Tiles(const Bounds& b) {
@@ -420,7 +485,8 @@ struct Tiles {
         n = na + max(0, (b.h1 + KT - 1) / KT - tb);
     }
     __device__ __forceinline__ int key0(int i) const {
-        return __builtin_amdgcn_readfirstlane(KT * (i < na ? i : tb + i - na));
+        const int j = n - 1 - i;
+        return __builtin_amdgcn_readfirstlane(KT * (j < na ? j : tb + j - na));
     }
 };
 
@@ -596,9 +662,10 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
     // The context through the buffer that does not hold the last tile: every
     // wave left it before the last tile's barrier.
     half_t* R = tbuf[(i1 - i0) & 1] + wave * 16 * HD;
+    t.close();
 #pragma unroll
     for (int u = 0; u < NQT; ++u) {
-        const float lt = sum4grp(t.l[u]);
+        const float lt = t.l[u][0];
         if constexpr (SPLIT) store_part<HD, NQT>(t.o, u, t.m[u], lt, lane, a, sp, p0 + 16 * u, h);
         else store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
     }
@@ -685,10 +752,11 @@ __global__ __launch_bounds__(PPW * LLMTIE_WAVE, 1) void ranges_pp_kernel(RangesA
         if (!second) turn(q + 1);
     }
     half_t* R = tbuf[0] + wave * 16 * HD;
+    t.close();
     static_assert(PPW * 16 * HD <= (KF + VF) * FH, "the waves' regions fit one buffer");
 #pragma unroll
     for (int u = 0; u < NQT; ++u) {
-        const float lt = sum4grp(t.l[u]);
+        const float lt = t.l[u][0];
         store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
     }
 }
