@@ -133,6 +133,37 @@ def test_prompt_random(gpu, seed):
     close(got, want, tol, (rows, past, table, shape))
 
 
+@pytest.mark.parametrize("kv", [32, 64, 128])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("c", [
+    (1024, 0, {}, False), (1030, 77, dict(starts=[0, 300, 301, 900, 1010], prefix=[100, 1, 599, 20]), True),
+    (1100, 40, dict(window=130, shared=5), True), (1024, 0, dict(causal=False), True),
+], ids=lambda c: f"{c[0]}+{c[1]}-{'-'.join(c[2])}")
+def test_prompt_of_many_workgroups(gpu, kv, hd, c):
+    """Enough row blocks for the eight-wave kernel, in each division of heads over its waves; some groups of heads
+    are compared. Where documents are, one of them holds values that are not finite."""
+    rows, past, table, bias = c
+    heads, keys = 128, past + rows
+    group = heads // kv
+    k, v, q = f16(1, 1, kv, keys, hd), f16(2, 1, kv, keys, hd), f16(3, rows, heads, hd, scale=3.0)
+    odd = "starts" in table
+    if odd:
+        k[0, :, past + 299], v[0, :, past + 299], v[0, :, past + 298, ::3] = math.nan, math.nan, -math.inf
+    t = {n: torch.tensor(x, dtype=torch.int32).cuda() if isinstance(x, list) else x for n, x in table.items()}
+    sl = slopes_of(heads)
+    got = gpu.flash_attn_ranges(q.cuda().view(-1), 0, heads * hd, cache_of(k, v), 0, gpu.key_ranges(rows, past, **t), rows,
+                                past, heads, 0.1, slopes=sl.cuda() if bias else None)
+    seen = ref.visible(ref.ranges(rows, past, **table), keys)
+    part = slice(300, rows) if odd else slice(0, rows)
+    kvs = [0, kv // 2 - 1, kv - 1]
+    hs = [h for x in kvs for h in range(x * group, x * group + group)]
+    want, tol = ref.attend(q[part][:, hs], k[0, kvs], v[0, kvs], seen[part], torch.arange(past, keys)[part], 0.1,
+                           slopes=sl[hs] if bias else None)
+    close(got.view(rows, heads, hd)[part][:, hs].contiguous(), want, tol)
+    if odd:
+        assert torch.isnan(got.view(rows, -1)[299]).all() and not torch.isnan(got.view(rows, -1)[300:]).any()
+
+
 def test_prompt_rows_of_a_longer_stride_and_odd_offset(gpu):
     """Queries inside wider rows, aligned or not."""
     rows, heads, kv, hd = 37, 8, 2, 128

@@ -1160,7 +1160,11 @@ int score_checks(float scale, float softcap, const float* slopes, size_t slopes_
 }
 
 // Runs that a prompt's row blocks are cut into (1: whole) when they are few and
-// their keys many.
+// their keys many: two workgroups a compute unit, of four tiles or more. Us, as
+// planned / whole: 173 rows after 3011 of 32/8/128 28.5 / 56.7 (5 runs; 4 29.5, 8
+// 31.4), 16 after 3000 16.5 / 56.8 (11; 8 17.2, 16 17.2), 100 after 7000 31.4 /
+// 124, 40 after 1000 12.5 / 19.7, 400 after 1500 31.5 / 33.2 (2; 4 35.7); 40 after
+// 2000 of 20/20/64 12.0 / 29.9; 1000 rows of 32/8/128 (504 blocks, whole) in 2 34.4 / 24.1.
 size_t plan_range_splits(size_t tq, size_t keys, size_t heads, size_t kv_heads) {
     const size_t group = heads / kv_heads;
     const size_t gb = group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
@@ -1361,8 +1365,13 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
         if (off16(ws)) return refuse("a workspace off 16 bytes");
     }
     const int nqt = splits > 1 ? 1 : pick_nqt(tq, heads, gb);
-    const size_t ppi = smul((tq + 64 * (4 / gb) - 1) / (64 * (4 / gb)), heads / gb);
-    const bool pp = splits == 1 && ppi >= (getenv("XP") ? atoi(getenv("XP")) : 1024);
+    // The eight-wave kernel for head_dim 128 and no cap, where its workgroups of
+    // 64 rows a head are two a compute unit. 32/8/128, us, eight waves / four:
+    // 8192 rows 510 / 561, biased 502 / 549, capped 675 / 667; 4096 148 / 164; 1999
+    // 62 / 51; 3968 of 40/40/128 220 / 214, before 214 / 228; 8192 of 32/8/64 352 / 319.
+    const size_t blocks8 = smul((tq + 64 * (4 / gb) - 1) / (64 * (4 / gb)), heads / gb);
+    const bool pp =
+        splits == 1 && head_dim == 128 && softcap == 0.0f && blocks8 >= 2 * (size_t)compute_units();
     const size_t items = smul((tq + 16 * nqt * (4 / gb) - 1) / (16 * nqt * (4 / gb)), heads / gb, splits);
     if (items > MAX_WGS) return overrun_slice(items, MAX_WGS);
     RangesArgs a{};

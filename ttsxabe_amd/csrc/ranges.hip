@@ -678,7 +678,10 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
 // (with the instructions of cap and bias) issues beside the other's MFMAs. Tiles rotate
 // through three buffers: period q reads K of tile q and V of tile q - 1, tile q +
 // 1 is issued at its start and waited for at its end. The arithmetic of a row is
-// ranges_kernel's, in the same order.
+// ranges_kernel's, in the same order. Not for capped scores: their softmax is
+// longer than the products, so a period waits for it (8192 rows of 32/8/128 675
+// against 667 us; without a cap 510 against 561, 1080 TF, of 1147 that the
+// library's product reaches at 8192^3).
 constexpr int PPW = 8;
 
 template <int HD, int MODE>
@@ -835,7 +838,8 @@ hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStrea
                            dim3(RT), 0, st, a.ws, a.out, rows, a.splits);                                        \
         return hipGetLastError();                                                                                \
     }
-#define RM(HD, M) RP(HD, M) RL(HD, M, 1) RL(HD, M, 2) RS(HD, M)
+#define RM(HD, M) RL(HD, M, 1) RL(HD, M, 2) RS(HD, M)
+    RP(128, 0) RP(128, SM_BIAS)
     RM(64, 0) RM(64, 1) RM(64, 2) RM(64, 3) RM(128, 0) RM(128, 1) RM(128, 2) RM(128, 3)
 #undef RM
 #undef RS
