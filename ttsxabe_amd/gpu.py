@@ -561,34 +561,41 @@ class Gpu:
                                             cache.cap))
 
     # ------------------------------- key ranges and rotary positions by row
+    #
+    # These calls are a launch or two of a few microseconds, and their host work
+    # sets the pace of small ones: checks are one call a tensor, and a result is
+    # returned as it was allocated (a view of it costs as much as the allocation).
 
     def _run(self, fn, *args):
         """A call whose launches go to this Gpu's device, whichever is current."""
-        if torch._C._cuda_getDevice() == self.device.index:
-            _check(fn(self._stream(), *args))
+        i = self.device.index
+        if torch._C._cuda_getDevice() == i:
+            status = fn(torch._C._cuda_getCurrentRawStream(i), *args)
         else:
             with torch.cuda.device(self.device):
-                _check(fn(self._stream(), *args))
+                status = fn(self._stream(), *args)
+        if status:
+            _check(status)
 
-    def _here(self, *tensors):
-        """Checks of (tensor, dtypes, name): as _need, and on this Gpu's device."""
-        for t, dtypes, what in tensors:
+    def _on(self, t, dtypes, what):
+        """As _need, and on this Gpu's device."""
+        if t is not None and (t.get_device() != self.device.index or t.dtype not in dtypes or not t.is_contiguous()):
             _need(t, dtypes, what)
-            if t is not None and t.device != self.device:
-                raise InvalidArgument(f"{what} is on {t.device}, not on {self.device}")
+            raise InvalidArgument(f"{what} is on {t.device}, not on {self.device}")
 
     def key_ranges(self, rows, past=0, starts=None, prefix=None, causal=True, window=0, shared=0) -> KeyRanges:
         """Which keys each of `rows` rows behind `past` positions sees (new; see
         llmtie_key_ranges): documents from `starts` (int32, one more than there
         are), `prefix` leading rows of each that its rows all see, a `window`,
         `shared` leading positions that every row sees."""
-        self._here((starts, _I32, "starts"), (prefix, _I32, "prefix"))
-        if min(rows, past, window, shared) < 0:
+        self._on(starts, _I32, "starts")
+        self._on(prefix, _I32, "prefix")
+        if rows < 0 or past < 0 or window < 0 or shared < 0:
             raise InvalidArgument("a negative count")
-        buf = torch.empty(4 * max(rows, 1), dtype=torch.int32, device=self.device)
-        table, pos = buf[: 3 * rows].view(3, rows), buf[3 * rows: 4 * rows]
+        table = torch.empty((3, rows), dtype=torch.int32, device=self.device)
+        pos = torch.empty(rows, dtype=torch.int32, device=self.device)
         self._run(self._L.llmtie_key_ranges, _p(starts), _n(starts), _p(prefix), _n(prefix), rows, past,
-                  int(bool(causal)), window, shared, _p(table), _n(table), _p(pos), _n(pos))
+                  1 if causal else 0, window, shared, table.data_ptr(), 3 * rows, pos.data_ptr(), rows)
         most = past + rows
         if causal and window and prefix is None:
             most = min(most, window + shared)
@@ -599,17 +606,23 @@ class Gpu:
         """Rotary positions by row (new): t rows of `heads` heads at x[off + r *
         stride ..], row r at pos[r] (int32 tensor; an int: pos + r), into `out`
         (f32 or f16; default in place)."""
-        first = 0 if isinstance(pos, torch.Tensor) else int(pos)
-        posd = pos if isinstance(pos, torch.Tensor) else None
         if out is None:
             out, out_off, out_stride = x, off, stride
-        self._here((x, _F32, "x"), (posd, _I32, "pos"), (freq_div, _F32, "freq_div"), (out, _F32 + _H16, "out"))
-        if min(off, stride, first, t, heads, head_dim, rot_dim, out_off) < 0:
+        elif out_stride is None:
+            out_stride = heads * head_dim
+        self._on(x, _F32, "x")
+        self._on(out, _F32 + _H16, "out")
+        self._on(freq_div, _F32, "freq_div")
+        if isinstance(pos, torch.Tensor):
+            self._on(pos, _I32, "pos")
+            at = pos.data_ptr(), pos.numel(), 0
+        else:
+            at = None, 0, int(pos)
+        if min(off, stride, at[2], t, heads, head_dim, rot_dim, out_off, out_stride) < 0:
             raise InvalidArgument("a negative count")
-        self._run(self._L.llmtie_rope_rows, _p(x), _n(x), off, stride, _p(out), _n(out), out_off,
-                  heads * head_dim if out_stride is None else out_stride, int(out.dtype != torch.float32), _p(posd),
-                  _n(posd), first, _p(freq_div), _n(freq_div), t, heads, head_dim, rot_dim, theta, mscale,
-                  int(bool(interleaved)))
+        self._run(self._L.llmtie_rope_rows, x.data_ptr(), x.numel(), off, stride, out.data_ptr(), out.numel(), out_off,
+                  out_stride, 0 if out.dtype is torch.float32 else 1, *at, _p(freq_div), _n(freq_div), t, heads,
+                  head_dim, rot_dim, theta, mscale, 1 if interleaved else 0)
 
     def t16_rope_store(self, q, q_off, k, k_off, v, v_off, stride, pos, slot, index, freq_div, rows, heads, rot_dim,
                        theta, mscale, interleaved, cache: TiledCache16, q_out=None, q_out_off=0, q_out_stride=None):
@@ -617,65 +630,89 @@ class Gpu:
         projections (`stride` apart, one stacked tensor or three) to position
         index[r] of slot slot[r] of a tiled cache; q (None: none) into q_out (f32
         or f16; default in place)."""
-        if q is not None and q_out is None:
-            q_out, q_out_off, q_out_stride = q, q_off, stride
-        self._here((q, _F32, "q"), (k, _F32, "k"), (v, _F32, "v"), (pos, _I32, "pos"), (slot, _I32, "slot"),
-                   (index, _I32, "index"), (freq_div, _F32, "freq_div"), (q_out, _F32 + _H16, "q_out"),
-                   (cache.data, _H16, "cache"))
-        if min(q_off, k_off, v_off, stride, rows, heads, rot_dim, q_out_off) < 0:
+        self._on(k, _F32, "k")
+        self._on(v, _F32, "v")
+        f16 = 0
+        if q is None:
+            q_out_stride = 0
+        else:
+            self._on(q, _F32, "q")
+            if q_out is None:
+                q_out, q_out_off, q_out_stride = q, q_off, stride
+            else:
+                self._on(q_out, _F32 + _H16, "q_out")
+                f16 = 0 if q_out.dtype is torch.float32 else 1
+                if q_out_stride is None:
+                    q_out_stride = heads * cache.head_dim
+        for t, what in ((pos, "pos"), (slot, "slot"), (index, "index")):
+            self._on(t, _I32, what)
+            if t.numel() < rows:
+                raise SliceOverrun(f"reading to {rows} in a buffer of {t.numel()}", (rows, t.numel()))
+        self._on(freq_div, _F32, "freq_div")
+        self._on(cache.data, _H16, "cache")
+        if min(q_off, k_off, v_off, stride, rows, heads, rot_dim, q_out_off, q_out_stride) < 0:
             raise InvalidArgument("a negative count")
-        n = min(_n(pos), _n(slot), _n(index))
-        if n < rows:
-            raise SliceOverrun(f"reading to {rows} in a buffer of {n}", (rows, n))
         self._run(self._L.llmtie_t16_rope_store, _p(q), _n(q), q_off, stride, _p(q_out), _n(q_out), q_out_off,
-                  heads * cache.head_dim if q_out_stride is None else q_out_stride,
-                  int(q_out is not None and q_out.dtype != torch.float32), _p(k), _n(k), k_off, stride, _p(v), _n(v),
-                  v_off, stride, _p(pos), _p(slot), _p(index), n, _p(freq_div), _n(freq_div), rows, heads,
-                  cache.kv_heads, cache.head_dim, rot_dim, theta, mscale, int(bool(interleaved)), _p(cache.data),
-                  _n(cache.data), cache.slots, cache.cap)
+                  q_out_stride, f16, k.data_ptr(), k.numel(), k_off, stride, v.data_ptr(), v.numel(), v_off, stride,
+                  pos.data_ptr(), slot.data_ptr(), index.data_ptr(), rows, _p(freq_div), _n(freq_div), rows, heads,
+                  cache.kv_heads, cache.head_dim, rot_dim, theta, mscale, 1 if interleaved else 0,
+                  cache.data.data_ptr(), cache.data.numel(), cache.slots, cache.cap)
 
     def flash_attn_ranges(self, q, q_off, q_stride, cache: TiledCache16, slot, ranges: KeyRanges, tq, past, heads,
                           scale, softcap=0.0, slopes=None):
         """Attention of tq rows (f16) over their key ranges of a slot of a tiled
         cache (new), scores capped (`softcap`) or biased by distance (`slopes`,
         one a head). Returns the f16 context [tq * heads * head_dim]."""
-        self._here((q, _H16, "q"), (cache.data, _H16, "cache"), (ranges.table, _I32, "ranges"),
-                   (slopes, _F32, "slopes"))
+        data, table, hd = cache.data, ranges.table, cache.head_dim
+        self._on(q, _H16, "q")
+        self._on(data, _H16, "cache")
+        self._on(table, _I32, "ranges")
+        self._on(slopes, _F32, "slopes")
         if min(q_off, q_stride, slot, tq, past, heads, ranges.max_keys) < 0:
             raise InvalidArgument("a negative count")
-        n = tq * heads * cache.head_dim
-        out = torch.empty(max(n, 1), dtype=torch.float16, device=self.device)
-        ws, keys = None, min(ranges.max_keys or past + tq, past + tq)
+        n = tq * heads * hd
+        out = torch.empty(n, dtype=torch.float16, device=self.device)
+        ws, floats, keys = None, 0, past + tq
+        if ranges.max_keys:
+            keys = min(ranges.max_keys, keys)
         if keys > 512:  # fewer are never cut
-            floats = self._L.llmtie_flash_attn_ranges_workspace(tq, keys, heads, cache.kv_heads, cache.head_dim)
+            floats = self._L.llmtie_flash_attn_ranges_workspace(tq, keys, heads, cache.kv_heads, hd)
             if floats:
                 try:
                     ws = torch.empty(floats, dtype=torch.float32, device=self.device)
                 except torch.OutOfMemoryError:
-                    pass  # whole, it needs nothing beside its output
-        self._run(self._L.llmtie_flash_attn_ranges_t16, _p(q), _n(q), q_off, q_stride, _p(cache.data), _n(cache.data),
-                  cache.slots, slot, _p(ranges.table), _n(ranges.table), ranges.max_keys, _p(out), n, tq, past, heads,
-                  cache.kv_heads, cache.head_dim, cache.cap, scale, softcap, _p(slopes), _n(slopes), _p(ws), _n(ws))
-        return out[:n]
+                    floats = 0  # whole, it needs nothing beside its output
+        self._run(self._L.llmtie_flash_attn_ranges_t16, q.data_ptr(), q.numel(), q_off, q_stride, data.data_ptr(),
+                  data.numel(), cache.slots, slot, table.data_ptr(), table.numel(), ranges.max_keys, out.data_ptr(), n,
+                  tq, past, heads, cache.kv_heads, hd, cache.cap, scale, softcap, _p(slopes), _n(slopes), _p(ws),
+                  floats)
+        return out
 
     def attn_decode_ranges(self, q, q_off, q_stride, cache: TiledCache16, tk_dev, slot_dev, max_tk, heads, scale,
                            scratch, lo_dev=None, window=0, shared=0, softcap=0.0, slopes=None, out=None):
         """One token of each of len(tk_dev) sequences over their slots of a tiled
         cache (new): the first `shared` positions and those from max(lo_dev, tk
         - window) on, scores as in flash_attn_ranges. Returns the f32 context."""
-        self._here((q, _F32, "q"), (cache.data, _H16, "cache"), (tk_dev, _I32, "tk"), (slot_dev, _I32, "slot"),
-                   (lo_dev, _I32, "lo"), (slopes, _F32, "slopes"), (out, _F32, "out"))
+        data = cache.data
+        self._on(q, _F32, "q")
+        self._on(data, _H16, "cache")
+        self._on(tk_dev, _I32, "tk")
+        self._on(slopes, _F32, "slopes")
+        nseq = tk_dev.numel()
+        for t, what in ((slot_dev, "slot"), (lo_dev, "lo")):
+            if t is not None:
+                self._on(t, _I32, what)
+                if t.numel() < nseq:
+                    raise SliceOverrun(f"reading to {nseq} in a buffer of {t.numel()}", (nseq, t.numel()))
         if min(q_off, q_stride, max_tk, heads, window, shared) < 0:
             raise InvalidArgument("a negative count")
-        nseq = tk_dev.numel()
-        for t in (slot_dev, lo_dev):
-            if t is not None and t.numel() < nseq:
-                raise SliceOverrun(f"reading to {nseq} in a buffer of {t.numel()}", (nseq, t.numel()))
         n = nseq * heads * cache.head_dim
         if out is None:
-            out = torch.empty(max(n, 1), dtype=torch.float32, device=self.device)
-        self._run(self._L.llmtie_attn_decode_ranges_t16, _p(q), _n(q), q_off, q_stride, _p(cache.data),
-                  _n(cache.data), cache.slots, _p(tk_dev), _p(slot_dev), _p(lo_dev), nseq, max_tk, window, shared,
+            out = torch.empty(n, dtype=torch.float32, device=self.device)
+        else:
+            self._on(out, _F32, "out")
+        self._run(self._L.llmtie_attn_decode_ranges_t16, q.data_ptr(), q.numel(), q_off, q_stride, data.data_ptr(),
+                  data.numel(), cache.slots, tk_dev.data_ptr(), _p(slot_dev), _p(lo_dev), nseq, max_tk, window, shared,
                   heads, cache.kv_heads, cache.head_dim, cache.cap, scale, softcap, _p(slopes), _n(slopes),
-                  scratch.handle, _p(out), _n(out))
-        return out[:n]
+                  scratch.handle, out.data_ptr(), out.numel())
+        return out if out.numel() == n else out[:n]
