@@ -1285,6 +1285,7 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
     if (rows > 1 && (k_stride < nk || v_stride < nk)) return overrun_slice(nk, std::min(k_stride, v_stride));
     if (reach(k_off, rows, k_stride, nk) > k_len) return overrun_slice(reach(k_off, rows, k_stride, nk), k_len);
     if (reach(v_off, rows, v_stride, nk) > v_len) return overrun_slice(reach(v_off, rows, v_stride, nk), v_len);
+    if (rows > (size_t)1 << 26) return overrun_slice(rows, (size_t)1 << 26);  // workgroups of a launch
     if (rows == 0) return ok();
     if (!k || !v || !pos || !slot || !index || !cache || (q && !q_out)) return invalid("a buffer");
     if (off16(cache)) return refuse("a cache off 16 bytes");
