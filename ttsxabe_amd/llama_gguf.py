@@ -16,7 +16,7 @@ the original ones: original row k * hd/2 + i of a head is stored at row
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 
 import numpy as np
 
@@ -40,6 +40,11 @@ class LlamaConfig:
     layers: int
     theta: float
     eps: float
+    # What LlamaBatch's rotary takes beside these: rotated dims of a head (0:
+    # all), (kind, factor, original positions) of a long context, pairs (2i, 2i + 1).
+    rope_dim: int = 0
+    rope_scaling: tuple | None = None
+    rope_interleaved: bool = False
 
 
 def config_from_gguf(f: GgufFile) -> LlamaConfig:
@@ -79,9 +84,14 @@ def config_from_gguf(f: GgufFile) -> LlamaConfig:
     kv = need("llama.attention.head_count_kv")
     if kv == 0 or heads % kv:
         raise LlamaGgufError(f"{heads} query heads do not group over {kv} kv heads")
+    kind, factor = f.get_str("llama.rope.scaling.type"), f.get_f32("llama.rope.scaling.factor")
+    scaling = None
+    if kind in ("linear", "yarn") and factor is not None:
+        scaling = (kind, factor, f.get_u32("llama.rope.scaling.original_context_length") or 8192)
     return LlamaConfig(vocab=vocab, hidden=hidden, heads=heads, kv_heads=kv, head_dim=hd,
                        ffn=need("llama.feed_forward_length"), layers=need("llama.block_count"),
-                       theta=need_f("llama.rope.freq_base"), eps=need_f("llama.attention.layer_norm_rms_epsilon"))
+                       theta=need_f("llama.rope.freq_base"), eps=need_f("llama.attention.layer_norm_rms_epsilon"),
+                       rope_dim=f.get_u32("llama.rope.dimension_count") or 0, rope_scaling=scaling)
 
 
 def unpermute_rope(w: np.ndarray, heads: int) -> np.ndarray:
@@ -99,13 +109,18 @@ def permute_rope(w: np.ndarray, heads: int) -> np.ndarray:
     return w.reshape(heads, 2, hd // 2, -1).transpose(0, 2, 1, 3).reshape(w.shape)
 
 
-def load_llama_gguf(path_or_file):
-    """(config, weights) for `LlamaStack` from a GGUF Llama: every tensor
+def load_llama_gguf(path_or_file, interleaved: bool = False):
+    """(config, weights) for `LlamaStack` or `LlamaBatch` from a GGUF Llama
+    (`interleaved`: `attn_q` and `attn_k` as the file holds them, for
+    `LlamaBatch`'s interleaved rotation): every tensor
     decoded to f32 and checked against the geometry (weights.rs:180-230);
     `output.weight` absent means tied embeddings; `rope_freqs.weight`, when
     present (Llama-3 frequency scaling), is bound as the RoPE divisors."""
     f = path_or_file if isinstance(path_or_file, GgufFile) else GgufFile.open(path_or_file)
     c = config_from_gguf(f)
+    if interleaved:
+        c = replace(c, rope_interleaved=True)
+    order = (lambda w, heads: w) if interleaved else unpermute_rope
     qd, kvd = c.heads * c.head_dim, c.kv_heads * c.head_dim
 
     def get(name, shape):
@@ -122,8 +137,8 @@ def load_llama_gguf(path_or_file):
     for l in range(c.layers):
         p = f"blk.{l}"
         w[f"{l}.attn_norm"] = get(f"{p}.attn_norm.weight", (c.hidden,))
-        w[f"{l}.wq"] = unpermute_rope(get(f"{p}.attn_q.weight", (qd, c.hidden)), c.heads)
-        w[f"{l}.wk"] = unpermute_rope(get(f"{p}.attn_k.weight", (kvd, c.hidden)), c.kv_heads)
+        w[f"{l}.wq"] = order(get(f"{p}.attn_q.weight", (qd, c.hidden)), c.heads)
+        w[f"{l}.wk"] = order(get(f"{p}.attn_k.weight", (kvd, c.hidden)), c.kv_heads)
         w[f"{l}.wv"] = get(f"{p}.attn_v.weight", (kvd, c.hidden))
         w[f"{l}.wo"] = get(f"{p}.attn_output.weight", (c.hidden, qd))
         w[f"{l}.ffn_norm"] = get(f"{p}.ffn_norm.weight", (c.hidden,))
