@@ -395,7 +395,7 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
  * + rot_dim / 2) or, `interleaved`, (2d, 2d + 1), by the angle pos * theta^(-2d /
  * rot_dim) / freq_div[d] (freq_div NULL: 1; rot_dim / 2 floats, device), the
  * rotated values times mscale. Angles are formed in f64 (llmtie_rope's are the
- * reference's f32 ones). */
+ * reference's f32 ones). At most 2^26 rows a call, of fewer than 2^29 values each. */
 
 /* t rows of `heads` heads from x[off + r * stride ..] into out[out_off + r *
  * out_stride ..], f32 or (out_f16) f16. out may be x itself (the same rows, f32)

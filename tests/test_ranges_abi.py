@@ -178,3 +178,14 @@ def test_scaling_tables():
         rope_scaling(64, 1e4, "yarn", 0.5)
     with pytest.raises(OddHeadDim):
         rope_scaling(63, 1e4, "linear", 2.0)
+
+
+def test_rotary_sizes():
+    """A row index behind the last workgroup's stays an int, and so do a thread's items."""
+    n = 2**26
+    assert rope(t=n + 1, heads=1, hd=2, rot=2, stride=2, out_stride=2) == 4
+    assert rope(t=2**31 - 1, heads=1, hd=2, rot=2, stride=2, out_stride=2) == 4
+    assert rope(t=1, heads=2**22 + 1, stride=2**29 + 128, out_stride=2**29 + 128) == 4
+    assert store(rows=n + 1, index_len=n + 1) == 4
+    assert store(q=N, rows=1, kv=2**23 + 1, hd=64, rot=64, k_stride=2**30, v_stride=2**30, slots=1, cap=32,
+                 cache_len=2**62) == 4

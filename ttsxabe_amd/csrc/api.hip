@@ -1182,7 +1182,9 @@ int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows,
     if (hd > 1024) return refuse("a rotary head wider than 1024");
     if (!(theta > 0.0f) || !std::isfinite(theta) || !std::isfinite(mscale))
         return refuse("a rotary base that is not positive, or a multiplier that is not finite");
-    if (int r = over_int(rows, smul(heads, hd), sadd(first, rows))) return r;
+    // Workgroups of a launch, and its rows and threads' items, are ints.
+    if (rows > (size_t)1 << 26) return overrun_slice(rows, (size_t)1 << 26);
+    if (int r = over_int(smul(heads, hd, 4), sadd(first, rows))) return r;
     if (has_pos && pos_len < rows) return overrun_slice(rows, pos_len);
     if (has_div && div_len < rot / 2) return overrun_slice(rot / 2, div_len);
     return LLMTIE_OK;
@@ -1285,7 +1287,6 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
     if (rows > 1 && (k_stride < nk || v_stride < nk)) return overrun_slice(nk, std::min(k_stride, v_stride));
     if (reach(k_off, rows, k_stride, nk) > k_len) return overrun_slice(reach(k_off, rows, k_stride, nk), k_len);
     if (reach(v_off, rows, v_stride, nk) > v_len) return overrun_slice(reach(v_off, rows, v_stride, nk), v_len);
-    if (rows > (size_t)1 << 26) return overrun_slice(rows, (size_t)1 << 26);  // workgroups of a launch
     if (rows == 0) return ok();
     if (!k || !v || !pos || !slot || !index || !cache || (q && !q_out)) return invalid("a buffer");
     if (off16(cache)) return refuse("a cache off 16 bytes");
