@@ -329,8 +329,8 @@ int llmtie_rope_cache_q8(void* stream, float* q, size_t q_len, size_t q_off, con
  *
  * where softcap c = 0 stands for no cap, slopes NULL (else [heads] f32, device)
  * for no bias, and i and j are cache positions: a row's own and the key's. The
- * scale is positive (1e-30 to 1e30), the cap 0 or 0.001 to 1000. A row that sees no key gets
- * zeros. Keys that a row does not see contribute nothing to it, whatever they hold. */
+ * scale is 1e-15 to 1e15, the cap 0 or 0.001 to 1000, a slope 0 to 1e15. A row that sees no
+ * key gets zeros. Keys that a row does not see contribute nothing to it, whatever they hold. */
 
 /* Which keys the rows of a packed prompt see: made once for all layers. Row r
  * (of `rows`) is at cache position i = past + r. starts (device, starts_len =

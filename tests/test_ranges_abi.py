@@ -189,3 +189,8 @@ def test_rotary_sizes():
     assert store(rows=n + 1, index_len=n + 1) == 4
     assert store(q=N, rows=1, kv=2**23 + 1, hd=64, rot=64, k_stride=2**30, v_stride=2**30, slots=1, cap=32,
                  cache_len=2**62) == 4
+
+
+def test_score_scales():
+    for scale in (9e-16, 1.1e15, 1e30, 1e-30):
+        assert prompt(scale=scale) == 10 and decode(scale=scale) == 10, scale

@@ -308,7 +308,7 @@ def test_decode_random(gpu, seed):
 
 
 @pytest.mark.parametrize("c", [
-    # Batches whose bound is long: every workgroup an equal run of all their blocks, across heads.
+    # Batches whose bound is long: several runs a head, streamed loads, lengths that leave runs without blocks.
     ([4096, 1, 700, 0, 2999, 33, 64, 1500, 4000], (32, 8, 128), 0, 0, 50.0, False),
     ([5] * 9, (32, 8, 128), 0, 0, 0.0, False),
     ([4096] * 9, (16, 8, 128), 0, 0, 0.0, True),
@@ -458,6 +458,49 @@ def test_a_cache_past_32_bits(gpu):
                                  torch.tensor([slots - 1], dtype=torch.int32).cuda(), cap, heads, 0.1, DecodeScratch())
     want, tol = ref.attend(q[2:].float(), k[0], v[0], seen[2:], torch.tensor([cap - 1]), 0.1, decode=True)
     close(got, want, tol)
+
+
+def test_distances_past_2_to_the_24(gpu):
+    """Positions that f32 does not hold: a bias by distance there is that of the same rows near 0."""
+    from ttsxabe_amd.gpu import TiledCache16
+    heads, hd, rows, base = 4, 64, 43, 2**24 + 960
+    cap = base + 96
+    cache = TiledCache16(1, hd, cap, zero=False)
+    k, v = f16(1, 1, 1, 96, hd), f16(2, 1, 1, 96, hd)
+    cache.data[-(96 * hd * 2):] = ref.tile(k, v).cuda()
+    q, slopes = f16(3, rows, heads, hd), slopes_of(heads)
+    i = torch.arange(96 - rows, 96)
+    table = torch.stack([torch.zeros(rows), torch.zeros(rows), (i + 1.0 + torch.arange(rows) % 9).clamp(max=96)]).int()
+    want, tol = ref.attend(q, k[0], v[0], ref.visible(table, 96), i, 0.1, 0.0, slopes)
+    from ttsxabe_amd.gpu import KeyRanges
+    there = table.clone()
+    there[1:] += base
+    got = gpu.flash_attn_ranges(q.cuda().view(-1), 0, heads * hd, cache, 0, KeyRanges(there.cuda(), None, 96), rows,
+                                cap - rows, heads, 0.1, slopes=slopes.cuda())
+    close(got, want, tol)
+
+
+@pytest.mark.parametrize("softcap", [0.0, 7.0])
+@pytest.mark.parametrize("scale", [1e-15, 1e12, 1e15])
+def test_extreme_scales(gpu, scale, softcap):
+    """Every key of a row far below zero, and scores that are all alike. (With distinct integers as products the
+    largest score is exactly known: one key has all the weight, or with a cap those of its sign do.)"""
+    from ttsxabe_amd.gpu import DecodeScratch
+    heads, hd, n = 4, 64, 70
+    k, v = torch.zeros(1, 1, n, hd, dtype=torch.float16), f16(2, 1, 1, n, hd)
+    k[0, 0, :, 0] = -1.0 - torch.randperm(n, generator=torch.Generator().manual_seed(1)).half()
+    q = torch.zeros(n, heads, hd, dtype=torch.float16)
+    q[:, :, 0] = 3.0
+    want, tol = ref.attend(q, k[0], v[0], ref.visible(ref.ranges(n), n), torch.arange(n), scale, softcap)
+    if scale > 1.0:  # products are exact here, the weights 0 and 1 (or, capped, all alike)
+        tol = ref.H * 2 * v.double().abs().amax() + 2.0 ** -20 + 0 * tol
+    cache = cache_of(k, v)
+    got = gpu.flash_attn_ranges(q.cuda().view(-1), 0, heads * hd, cache, 0, gpu.key_ranges(n), n, 0, heads, scale, softcap)
+    close(got, want, tol)
+    got = gpu.attn_decode_ranges(q[-1:].float().cuda().view(-1), 0, heads * hd, cache,
+                                 torch.tensor([n], dtype=torch.int32).cuda(), None, n, heads, scale, DecodeScratch(),
+                                 softcap=softcap)
+    close(got, want[-1:], tol[-1:])
 
 
 def test_refusals(gpu):

@@ -1149,10 +1149,11 @@ constexpr size_t MAX_WGS = ((size_t)1 << 24) - 1;
 constexpr int RD_WHOLE = 20;
 constexpr size_t RD_STREAM_BYTES = (size_t)128 << 20;
 
-// What the score arguments must be. (The kernels keep running maxima of raw
-// products, so the scale is positive.)
+// What the score arguments must be: every logit of finite queries and keys is
+// then above the reference maximum that a row starts from, -1e30, and twice a
+// slope over the scale is finite.
 int score_checks(float scale, float softcap, const float* slopes, size_t slopes_len, size_t heads) {
-    if (!(scale >= 1e-30f) || !(scale <= 1e30f)) return refuse("a score scale that is not in 1e-30 to 1e30");
+    if (!(scale >= 1e-15f) || !(scale <= 1e15f)) return refuse("a score scale that is not in 1e-15 to 1e15");
     if (softcap != 0.0f && !(softcap >= 1e-3f && softcap <= 1e3f))
         return refuse("a score cap that is neither 0 nor in 0.001 to 1000");
     if (slopes && slopes_len < heads) return overrun_slice(heads, slopes_len);

@@ -10,6 +10,7 @@
 // A row that sees no key is zeros. Keys a row does not see contribute nothing,
 // whatever they hold. The cache is the tiled f16 one (kvlayout.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "decode.h"
@@ -287,7 +288,7 @@ struct RangeTile {
                 const float k2 = 2.0f * slope2 / mul;
 #pragma unroll
                 for (int u = 0; u < NQT; ++u) {
-                    const float d0 = (float)min(pos0 + 16 * u + (lane & 15), last) - (float)(kv0 + 8 * grp);
+                    const float d0 = (float)(min(pos0 + 16 * u + (lane & 15), last) - kv0 - 8 * grp);
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -344,8 +345,16 @@ struct RangeTile {
                 if constexpr ((MODE & SM_BIAS) != 0) off = __builtin_fmaf(sl, (float)c, off);
                 return __builtin_fmaf(s, mul, off);
             };
-            auto form = [&]() __attribute__((always_inline)) {
-                const float off = at - m[u];
+            auto form = [&](auto moved) __attribute__((always_inline)) {
+                // Less m in the offset; behind a move in a step of its own, so
+                // that the key m was taken from has a weight of exactly 1 (of
+                // logits past 2^24 the offset's rounding is more than a weight).
+                constexpr bool M = decltype(moved)::value;
+                const float off = M ? at : at - m[u], ref = M ? m[u] : 0.0f;
+                auto weight = [&](float s, int c) __attribute__((always_inline)) {
+                    const float x = logit(s, c, off);
+                    return to_h(ex2(M ? x - ref : x));
+                };
                 half2_t top;
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
@@ -354,15 +363,15 @@ struct RangeTile {
 #pragma unroll
                         for (int r = 0; r < 4; r += 2) {
                             half2_t p;
-                            p[0] = to_h(ex2(logit(sc[hf][T][u][r], 32 * hf + 4 * T + r, off)));
-                            p[1] = to_h(ex2(logit(sc[hf][T][u][r + 1], 32 * hf + 4 * T + r + 1, off)));
+                            p[0] = weight(sc[hf][T][u][r], 32 * hf + 4 * T + r);
+                            p[1] = weight(sc[hf][T][u][r + 1], 32 * hf + 4 * T + r + 1);
                             pb[hf][u][4 * T + r] = p[0];
                             pb[hf][u][4 * T + r + 1] = p[1];
                             top = hf | T | r ? __builtin_elementwise_max(top, p) : p;
                         }
                 return fmaxf((float)top[0], (float)top[1]);
             };
-            if (__any(!(form() <= 32768.0f))) {
+            if (__any(!(form(std::false_type{}) <= 32768.0f))) {
                 float mx = ninf();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
@@ -377,7 +386,7 @@ struct RangeTile {
                 l[u] *= fac;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) o[t][u] *= fac;
-                form();
+                form(std::true_type{});
             }
         }
     }
