@@ -194,3 +194,37 @@ def test_rotary_sizes():
 def test_score_scales():
     for scale in (9e-16, 1.1e15, 1e30, 1e-30):
         assert prompt(scale=scale) == 10 and decode(scale=scale) == 10, scale
+
+
+def test_scaling_refusals():
+    from ttsxabe_amd.gpu import InvalidArgument, rope_scaling
+    for theta in (1.0, 0.5, math.nan):
+        with pytest.raises(InvalidArgument):
+            rope_scaling(64, theta, "yarn", 4.0, device="cpu")
+    for kind in ("linear", "ntk", "yarn"):
+        for factor in (math.inf, math.nan, 0.0):
+            with pytest.raises(InvalidArgument):
+                rope_scaling(64, 1e4, kind, factor, device="cpu")
+
+
+def test_a_gguf_that_rotates_a_part_of_its_heads(tmp_path):
+    """Its own order keeps the count of rotated dims; unpermuted (whole) heads are rotated whole, as before."""
+    import numpy as np
+
+    from oracle.stack import StackConfig, random_weights
+    from tests.test_gguf import llama_gguf
+    from ttsxabe_amd.llama_gguf import load_llama_gguf
+    cfg = StackConfig()
+    llama_gguf(tmp_path / "m.gguf", cfg, random_weights(cfg, 1))
+    f = load_llama_gguf(tmp_path / "m.gguf")[0]
+    assert f.rope_dim == 0 and not f.rope_interleaved
+    from ttsxabe_amd import llama_gguf as m
+    config = m.config_from_gguf
+    try:
+        m.config_from_gguf = lambda f: m.replace(config(f), rope_dim=cfg.head_dim // 2)
+        whole, a = m.load_llama_gguf(tmp_path / "m.gguf")
+        part, b = m.load_llama_gguf(tmp_path / "m.gguf", interleaved=True)
+    finally:
+        m.config_from_gguf = config
+    assert whole.rope_dim == 0 and part.rope_dim == cfg.head_dim // 2 and part.rope_interleaved
+    assert np.array_equal(m.unpermute_rope(b["0.wq"], cfg.heads), a["0.wq"])

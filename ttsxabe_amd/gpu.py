@@ -251,7 +251,7 @@ def rope_scaling(rot_dim: int, theta: float, kind: str = "none", factor: float =
         raise InvalidArgument(f"unknown rotary scaling {kind!r}")
     if rot_dim % 2 or rot_dim < 0:
         raise OddHeadDim(f"a rotary head of odd width {rot_dim}", (rot_dim,))
-    if not (factor >= 1.0 and theta > 0.0 and original > 0 and beta_fast > beta_slow > 0.0):
+    if not (math.inf > factor >= 1.0 and math.inf > theta > 0.0 and original > 0 and beta_fast > beta_slow > 0.0):
         raise InvalidArgument("a rotary scaling wants factor >= 1, theta, original > 0 and beta_fast > beta_slow > 0")
     n = rot_dim // 2
     if kind == "none" or factor == 1.0 or n == 0:
@@ -260,6 +260,8 @@ def rope_scaling(rot_dim: int, theta: float, kind: str = "none", factor: float =
         return None, theta * factor ** (rot_dim / (rot_dim - 2)) if rot_dim > 2 else theta, 1.0
     if kind == "linear":
         return torch.full((n,), factor, dtype=torch.float32, device=device), theta, 1.0
+    if not theta > 1.0:
+        raise InvalidArgument("yarn wants frequencies that fall: theta > 1")
     # The dim whose frequency turns b times within `original` positions.
     def at(b):
         return n * math.log(original / (b * 2.0 * math.pi)) / math.log(theta)

@@ -112,14 +112,16 @@ def permute_rope(w: np.ndarray, heads: int) -> np.ndarray:
 def load_llama_gguf(path_or_file, interleaved: bool = False):
     """(config, weights) for `LlamaStack` or `LlamaBatch` from a GGUF Llama
     (`interleaved`: `attn_q` and `attn_k` as the file holds them, for
-    `LlamaBatch`'s interleaved rotation): every tensor
+    `LlamaBatch`'s interleaved rotation of the file's rope.dimension_count dims;
+    without it they are rotated as whole heads): every tensor
     decoded to f32 and checked against the geometry (weights.rs:180-230);
     `output.weight` absent means tied embeddings; `rope_freqs.weight`, when
     present (Llama-3 frequency scaling), is bound as the RoPE divisors."""
     f = path_or_file if isinstance(path_or_file, GgufFile) else GgufFile.open(path_or_file)
     c = config_from_gguf(f)
-    if interleaved:
-        c = replace(c, rope_interleaved=True)
+    # Unpermuted heads are whole ones, rotated whole; the file's own order also
+    # serves heads of which it rotates the first dims only.
+    c = replace(c, rope_interleaved=True) if interleaved else replace(c, rope_dim=0)
     order = (lambda w, heads: w) if interleaved else unpermute_rope
     qd, kvd = c.heads * c.head_dim, c.kv_heads * c.head_dim
 
