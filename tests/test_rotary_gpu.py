@@ -191,3 +191,27 @@ def test_refusals(gpu):
     with pytest.raises(SliceOverrun):
         gpu.t16_rope_store(x, 0, x, 0, x, 0, 256, pos, pos[:3], pos, None, 4, 4, 64, THETA, 1.0, False,
                            TiledCache16(1, 64, 32))
+
+
+@pytest.mark.parametrize("offset", [0, 5])
+def test_more_rows_than_workgroups(gpu, offset):
+    """Rows behind the last workgroup's follow at the launch's stride, alone and with a store."""
+    from ttsxabe_amd.gpu import TiledCache16
+    rows, hd = 70001, 64
+    x = rows_of(7, rows, 3 * hd)
+    want = ref.rotate(x.view(rows, 3, hd)[:, :2], torch.arange(rows), hd, THETA)
+    tol = allowed(x.view(rows, 3, hd)[:, :2], hd, False, 1.0, False)
+    half = allowed(x.view(rows, 3, hd)[:, :2], hd, False, 1.0, True)
+    cache = TiledCache16(1, hd, rows + offset, zero=False)
+    d, q = x.cuda().view(-1), torch.empty(rows * hd, dtype=torch.float32, device="cuda")
+    at = torch.arange(rows, dtype=torch.int32).cuda()
+    gpu.t16_rope_store(d, 0, d, hd, d, 2 * hd, 3 * hd, at, torch.zeros_like(at), at + offset, None, rows, 1, hd, THETA, 1.0,
+                       False, cache, q_out=q)
+    assert ((q.cpu().double().view(rows, hd) - want[:, 0]).abs() <= tol[:, 0]).all()
+    k, v = ref.untile(cache.data.cpu(), 1, 1, hd, rows + offset)
+    assert ((k[0, 0, offset:].double() - want[:, 1]).abs() <= half[:, 1]).all()
+    assert torch.equal(v[0, 0, offset:], x[:, 2 * hd:].half())
+    gpu.rope_rows(d, 0, 3 * hd, 0, None, rows, 2, hd, hd, THETA)
+    got = d.cpu().view(rows, 3, hd)
+    assert ((got[:, :2].double() - want).abs() <= tol).all()
+    assert torch.equal(got[:, 2], x[:, 2 * hd:])
