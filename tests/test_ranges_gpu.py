@@ -503,6 +503,12 @@ def test_extreme_scales(gpu, scale, softcap):
     close(got, want[-1:], tol[-1:])
 
 
+@pytest.mark.parametrize("nqt", ["1", "2", "4"])
+def test_prompt_under_the_tile_override(gpu, monkeypatch, nqt):
+    monkeypatch.setenv("LLMTIE_PREFILL_NQT", nqt)
+    close(*prompt(gpu, 70, 30, (4, 2, 64), {}, 0.0, False)[:3])
+
+
 def test_refusals(gpu):
     from ttsxabe_amd.gpu import DecodeScratch, InvalidArgument, SliceOverrun, TiledCache16
     cache = TiledCache16(2, 64, 40)

@@ -1367,7 +1367,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
         if (ws_len < need) return overrun_slice(need, ws_len);
         if (off16(ws)) return refuse("a workspace off 16 bytes");
     }
-    const int nqt = splits > 1 ? 1 : pick_nqt(tq, heads, gb);
+    const int nqt = splits > 1 ? 1 : std::min(2, pick_nqt(tq, heads, gb));
     // The eight-wave kernel for head_dim 128 and no cap, where its workgroups of
     // 64 rows a head are two a compute unit. 32/8/128, us, eight waves / four:
     // 8192 rows 510 / 561, biased 502 / 549, capped 675 / 667; 4096 148 / 164; 1999
