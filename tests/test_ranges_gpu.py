@@ -140,7 +140,7 @@ def test_prompt_random(gpu, seed):
     (1100, 40, dict(window=130, shared=5), True), (1024, 0, dict(causal=False), True),
 ], ids=lambda c: f"{c[0]}+{c[1]}-{'-'.join(c[2])}")
 def test_prompt_of_many_workgroups(gpu, kv, hd, c):
-    """Enough row blocks for the eight-wave kernel, in each division of heads over its waves; some groups of heads
+    """Enough row blocks for two query tiles a wave, in each division of heads over its waves; some groups of heads
     are compared. Where documents are, one of them holds values that are not finite."""
     rows, past, table, bias = c
     heads, keys = 128, past + rows

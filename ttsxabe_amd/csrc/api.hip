@@ -1162,10 +1162,10 @@ int score_checks(float scale, float softcap, const float* slopes, size_t slopes_
 
 // Runs that a prompt's row blocks are cut into (1: whole) when they are few and
 // their keys many: two workgroups a compute unit, of four tiles or more. Us, as
-// planned / whole: 173 rows after 3011 of 32/8/128 28.5 / 56.7 (5 runs; 4 29.5, 8
-// 31.4), 16 after 3000 16.5 / 56.8 (11; 8 17.2, 16 17.2), 100 after 7000 31.4 /
-// 124, 40 after 1000 12.5 / 19.7, 400 after 1500 31.5 / 33.2 (2; 4 35.7); 40 after
-// 2000 of 20/20/64 12.0 / 29.9; 1000 rows of 32/8/128 (504 blocks, whole) in 2 34.4 / 24.1.
+// planned / whole: 173 rows after 3011 of 32/8/128 26.9 / 44.7 (5 runs; 4 28.8, 8
+// 29.0), 16 after 3000 15.6 / 42.1 (11; 8 15.5, 16 16.2), 100 after 7000 28.8 / 91
+// (9; 4 32.5), 40 after 1000 12.2 / 17.8, 400 after 1500 30.7 / 30.0 (2; 4 34.3); 40 after
+// 2000 of 20/20/64 11.1 / 21.0; 1000 rows of 32/8/128 (504 blocks, whole) in 2 33.4 / 21.8.
 size_t plan_range_splits(size_t tq, size_t keys, size_t heads, size_t kv_heads) {
     const size_t group = heads / kv_heads;
     const size_t gb = group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
@@ -1173,6 +1173,23 @@ size_t plan_range_splits(size_t tq, size_t keys, size_t heads, size_t kv_heads) 
     const size_t cus = (size_t)compute_units(), tiles = (keys + 63) / 64;
     if (items >= cus || tiles <= 8) return 1;
     return std::max<size_t>(1, std::min<size_t>(std::min<size_t>(32, tiles / 4), 2 * cus / items));
+}
+
+// 16-row query tiles a wave (each K and V fragment read from LDS serves both of
+// two). Two where the launch then still has workgroups enough: two a compute unit, fewer
+// where the rows are alike (no fewer positions before them than there are rows,
+// so that none ends early), more where a score takes longer than its reads (head_dim 64).
+// Us, one / two; workgroups at two: 304 (1200 rows of 32/8/128) 26.7 / 33.3, after
+// 4000 134 / 126; 440, after 4000 169 / 151; 504 47.0 / 54.0, capped 53 / 67, after 186 / 165;
+// 656 75.6 / 72.1, capped 87.4 / 86.9; 1000 156 / 126. head_dim 64: 440 (1750 of 32/8) after
+// 4000 96 / 100; 640 (4000 of 20/20) 102 / 92, after 305 / 183, capped 119 / 156; 656 (2600 of
+// 32/8) 44.5 / 51.3, after 150 / 137; 1000 88 / 85, capped 116 / 115.
+int range_tiles(size_t tq, size_t past, size_t heads, size_t hd, int gb, bool capped) {
+    if (getenv("LLMTIE_PREFILL_NQT")) return std::min(2, pick_nqt(tq, heads, gb));
+    const size_t rows = 32 * (4 / gb), wgs = (tq + rows - 1) / rows * (heads / gb);
+    const size_t cus = (size_t)compute_units();
+    if (past >= tq) return wgs >= (hd == 128 ? cus + cus / 8 : 2 * cus) ? 2 : 1;
+    return wgs >= (hd == 128 ? 2 * cus : capped ? 4 * cus - cus / 8 : 5 * cus / 2) ? 2 : 1;
 }
 
 int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows, size_t heads, size_t pos_len,
@@ -1367,14 +1384,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
         if (ws_len < need) return overrun_slice(need, ws_len);
         if (off16(ws)) return refuse("a workspace off 16 bytes");
     }
-    const int nqt = splits > 1 ? 1 : std::min(2, pick_nqt(tq, heads, gb));
-    // The eight-wave kernel for head_dim 128 and no cap, where its workgroups of
-    // 64 rows a head are two a compute unit. 32/8/128, us, eight waves / four:
-    // 8192 rows 510 / 561, biased 502 / 549, capped 675 / 667; 4096 148 / 164; 1999
-    // 62 / 51; 3968 of 40/40/128 220 / 214, before 214 / 228; 8192 of 32/8/64 352 / 319.
-    const size_t blocks8 = smul((tq + 64 * (4 / gb) - 1) / (64 * (4 / gb)), heads / gb);
-    const bool pp =
-        splits == 1 && head_dim == 128 && softcap == 0.0f && blocks8 >= 2 * (size_t)compute_units();
+    const int nqt = splits > 1 ? 1 : range_tiles(tq, past, heads, head_dim, gb, softcap != 0.0f);
     const size_t items = smul((tq + 16 * nqt * (4 / gb) - 1) / (16 * nqt * (4 / gb)), heads / gb, splits);
     if (items > MAX_WGS) return overrun_slice(items, MAX_WGS);
     RangesArgs a{};
@@ -1397,7 +1407,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
     a.splits = (int)splits;
     a.ws = ws;
     a.qal = !off16(a.q) && a.q_stride % 8 == 0;
-    return launched("flash_attn_ranges", launch_ranges((int)head_dim, nqt, pp, a, S(stream)));
+    return launched("flash_attn_ranges", launch_ranges((int)head_dim, nqt, a, S(stream)));
 }
 
 int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,

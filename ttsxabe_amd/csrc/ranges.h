@@ -36,8 +36,8 @@ struct RangesArgs {
     int nrb, grid8, xcd;
     int qal;                // query rows are 16-byte aligned
 };
-// nqt: 16-row query tiles a wave (1 or 2); pp: the eight-wave kernel.
-hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStream_t st);
+// nqt: 16-row query tiles a wave (1 or 2).
+hipError_t launch_ranges(int hd, int nqt, const RangesArgs& a, hipStream_t st);
 
 struct RangesDecodeArgs {
     const float* q;         // sequence s's heads at s * q_stride

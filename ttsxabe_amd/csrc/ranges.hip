@@ -268,7 +268,7 @@ struct RangeTile {
     // clocks, whatever it is: four a score here and three in softmax(), which
     // the cap needs instead of three, set the time of a capped prompt. (A
     // cubic in x^2 for scores under half the cap, no transcendentals but 9.5
-    // instructions: 8192 rows of 32/8/128 661 us.)
+    // instructions, was no faster.)
     __device__ __forceinline__ void logits(int kv0, bool whole) {
         if constexpr ((MODE & SM_CAP) != 0) {
 #pragma unroll
@@ -449,14 +449,14 @@ struct RangeTile {
 };
 
 // Whether some value of a tile is not finite, as this wave's share of a look by
-// all W waves of the workgroup shows.
-template <int HD, int W>
+// all waves of the workgroup shows.
+template <int HD>
 __device__ __forceinline__ bool odd_values(const half_t* vt, int tid) {
     const uint4* v = reinterpret_cast<const uint4*>(vt);
     uint32_t x = 0;
 #pragma unroll
-    for (int k = 0; k < 2 * (HD / 16) / W; ++k) {
-        const uint4 y = v[tid + W * 64 * k];
+    for (int k = 0; k < 2 * (HD / 16) / RW; ++k) {
+        const uint4 y = v[tid + RT * k];
         x |= not_finite(y.x) | not_finite(y.y) | not_finite(y.z) | not_finite(y.w);
     }
     return __any(x != 0);
@@ -471,8 +471,7 @@ __device__ __forceinline__ void lds_barrier() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// The bounds of all W waves' rows (a barrier).
-template <int W>
+// The bounds of all waves' rows (a barrier).
 __device__ __forceinline__ Bounds together(const Bounds& mine, int (*wb)[6], int wave, int lane) {
     if (lane == 0) {
         wb[wave][0] = mine.f0, wb[wave][1] = mine.f1, wb[wave][2] = mine.l0;
@@ -481,7 +480,7 @@ __device__ __forceinline__ Bounds together(const Bounds& mine, int (*wb)[6], int
     __syncthreads();
     Bounds b = mine;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
+    for (int w = 0; w < RW; ++w) {
         b.f0 = min(b.f0, wb[w][0]), b.f1 = max(b.f1, wb[w][1]), b.l0 = min(b.l0, wb[w][2]);
         b.l1 = max(b.l1, wb[w][3]), b.h0 = min(b.h0, wb[w][4]), b.h1 = max(b.h1, wb[w][5]);
     }
@@ -509,19 +508,19 @@ struct Tiles {
 };
 
 // Takes the values that are not finite out of a tile in LDS (a weight of 0 must
-// not meet them: a row may not see their keys), by all threads of a workgroup
-// of W waves: they become 0, and sp[dim] holds which of the 64 keys had +inf or
+// not meet them: a row may not see their keys), by all threads of a
+// workgroup: they become 0, and sp[dim] holds which of the 64 keys had +inf or
 // NaN there (x, y) and -inf or NaN (z, w). Barriers before and after are the
 // caller's.
-template <int HD, int W>
+template <int HD>
 __device__ __forceinline__ void screen_clear(uint4* sp, int tid) {
     if (tid < HD) sp[tid] = make_uint4(0, 0, 0, 0);
 }
-template <int HD, int W>
+template <int HD>
 __device__ __forceinline__ void screen(half_t* vt, uint4* sp, int tid) {
     constexpr int NT = HD / 16;
     uint4* v = reinterpret_cast<uint4*>(vt);
-    for (int c = tid; c < 2 * NT * 64; c += W * 64) {
+    for (int c = tid; c < 2 * NT * 64; c += RT) {
         const int hf = c / (NT * 64), dim = 16 * (c / 64 % NT) + (c & 15), key = 8 * (c >> 4 & 3);
         uint4 y = v[c];
         uint32_t* w = &y.x;
@@ -543,16 +542,16 @@ __device__ __forceinline__ void screen(half_t* vt, uint4* sp, int tid) {
     }
 }
 
-// Fragments of one tile into LDS by direct loads, W waves taking every W-th:
+// Fragments of one tile into LDS by direct loads, its waves taking every fourth:
 // per-lane offsets fixed for the launch, a scalar one a load. Where the tile's
 // second block lies past the last one that holds keys, both halves come from
 // the first, so every address lies in a live block.
-template <int HD, int W>
+template <int HD>
 struct RangeLoad {
     static constexpr int NS = HD / 32, NT = HD / 16, KF = 4 * NS, VF = 2 * NT, FH = 64 * 8;
-    static constexpr int KI = KF / W, VI = VF / W, KFB = KF / 2;
+    static constexpr int KI = KF / RW, VI = VF / RW, KFB = KF / 2;
     static constexpr uint32_t BLK = 128 * HD;  // bytes of a block
-    static_assert(KF % W == 0 && (KFB % W == 0 || W == 2 * KFB), "a wave's fragments are W apart");
+    static_assert(KFB % RW == 0, "a load takes the same block for every wave");
     const uint16_t* head;
     int w0, lastb;
     uint32_t off;
@@ -560,7 +559,7 @@ struct RangeLoad {
         : head(a.cache + (size_t)kh * tiled_nblk(a.cap) * (BLK / 2)),
           w0(__builtin_amdgcn_readfirstlane(wave)),
           lastb((a.past + a.tq - 1) >> 5),
-          off(16u * lane + 1024u * (wave % KFB)) {}
+          off(16u * lane + 1024u * wave) {}
     __device__ __forceinline__ void operator()(int kv0, half_t* dst) const {
         half_t* l = dst + w0 * FH;
         const int b = kv0 >> 5;
@@ -569,10 +568,9 @@ struct RangeLoad {
             const_cast<uint16_t*>(head) + (size_t)b * (BLK / 2), 0, 2 * (int)BLK, 0x00020000);
 #pragma unroll
         for (int i = 0; i < KI + VI; ++i) {
-            const int f = W * (i < KI ? i : i - KI);  // of its area, for wave 0
-            const int blk = KFB % W == 0 ? f / KFB : w0 / KFB;
+            const int f = RW * (i < KI ? i : i - KI);  // of its area, for wave 0
             const uint32_t in = (i < KI ? 0u : 64u * HD) + 1024u * (f % KFB);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l + W * i * FH, 16, (int)off, blk * second + in, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l + RW * i * FH, 16, (int)off, f / KFB * second + in, 0, 0);
         }
     }
 };
@@ -641,11 +639,11 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
     }
     const int h = gy * gb + wave % gb, kh = gy * gb / group;
     const int p0 = bx * pb + (wave / gb) * QPW;
-    const RangeLoad<HD, RW> issue(a, kh, lane, wave);
+    const RangeLoad<HD> issue(a, kh, lane, wave);
 
     Tile t;
     const Bounds mine = t.start(a, p0, h, lane, wrg[wave]);
-    const Bounds all = together<RW>(mine, wb, wave, lane);
+    const Bounds all = together(mine, wb, wave, lane);
     const Tiles tiles(all);
     int i0 = 0, i1 = tiles.n;
     if constexpr (SPLIT) {
@@ -665,14 +663,14 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
         bool bad = false;
         if (!all.whole(kv0)) {
             // Some row does not see some key: are all its values finite?
-            const bool any = odd_values<HD, RW>(cur + KF * FH, tid);
+            const bool any = odd_values<HD>(cur + KF * FH, tid);
             if (lane == 0) wbad[wave] = any;
             lds_barrier();
             bad = (wbad[0] | wbad[1] | wbad[2] | wbad[3]) != 0;
             if (bad) {
-                screen_clear<HD, RW>(sp_, tid);
+                screen_clear<HD>(sp_, tid);
                 lds_barrier();
-                screen<HD, RW>(cur + KF * FH, sp_, tid);
+                screen<HD>(cur + KF * FH, sp_, tid);
                 lds_barrier();
             }
         }
@@ -695,99 +693,6 @@ __global__ __launch_bounds__(RT, 2) void ranges_kernel(RangesArgs a) {
         const float lt = t.l[u][0];
         if constexpr (SPLIT) store_part<HD, NQT>(t.o, u, t.m[u], lt, lane, a, sp, p0 + 16 * u, h);
         else store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
-    }
-}
-
-// Long prompts: eight waves in two groups of four that share each tile; waves w
-// and w + 4 share a SIMD. In the period between two barriers the first group
-// computes O += V^T P^T of tile q - 1, S of tile q and its softmax, the second
-// the softmax of tile q - 1, then the same products, so that one wave's softmax
-// (with the instructions of cap and bias) issues beside the other's MFMAs. Tiles rotate
-// through three buffers: period q reads K of tile q and V of tile q - 1, tile q +
-// 1 is issued at its start and waited for at its end. The arithmetic of a row is
-// ranges_kernel's, in the same order. Not for capped scores: their softmax is
-// longer than the products, so a period waits for it (8192 rows of 32/8/128 675
-// against 667 us; without a cap 510 against 561, 1080 TF, of 1147 that the
-// library's product reaches at 8192^3).
-constexpr int PPW = 8;
-
-template <int HD, int MODE>
-__global__ __launch_bounds__(PPW * LLMTIE_WAVE, 1) void ranges_pp_kernel(RangesArgs a) {
-    constexpr int NQT = 2;
-    using Tile = RangeTile<HD, MODE, NQT>;
-    constexpr int FH = Tile::FH, KF = Tile::KF, VF = Tile::VF, QPW = 16 * NQT;
-    __shared__ __attribute__((aligned(16))) half_t tbuf[3][(KF + VF) * FH];
-    __shared__ int wrg[PPW][3 * QPW];
-    __shared__ int wb[PPW][6];
-    __shared__ int wbad[2][PPW];
-    __shared__ uint4 sp_[HD];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const bool second = wave >= 4;
-    const int wl = wave & 3, gb = a.gb, gpr = QPW * (4 / gb), group = a.heads / a.kv_heads;
-    const int item = a.xcd ? (int)(blockIdx.x % 8) * a.grid8 + (int)(blockIdx.x / 8) : (int)blockIdx.x;
-    const int gy = item / a.nrb, bx = a.nrb - 1 - item % a.nrb;
-    const int h = gy * gb + wl % gb, kh = gy * gb / group;
-    const int p0 = bx * 2 * gpr + (second ? gpr : 0) + (wl / gb) * QPW;
-    const RangeLoad<HD, PPW> issue(a, kh, lane, wave);
-    Tile t;
-    const Bounds mine = t.start(a, p0, h, lane, wrg[wave]);
-    const Bounds all = together<PPW>(mine, wb, wave, lane);
-    const Tiles tiles(all);
-    const int n = tiles.n;
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-        if (j < n) issue(tiles.key0(j), tbuf[j]);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    bool bad = false;  // tile q - 1 had values that are not finite
-    auto open = [&](int q) __attribute__((always_inline)) {
-        if (q >= 2 && q + 1 < n) issue(tiles.key0(q + 1), tbuf[(q + 1) % 3]);
-        bad = false;
-        if (q >= 1 && q <= n && !all.whole(tiles.key0(q - 1))) {
-            int x = 0;
-#pragma unroll
-            for (int w = 0; w < PPW; ++w) x |= wbad[(q + 1) & 1][w];
-            bad = __builtin_amdgcn_readfirstlane(x) != 0;
-            if (bad) {
-                screen_clear<HD, PPW>(sp_, tid);
-                __syncthreads();
-                screen<HD, PPW>(tbuf[(q + 2) % 3] + KF * FH, sp_, tid);
-                __syncthreads();
-            }
-        }
-        if (q < n && !all.whole(tiles.key0(q))) {
-            const bool any = odd_values<HD, PPW>(tbuf[q % 3] + KF * FH, tid);
-            if (lane == 0) wbad[q & 1][wave] = any;
-        }
-    };
-    auto turn = [&](int q) __attribute__((always_inline)) {
-        __builtin_amdgcn_s_waitcnt(0);  // the tile issued at the start of this period
-        __syncthreads();
-        open(q);
-    };
-    open(0);
-    bool done = false;
-    for (int q = 0; q <= n; ++q) {
-        if (done) {
-            t.values(tbuf[(q + 2) % 3]);
-            if (bad) t.specials(sp_, tiles.key0(q - 1));
-        }
-        const int kv0 = tiles.key0(q);
-        done = q < n && mine.touches(kv0);
-        if (done) t.scores(tbuf[q % 3]);
-        // One barrier a period, behind the scores or behind the softmax: the
-        // waves' instructions are the same, half a period apart.
-        if (second) turn(q + 1);
-        if (done) t.softmax(kv0, mine.whole(kv0));
-        if (!second) turn(q + 1);
-    }
-    half_t* R = tbuf[0] + wave * 16 * HD;
-    t.close();
-    static_assert(PPW * 16 * HD <= (KF + VF) * FH, "the waves' regions fit one buffer");
-#pragma unroll
-    for (int u = 0; u < NQT; ++u) {
-        const float lt = t.l[u][0];
-        store_rows<HD, NQT>(R, t.o, u, lt > 0.0f || lt != lt ? 1.0f / lt : 0.0f, lane, a, p0 + 16 * u, h);
     }
 }
 
@@ -839,20 +744,15 @@ __global__ __launch_bounds__(RT) void ranges_merge_kernel(const float* ws, uint1
     *reinterpret_cast<half8*>(out + 8 * i) = y;
 }
 
-hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStream_t st) {
+hipError_t launch_ranges(int hd, int nqt, const RangesArgs& a, hipStream_t st) {
     RangesArgs b = a;
-    const int pb = pp ? 64 * (4 / a.gb) : 16 * nqt * (RW / a.gb);
+    const int pb = 16 * nqt * (RW / a.gb);
     b.nrb = (a.tq + pb - 1) / pb;
     const unsigned items = (unsigned)b.nrb * (unsigned)(a.heads / a.gb) * (unsigned)a.splits;
     b.xcd = items % 8 == 0;
     b.grid8 = (int)(items / 8);
     const int mode = (a.softcap > 0.0f ? SM_CAP : 0) | (a.slopes ? SM_BIAS : 0);
     const long rows = (long)a.tq * a.heads;
-#define RP(HD, M)                                                                                                \
-    if (hd == HD && mode == M && pp) {                                                                           \
-        hipLaunchKernelGGL((ranges_pp_kernel<HD, M>), dim3(items), dim3(PPW * LLMTIE_WAVE), 0, st, b);           \
-        return hipGetLastError();                                                                                \
-    }
 #define RL(HD, M, N)                                                                                             \
     if (hd == HD && mode == M && nqt == N && a.splits == 1) {                                                    \
         hipLaunchKernelGGL((ranges_kernel<HD, M, N, false>), dim3(items), dim3(RT), 0, st, b);                   \
@@ -866,12 +766,10 @@ hipError_t launch_ranges(int hd, int nqt, bool pp, const RangesArgs& a, hipStrea
         return hipGetLastError();                                                                                \
     }
 #define RM(HD, M) RL(HD, M, 1) RL(HD, M, 2) RS(HD, M)
-    RP(128, 0) RP(128, SM_BIAS)
     RM(64, 0) RM(64, 1) RM(64, 2) RM(64, 3) RM(128, 0) RM(128, 1) RM(128, 2) RM(128, 3)
 #undef RM
 #undef RS
 #undef RL
-#undef RP
     return hipErrorInvalidValue;
 }
 
