@@ -228,3 +228,13 @@ def test_a_gguf_that_rotates_a_part_of_its_heads(tmp_path):
         m.config_from_gguf = config
     assert whole.rope_dim == 0 and part.rope_dim == cfg.head_dim // 2 and part.rope_interleaved
     assert np.array_equal(m.unpermute_rope(b["0.wq"], cfg.heads), a["0.wq"])
+
+
+@pytest.mark.parametrize("names", ["Gpu, DecodeScratch, TiledCache16, KeyRanges, rope_scaling", "gpu", "rope_scaling"])
+def test_names_of_the_package(names):
+    """In a process that has not imported the mirror yet."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    subprocess.run([sys.executable, "-c", f"from ttsxabe_amd import {names}"], check=True,
+                   cwd=Path(__file__).resolve().parent.parent)
