@@ -377,7 +377,9 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
  * 1. The three arrays are on the device and may change between replays of a
  * captured call. Lengths are clamped to cap; max_tk plans the launch for the
  * lengths to come (longer ones are attended too, less evenly spread) and decides
- * with it how keys are divided: results under two bounds agree to rounding. A
+ * with it how keys are divided: results under two bounds agree to rounding. (An
+ * eager call of the most sequences and the largest max_tk sizes the scratch for
+ * every smaller one that is captured.) A
  * sequence whose slot is out of range gets a NaN row, one that sees no key
  * zeros. GQA groups up to 16. out = [nseq, heads*head_dim] f32, 16-byte aligned
  * as the cache is. */

@@ -412,6 +412,37 @@ def test_decode_captured_follows_its_lengths(gpu):
                 assert not got.view(n, -1)[i].any()
 
 
+@pytest.mark.parametrize("cap", [1500, 6500])
+def test_decode_captured_after_a_larger_batch(gpu, cap):
+    """One eager call of the largest batch sizes the scratch for smaller ones, whose heads are cut into more runs."""
+    from ttsxabe_amd.gpu import DecodeScratch
+    heads, kv, hd, slots = 8, 8, 64, 3
+    k, v = f16(1, slots, kv, cap, hd), f16(2, slots, kv, cap, hd)
+    cache, scratch = cache_of(k, v), DecodeScratch()
+    q = torch.randn(100, heads, hd, generator=torch.Generator().manual_seed(3))
+    d = q.cuda().view(-1)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32).cuda()  # noqa: E731
+    gpu.attn_decode_ranges(d, 0, heads * hd, cache, i32([100] * 100), i32([0] * 100), cap, heads, 0.1, scratch)
+    for n in (1, 3, 25, 40):
+        for bound in (cap, 1000):
+            lens = [min(bound, 300 * (i % 5) + 1) for i in range(n)]
+            tk, slot = i32(lens), i32([i % slots for i in range(n)])
+            out = torch.zeros(n * heads * hd, device="cuda")
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                gpu.attn_decode_ranges(d, 0, heads * hd, cache, tk, slot, bound, heads, 0.1, scratch, out=out)
+            for turn in range(3):
+                out.zero_()
+                g.replay()
+                torch.cuda.synchronize()
+                for i in range(n) if turn == 2 else (0, n - 1):
+                    want, tol = ref.attend(q[i:i + 1], k[i % slots, :, :lens[i]], v[i % slots, :, :lens[i]],
+                                           torch.ones(1, lens[i], dtype=torch.bool), torch.tensor([lens[i] - 1]), 0.1,
+                                           decode=True)
+                    close(out.view(n, heads, hd)[i:i + 1], want, tol, (n, bound, i))
+
+
 def test_prompt_captured(gpu):
     """A cut prompt in a graph: its workspace is the graph's own, and two graphs do not share it."""
     rows, past, heads, kv, hd = 40, 1200, 8, 2, 128

@@ -1147,6 +1147,7 @@ constexpr size_t MAX_WGS = ((size_t)1 << 24) - 1;
 // Batched decode over key ranges: blocks of a head kept in one workgroup, and the
 // bytes (half of the 256 MB Infinity Cache) past which a launch streams.
 constexpr int RD_WHOLE = 20;
+constexpr size_t RD_LONG = 192;  // blocks of a bound under which lengths may differ much
 constexpr size_t RD_STREAM_BYTES = (size_t)128 << 20;
 
 // What the score arguments must be: every logit of finite queries and keys is
@@ -1190,6 +1191,26 @@ int range_tiles(size_t tq, size_t past, size_t heads, size_t hd, int gb, bool ca
     const size_t cus = (size_t)compute_units();
     if (past >= tq) return wgs >= (hd == 128 ? cus + cus / 8 : 2 * cus) ? 2 : 1;
     return wgs >= (hd == 128 ? 2 * cus : capped ? 4 * cus - cus / 8 : 5 * cus / 2) ? 2 : 1;
+}
+
+// Workgroups that a decode cuts each (sequence, kv head) into: those that fill the
+// compute units once without a second round, or twice where the launch
+// streams; a launch just past a round waits for it. Us at runs (workgroups): 40 heads of 3000 keys of 128 dims 6 (240) 16.5, 7
+// (280) 18.2, 12 (480) 17.6; 80 of 3000 3 (240) 26.3, 4 (320) 29.4, 6 (480) 26.4; streamed, 40 of
+// 8000 5 (200) 32.7, 6 31.7, 12 (480) 31.1, 13 (520) 36.4; 96 of 8000 2 67.7, 3 81.7, 5 (480) 66.2, 6 73.6;
+// 160 of 500-5000 1 59.9, 2 50.2, 3 (480) 49.1, 4 50.2. (Very uneven ones can gain by more: 96 of
+// 20-8000 5 45.1, 6 37.9; of 256-8192 47.7, 45.5.)
+// Heads that fill the compute units by themselves are whole, unless the bound is so long that
+// lengths under it differ much: 176 of 256-8192 89.8 / 70.2 in four, 224 93.9 / 92.7, 256 103.8 / 100.7 (two 98.8),
+// 320 159 / 127, 448 184 / 167, 640 of 64 dims 135 / 119, but 224 of 1000-4000 53.6 / 59.1 and 256 of 2500 53.0 / 62.5.
+// Some more than one a compute unit are two runs: 288 of 1000-4000 78.0 / 73.5, 320 of 2500 79.4 / 73.4,
+// 448 90.3 / 98.6; behind a window of 1024 34.8 / 37.1.
+size_t range_runs(size_t units, size_t blocks, bool streams) {
+    const size_t cus = (size_t)compute_units(), one = std::max<size_t>(1, cus / units), two = 2 * cus / units;
+    if (!streams) return one;
+    if (two >= 3) return two;
+    if (units <= 3 * cus && blocks >= RD_LONG) return units == cus ? 2 : 4;
+    return units > cus && units <= cus + cus / 2 && blocks >= 64 ? 2 : 1;
 }
 
 int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows, size_t heads, size_t pos_len,
@@ -1436,27 +1457,24 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     const size_t group = heads / kv_heads, units = smul(nseq, kv_heads);
     const size_t keys = window ? std::min(max_tk, sadd(window, shared)) : max_tk;
     const size_t blocks = (keys + 31) / 32;
-    // Runs of a head: as many as bring the launch to one workgroup a compute
-    // unit, of four blocks (one a wave) or more; a head of up to RD_WHOLE blocks is
-    // one run (a merge costs ~3 us). Us, whole / cut: 1 sequence of 32/8/128, 14
+    // Runs of a head, of four blocks (one a wave) or more; a head of up to RD_WHOLE
+    // blocks is one run (a merge costs ~3 us). Us, whole / cut: 1 sequence of 32/8/128, 14
     // blocks 6.8 / 7.5, 18 7.5 / 7.5, 28 8.9 / 7.5; of 20/20/64, 18 5.9 / 7.2, 28
     // 7.0 / 7.3; 16 sequences of 32/8/128, 18 blocks 12.2 / 12.9, 28 16.0 / 15.7.
-    // Twice the workgroups: 1 sequence of 4001 10.0 / 10.0; 4 of 200-6000 15.4 / 15.0;
-    // 16 of 50-600 12.8 / 10.9; 8 of 2000 over 8 heads of 64, 11.9 / 11.3.
+    const size_t span = 4;
+    const size_t most = std::min<size_t>(DECODE_MAX_SPLITS, DECODE_MAX_SPLIT_ROWS / group);
     // Past half the Infinity Cache a launch streams: what it reads cannot be
     // kept until it is read again, and loads that do not try read faster (32
     // sequences of 256-8192, 113 / 101 us; 4 of 200-6000, which fit, 15.2 / 16.6).
-    // Two workgroups a compute unit then even out the lengths: 32 of 256-8192, 101
-    // / 108; 32 of 4096, 88 / 85.
-    const size_t span = 4;
-    const size_t most = std::min<size_t>(DECODE_MAX_SPLITS, DECODE_MAX_SPLIT_ROWS / group);
     const bool streams = smul(smul(units, blocks), 128, head_dim) > RD_STREAM_BYTES;
-    const size_t target = (size_t)compute_units() * (streams ? 2 : 1);
-    const size_t splits =
-        std::max<size_t>(1, std::min(std::min((blocks + span - 1) / span, most), (target + units - 1) / units));
+    const size_t runs = range_runs(units, blocks, streams);
+    const size_t splits = std::max<size_t>(1, std::min(std::min((blocks + span - 1) / span, most), runs));
     if (smul(units, splits) > MAX_WGS) return overrun_slice(smul(units, splits), MAX_WGS);
     const size_t parts = smul(units, splits, n / kv_heads);
-    const size_t floats = splits > 1 ? sadd(parts, smul(units, splits, 2 * group)) : 0;
+    // Room for the runs of any smaller batch under this bound too (they can be
+    // more): one eager call of the largest sizes a scratch for captured ones.
+    const size_t room = (size_t)compute_units() * (blocks >= RD_LONG ? 12 : 2);
+    const size_t floats = smul(std::max(smul(units, splits), room), group, head_dim + 2);
     if (int r = ensure_scratch(scratch, floats, smul(units, CTR_STRIDE), S(stream))) return r;
     RangesDecodeArgs a{};
     a.q = q + q_off;
