@@ -412,6 +412,13 @@ def test_decode_captured_follows_its_lengths(gpu):
                 assert not got.view(n, -1)[i].any()
 
 
+@pytest.mark.parametrize("softcap", [0.25, 2.0, 4.0, 8.0, 200.0])
+@pytest.mark.parametrize("shape", [(8, 2, 64), (4, 4, 128)])
+def test_decode_scores_on_both_sides_of_the_series(gpu, shape, softcap):
+    """Blocks whose scores are all small against the cap, some beyond 0.45 of it, and all beyond."""
+    close(*decode(gpu, [700, 33, 1], 700, shape, 0, 0, softcap, False))
+
+
 @pytest.mark.parametrize("cap", [1500, 6500])
 def test_decode_captured_after_a_larger_batch(gpu, cap):
     """One eager call of the largest batch sizes the scratch for smaller ones, whose heads are cut into more runs."""
