@@ -1194,17 +1194,19 @@ int range_tiles(size_t tq, size_t past, size_t heads, size_t hd, int gb, bool ca
 }
 
 // Workgroups that a decode cuts each (sequence, kv head) into: those that fill the
-// compute units once without a second round, or twice where the launch
-// streams; a launch just past a round waits for it. Us at runs (workgroups): 40 heads of 3000 keys of 128 dims 6 (240) 16.5, 7
-// (280) 18.2, 12 (480) 17.6; 80 of 3000 3 (240) 26.3, 4 (320) 29.4, 6 (480) 26.4; streamed, 40 of
-// 8000 5 (200) 32.7, 6 31.7, 12 (480) 31.1, 13 (520) 36.4; 96 of 8000 2 67.7, 3 81.7, 5 (480) 66.2, 6 73.6;
-// 160 of 500-5000 1 59.9, 2 50.2, 3 (480) 49.1, 4 50.2. (Very uneven ones can gain by more: 96 of
-// 20-8000 5 45.1, 6 37.9; of 256-8192 47.7, 45.5.)
-// Heads that fill the compute units by themselves are whole, unless the bound is so long that
-// lengths under it differ much: 176 of 256-8192 89.8 / 70.2 in four, 224 93.9 / 92.7, 256 103.8 / 100.7 (two 98.8),
-// 320 159 / 127, 448 184 / 167, 640 of 64 dims 135 / 119, but 224 of 1000-4000 53.6 / 59.1 and 256 of 2500 53.0 / 62.5.
-// Some more than one a compute unit are two runs: 288 of 1000-4000 78.0 / 73.5, 320 of 2500 79.4 / 73.4,
-// 448 90.3 / 98.6; behind a window of 1024 34.8 / 37.1.
+// compute units once without a second round, or twice where the launch streams; a
+// launch just past a round waits for it. Us at runs (workgroups): 40 heads of 3000
+// keys of 128 dims 6 (240) 16.5, 7 (280) 18.2, 12 (480) 17.6; 80 of 3000 3 (240) 26.3,
+// 4 (320) 29.4, 6 (480) 26.4; streamed, 40 of 8000 5 (200) 32.7, 6 31.7, 12 (480) 31.1,
+// 13 (520) 36.4; 96 of 8000 2 67.7, 3 81.7, 5 (480) 66.2, 6 73.6; 160 of 500-5000 1 59.9,
+// 2 50.2, 3 (480) 49.1, 4 50.2. (Very uneven ones can gain by more: 96 of 20-8000 5
+// 45.1, 6 37.9; of 256-8192 47.7, 45.5.)
+// Heads that fill the compute units by themselves are whole, unless the bound is so
+// long that lengths under it differ much, whole / in four: 176 of 256-8192 89.8 /
+// 70.2, 224 93.9 / 92.7, 256 103.8 / 100.7 (in two 98.8), 320 159 / 127, 448 184 / 167,
+// 640 of 64 dims 135 / 119, but 224 of 1000-4000 53.6 / 59.1, 256 of 2500 53.0 / 62.5.
+// Some more than one a compute unit are two runs: 288 of 1000-4000 78.0 / 73.5, 320 of
+// 2500 79.4 / 73.4, 448 90.3 / 98.6; behind a window of 1024 34.8 / 37.1.
 size_t range_runs(size_t units, size_t blocks, bool streams) {
     const size_t cus = (size_t)compute_units(), one = std::max<size_t>(1, cus / units), two = 2 * cus / units;
     if (!streams) return one;
