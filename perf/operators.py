@@ -185,9 +185,6 @@ def prepare(case, seed):
     c = dict(case)
     g = _gen(seed)
     s = {"c": c}
-    if own:  # the handle that such a program keeps
-        from ttsxabe_amd.gpu import DecodeScratch, Gpu, KeyRanges, TiledCache16
-        s["gpu"] = Gpu(0)
     if c["kind"] == "ranges":
         starts = _starts(c)
         prefix = _prefix(c, starts)
@@ -232,7 +229,9 @@ def prepare(case, seed):
         s["tk"] = _ints(_lengths(c))
         s["slot"] = torch.randperm(c["nseq"], generator=g, device="cuda").to(torch.int32)
         s["slopes"] = _slopes(c)
-    if own:  # and the cache, the row table and the scratch
+    if own:  # the handles that such a program keeps
+        from ttsxabe_amd.gpu import DecodeScratch, Gpu, KeyRanges, TiledCache16
+        s["gpu"] = Gpu(0)
         slots = c.get("slots", c.get("nseq", 1))
         s["tiled"] = TiledCache16.of(s["cache"], c["kv"], c["hd"], s.get("cap", c.get("cap")), slots=slots)
         if c["kind"] == "prefill":
@@ -372,7 +371,12 @@ def _plain(s):
 
 
 def _kernels(s):
-    c, g = s["c"], s["gpu"]
+    c = s["c"]
+    if c["kind"] in ("ranges", "rope"):
+        from ttsxabe_amd.gpu import Gpu
+        g = Gpu(0)
+    else:
+        g = s["gpu"]
     if c["kind"] == "ranges":
         r = g.key_ranges(c["rows"], c["past"], s["starts"], s["prefix"], c["causal"], c["window"], c["shared"])
         return [*r.table, r.pos]
