@@ -780,8 +780,9 @@ hipError_t launch_ranges(int hd, int nqt, const RangesArgs& a, hipStream_t st) {
 // waves taking every fourth block; the <= 16 query heads of the group are the
 // 16 columns of the MFMA tile, so a key and value is read once for all of them.
 // The products are S^T = K Q^T and O^T = V^T P^T as in the prompts' kernel, with
-// q and P as the sums of two f16 (22 bits of each), so the context carries f32's
-// precision off the f16 cache. What bounds it is reading K and V: the next
+// q and P as the sums of two f16 (22 bits of each, P's down to 2^-17 of the
+// largest and 2^-40 of it below that), so the context carries f32's precision
+// off the f16 cache. What bounds it is reading K and V: the next
 // block's 16 loads a lane are in flight while one is computed.
 //
 // The lengths are on the device, so the launch has `splits` runs a head for any
@@ -790,6 +791,12 @@ hipError_t launch_ranges(int hd, int nqt, const RangesArgs& a, hipStream_t st) {
 // coherent stores, counts its arrivals, and the last one merges them in order
 // (the results do not depend on which that is).
 constexpr int RD_MAX_ROWS = 1024;  // splits * group at most
+// A weight is formed as 2^(s - m + RD_LIFT), m the largest score: what f16's
+// smallest half step, 2^-25, takes from it is then 2^-40 of the largest weight
+// (unlifted, keys 25 below a dominant one were in l and not in O). O and l
+// carry the same factor, and 2^15 is within f16. Its addition is not seen in
+// the time (32 sequences of 256-8192 96.2 us with and without it, one of 4001 9.6).
+constexpr float RD_LIFT = 15.0f;
 
 // c2 tanh(c1 s) of a lane's eight scores, c1 c2 = sl2. For |x| up to 0.45 the
 // series of tanh x / x to x^12, 2^-25.6 off there; where a lane's score is
@@ -942,7 +949,8 @@ __global__ __launch_bounds__(RT, 2) void ranges_decode_kernel(RangesDecodeArgs a
         for (int T = 0; T < 2; ++T)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float p = ex2(sc[T][r] - m);
+                // (The difference first: the key m is has 0, however large m is.)
+                const float p = ex2((sc[T][r] - m) + RD_LIFT);
                 l += p;
                 half_t hi_, lo_;
                 split_h(p, hi_, lo_);
