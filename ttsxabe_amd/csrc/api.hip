@@ -1148,6 +1148,7 @@ constexpr size_t MAX_WGS = ((size_t)1 << 24) - 1;
 // bytes (half of the 256 MB Infinity Cache) past which a launch streams.
 constexpr int RD_WHOLE = 20;
 constexpr size_t RD_LONG = 192;  // blocks of a bound under which lengths may differ much
+constexpr size_t RD_TWO = 64;    // and from which heads past a round are two runs
 constexpr size_t RD_STREAM_BYTES = (size_t)128 << 20;
 
 // What the score arguments must be: every logit of finite queries and keys is
@@ -1212,7 +1213,13 @@ size_t range_runs(size_t units, size_t blocks, bool streams) {
     if (!streams) return one;
     if (two >= 3) return two;
     if (units <= 3 * cus && blocks >= RD_LONG) return units == cus ? 2 : 4;
-    return units > cus && units <= cus + cus / 2 && blocks >= 64 ? 2 : 1;
+    return units > cus && units <= cus + cus / 2 && blocks >= RD_TWO ? 2 : 1;
+}
+// The most partials (a workgroup's each) that range_runs leaves to any batch, of
+// bounds up to `blocks`: four runs of three heads a compute unit, two of one and a
+// half, or twice the compute units.
+size_t range_room(size_t blocks) {
+    return (size_t)compute_units() * (blocks >= RD_LONG ? 12 : blocks >= RD_TWO ? 3 : 2);
 }
 
 int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows, size_t heads, size_t pos_len,
@@ -1475,8 +1482,7 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     const size_t parts = smul(units, splits, n / kv_heads);
     // Room for the runs of any smaller batch under this bound too (they can be
     // more): one eager call of the largest sizes a scratch for captured ones.
-    const size_t room = (size_t)compute_units() * (blocks >= RD_LONG ? 12 : 2);
-    const size_t floats = smul(std::max(smul(units, splits), room), group, head_dim + 2);
+    const size_t floats = smul(std::max(smul(units, splits), range_room(blocks)), group, head_dim + 2);
     if (int r = ensure_scratch(scratch, floats, smul(units, CTR_STRIDE), S(stream))) return r;
     RangesDecodeArgs a{};
     a.q = q + q_off;
