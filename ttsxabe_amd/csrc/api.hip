@@ -1203,16 +1203,21 @@ int range_tiles(size_t tq, size_t past, size_t heads, size_t hd, int gb, bool ca
 // 2 50.2, 3 (480) 49.1, 4 50.2. (Very uneven ones can gain by more: 96 of 20-8000 5
 // 45.1, 6 37.9; of 256-8192 47.7, 45.5.)
 // Heads that fill the compute units by themselves are whole, unless the bound is so
-// long that lengths under it differ much, whole / in four: 176 of 256-8192 89.8 /
-// 70.2, 224 93.9 / 92.7, 256 103.8 / 100.7 (in two 98.8), 320 159 / 127, 448 184 / 167,
-// 640 of 64 dims 135 / 119, but 224 of 1000-4000 53.6 / 59.1, 256 of 2500 53.0 / 62.5.
+// long that lengths under it differ much: then four runs. Means of eight batches of
+// 32/8/128 under 8192, capped, whole / in two / in four: of 256-8192 224 heads 93.7 /
+// 93.6 / 89.9, 240 96.8 / 96.9 / 95.4, 256 100.6 / 101.0 / 100.0; of 64-8192 over their
+// logarithm 70.2 / 48.5 / 45.0, 70.7 / 49.3 / 47.9, 71.3 / 50.3 / 49.9; but of 4096-8192 113.6 /
+// 115.4 / 118.2, 120.3 / 123.2 / 124.4, 126.9 / 130.2 / 132.4. Means of three batches of 256-8192:
+// 264 heads 126 / 108 / 108, 288 160 / 117 / 118, 384 176 / 159 / 151; 448 184 / - / 167, 640 of 64
+// dims 135 / - / 119. (Under 192 blocks whole: 224 of 1000-4000 53.6 / - / 59.1, 256 of 2500
+// 53.0 / - / 62.5.)
 // Some more than one a compute unit are two runs: 288 of 1000-4000 78.0 / 73.5, 320 of
 // 2500 79.4 / 73.4, 448 90.3 / 98.6; behind a window of 1024 34.8 / 37.1.
 size_t range_runs(size_t units, size_t blocks, bool streams) {
     const size_t cus = (size_t)compute_units(), one = std::max<size_t>(1, cus / units), two = 2 * cus / units;
     if (!streams) return one;
     if (two >= 3) return two;
-    if (units <= 3 * cus && blocks >= RD_LONG) return units == cus ? 2 : 4;
+    if (units <= 3 * cus && blocks >= RD_LONG) return 4;
     return units > cus && units <= cus + cus / 2 && blocks >= RD_TWO ? 2 : 1;
 }
 // The most partials (a workgroup's each) that range_runs leaves to any batch, of
