@@ -27,13 +27,22 @@ from .gpu import CacheOverrun, DecodeScratch, Gpu, InvalidArgument, TiledCache16
 
 class LlamaStack:
     """`layout`: "reference" (K [kv][cap][hd] + V [kv][hd][cap] f16, the
-    reference's cache) or "tiled" (the fragment-order cache)."""
+    reference's cache) or "tiled" (the fragment-order cache). Plain scores, and
+    whole heads rotated in halves at unscaled positions: a configuration that asks for
+    others is refused."""
 
     def __init__(self, gpu: Gpu, cfg, weights: dict, layout: str = "reference"):
         if layout not in ("reference", "tiled"):
             raise ValueError(f"unknown cache layout {layout!r}")
-        if getattr(cfg, "rope_interleaved", False) or getattr(cfg, "softcap", 0.0):
-            raise ValueError("interleaved rotary weights and capped scores are LlamaBatch's")
+        kind, factor, _ = getattr(cfg, "rope_scaling", None) or ("none", 1.0, 0)
+        for what, has in (("interleaved rotary weights", getattr(cfg, "rope_interleaved", False)),
+                          ("capped scores", getattr(cfg, "softcap", 0.0)),
+                          ("a window", getattr(cfg, "window", 0)),
+                          ("biased scores", getattr(cfg, "slopes", None) is not None),
+                          ("partly rotated heads", (getattr(cfg, "rope_dim", 0) or cfg.head_dim) != cfg.head_dim),
+                          ("scaled rotary positions", kind != "none" and factor != 1.0)):
+            if has:
+                raise ValueError(f"a configuration with {what}, which LlamaBatch computes")
         self.g, self.cfg, self.layout = gpu, cfg, layout
         dev = gpu.device
         self.w = {k: torch.from_numpy(np.ascontiguousarray(v)).to(dev) for k, v in weights.items()}
