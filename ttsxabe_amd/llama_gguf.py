@@ -87,7 +87,11 @@ def config_from_gguf(f: GgufFile) -> LlamaConfig:
     kind, factor = f.get_str("llama.rope.scaling.type"), f.get_f32("llama.rope.scaling.factor")
     scaling = None
     if kind in ("linear", "yarn") and factor is not None:
-        scaling = (kind, factor, f.get_u32("llama.rope.scaling.original_context_length") or 8192)
+        # The file's whole context is the original one where no other is named. (Linear positions need neither.)
+        original = f.get_u32("llama.rope.scaling.original_context_length") or f.get_u32("llama.context_length")
+        if kind == "yarn" and not original:
+            raise LlamaGgufError("missing metadata `llama.rope.scaling.original_context_length`")
+        scaling = (kind, factor, original or 8192)
     return LlamaConfig(vocab=vocab, hidden=hidden, heads=heads, kv_heads=kv, head_dim=hd,
                        ffn=need("llama.feed_forward_length"), layers=need("llama.block_count"),
                        theta=need_f("llama.rope.freq_base"), eps=need_f("llama.attention.layer_norm_rms_epsilon"),
