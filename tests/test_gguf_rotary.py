@@ -74,3 +74,18 @@ def test_rotated_dims(tmp_path):
     assert c.rope_dim == 16 and c.rope_interleaved
     c, _ = load_llama_gguf(f)
     assert c.rope_dim == 0 and not c.rope_interleaved
+
+
+@pytest.mark.parametrize("more,what", [
+    (scaling("longrope", 4.0, 4096), "longrope"), (scaling("other"), "other"),
+    ({**scaling("yarn", 4.0, 4096), "llama.rope.scaling.attn_factor": (gguf.F32, 0.75)}, "attn_factor"),
+], ids=["longrope", "other", "attn_factor"])
+def test_scalings_that_are_not_computed_are_refused(tmp_path, more, what):
+    f = with_metadata(tmp_path / "m.gguf", more)
+    with pytest.raises(LlamaGgufError, match=what):
+        config_from_gguf(f)
+
+
+def test_a_factor_of_one_multiplies_nothing(tmp_path):
+    m = {**scaling("linear", 4.0, 4096), "llama.rope.scaling.attn_factor": (gguf.F32, 1.0)}
+    assert config_from_gguf(with_metadata(tmp_path / "m.gguf", m)).rope_scaling == ("linear", 4.0, 4096)

@@ -92,6 +92,10 @@ def config_from_gguf(f: GgufFile) -> LlamaConfig:
         if kind == "yarn" and not original:
             raise LlamaGgufError("missing metadata `llama.rope.scaling.original_context_length`")
         scaling = (kind, factor, original or 8192)
+    elif kind not in (None, "none", "linear", "yarn"):
+        raise LlamaGgufError(f"rotary scaling `{kind}`, wanted `linear` or `yarn`")
+    if scaling and (f.get_f32("llama.rope.scaling.attn_factor") or 1.0) != 1.0:
+        raise LlamaGgufError("metadata `llama.rope.scaling.attn_factor`, for which there is no multiplier")
     return LlamaConfig(vocab=vocab, hidden=hidden, heads=heads, kv_heads=kv, head_dim=hd,
                        ffn=need("llama.feed_forward_length"), layers=need("llama.block_count"),
                        theta=need_f("llama.rope.freq_base"), eps=need_f("llama.attention.layer_norm_rms_epsilon"),
