@@ -42,3 +42,20 @@ def test_a_plain_stack_takes_what_changes_nothing(extra):
     cfg = Config(**extra)
     with pytest.raises(LookupError):
         LlamaStack(Device(), cfg, random_weights(cfg, 1))
+
+
+@pytest.mark.parametrize("token", [64, -1, 2**31, 2**40])
+def test_a_batch_refuses_a_token_that_has_no_embedding(token):
+    """Before anything is launched (on a device such an index ends the process), and the sequences stay."""
+    import torch
+
+    from ttsxabe_amd.gpu import InvalidArgument
+    from ttsxabe_amd.stack import LlamaBatch
+    b = object.__new__(LlamaBatch)
+    b.g, b.cfg, b.slots, b.cap, b.length, b.window, b.shared = None, StackConfig(vocab=64), 2, 32, [5, 0], 0, 0
+    b.w = {"embed": torch.zeros(64, 4)}
+    with pytest.raises(InvalidArgument):
+        b.prefill([[1, 2], [3, token]], [0, 1])
+    with pytest.raises(InvalidArgument):
+        b.step([1, token], [0, 1])
+    assert b.length == [5, 0]

@@ -161,7 +161,10 @@ class LlamaBatch:
     def _ints(self, v):
         return torch.tensor(v, dtype=torch.int32, device=self.g.device)
 
-    def _check(self, slots, new):
+    def _check(self, slots, new, ids):
+        # (An id past the embedding ends the process from the device.)
+        if any(not 0 <= t < len(self.w["embed"]) for t in ids):
+            raise InvalidArgument(f"a token that is not one of {len(self.w['embed'])}")
         if len(set(slots)) < len(slots) or any(not 0 <= s < self.slots for s in slots):
             raise InvalidArgument(f"slots {slots} of {self.slots}")
         for s, n in zip(slots, new):
@@ -198,10 +201,11 @@ class LlamaBatch:
         lens = [len(p) for p in prompts]
         if len(slots) != len(prompts) or not prompts:
             raise InvalidArgument("a slot for each prompt")
+        tokens = [int(t) for p in prompts for t in p]
         before = self.length
         self.length = [0 if s in set(slots) else n for s, n in enumerate(before)]
         try:
-            self._check(slots, lens)
+            self._check(slots, lens, tokens)
         except Exception:
             self.length = before
             raise
@@ -232,8 +236,7 @@ class LlamaBatch:
             return g.flash_attn_ranges(q, 0, c.heads * c.head_dim, self.packed, 0, r, n, 0, c.heads, self.scale,
                                        **self.scores)
 
-        ids = torch.tensor([t for p in prompts for t in p], device=g.device)
-        h = self._layers(ids, attend)[torch.tensor(starts[1:], device=g.device) - 1]
+        h = self._layers(torch.tensor(tokens, device=g.device), attend)[torch.tensor(starts[1:], device=g.device) - 1]
         for s, m in zip(slots, lens):
             self.length[s] = m
         return self._norm(h, self.w["norm"]) @ self.w["lm_head"].T
@@ -243,7 +246,8 @@ class LlamaBatch:
         c, g = self.cfg, self.g
         if len(ids) != len(slots) or not slots:
             raise InvalidArgument("a token for each slot")
-        self._check(slots, [1] * len(slots))
+        ids = [int(t) for t in ids]
+        self._check(slots, [1] * len(slots), ids)
         at = [self.length[s] for s in slots]
         pos, slot, tk = self._ints(at), self._ints(list(slots)), self._ints([p + 1 for p in at])
         q = torch.empty(len(ids) * c.heads * c.head_dim, dtype=torch.float32, device=g.device)
@@ -253,7 +257,7 @@ class LlamaBatch:
             return g.attn_decode_ranges(q, 0, c.heads * c.head_dim, self.cache[l], tk, slot, max(at) + 1, c.heads,
                                         self.scale, self.scratch, window=self.window, shared=self.shared, **self.scores)
 
-        h = self._layers(torch.tensor(list(ids), device=g.device), attend)
+        h = self._layers(torch.tensor(ids, device=g.device), attend)
         for s in slots:
             self.length[s] += 1
         return self._norm(h, self.w["norm"]) @ self.w["lm_head"].T
