@@ -579,19 +579,24 @@ class Gpu:
         if status:
             _check(status)
 
-    def _on(self, t, dtypes, what):
-        """As _need, and on this Gpu's device."""
-        if t is not None and (t.get_device() != self.device.index or t.dtype not in dtypes or not t.is_contiguous()):
+    def _on(self, t, dtypes, what, least=0):
+        """As _need, on this Gpu's device, and of `least` elements. (An empty
+        tensor has no address, which an entry point would take for none given.)"""
+        if t is None:
+            return
+        if t.get_device() != self.device.index or t.dtype not in dtypes or not t.is_contiguous():
             _need(t, dtypes, what)
             raise InvalidArgument(f"{what} is on {t.device}, not on {self.device}")
+        if t.numel() < least:
+            raise SliceOverrun(f"reading to {least} in a buffer of {t.numel()}", (least, t.numel()))
 
     def key_ranges(self, rows, past=0, starts=None, prefix=None, causal=True, window=0, shared=0) -> KeyRanges:
         """Which keys each of `rows` rows behind `past` positions sees (new; see
         llmtie_key_ranges): documents from `starts` (int32, one more than there
         are), `prefix` leading rows of each that its rows all see, a `window`,
         `shared` leading positions that every row sees."""
-        self._on(starts, _I32, "starts")
-        self._on(prefix, _I32, "prefix")
+        self._on(starts, _I32, "starts", 1)
+        self._on(prefix, _I32, "prefix", 1 if starts is None else starts.numel() - 1)
         if rows < 0 or past < 0 or window < 0 or shared < 0:
             raise InvalidArgument("a negative count")
         table = torch.empty((3, rows), dtype=torch.int32, device=self.device)
@@ -614,9 +619,9 @@ class Gpu:
             out_stride = heads * head_dim
         self._on(x, _F32, "x")
         self._on(out, _F32 + _H16, "out")
-        self._on(freq_div, _F32, "freq_div")
+        self._on(freq_div, _F32, "freq_div", rot_dim // 2)
         if isinstance(pos, torch.Tensor):
-            self._on(pos, _I32, "pos")
+            self._on(pos, _I32, "pos", t)
             at = pos.data_ptr(), pos.numel(), 0
         else:
             at = None, 0, int(pos)
@@ -647,10 +652,8 @@ class Gpu:
                 if q_out_stride is None:
                     q_out_stride = heads * cache.head_dim
         for t, what in ((pos, "pos"), (slot, "slot"), (index, "index")):
-            self._on(t, _I32, what)
-            if t.numel() < rows:
-                raise SliceOverrun(f"reading to {rows} in a buffer of {t.numel()}", (rows, t.numel()))
-        self._on(freq_div, _F32, "freq_div")
+            self._on(t, _I32, what, rows)
+        self._on(freq_div, _F32, "freq_div", rot_dim // 2)
         self._on(cache.data, _H16, "cache")
         if min(q_off, k_off, v_off, stride, rows, heads, rot_dim, q_out_off, q_out_stride) < 0:
             raise InvalidArgument("a negative count")
@@ -669,7 +672,7 @@ class Gpu:
         self._on(q, _H16, "q")
         self._on(data, _H16, "cache")
         self._on(table, _I32, "ranges")
-        self._on(slopes, _F32, "slopes")
+        self._on(slopes, _F32, "slopes", heads)
         if min(q_off, q_stride, slot, tq, past, heads, ranges.max_keys) < 0:
             raise InvalidArgument("a negative count")
         n = tq * heads * hd
@@ -699,13 +702,10 @@ class Gpu:
         self._on(q, _F32, "q")
         self._on(data, _H16, "cache")
         self._on(tk_dev, _I32, "tk")
-        self._on(slopes, _F32, "slopes")
+        self._on(slopes, _F32, "slopes", heads)
         nseq = tk_dev.numel()
-        for t, what in ((slot_dev, "slot"), (lo_dev, "lo")):
-            if t is not None:
-                self._on(t, _I32, what)
-                if t.numel() < nseq:
-                    raise SliceOverrun(f"reading to {nseq} in a buffer of {t.numel()}", (nseq, t.numel()))
+        self._on(slot_dev, _I32, "slot", nseq)
+        self._on(lo_dev, _I32, "lo", nseq)
         if min(q_off, q_stride, max_tk, heads, window, shared) < 0:
             raise InvalidArgument("a negative count")
         n = nseq * heads * cache.head_dim
