@@ -413,7 +413,8 @@ int llmtie_rope_rows(void* stream, const float* x, size_t x_len, size_t off, siz
  * launch. pos, slot and index are device arrays of index_len >= rows entries. A
  * row whose slot or index is out of range stores nothing (its q is rotated);
  * no two rows of a call may name the same place. The projections may be one
- * stacked buffer. */
+ * stacked buffer: q rotated in place then lies beside k and v at the one stride of all
+ * three, and another q_out lies apart from them. */
 int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
                           size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
                           size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,

@@ -1248,6 +1248,15 @@ bool overlap(const void* a, size_t an, const void* b, size_t bn) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + bn && y < x + an;
 }
+// Whether some of `rows` rows of an floats from a on, sa apart, shares a byte with
+// one of bn from b on, sb apart. (Two strides through the same memory: taken for it.)
+bool rows_overlap(const float* a, size_t an, size_t sa, const float* b, size_t bn, size_t sb, size_t rows) {
+    if (!overlap(a, reach(0, rows, sa, an) * 4, b, reach(0, rows, sb, bn) * 4)) return false;
+    if (rows == 1 || sa != sb) return true;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), s = sa * 4;
+    const uintptr_t d = x <= y ? (y - x) % s : (s - (x - y) % s) % s;  // where b's row begins in a's stride
+    return d < an * 4 || d + bn * 4 > s;
+}
 
 }  // namespace
 
@@ -1353,6 +1362,9 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
                       overlap(k + k_off, reach(0, rows, k_stride, nk) * 4, o, on) ||
                       overlap(v + v_off, reach(0, rows, v_stride, nk) * 4, o, on)))
             return refuse("rotated queries that overlap a source but are not their own");
+        if (same && (rows_overlap(q + q_off, n, q_stride, k + k_off, nk, k_stride, rows) ||
+                     rows_overlap(q + q_off, n, q_stride, v + v_off, nk, v_stride, rows)))
+            return refuse("queries rotated in place that lie over k's or v's rows");
         a.q = q + q_off;
         a.qo = const_cast<char*>(o);
     }
