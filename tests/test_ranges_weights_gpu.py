@@ -54,3 +54,34 @@ def test_decode_keeps_what_many_small_weights_add(gpu, shape, gap, softcap, n, n
         tol = want * (ref.U * (8 * top + 16 * softcap + 4 * n + 8) + 2.0 ** -22 + small)
         for i in range(s, nseq, 3):
             close(got[i], want, tol, (s, i))
+
+
+@pytest.mark.parametrize("softcap", [0.0, 100.0])
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("shape", [(128, 1, 128), (256, 1, 64)])
+@pytest.mark.parametrize("keys", [2 ** 15, 2 ** 17])
+def test_prompts_keep_what_many_small_weights_add(gpu, shape, gap, softcap, keys):
+    """Rows enough that no launch cuts the keys: every row's own key, in its first tile, has nearly all the weight, and
+    its value is 0. Allowed, of the context (all of it the other keys'): a half step of f16's smallest for each weight,
+    2^-25 and as many binades down as the keys are doublings of 2^13, of the largest weight; the scores' 4 u |s| nats,
+    the cap's 16 u c; h of each weight and of the output; sums over n keys, u each, of O and of l."""
+    heads, kv, hd = shape
+    rows = hd
+    past = keys - rows
+    g = torch.Generator().manual_seed(keys)
+    k = torch.zeros(1, kv, keys, hd, dtype=torch.float16)
+    v = (1.0 + torch.rand(1, kv, keys, hd, generator=g)).to(torch.float16)
+    q = torch.zeros(rows, heads, hd, dtype=torch.float16)
+    for r in range(rows):
+        q[r, :, r], k[0, 0, past + r, r], v[0, 0, past + r] = 1.0, gap, 0.0
+    got = gpu.flash_attn_ranges(q.cuda().view(-1), 0, heads * hd, cache_of(k, v), 0, gpu.key_ranges(rows, past), rows, past,
+                                heads, 1.0, softcap)
+    top = softcap * math.tanh(gap / softcap) if softcap else gap
+    others = torch.arange(past, keys).double()  # keys before a row's own
+    want = v[0, 0].double().sum(0)[None] / (math.exp(top) + others[:, None])
+    small = 2.0 ** -25 * 2.0 ** 13 / keys * math.exp(top)
+    tol = want * (small + 2 * ref.H + ref.U * (8 * top + 16 * softcap + 2 * keys)) + 2.0 ** -25
+    got = got.view(rows, heads, hd).cpu()
+    for h in (0, heads // 2, heads - 1):
+        close(got[:, h].contiguous(), want, tol, h)
+    assert torch.equal(got, got[:, :1].expand_as(got))

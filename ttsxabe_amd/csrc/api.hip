@@ -1227,6 +1227,21 @@ size_t range_room(size_t blocks) {
     return (size_t)compute_units() * (blocks >= RD_LONG ? 12 : blocks >= RD_TWO ? 3 : 2);
 }
 
+// Binades that a prompt's row forms its largest weight above 1. A weight's
+// rounding to f16 is at most 2^-25 where it is small, 2^(-25 - lift) of the
+// largest: over 2^13 keys 2^-12 of it, half of a weight's own rounding, and each
+// doubling of the keys wants one more. (At 0, a key 25 binades above 2^17 others,
+// with its tile the first, rounded all of them away, 0.4 % of the context.) Not seen
+// in the time where it is wanted, us at 0 / so: 1000 rows of 32/8/128 behind 31000 593 / 593
+// (2), behind 130000 2444 / 2437 (4), capped 2982 / 2985. More than that costs: lifted
+// rows leave f16's range sooner, and a tile that moves the reference is formed twice
+// (8192 rows at 0 / 5 / 8 / 11 490 / 496 / 507 / 517, capped 585 / 590 / 595 / 613).
+float range_lift(size_t keys) {
+    int lift = 0;
+    while (lift < 10 && keys > (size_t)1 << (13 + lift)) ++lift;
+    return (float)lift;
+}
+
 int rotary_checks(size_t hd, size_t rot, float theta, float mscale, size_t rows, size_t heads, size_t pos_len,
                   bool has_pos, size_t first, bool has_div, size_t div_len) {
     if (hd % 2 != 0 || hd == 0) return fail(LLMTIE_ODD_HEAD_DIM, hd, 0, 0, 0, "a rotary head of odd width %zu", hd);
@@ -1450,6 +1465,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
     a.cap = (int)cap;
     a.scale = scale;
     a.softcap = softcap;
+    a.lift = range_lift(past + tq);
     a.gb = gb;
     a.splits = (int)splits;
     a.ws = ws;

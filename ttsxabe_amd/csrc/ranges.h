@@ -27,6 +27,7 @@ struct RangesArgs {
     long q_stride;
     int tq, past, heads, kv_heads, cap;
     float scale, softcap;   // softcap 0: none
+    float lift;             // binades that a row's largest weight is formed above 1 (0 to 10)
     int gb;                 // query heads of a workgroup (1, 2 or 4)
     int splits;             // runs of a row block's tiles (1: whole)
     float* ws;              // splits > 1: splits * tq * heads * (hd + 2) floats

@@ -137,6 +137,7 @@ struct RangeTile {
     half8 pb[2][NQT];
     float mul, add;  // a logit (log2 units) is mul * (what logits() leaves) + add + the bias
     float kc;        // SM_CAP: 2 log2(e) scale / c
+    float lift;      // a row's reference is set so far below its largest score
     float slope2;    // SM_BIAS: slope * log2(e)
     int grp, lane;
 
@@ -175,6 +176,7 @@ struct RangeTile {
         last = ktot - 1;
         mul = a.scale * LLMTIE_LOG2E;
         add = 0.0f;
+        lift = a.lift;
         if constexpr ((MODE & SM_CAP) != 0) {
             kc = 2.0f * LLMTIE_LOG2E * (a.scale / a.softcap);
             add = a.softcap * LLMTIE_LOG2E;
@@ -322,11 +324,13 @@ struct RangeTile {
     __device__ __forceinline__ float side(int kv0) const { return kv0 >= pos0 + QPW - 1 ? -slope2 : slope2; }
 
     // The online softmax of the tile in log2 units. P = 2^(s - m) is formed
-    // against the row's reference max m, which moves only when a weight passes
-    // 2^15 (a key 15 above m, or the first one seen): O and l carry the same
-    // factor, so O / l does not depend on where m sits, P stays inside f16, and
-    // the tile's max is taken on the rare tiles that move m. P is rounded to f16
-    // for the product (2^-11 of each weight, as the f16 context's own rounding);
+    // against the row's reference m, which moves only when a weight passes 2^15
+    // (a key 15 above m, or the first one seen), to `lift` below the row's
+    // largest score: O and l carry the same factor, so O / l does not depend on
+    // where m sits, P stays inside f16, and the tile's max is taken on the rare
+    // tiles that move m. P is rounded to f16 for the product (2^-11 of each
+    // weight, as the f16 context's own rounding, and at most 2^-25 where it is
+    // small: 2^(-25 - lift) of the largest, which over all keys is 2^-12 of it);
     // l is the sum of the rounded weights at f32, by the matrix unit (a product
     // with ones in values()): 16 additions a row and lane less, beside a
     // packed maximum that watches for 2^15.
@@ -380,7 +384,8 @@ struct RangeTile {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             mx = fmaxf(mx, logit(sc[hf][T][u][r], 32 * hf + 4 * T + r, at));
-                const float mn = fmaxf(m[u], max4grp(mx));
+                mx = max4grp(mx);
+                const float mn = fmaxf(m[u], fabsf(mx) < 0x1p23f ? mx - lift : mx);
                 const float fac = ex2(m[u] - mn);
                 m[u] = mn;
                 l[u] *= fac;
