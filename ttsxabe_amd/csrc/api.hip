@@ -1513,10 +1513,12 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     const size_t splits = std::max<size_t>(1, std::min(std::min((blocks + span - 1) / span, most), runs));
     if (smul(units, splits) > MAX_WGS) return overrun_slice(smul(units, splits), MAX_WGS);
     const size_t parts = smul(units, splits, n / kv_heads);
-    // Room for the runs of any smaller batch under this bound too (they can be
-    // more): one eager call of the largest sizes a scratch for captured ones.
-    const size_t floats = smul(std::max(smul(units, splits), range_room(blocks)), group, head_dim + 2);
-    if (int r = ensure_scratch(scratch, floats, smul(units, CTR_STRIDE), S(stream))) return r;
+    // An eager call makes room for the runs of any smaller batch under its bound too
+    // (they can be more): one of the largest sizes a scratch for captured ones.
+    const size_t row = smul(group, head_dim + 2);
+    if (int r = ensure_scratch(scratch, smul(units, splits, row), smul(units, CTR_STRIDE), S(stream),
+                               smul(range_room(blocks), row)))
+        return r;
     RangesDecodeArgs a{};
     a.q = q + q_off;
     a.cache = cache;
