@@ -163,8 +163,9 @@ class LlamaBatch:
 
     def _check(self, slots, new, ids):
         # (An id past the embedding ends the process from the device.)
-        if any(not 0 <= t < len(self.w["embed"]) for t in ids):
-            raise InvalidArgument(f"a token that is not one of {len(self.w['embed'])}")
+        vocab = len(self.w["embed"])
+        if ids and not (min(ids) >= 0 and max(ids) < vocab):
+            raise InvalidArgument(f"a token that is not one of {vocab}")
         if len(set(slots)) < len(slots) or any(not 0 <= s < self.slots for s in slots):
             raise InvalidArgument(f"slots {slots} of {self.slots}")
         for s, n in zip(slots, new):
