@@ -358,7 +358,8 @@ int llmtie_key_ranges(void* stream, const int32_t* starts, size_t starts_len, co
  * plan alone (0: past + tq). ws: a workspace of
  * llmtie_flash_attn_ranges_workspace floats, 16-byte aligned, for launches of
  * few rows over many keys, which are then cut into runs of keys and merged by a
- * second launch (0 floats: not cut; NULL: never cut). It is written and read on
+ * second launch (0 floats, or NULL: not cut). Its size is asked for with the
+ * call's own max_keys, past + tq in place of 0. It is written and read on
  * `stream` by this call alone; concurrent calls need one each. cache and out
  * are 16-byte aligned. */
 size_t llmtie_flash_attn_ranges_workspace(size_t tq, size_t max_keys, size_t heads, size_t kv_heads, size_t head_dim);

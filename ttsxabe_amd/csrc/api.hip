@@ -1440,7 +1440,7 @@ int llmtie_flash_attn_ranges_t16(void* stream, const uint16_t* q, size_t q_len, 
     const size_t group = heads / kv_heads;
     const int gb = group % 4 == 0 ? 4 : (group % 2 == 0 ? 2 : 1);
     const size_t keys = std::min(max_keys ? max_keys : IMAX, past + tq);
-    const size_t splits = ws ? plan_range_splits(tq, keys, heads, kv_heads) : 1;
+    const size_t splits = ws && ws_len ? plan_range_splits(tq, keys, heads, kv_heads) : 1;
     if (splits > 1) {
         const size_t need = smul(smul(splits, tq, heads), head_dim + 2);
         if (ws_len < need) return overrun_slice(need, ws_len);
