@@ -424,6 +424,106 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
                           size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
                           int interleaved, uint16_t* cache, size_t cache_len, size_t slots, size_t cap);
 
+/* ------------------------------------------------ a cache in pages (new)
+ *
+ * No counterpart in the reference. The tiled f16 cache with its slots taken as
+ * pages of `page` positions (a power of two from 32 to 4096; llmtie_t16_cache_len(..,
+ * page) halves each): a sequence lies where row t of a table says, table[t *
+ * table_cols + p] being the page of its positions p * page .. (device int32, of
+ * table_rows rows; entries behind a sequence's last page are not read). At most
+ * 2^30 positions a sequence. Query rows are a token of each sequence, or rows of
+ * prompts: row r is at position tk_dev[r] - 1 of table row row_dev[r] (row_dev NULL:
+ * row r) and sees some of the tk_dev[r] first positions. A row that sees no key gets
+ * zeros; one whose table row does not exist, or that needs a page the cache does not
+ * have, NaN. Keys that a row does not see contribute nothing, whatever they hold.
+ * Lengths, tables and rows may change between replays of captured calls. Scores
+ * are those of the key ranges above, with the same bounds of their arguments. */
+
+/* llmtie_t16_rope_store into pages: row r to position index[r] of table row
+ * seq[r]. Rows whose table row, position or page does not exist store nothing. */
+int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
+                            size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
+                            size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
+                            size_t v_stride, const int32_t* pos, const int32_t* seq, const int32_t* index,
+                            size_t index_len, const int32_t* table, size_t table_len, size_t table_rows,
+                            size_t table_cols, const float* freq_div, size_t div_len, size_t rows, size_t heads,
+                            size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
+                            int interleaved, uint16_t* cache, size_t cache_len, size_t pages, size_t page);
+
+/* The plan of a step's attention, made once for all its layers (plan: device
+ * int32, llmtie_page_plan_len of them, written on `stream`; read by the calls it
+ * is for). Row r of nseq sees of its first tk_dev[r] positions the first `shared`
+ * ones and those from max(lo_dev[r], tk_dev[r] - window) on (lo_dev NULL: 0; window
+ * 0: none). Rows starts[g] up to starts[g + 1] (device, groups + 1 entries, never
+ * decreasing; groups 0: none) promise that their tables' rows name the same pages
+ * for positions below prefix[g]: what all of them see of these is then read and
+ * attended once for up to 32 / (heads / kv_heads) rows together. A prefix counts in
+ * whole blocks of 32 positions and no further than the shortest row's length. max_tk is the
+ * longest length or near it (it says which launch is made; longer rows are attended too).
+ * GQA groups up to 16, at most 1024 groups and 2^20 rows. */
+size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads);
+int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev, const int32_t* lo_dev, size_t nseq,
+                     const int32_t* starts, const int32_t* prefix, size_t groups, size_t max_tk, size_t window,
+                     size_t shared, size_t table_rows, size_t table_cols, size_t page, size_t heads, size_t kv_heads,
+                     size_t head_dim, int32_t* plan, size_t plan_len);
+
+/* Attention of nseq query rows (f32, row r at q[q_off + r * q_stride ..], magnitudes
+ * up to 65504) over what the plan says; plan, tk_dev and the sizes are those that
+ * it was made with (rows are NaN under a plan of other sizes). ws: a workspace of
+ * llmtie_attn_paged_workspace floats, 16-byte aligned, written and read on `stream` by this
+ * call alone. out = [nseq, heads*head_dim] f32, 16-byte aligned as the cache is. */
+size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads,
+                                   size_t head_dim);
+int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                             const uint16_t* cache, size_t cache_len, size_t pages, size_t page, const int32_t* table,
+                             size_t table_len, size_t table_rows, size_t table_cols, const int32_t* tk_dev,
+                             const int32_t* plan, size_t plan_len, size_t nseq, size_t groups, size_t max_tk,
+                             size_t heads, size_t kv_heads, size_t head_dim, float scale, float softcap,
+                             const float* slopes, size_t slopes_len, float* ws, size_t ws_len, float* out,
+                             size_t out_len);
+
+/* The same over `count` pages of each (row, kv head): chosen[(r * kv_heads + h) *
+ * count ..] are numbers of pages within the sequence (device int32, as
+ * llmtie_select_pages leaves them, any order; ones below 0 or with no position that
+ * the row has name nothing, a page named twice counts twice). Row r sees those of
+ * their positions that are below tk_dev[r]. */
+size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
+                                      size_t head_dim);
+int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                                const uint16_t* cache, size_t cache_len, size_t pages, size_t page,
+                                const int32_t* table, size_t table_len, size_t table_rows, size_t table_cols,
+                                const int32_t* tk_dev, const int32_t* row_dev, const int32_t* chosen, size_t chosen_len,
+                                size_t count, size_t nseq, size_t heads, size_t kv_heads, size_t head_dim, float scale,
+                                float softcap, const float* slopes, size_t slopes_len, float* ws, size_t ws_len,
+                                float* out, size_t out_len);
+
+/* The greatest and the least key of pages, dim by dim: bounds[((page * kv_heads +
+ * h) * 2 + 0) * head_dim ..] and [.. + 1 ..] (f16; NaN where a key is) over the positions below tk_dev[r] of
+ * every page of row r's sequence that holds one from low_dev[r] (NULL: 0) up to
+ * tk_dev[r]. Pages without one, and those the cache does not have, are left as they
+ * are. max_new is how many positions that is at most, or near it. No two rows of a
+ * call may give one page different lengths. cache and bounds are 16-byte aligned. */
+int llmtie_page_bounds(void* stream, const uint16_t* cache, size_t cache_len, size_t pages, size_t page,
+                       const int32_t* table, size_t table_len, size_t table_rows, size_t table_cols,
+                       const int32_t* row_dev, const int32_t* low_dev, const int32_t* tk_dev, size_t nseq,
+                       size_t max_new, size_t kv_heads, size_t head_dim, uint16_t* bounds, size_t bounds_len);
+
+/* The `count` pages of its sequence that each (row, kv head) attends: the first
+ * `first` and the last `last` ones, and of the others those with the largest
+ *   max over the heads of the kv head of  sum_d max(q_d, 0) greatest_d + min(q_d, 0) least_d,
+ * which no product of those heads with a key of the page exceeds; formed in f64, a NaN
+ * as +inf (and a page that the cache does not have), ties to the lowest number.
+ * chosen [nseq, kv_heads, count] in rising order, -1 behind the last where the
+ * sequence has fewer. Lengths are clamped to the pages of max_tk. ws:
+ * llmtie_select_pages_workspace doubles, 16-byte aligned, as the attention's. */
+size_t llmtie_select_pages_workspace(size_t nseq, size_t max_tk, size_t page, size_t count, size_t kv_heads);
+int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                        const uint16_t* bounds, size_t bounds_len, size_t pages, size_t page, const int32_t* table,
+                        size_t table_len, size_t table_rows, size_t table_cols, const int32_t* tk_dev,
+                        const int32_t* row_dev, size_t nseq, size_t max_tk, size_t heads, size_t kv_heads,
+                        size_t head_dim, size_t count, size_t first, size_t last, double* ws, size_t ws_len,
+                        int32_t* chosen, size_t chosen_len);
+
 #ifdef __cplusplus
 }
 #endif

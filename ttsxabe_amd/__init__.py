@@ -14,7 +14,8 @@ __version__ = "0.1.0"
 def __getattr__(name):
     # The torch-facing host mirror is imported lazily so that building the
     # library does not need torch.
-    if name in ("Gpu", "DecodeScratch", "Q8", "KvCacheQ8", "TiledCache16", "KeyRanges", "rope_scaling", "gpu"):
+    if name in ("Gpu", "DecodeScratch", "Q8", "KvCacheQ8", "TiledCache16", "KeyRanges", "rope_scaling", "PagedCache16",
+                "PagePlan", "gpu"):
         # (`from . import gpu` would ask this function for the module first.)
         _g = importlib.import_module(".gpu", __name__)
         return _g if name == "gpu" else getattr(_g, name)

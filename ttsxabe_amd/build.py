@@ -20,7 +20,7 @@ LIB = PKG / "libllmtie_hip.so"
 # library so the attention ABI stays the reference's operators only.
 PEAKS_LIB = PKG / "libllmtie_peaks.so"
 PEAKS_SRC = "peaks.hip"
-SOURCES = ["api.hip", "decode.hip", "prefill.hip", "kvcache.hip", "ranges.hip", "rotary.hip"]
+SOURCES = ["api.hip", "decode.hip", "prefill.hip", "kvcache.hip", "ranges.hip", "rotary.hip", "paged.hip", "pages.hip"]
 ARCH = "gfx950"
 # Packed-FP32 instructions stay off (they have given silent wrong results on
 # this pool); -O3 would otherwise form them from ordinary float code.

@@ -18,6 +18,7 @@
 #include "decode.h"
 #include "kvlayout.h"
 #include "kvcache.h"
+#include "paged.h"
 #include "prefill.h"
 #include "ranges.h"
 #include "rotary.h"
@@ -1273,6 +1274,104 @@ bool rows_overlap(const float* a, size_t an, size_t sa, const float* b, size_t b
     return d < an * 4 || d + bn * 4 > s;
 }
 
+// A page table [rows][cols], and whether there is one.
+struct TableArg {
+    const int32_t* ids = nullptr;
+    size_t len = 0, rows = 0, cols = 0;
+    bool given = false;
+};
+int page_shift(size_t page) {
+    int s = 0;
+    while (((size_t)1 << s) < page) ++s;
+    return s;
+}
+// Positions fit an int with room to spare, pages are whole blocks.
+int table_checks(const TableArg& t, size_t page) {
+    if (page < 32 || page > 4096 || (page & (page - 1)) != 0) return refuse("a page that is not a power of two from 32 to 4096");
+    if (int r = over_int(t.rows, t.cols)) return r;
+    if (smul(t.cols, page) > (size_t)1 << 30) return overrun_slice(smul(t.cols, page), (size_t)1 << 30);
+    if (t.len < smul(t.rows, t.cols)) return overrun_slice(smul(t.rows, t.cols), t.len);
+    return LLMTIE_OK;
+}
+
+int rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
+               size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
+               size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
+               size_t v_stride, const int32_t* pos, const int32_t* slot, const int32_t* index,
+               size_t index_len, const float* freq_div, size_t div_len, size_t rows, size_t heads,
+               size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
+               int interleaved, uint16_t* cache, size_t cache_len, size_t slots, size_t cap, const TableArg& table) {
+    if (!(head_dim == 64 || head_dim == 128) || kv_heads == 0) return unsupported(head_dim, heads, kv_heads);
+    if (int r = rotary_checks(head_dim, rot_dim, theta, mscale, rows, std::max(heads, kv_heads), index_len, true, 0,
+                              freq_div != nullptr, div_len))
+        return r;
+    if (int r = over_int(cap, slots, kv_heads)) return r;
+    if (table.given)
+        if (int r = table_checks(table, cap)) return r;
+    const size_t need = smul(slots, llmtie_t16_cache_len(kv_heads, head_dim, cap));
+    if (cache_len < need) return overrun_slice(need, cache_len);
+    const size_t n = smul(heads, head_dim), nk = smul(kv_heads, head_dim);
+    const size_t es = q_out_f16 ? 2 : 4;
+    if (q) {
+        if (rows > 1 && (q_stride < n || q_out_stride < n)) return overrun_slice(n, std::min(q_stride, q_out_stride));
+        if (reach(q_off, rows, q_stride, n) > q_len) return overrun_slice(reach(q_off, rows, q_stride, n), q_len);
+        if (reach(q_out_off, rows, q_out_stride, n) > q_out_len)
+            return overrun_slice(reach(q_out_off, rows, q_out_stride, n), q_out_len);
+    }
+    if (rows > 1 && (k_stride < nk || v_stride < nk)) return overrun_slice(nk, std::min(k_stride, v_stride));
+    if (reach(k_off, rows, k_stride, nk) > k_len) return overrun_slice(reach(k_off, rows, k_stride, nk), k_len);
+    if (reach(v_off, rows, v_stride, nk) > v_len) return overrun_slice(reach(v_off, rows, v_stride, nk), v_len);
+    if (rows == 0) return ok();
+    if (!k || !v || !pos || !slot || !index || !cache || (q && !q_out) || (table.given && !table.ids))
+        return invalid("a buffer");
+    if (off16(cache)) return refuse("a cache off 16 bytes");
+    RotaryArgs a{};
+    if (q && heads) {
+        const char* o = static_cast<char*>(q_out) + q_out_off * es;
+        const size_t on = reach(0, rows, q_out_stride, n) * es;
+        const bool same =
+            !q_out_f16 && o == reinterpret_cast<const char*>(q + q_off) && (q_stride == q_out_stride || rows == 1);
+        if (!same && (overlap(q + q_off, reach(0, rows, q_stride, n) * 4, o, on) ||
+                      overlap(k + k_off, reach(0, rows, k_stride, nk) * 4, o, on) ||
+                      overlap(v + v_off, reach(0, rows, v_stride, nk) * 4, o, on)))
+            return refuse("rotated queries that overlap a source but are not their own");
+        if (same && (rows_overlap(q + q_off, n, q_stride, k + k_off, nk, k_stride, rows) ||
+                     rows_overlap(q + q_off, n, q_stride, v + v_off, nk, v_stride, rows)))
+            return refuse("queries rotated in place that lie over k's or v's rows");
+        a.q = q + q_off;
+        a.qo = const_cast<char*>(o);
+    }
+    a.k = k + k_off;
+    a.v = v + v_off;
+    a.pos = pos;
+    a.slot = slot;
+    a.index = index;
+    a.div = freq_div;
+    a.cache = cache;
+    a.q_stride = rows > 1 ? (long)q_stride : 0;
+    a.qo_stride = rows > 1 ? (long)q_out_stride : 0;
+    a.k_stride = rows > 1 ? (long)k_stride : 0;
+    a.v_stride = rows > 1 ? (long)v_stride : 0;
+    a.rows = (int)rows;
+    a.heads = (int)heads;
+    a.kv = (int)kv_heads;
+    a.hd = (int)head_dim;
+    a.rot = (int)rot_dim;
+    a.interleaved = interleaved ? 1 : 0;
+    a.qo_f16 = q_out_f16 ? 1 : 0;
+    a.slots = (int)slots;
+    a.cap = (int)cap;
+    a.mscale = mscale;
+    a.log2_theta = std::log2((double)theta);
+    if (table.given) {
+        a.table = table.ids;
+        a.trows = (int)table.rows;
+        a.tcols = (int)table.cols;
+        a.shift = page_shift(cap);
+    }
+    return launched(table.given ? "paged_rope_store" : "t16_rope_store", launch_rotary(a, true, S(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1346,66 +1445,9 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
                           size_t index_len, const float* freq_div, size_t div_len, size_t rows, size_t heads,
                           size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
                           int interleaved, uint16_t* cache, size_t cache_len, size_t slots, size_t cap) {
-    if (!(head_dim == 64 || head_dim == 128) || kv_heads == 0) return unsupported(head_dim, heads, kv_heads);
-    if (int r = rotary_checks(head_dim, rot_dim, theta, mscale, rows, std::max(heads, kv_heads), index_len, true, 0,
-                              freq_div != nullptr, div_len))
-        return r;
-    if (int r = over_int(cap, slots, kv_heads)) return r;
-    const size_t need = smul(slots, llmtie_t16_cache_len(kv_heads, head_dim, cap));
-    if (cache_len < need) return overrun_slice(need, cache_len);
-    const size_t n = smul(heads, head_dim), nk = smul(kv_heads, head_dim);
-    const size_t es = q_out_f16 ? 2 : 4;
-    if (q) {
-        if (rows > 1 && (q_stride < n || q_out_stride < n)) return overrun_slice(n, std::min(q_stride, q_out_stride));
-        if (reach(q_off, rows, q_stride, n) > q_len) return overrun_slice(reach(q_off, rows, q_stride, n), q_len);
-        if (reach(q_out_off, rows, q_out_stride, n) > q_out_len)
-            return overrun_slice(reach(q_out_off, rows, q_out_stride, n), q_out_len);
-    }
-    if (rows > 1 && (k_stride < nk || v_stride < nk)) return overrun_slice(nk, std::min(k_stride, v_stride));
-    if (reach(k_off, rows, k_stride, nk) > k_len) return overrun_slice(reach(k_off, rows, k_stride, nk), k_len);
-    if (reach(v_off, rows, v_stride, nk) > v_len) return overrun_slice(reach(v_off, rows, v_stride, nk), v_len);
-    if (rows == 0) return ok();
-    if (!k || !v || !pos || !slot || !index || !cache || (q && !q_out)) return invalid("a buffer");
-    if (off16(cache)) return refuse("a cache off 16 bytes");
-    RotaryArgs a{};
-    if (q && heads) {
-        const char* o = static_cast<char*>(q_out) + q_out_off * es;
-        const size_t on = reach(0, rows, q_out_stride, n) * es;
-        const bool same =
-            !q_out_f16 && o == reinterpret_cast<const char*>(q + q_off) && (q_stride == q_out_stride || rows == 1);
-        if (!same && (overlap(q + q_off, reach(0, rows, q_stride, n) * 4, o, on) ||
-                      overlap(k + k_off, reach(0, rows, k_stride, nk) * 4, o, on) ||
-                      overlap(v + v_off, reach(0, rows, v_stride, nk) * 4, o, on)))
-            return refuse("rotated queries that overlap a source but are not their own");
-        if (same && (rows_overlap(q + q_off, n, q_stride, k + k_off, nk, k_stride, rows) ||
-                     rows_overlap(q + q_off, n, q_stride, v + v_off, nk, v_stride, rows)))
-            return refuse("queries rotated in place that lie over k's or v's rows");
-        a.q = q + q_off;
-        a.qo = const_cast<char*>(o);
-    }
-    a.k = k + k_off;
-    a.v = v + v_off;
-    a.pos = pos;
-    a.slot = slot;
-    a.index = index;
-    a.div = freq_div;
-    a.cache = cache;
-    a.q_stride = rows > 1 ? (long)q_stride : 0;
-    a.qo_stride = rows > 1 ? (long)q_out_stride : 0;
-    a.k_stride = rows > 1 ? (long)k_stride : 0;
-    a.v_stride = rows > 1 ? (long)v_stride : 0;
-    a.rows = (int)rows;
-    a.heads = (int)heads;
-    a.kv = (int)kv_heads;
-    a.hd = (int)head_dim;
-    a.rot = (int)rot_dim;
-    a.interleaved = interleaved ? 1 : 0;
-    a.qo_f16 = q_out_f16 ? 1 : 0;
-    a.slots = (int)slots;
-    a.cap = (int)cap;
-    a.mscale = mscale;
-    a.log2_theta = std::log2((double)theta);
-    return launched("t16_rope_store", launch_rotary(a, true, S(stream)));
+    return rope_store(stream, q, q_len, q_off, q_stride, q_out, q_out_len, q_out_off, q_out_stride, q_out_f16, k, k_len,
+                      k_off, k_stride, v, v_len, v_off, v_stride, pos, slot, index, index_len, freq_div, div_len, rows,
+                      heads, kv_heads, head_dim, rot_dim, theta, mscale, interleaved, cache, cache_len, slots, cap, {});
 }
 
 size_t llmtie_flash_attn_ranges_workspace(size_t tq, size_t max_keys, size_t heads, size_t kv_heads, size_t head_dim) {
@@ -1545,6 +1587,317 @@ int llmtie_attn_decode_ranges_t16(void* stream, const float* q, size_t q_len, si
     a.scale = scale;
     a.softcap = softcap;
     return launched("attn_decode_ranges", launch_ranges_decode((int)head_dim, a, S(stream)));
+}
+
+}  // extern "C"
+
+// -------------------------------------------------------- a cache in pages
+
+namespace {
+
+constexpr size_t PG_MAX_ROWS = (size_t)1 << 20;
+
+// How a step over pages is divided, from what the host knows of it.
+struct PagedSizes {
+    size_t target, max_shared, max_own;
+    bool whole;
+};
+// Items of a kv head: two workgroups a compute unit. Rows that no group shares
+// anything of and whose bound is short are one item each.
+PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
+    PagedSizes s;
+    s.target = std::max<size_t>(1, 2 * (size_t)compute_units() / kv_heads);
+    s.whole = groups == 0 && (max_tk + 31) / 32 <= (size_t)RD_WHOLE;
+    s.max_own = s.whole ? nseq : nseq + s.target;
+    s.max_shared = groups ? nseq / (size_t)PG_TILE_ROWS((int)(heads / kv_heads)) + groups + s.target : 0;
+    return s;
+}
+int paged_checks(size_t nseq, size_t groups, size_t max_tk, const TableArg& t, size_t page, size_t heads, size_t kv_heads,
+                 size_t head_dim) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16)
+        return unsupported(head_dim, heads, kv_heads);
+    if (int r = table_checks(t, page)) return r;
+    if (int r = over_int(smul(heads, head_dim))) return r;
+    if (max_tk == 0 || max_tk > smul(t.cols, page)) return overrun_cache(max_tk, smul(t.cols, page));
+    if (nseq > PG_MAX_ROWS) return overrun_slice(nseq, PG_MAX_ROWS);
+    if (groups > (size_t)PG_GROUPS) return overrun_slice(groups, PG_GROUPS);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const size_t wgs = smul(sadd(z.max_shared, z.max_own), kv_heads);
+    if (wgs > MAX_WGS) return overrun_slice(wgs, MAX_WGS);
+    return LLMTIE_OK;
+}
+size_t paged_floats(const PagedSizes& z, size_t heads, size_t kv_heads, size_t head_dim) {
+    return smul(sadd(smul(z.max_own, heads), smul(z.max_shared, PG_COLS, kv_heads)), head_dim + 2);
+}
+Pages pages_of(const uint16_t* cache, const TableArg& t, size_t pages, size_t page) {
+    return Pages{cache, t.ids, (int)t.rows, (int)t.cols, page_shift(page), (int)pages};
+}
+
+// Workgroups of a (row, kv head) over its selected pages: those that fill the
+// compute units once, of four blocks or more.
+size_t selected_runs(size_t units, size_t blocks) {
+    return std::max<size_t>(1, std::min((blocks + 3) / 4, (size_t)compute_units() / std::max<size_t>(1, units)));
+}
+
+// Queries of nseq rows, a cache of pages, the context.
+int query_checks(const float* q, size_t q_len, size_t q_off, size_t q_stride, size_t nseq, size_t n, size_t out_len,
+                 size_t cache_len, size_t pages, size_t page, size_t kv_heads, size_t head_dim) {
+    if (int r = over_int(pages)) return r;
+    const size_t need = smul(pages, llmtie_t16_cache_len(kv_heads, head_dim, page));
+    if (cache_len < need) return overrun_slice(need, cache_len);
+    if (nseq > 1 && q_stride < n) return overrun_slice(n, q_stride);
+    if (reach(q_off, nseq, q_stride, n) > q_len) return overrun_slice(reach(q_off, nseq, q_stride, n), q_len);
+    if (out_len < smul(nseq, n)) return overrun_slice(smul(nseq, n), out_len);
+    return LLMTIE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
+                            size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
+                            size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
+                            size_t v_stride, const int32_t* pos, const int32_t* seq, const int32_t* index,
+                            size_t index_len, const int32_t* table, size_t table_len, size_t table_rows,
+                            size_t table_cols, const float* freq_div, size_t div_len, size_t rows, size_t heads,
+                            size_t kv_heads, size_t head_dim, size_t rot_dim, float theta, float mscale,
+                            int interleaved, uint16_t* cache, size_t cache_len, size_t pages, size_t page) {
+    return rope_store(stream, q, q_len, q_off, q_stride, q_out, q_out_len, q_out_off, q_out_stride, q_out_f16, k, k_len,
+                      k_off, k_stride, v, v_len, v_off, v_stride, pos, seq, index, index_len, freq_div, div_len, rows,
+                      heads, kv_heads, head_dim, rot_dim, theta, mscale, interleaved, cache, cache_len, pages, page,
+                      TableArg{table, table_len, table_rows, table_cols, true});
+}
+
+size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
+    if (kv_heads == 0 || heads == 0 || heads % kv_heads != 0 || heads / kv_heads > 16 || nseq > PG_MAX_ROWS) return 0;
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const size_t rows = smul(nseq, PG_ROW);
+    return sadd(sadd(PG_HEAD + rows, rows % 16), smul(sadd(z.max_shared, z.max_own), PG_ITEM));
+}
+
+int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev, const int32_t* lo_dev, size_t nseq,
+                     const int32_t* starts, const int32_t* prefix, size_t groups, size_t max_tk, size_t window,
+                     size_t shared, size_t table_rows, size_t table_cols, size_t page, size_t heads, size_t kv_heads,
+                     size_t head_dim, int32_t* plan, size_t plan_len) {
+    const TableArg t{nullptr, SIZE_MAX, table_rows, table_cols, true};
+    if (int r = paged_checks(nseq, groups, max_tk, t, page, heads, kv_heads, head_dim)) return r;
+    if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
+    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, heads, kv_heads);
+    if (plan_len < need) return overrun_slice(need, plan_len);
+    if (nseq == 0) return ok();
+    if (!tk_dev || !plan || (groups && (!starts || !prefix))) return invalid("a buffer");
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    PagePlanArgs a{};
+    a.tk = tk_dev;
+    a.row = row_dev;
+    a.lo = lo_dev;
+    a.starts = groups ? starts : nullptr;
+    a.prefix = prefix;
+    a.plan = plan;
+    a.nseq = (int)nseq;
+    a.groups = (int)groups;
+    a.window = (int)std::min(window, IMAX);
+    a.shared = (int)std::min(shared, IMAX);
+    a.rows = (int)table_rows;
+    a.cols = (int)table_cols;
+    a.shift = page_shift(page);
+    a.group = (int)(heads / kv_heads);
+    a.kv_heads = (int)kv_heads;
+    a.max_shared = (int)z.max_shared;
+    a.max_own = (int)z.max_own;
+    a.target = (int)z.target;
+    a.whole = z.whole ? 1 : 0;
+    return launched("page_plan", launch_page_plan(a, S(stream)));
+}
+
+size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads,
+                                   size_t head_dim) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16 || nseq == 0 || nseq > PG_MAX_ROWS)
+        return 0;
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    return z.whole ? 0 : paged_floats(z, heads, kv_heads, head_dim);
+}
+
+int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                             const uint16_t* cache, size_t cache_len, size_t pages, size_t page, const int32_t* table,
+                             size_t table_len, size_t table_rows, size_t table_cols, const int32_t* tk_dev,
+                             const int32_t* plan, size_t plan_len, size_t nseq, size_t groups, size_t max_tk,
+                             size_t heads, size_t kv_heads, size_t head_dim, float scale, float softcap,
+                             const float* slopes, size_t slopes_len, float* ws, size_t ws_len, float* out,
+                             size_t out_len) {
+    const TableArg t{table, table_len, table_rows, table_cols, true};
+    if (int r = paged_checks(nseq, groups, max_tk, t, page, heads, kv_heads, head_dim)) return r;
+    if (int r = score_checks(scale, softcap, slopes, slopes_len, heads)) return r;
+    const size_t n = smul(heads, head_dim);
+    if (int r = query_checks(q, q_len, q_off, q_stride, nseq, n, out_len, cache_len, pages, page, kv_heads, head_dim))
+        return r;
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, heads, kv_heads);
+    if (plan_len < need) return overrun_slice(need, plan_len);
+    const size_t floats = z.whole ? 0 : paged_floats(z, heads, kv_heads, head_dim);
+    if (nseq == 0) return ok();
+    if (ws_len < floats) return overrun_slice(floats, ws_len);
+    if (!q || !cache || !table || !tk_dev || !plan || !out || (floats && !ws)) return invalid("a buffer");
+    if (off16(cache) || off16(out) || off16(ws)) return refuse("a cache, a context or a workspace off 16 bytes");
+    PagedArgs a{};
+    a.p = pages_of(cache, t, pages, page);
+    a.q = q + q_off;
+    a.out = out;
+    a.tk = tk_dev;
+    a.slopes = slopes;
+    a.plan = plan;
+    a.part = ws;
+    a.q_stride = nseq > 1 ? (long)q_stride : 0;
+    a.nseq = (int)nseq;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads);
+    a.max_shared = (int)z.max_shared;
+    a.max_own = (int)z.max_own;
+    a.runs = 1;
+    a.stream = groups == 0 && smul(smul(nseq, kv_heads), (max_tk + 31) / 32, 128 * head_dim) > RD_STREAM_BYTES;
+    a.merge = z.whole ? 0 : 1;
+    a.scale = scale;
+    a.softcap = softcap;
+    return launched("attn_decode_paged", launch_paged((int)head_dim, a, S(stream)));
+}
+
+size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
+                                      size_t head_dim) {
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || nseq == 0) return 0;
+    const size_t runs = selected_runs(smul(nseq, kv_heads), smul(count, (page + 31) / 32));
+    return runs > 1 ? smul(smul(nseq, heads, runs), head_dim + 2) : 0;
+}
+
+int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                                const uint16_t* cache, size_t cache_len, size_t pages, size_t page,
+                                const int32_t* table, size_t table_len, size_t table_rows, size_t table_cols,
+                                const int32_t* tk_dev, const int32_t* row_dev, const int32_t* chosen, size_t chosen_len,
+                                size_t count, size_t nseq, size_t heads, size_t kv_heads, size_t head_dim, float scale,
+                                float softcap, const float* slopes, size_t slopes_len, float* ws, size_t ws_len,
+                                float* out, size_t out_len) {
+    const TableArg t{table, table_len, table_rows, table_cols, true};
+    if (int r = paged_checks(nseq, 0, 1, t, page, heads, kv_heads, head_dim)) return r;
+    if (int r = score_checks(scale, softcap, slopes, slopes_len, heads)) return r;
+    const size_t n = smul(heads, head_dim), units = smul(nseq, kv_heads);
+    if (int r = query_checks(q, q_len, q_off, q_stride, nseq, n, out_len, cache_len, pages, page, kv_heads, head_dim))
+        return r;
+    if (smul(count, page) > (size_t)1 << 30) return overrun_slice(smul(count, page), (size_t)1 << 30);
+    if (chosen_len < smul(units, count)) return overrun_slice(smul(units, count), chosen_len);
+    if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
+    if (nseq == 0) return ok();
+    const size_t runs = selected_runs(units, smul(count, page / 32));
+    if (smul(units, runs) > MAX_WGS) return overrun_slice(smul(units, runs), MAX_WGS);
+    const size_t floats = llmtie_attn_selected_workspace(nseq, count, page, heads, kv_heads, head_dim);
+    if (ws_len < floats) return overrun_slice(floats, ws_len);
+    if (!q || !cache || !table || !tk_dev || (count && !chosen) || !out || (floats && !ws)) return invalid("a buffer");
+    if (off16(cache) || off16(out) || off16(ws)) return refuse("a cache, a context or a workspace off 16 bytes");
+    PagedArgs a{};
+    a.p = pages_of(cache, t, pages, page);
+    a.q = q + q_off;
+    a.out = out;
+    a.tk = tk_dev;
+    a.row = row_dev;
+    a.chosen = chosen;
+    a.slopes = slopes;
+    a.part = ws;
+    a.q_stride = nseq > 1 ? (long)q_stride : 0;
+    a.nseq = (int)nseq;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads);
+    a.max_own = (int)(nseq * runs);
+    a.count = (int)count;
+    a.runs = (int)runs;
+    a.merge = runs > 1 ? 1 : 0;
+    a.scale = scale;
+    a.softcap = softcap;
+    return launched("attn_decode_selected", launch_paged((int)head_dim, a, S(stream)));
+}
+
+int llmtie_page_bounds(void* stream, const uint16_t* cache, size_t cache_len, size_t pages, size_t page,
+                       const int32_t* table, size_t table_len, size_t table_rows, size_t table_cols,
+                       const int32_t* row_dev, const int32_t* low_dev, const int32_t* tk_dev, size_t nseq,
+                       size_t max_new, size_t kv_heads, size_t head_dim, uint16_t* bounds, size_t bounds_len) {
+    if (!llmtie_supports_flash(head_dim, kv_heads, kv_heads)) return unsupported(head_dim, kv_heads, kv_heads);
+    const TableArg t{table, table_len, table_rows, table_cols, true};
+    if (int r = table_checks(t, page)) return r;
+    if (int r = over_int(pages, smul(kv_heads, head_dim))) return r;
+    const size_t need = smul(pages, llmtie_t16_cache_len(kv_heads, head_dim, page));
+    if (cache_len < need) return overrun_slice(need, cache_len);
+    const size_t want = smul(pages, smul(2, kv_heads, head_dim));
+    if (bounds_len < want) return overrun_slice(want, bounds_len);
+    if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
+    // Pages that so many new positions touch at most; more are taken in turn.
+    const size_t per = std::min(table_cols, sadd(std::min(max_new, (size_t)1 << 30) / page, 2));
+    const size_t waves = smul(smul(nseq, per), kv_heads, head_dim / 32);
+    if (waves / 4 >= MAX_WGS) return overrun_slice(waves / 4, MAX_WGS);
+    if (nseq == 0 || per == 0 || pages == 0) return ok();
+    if (!cache || !table || !tk_dev || !bounds) return invalid("a buffer");
+    if (off16(cache) || off16(bounds)) return refuse("a cache or bounds off 16 bytes");
+    PageBoundsArgs a{};
+    a.p = pages_of(cache, t, pages, page);
+    a.row = row_dev;
+    a.low = low_dev;
+    a.tk = tk_dev;
+    a.bounds = bounds;
+    a.nseq = (int)nseq;
+    a.kv_heads = (int)kv_heads;
+    a.per = (int)per;
+    return launched("page_bounds", launch_page_bounds((int)head_dim, a, S(stream)));
+}
+
+size_t llmtie_select_pages_workspace(size_t nseq, size_t max_tk, size_t page, size_t count, size_t kv_heads) {
+    if (page == 0) return 0;
+    const size_t wide = max_tk / page + (max_tk % page != 0);
+    return wide > count ? smul(nseq, kv_heads, wide) : 0;
+}
+
+int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
+                        const uint16_t* bounds, size_t bounds_len, size_t pages, size_t page, const int32_t* table,
+                        size_t table_len, size_t table_rows, size_t table_cols, const int32_t* tk_dev,
+                        const int32_t* row_dev, size_t nseq, size_t max_tk, size_t heads, size_t kv_heads,
+                        size_t head_dim, size_t count, size_t first, size_t last, double* ws, size_t ws_len,
+                        int32_t* chosen, size_t chosen_len) {
+    const TableArg t{table, table_len, table_rows, table_cols, true};
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16)
+        return unsupported(head_dim, heads, kv_heads);
+    if (int r = table_checks(t, page)) return r;
+    if (int r = over_int(smul(heads, head_dim), pages, count)) return r;
+    if (max_tk == 0 || max_tk > smul(table_cols, page)) return overrun_cache(max_tk, smul(table_cols, page));
+    if (count == 0 || sadd(first, last) > count) return refuse("fewer pages to select than are always kept, or none");
+    const size_t want = smul(pages, smul(2, kv_heads, head_dim)), n = smul(heads, head_dim), units = smul(nseq, kv_heads);
+    if (bounds_len < want) return overrun_slice(want, bounds_len);
+    if (nseq > 1 && q_stride < n) return overrun_slice(n, q_stride);
+    if (reach(q_off, nseq, q_stride, n) > q_len) return overrun_slice(reach(q_off, nseq, q_stride, n), q_len);
+    if (chosen_len < smul(units, count)) return overrun_slice(smul(units, count), chosen_len);
+    if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
+    if (sadd(units, 512) > MAX_WGS) return overrun_slice(units, MAX_WGS - 512);
+    const size_t need = llmtie_select_pages_workspace(nseq, max_tk, page, count, kv_heads);
+    if (ws_len < need) return overrun_slice(need, ws_len);
+    if (nseq == 0) return ok();
+    if (!q || !bounds || !table || !tk_dev || !chosen || (need && !ws)) return invalid("a buffer");
+    if (off16(bounds) || off16(ws)) return refuse("bounds or a workspace off 16 bytes");
+    SelectArgs a{};
+    a.q = q + q_off;
+    a.bounds = bounds;
+    a.table = table;
+    a.row = row_dev;
+    a.tk = tk_dev;
+    a.chosen = chosen;
+    a.score = ws;
+    a.q_stride = nseq > 1 ? (long)q_stride : 0;
+    a.nseq = (int)nseq;
+    a.kv_heads = (int)kv_heads;
+    a.group = (int)(heads / kv_heads);
+    a.rows = (int)table_rows;
+    a.cols = (int)table_cols;
+    a.shift = page_shift(page);
+    a.pages = (int)pages;
+    a.count = (int)count;
+    a.first = (int)first;
+    a.last = (int)last;
+    a.wide = (int)((max_tk + page - 1) / page);
+    return launched("select_pages", launch_select((int)head_dim, a, S(stream)));
 }
 
 }  // extern "C"

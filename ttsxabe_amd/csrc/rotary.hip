@@ -108,10 +108,16 @@ struct Unit {
 };
 
 // Block of row r's place for kv head kh, its position in it in kk; null for a
-// padding row.
+// padding row. PAGED: the row names a table row and a position of its sequence.
+template <bool PAGED>
 __device__ __forceinline__ half_t* home(const RotaryArgs& a, int r, int kh, int& kk) {
-    const int s = a.slot[r], i = a.index[r];
+    int s = a.slot[r], i = a.index[r];
     kk = i & 31;
+    if constexpr (PAGED) {
+        if (s < 0 || s >= a.trows || i < 0 || i >> a.shift >= a.tcols) return nullptr;
+        s = a.table[(size_t)s * a.tcols + (i >> a.shift)];
+        i &= a.cap - 1;
+    }
     if (s < 0 || s >= a.slots || i < 0 || i >= a.cap) return nullptr;
     return reinterpret_cast<half_t*>(a.cache) +
            (((size_t)s * a.kv + kh) * tiled_nblk(a.cap) + (i >> 5)) * (64 * (size_t)a.hd);
@@ -128,10 +134,10 @@ __device__ __forceinline__ void put_q(const RotaryArgs& a, int r, int h, const U
         st_vec<V>(static_cast<float*>(a.qo) + at + x.d1, x.y.x);
     }
 }
-template <int V>
+template <bool PAGED, int V>
 __device__ __forceinline__ void put_k(const RotaryArgs& a, int r, int h, const Unit<V>& x) {
     int kk;
-    half_t* b = home(a, r, h, kk);
+    half_t* b = home<PAGED>(a, r, h, kk);
     if (!b) return;
     st_vec<V>(b + t16_k_off(a.hd, kk, x.d0), x.x.x);
     st_vec<V>(b + t16_k_off(a.hd, kk, x.d1), x.y.x);
@@ -142,7 +148,7 @@ __device__ __forceinline__ void put_k(const RotaryArgs& a, int r, int h, const U
 // heads of 128 46.9 -> 42.5 us, 6.3 TB/s of reads and writes; with 96 of 128
 // dims rotated 54 -> 43; a turn of 127 4.9 -> 4.2. Loading two units a thread
 // before the angles took 30 registers more and was no faster: 45, 45.9, 4.6.)
-template <int V, bool STORE>
+template <int V, bool STORE, bool PAGED>
 __device__ __forceinline__ void row(const RotaryArgs& a, int r, int h0, int h1, float2* cs, int tid) {
     const int units = a.hd / (2 * V), nh = a.q ? a.heads : 0;
     const int t1 = min(h1, nh + (STORE ? a.kv : 0)), n = max(0, t1 - h0) * units;  // units to rotate
@@ -152,7 +158,7 @@ __device__ __forceinline__ void row(const RotaryArgs& a, int r, int h0, int h1, 
     };
     auto put = [&](int h, const Unit<V>& x) __attribute__((always_inline)) {
         if (!STORE || h < nh) put_q<V>(a, r, h, x);
-        else put_k<V>(a, r, h - nh, x);
+        else put_k<PAGED>(a, r, h - nh, x);
     };
     if (n > 0) {
         angles<1>(a, r, cs, tid);
@@ -177,7 +183,7 @@ __device__ __forceinline__ void row(const RotaryArgs& a, int r, int h0, int h1, 
                 for (int c = 0; c < V; ++c) x[i + c] = y.x[c];
             }
             int kk;
-            half_t* b = home(a, r, h, kk);
+            half_t* b = home<PAGED>(a, r, h, kk);
             if (!b) continue;
 #pragma unroll
             for (int i = 0; i < 4; ++i) b[32 * a.hd + t16_v_off(kk, d + i)] = to_h(x[i]);
@@ -191,7 +197,7 @@ __device__ __forceinline__ void row(const RotaryArgs& a, int r, int h0, int h1, 
 // the first row's cache position, so a run's rows do. Us, with k and v by row /
 // so: 4000 rows of 32/8/128 50.6 / 31.5 (147 MB; a copy of them 28.6), 1999 24.6 /
 // 16.0, 500 10.2 / 7.3, 100 5.0 / 5.1, 64 4.9 / 4.8; rows of a place each 32 4.5 / 6.5.
-template <int V>
+template <int V, bool PAGED>
 __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h1, float2* cs, int tid) {
     const int units = a.hd / (2 * V), half = a.rot / 2, k1 = min(h1, a.kv);
     if (h0 < k1) {
@@ -203,7 +209,7 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
             if (r < 0 || r >= a.rows) continue;
             Unit<V> x(a, a.k + (size_t)r * a.k_stride + (size_t)h * a.hd, u);
             x.turn(a, cs + p * half, u);
-            put_k<V>(a, r, h, x);
+            put_k<PAGED>(a, r, h, x);
         }
     }
     const int v0 = max(h0, a.kv);
@@ -211,7 +217,9 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
     bool run = r0 >= 0 && r0 + 8 <= a.rows;
     if (run) {
         const int s = a.slot[r0], i = a.index[r0];
-        run = (i & 7) == 0 && s >= 0 && s < a.slots && i >= 0 && i < a.cap - 7;
+        int kk;  // (a run of eight lies in one page)
+        run = (i & 7) == 0 && (PAGED ? home<PAGED>(a, r0, 0, kk) != nullptr
+                                     : s >= 0 && s < a.slots && i >= 0 && i < a.cap - 7);
         for (int p = 1; p < 8 && run; ++p) run = a.slot[r0 + p] == s && a.index[r0 + p] == i + p;
     }
     const int quads = a.hd / 4;
@@ -231,7 +239,7 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
         }
         int kk;
         if (run) {
-            half_t* b = home(a, r0, h, kk) + 32 * a.hd;
+            half_t* b = home<PAGED>(a, r0, h, kk) + 32 * a.hd;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 half8 y;
@@ -245,7 +253,7 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
         for (int p = 0; p < 8; ++p) {
             const int r = r0 + p;
             if (r < 0 || r >= a.rows) continue;
-            half_t* b = home(a, r, h, kk);
+            half_t* b = home<PAGED>(a, r, h, kk);
             if (!b) continue;
 #pragma unroll
             for (int i = 0; i < 4; ++i) b[32 * a.hd + t16_v_off(kk, d + i)] = to_h(x[p][i]);
@@ -256,7 +264,7 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
 // GROUPS: the first `g8` workgroups take k and v eight rows at a time, the
 // others q by row; else all by row. Rows past a launch's workgroups follow at
 // its stride.
-template <int V, bool STORE, bool GROUPS>
+template <int V, bool STORE, bool GROUPS, bool PAGED>
 __global__ __launch_bounds__(RO) void rotary_kernel(RotaryArgs a, int g8, int hpb8, int groups, int hpb, int heads) {
     extern __shared__ float2 cs[];
     const int tid = threadIdx.x;
@@ -264,14 +272,14 @@ __global__ __launch_bounds__(RO) void rotary_kernel(RotaryArgs a, int g8, int hp
         if ((int)blockIdx.x < g8) {
             const int per = (2 * a.kv + hpb8 - 1) / hpb8, g = (int)blockIdx.x / per, h0 = (int)blockIdx.x % per * hpb8;
             const int shift = a.index[0] & 7;
-            rows8<V>(a, 8 * g - shift, h0, min(2 * a.kv, h0 + hpb8), cs, tid);
+            rows8<V, PAGED>(a, 8 * g - shift, h0, min(2 * a.kv, h0 + hpb8), cs, tid);
             return;
         }
     }
     const int per = (heads + hpb - 1) / hpb, b = (int)blockIdx.x - (GROUPS ? g8 : 0);
     const int h0 = b % per * hpb, stride = ((int)gridDim.x - (GROUPS ? g8 : 0)) / per;
     for (int r = b / per; r < groups; r += stride) {
-        row<V, STORE && !GROUPS>(a, r, h0, min(heads, h0 + hpb), cs, tid);
+        row<V, STORE && !GROUPS, PAGED>(a, r, h0, min(heads, h0 + hpb), cs, tid);
         __syncthreads();  // the angles are read
     }
 }
@@ -300,12 +308,14 @@ hipError_t launch_rotary(const RotaryArgs& a, bool store, hipStream_t st) {
     const int rows = std::min(a.rows, 1 << 16);
     const dim3 grid((unsigned)(g8 + rows * per));
     const size_t lds = (size_t)(groups ? 8 : 1) * (a.rot / 2) * sizeof(float2);
-#define RO_(V, S, G)                                                                                              \
-    if ((vec ? 4 : 1) == V && store == S && groups == G) {                                                        \
-        hipLaunchKernelGGL((rotary_kernel<V, S, G>), grid, dim3(RO), lds, st, a, g8, hpb8, a.rows, hpb, heads);   \
+#define RO_(V, S, G, P)                                                                                           \
+    if ((vec ? 4 : 1) == V && store == S && groups == G && (a.table != nullptr) == P) {                           \
+        hipLaunchKernelGGL((rotary_kernel<V, S, G, P>), grid, dim3(RO), lds, st, a, g8, hpb8, a.rows, hpb, heads);   \
         return hipGetLastError();                                                                                 \
     }
-    RO_(4, false, false) RO_(4, true, false) RO_(4, true, true) RO_(1, false, false) RO_(1, true, false) RO_(1, true, true)
+    RO_(4, false, false, false) RO_(4, true, false, false) RO_(4, true, true, false) RO_(1, false, false, false)
+    RO_(1, true, false, false) RO_(1, true, true, false)
+    RO_(4, true, false, true) RO_(4, true, true, true) RO_(1, true, false, true) RO_(1, true, true, true)
 #undef RO_
     return hipErrorInvalidValue;
 }

@@ -27,7 +27,7 @@ __all__ = [
     "SplitHeadLost",
     "DecodeScratch",
     "Q8", "KvCacheQ8",
-    "TiledCache16", "KeyRanges", "rope_scaling", "Gpu",
+    "TiledCache16", "KeyRanges", "rope_scaling", "PagedCache16", "PagePlan", "Gpu",
 ]
 
 
@@ -234,6 +234,40 @@ class KeyRanges:
     table: torch.Tensor
     pos: torch.Tensor | None = None
     max_keys: int = 0
+
+
+class PagedCache16(TiledCache16):
+    """A tiled f16 cache for one layer in `pages` pages of `page` positions (a
+    power of two from 32 to 4096), which are its slots. A sequence's positions lie
+    where a row of a table (int32 [rows, pages of the longest]) says."""
+
+    def __init__(self, kv_heads: int, head_dim: int, pages: int, page: int, device="cuda", zero=True):
+        super().__init__(kv_heads, head_dim, page, device=device, zero=zero, slots=pages)
+        self.pages, self.page = pages, page
+
+    @classmethod
+    def of(cls, data, kv_heads: int, head_dim: int, pages: int, page: int):
+        """A cache over memory that the caller holds."""
+        self = super().of(data, kv_heads, head_dim, page, slots=pages)
+        self.pages, self.page = pages, page
+        return self
+
+
+@dataclass
+class PagePlan:
+    """What Gpu.page_plan made of a step's rows, for the attention of all layers: the
+    rows' lengths and tables, which it holds on to, and how the work is divided."""
+
+    data: torch.Tensor
+    tk: torch.Tensor
+    table: torch.Tensor
+    heads: int
+    kv_heads: int
+    head_dim: int
+    page: int
+    groups: int
+    max_tk: int
+    floats: int  # of the attention's workspace
 
 
 def rope_scaling(rot_dim: int, theta: float, kind: str = "none", factor: float = 1.0, original: int = 8192,
@@ -718,3 +752,171 @@ class Gpu:
                   heads, cache.kv_heads, cache.head_dim, cache.cap, scale, softcap, _p(slopes), _n(slopes),
                   scratch.handle, out.data_ptr(), out.numel())
         return out if out.numel() == n else out[:n]
+
+    # ------------------------------------------------------ a cache in pages
+
+    def _table(self, table):
+        """A page table's address, elements, rows and columns."""
+        self._on(table, _I32, "table")
+        if table.dim() != 2:
+            raise InvalidArgument("a table that is not [rows, pages]")
+        return table.data_ptr(), table.numel(), table.shape[0], table.shape[1]
+
+    def _room(self, n, dtype=torch.float32):
+        return torch.empty(n, dtype=dtype, device=self.device) if n else None
+
+    def paged_rope_store(self, q, q_off, k, k_off, v, v_off, stride, pos, seq, index, table, freq_div, rows, heads,
+                         rot_dim, theta, mscale, interleaved, cache: PagedCache16, q_out=None, q_out_off=0,
+                         q_out_stride=None):
+        """t16_rope_store into pages (new): row r to position index[r] of the
+        sequence whose pages are table[seq[r]]."""
+        self._on(k, _F32, "k")
+        self._on(v, _F32, "v")
+        f16 = 0
+        if q is None:
+            q_out_stride = 0
+        else:
+            self._on(q, _F32, "q")
+            if q_out is None:
+                q_out, q_out_off, q_out_stride = q, q_off, stride
+            else:
+                self._on(q_out, _F32 + _H16, "q_out")
+                f16 = 0 if q_out.dtype is torch.float32 else 1
+                if q_out_stride is None:
+                    q_out_stride = heads * cache.head_dim
+        for t, what in ((pos, "pos"), (seq, "seq"), (index, "index")):
+            self._on(t, _I32, what, rows)
+        self._on(freq_div, _F32, "freq_div", rot_dim // 2)
+        self._on(cache.data, _H16, "cache")
+        if min(q_off, k_off, v_off, stride, rows, heads, rot_dim, q_out_off, q_out_stride) < 0:
+            raise InvalidArgument("a negative count")
+        self._run(self._L.llmtie_paged_rope_store, _p(q), _n(q), q_off, stride, _p(q_out), _n(q_out), q_out_off,
+                  q_out_stride, f16, k.data_ptr(), k.numel(), k_off, stride, v.data_ptr(), v.numel(), v_off, stride,
+                  pos.data_ptr(), seq.data_ptr(), index.data_ptr(), rows, *self._table(table), _p(freq_div),
+                  _n(freq_div), rows, heads, cache.kv_heads, cache.head_dim, rot_dim, theta, mscale,
+                  1 if interleaved else 0, cache.data.data_ptr(), cache.data.numel(), cache.pages, cache.page)
+
+    def page_plan(self, tk_dev, row_dev, table, heads, cache: PagedCache16, max_tk, starts=None, prefix=None,
+                  lo_dev=None, window=0, shared=0) -> PagePlan:
+        """The plan of a step's attention for all its layers (new; see
+        llmtie_page_plan): len(tk_dev) rows, row r at position tk_dev[r] - 1 of the
+        sequence of table[row_dev[r]] (None: table[r]), which sees the first `shared`
+        positions and those from max(lo_dev, tk - window) on; rows starts[g] ..
+        starts[g + 1] - 1 hold positions below prefix[g] in the same pages."""
+        n = tk_dev.numel()
+        self._on(tk_dev, _I32, "tk")
+        self._on(row_dev, _I32, "row", n)
+        self._on(lo_dev, _I32, "lo", n)
+        groups = 0
+        if starts is not None:
+            self._on(starts, _I32, "starts", 1)
+            groups = starts.numel() - 1
+            if groups and prefix is None:
+                raise InvalidArgument("groups without their prefixes")
+            self._on(prefix, _I32, "prefix", groups)
+        elif prefix is not None:
+            raise InvalidArgument("prefixes without their groups")
+        _, _, rows, cols = self._table(table)
+        if min(max_tk, heads, window, shared) < 0:
+            raise InvalidArgument("a negative count")
+        kv, hd = cache.kv_heads, cache.head_dim
+        size = self._L.llmtie_page_plan_len(n, groups, max_tk, heads, kv)
+        plan = torch.empty(size, dtype=torch.int32, device=self.device)
+        self._run(self._L.llmtie_page_plan, tk_dev.data_ptr(), _p(row_dev), _p(lo_dev), n, _p(starts), _p(prefix), groups,
+                  max_tk, window, shared, rows, cols, cache.page, heads, kv, hd, plan.data_ptr(), size)
+        floats = self._L.llmtie_attn_paged_workspace(n, groups, max_tk, heads, kv, hd)
+        return PagePlan(plan, tk_dev, table, heads, kv, hd, cache.page, groups, max_tk, floats)
+
+    def attn_decode_paged(self, q, q_off, q_stride, cache: PagedCache16, plan: PagePlan, heads, scale, softcap=0.0,
+                          slopes=None, out=None):
+        """Attention of the plan's rows over their pages (new), what a group's rows
+        share once for all of them, scores as in flash_attn_ranges. Returns the f32
+        context [rows * heads * head_dim]."""
+        data, hd, kv, nseq = cache.data, cache.head_dim, cache.kv_heads, plan.tk.numel()
+        self._on(q, _F32, "q")
+        self._on(data, _H16, "cache")
+        self._on(plan.data, _I32, "plan")
+        self._on(slopes, _F32, "slopes", heads)
+        if (heads, kv, hd, cache.page) != (plan.heads, plan.kv_heads, plan.head_dim, plan.page):
+            raise InvalidArgument("a plan of other heads or pages")
+        if min(q_off, q_stride) < 0:
+            raise InvalidArgument("a negative count")
+        n = nseq * heads * hd
+        if out is None:
+            out = torch.empty(n, dtype=torch.float32, device=self.device)
+        else:
+            self._on(out, _F32, "out")
+        ws = self._room(plan.floats)
+        self._run(self._L.llmtie_attn_decode_paged, q.data_ptr(), q.numel(), q_off, q_stride, data.data_ptr(),
+                  data.numel(), cache.pages, cache.page, *self._table(plan.table), plan.tk.data_ptr(),
+                  plan.data.data_ptr(), plan.data.numel(), nseq, plan.groups, plan.max_tk, heads, kv, hd, scale, softcap,
+                  _p(slopes), _n(slopes), _p(ws), plan.floats, out.data_ptr(), out.numel())
+        return out if out.numel() == n else out[:n]
+
+    def attn_decode_selected(self, q, q_off, q_stride, cache: PagedCache16, table, row_dev, tk_dev, chosen, heads, scale,
+                             softcap=0.0, slopes=None, out=None):
+        """attn_decode_paged over the pages `chosen` (int32 [rows, kv_heads, count],
+        as select_pages returns them) of each row and kv head (new)."""
+        data, hd, kv, nseq = cache.data, cache.head_dim, cache.kv_heads, tk_dev.numel()
+        self._on(q, _F32, "q")
+        self._on(data, _H16, "cache")
+        self._on(tk_dev, _I32, "tk")
+        self._on(row_dev, _I32, "row", nseq)
+        self._on(chosen, _I32, "chosen")
+        self._on(slopes, _F32, "slopes", heads)
+        if chosen.dim() != 3 or chosen.shape[0] != nseq or chosen.shape[1] != kv:
+            raise InvalidArgument(f"pages chosen for {tuple(chosen.shape)}, not for [{nseq}, {kv}, ..]")
+        if min(q_off, q_stride, heads) < 0:
+            raise InvalidArgument("a negative count")
+        count, n = chosen.shape[2], nseq * heads * hd
+        if out is None:
+            out = torch.empty(n, dtype=torch.float32, device=self.device)
+        else:
+            self._on(out, _F32, "out")
+        floats = self._L.llmtie_attn_selected_workspace(nseq, count, cache.page, heads, kv, hd)
+        ws = self._room(floats)
+        self._run(self._L.llmtie_attn_decode_selected, q.data_ptr(), q.numel(), q_off, q_stride, data.data_ptr(),
+                  data.numel(), cache.pages, cache.page, *self._table(table), tk_dev.data_ptr(), _p(row_dev),
+                  chosen.data_ptr(), chosen.numel(), count, nseq, heads, kv, hd, scale, softcap, _p(slopes), _n(slopes),
+                  _p(ws), floats, out.data_ptr(), out.numel())
+        return out if out.numel() == n else out[:n]
+
+    def page_bounds(self, cache: PagedCache16, table, row_dev, low_dev, tk_dev, max_new, bounds):
+        """The greatest and the least key (f16 `bounds` [pages, kv_heads, 2, head_dim])
+        of the pages that hold positions low_dev[r] (None: 0) to tk_dev[r] of each
+        row's sequence, over its live positions; max_new of them or so (new)."""
+        nseq = tk_dev.numel()
+        self._on(cache.data, _H16, "cache")
+        self._on(tk_dev, _I32, "tk")
+        self._on(row_dev, _I32, "row", nseq)
+        self._on(low_dev, _I32, "low", nseq)
+        self._on(bounds, _H16, "bounds")
+        if max_new < 0:
+            raise InvalidArgument("a negative count")
+        self._run(self._L.llmtie_page_bounds, cache.data.data_ptr(), cache.data.numel(), cache.pages, cache.page,
+                  *self._table(table), _p(row_dev), _p(low_dev), tk_dev.data_ptr(), nseq, max_new, cache.kv_heads,
+                  cache.head_dim, bounds.data_ptr(), bounds.numel())
+
+    def select_pages(self, q, q_off, q_stride, bounds, table, row_dev, tk_dev, max_tk, heads, page, count, first=1,
+                     last=1):
+        """The `count` pages that each row and kv head attends (new): the first `first`
+        and `last` last ones and those whose `bounds` (page_bounds) allow the largest
+        product with one of its heads. Returns int32 [rows, kv_heads, count], rising,
+        -1 behind the last."""
+        nseq = tk_dev.numel()
+        self._on(q, _F32, "q")
+        self._on(bounds, _H16, "bounds")
+        self._on(tk_dev, _I32, "tk")
+        self._on(row_dev, _I32, "row", nseq)
+        if bounds.dim() != 4 or bounds.shape[2] != 2:
+            raise InvalidArgument("bounds that are not [pages, kv_heads, 2, head_dim]")
+        pages, kv, _, hd = bounds.shape
+        if min(q_off, q_stride, max_tk, heads, page, count, first, last) < 0:
+            raise InvalidArgument("a negative count")
+        chosen = torch.empty((nseq, kv, count), dtype=torch.int32, device=self.device)
+        room = self._L.llmtie_select_pages_workspace(nseq, max_tk, page, count, kv)
+        ws = self._room(room, torch.float64)
+        self._run(self._L.llmtie_select_pages, q.data_ptr(), q.numel(), q_off, q_stride, bounds.data_ptr(),
+                  bounds.numel(), pages, page, *self._table(table), tk_dev.data_ptr(), _p(row_dev), nseq, max_tk, heads,
+                  kv, hd, count, first, last, _p(ws), room, chosen.data_ptr(), chosen.numel())
+        return chosen
