@@ -408,7 +408,7 @@ def _kernels(s):
                            s["div"], n, heads, c["rot"], THETA, s["m"], c["pairs"] == "interleaved", s["paged"], q_out=q)
         return {"q": q, "cache": s["cache"]}
     if c["kind"] == "select":
-        return g.select_pages(s["q"], 0, heads * hd, s["bounds"], s["table"], s["row"], s["tk"], c["high"], heads,
+        return g.select_pages(s["q"], 0, heads * hd, s["bounds"], s["table"], s["row"], s["tk"], max(_ends(c)[0]), heads,
                               c["page"], c["count"], first=c["first"], last=c["last"])
     if c["kind"] == "decode":
         plan = s["plan"] if c["plan"] == "kept" else _plan(s)
