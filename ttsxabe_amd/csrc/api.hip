@@ -1599,17 +1599,21 @@ constexpr size_t PG_MAX_ROWS = (size_t)1 << 20;
 
 // How a step over pages is divided, from what the host knows of it.
 struct PagedSizes {
-    size_t target, max_shared, max_own;
+    size_t target, max_shared, max_own, items;
     bool whole;
 };
-// Items of a kv head: two workgroups a compute unit. Rows that no group shares
-// anything of and whose bound is short are one item each.
+// Items of a kv head: two workgroups a compute unit, fewer where the rows do not
+// hold four blocks for each. Rows that no group shares anything of and whose bound is
+// short are one item each.
 PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
     PagedSizes s;
-    s.target = std::max<size_t>(1, 2 * (size_t)compute_units() / kv_heads);
-    s.whole = groups == 0 && (max_tk + 31) / 32 <= (size_t)RD_WHOLE;
+    const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
+    s.target = std::max<size_t>(1, std::min(2 * (size_t)compute_units() / kv_heads, (nseq * blocks + 3) / 4));
+    s.whole = groups == 0 && blocks <= (size_t)RD_WHOLE;
+    const size_t tiles = groups ? nseq / (size_t)PG_TILE_ROWS((int)(heads / kv_heads)) + groups : 0;
     s.max_own = s.whole ? nseq : nseq + s.target;
-    s.max_shared = groups ? nseq / (size_t)PG_TILE_ROWS((int)(heads / kv_heads)) + groups + s.target : 0;
+    s.max_shared = groups ? tiles + s.target : 0;
+    s.items = s.whole ? nseq : nseq + tiles + s.target;
     return s;
 }
 int paged_checks(size_t nseq, size_t groups, size_t max_tk, const TableArg& t, size_t page, size_t heads, size_t kv_heads,
@@ -1687,6 +1691,7 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
     if (plan_len < need) return overrun_slice(need, plan_len);
     if (nseq == 0) return ok();
     if (!tk_dev || !plan || (groups && (!starts || !prefix))) return invalid("a buffer");
+    if (off16(plan)) return refuse("a plan off 16 bytes");
     const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
     PagePlanArgs a{};
     a.tk = tk_dev;
@@ -1754,6 +1759,7 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
     a.group = (int)(heads / kv_heads);
     a.max_shared = (int)z.max_shared;
     a.max_own = (int)z.max_own;
+    a.items = (int)z.items;
     a.runs = 1;
     a.stream = groups == 0 && smul(smul(nseq, kv_heads), (max_tk + 31) / 32, 128 * head_dim) > RD_STREAM_BYTES;
     a.merge = z.whole ? 0 : 1;

@@ -51,6 +51,7 @@ struct PagedArgs {
     long q_stride;
     int nseq, kv_heads, group;
     int max_shared, max_own;
+    int items;           // of a kv head, at most
     int count, runs;     // selected pages: how many, and the workgroups of a (row, kv head)
     int stream;          // more bytes than are worth keeping in the Infinity Cache
     int merge;           // some row may have partials

@@ -358,7 +358,7 @@ __global__ __launch_bounds__(PT, 2) void paged_kernel(PagedArgs a) {
     const int n = a.group * HD;
     const int* d = plan_items(a) + (size_t)PG_ITEM * item;
     if (!plan_fits(a)) {
-        for (int r = item; r < a.nseq; r += (int)(gridDim.x / (unsigned)a.kv_heads))
+        for (int r = item; r < a.nseq; r += a.items)
             fill(a.out + ((size_t)r * a.kv_heads + kh) * n, n, __builtin_nanf(""));
         return;
     }
@@ -409,15 +409,26 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     });
 }
 
-// The context of a (row, kv head) from its parts, in their order: M = max m,
+// The context of a row's query heads from its parts, in their order: M = max m,
 // O = sum 2^(m - M) O / sum 2^(m - M) l. A part in which a row sees no key has m =
-// RG_NOREF and l = 0.
+// RG_NOREF and l = 0. The threads are HD / 4 columns of four dims by phases of
+// the parts, whose loads go out together; a workgroup takes `heads` query heads of
+// a kv head, one where the launch is small (one sequence of 32 parts, all four
+// heads by one thread a column: 12.4 us).
+constexpr int PM_PARTS = 1088;  // parts of a row at most: each side's target and one
+
 template <int HD, bool PLAN>
-__global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {
-    const int kh = (int)(blockIdx.x % (unsigned)a.kv_heads), row = (int)(blockIdx.x / (unsigned)a.kv_heads);
-    const int tid = threadIdx.x;
+__global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a, int heads) {
+    constexpr int C = HD / 4, R = PT / C, U = 4;
+    __shared__ float wt[PM_PARTS];
+    __shared__ floatx4 red[PT];
+    const int per = a.group / heads;
+    const int kh = (int)(blockIdx.x / (unsigned)per % (unsigned)a.kv_heads);
+    const int row = (int)(blockIdx.x / (unsigned)(per * a.kv_heads));
+    const int g0 = (int)(blockIdx.x % (unsigned)per) * heads;
+    const int tid = threadIdx.x, c = tid % C, phase = tid / C, lane = tid & 63;
     int o0 = row * a.runs, on = a.runs, s0 = 0, sn = 0, step = 0, col = 0;
-    float* out = a.out + ((size_t)row * a.kv_heads + kh) * a.group * HD;
+    float* out = a.out + (((size_t)row * a.kv_heads + kh) * a.group + g0) * HD;
     if constexpr (PLAN) {
         if (!plan_fits(a)) return;
         const int* d = a.plan + PG_HEAD + (size_t)PG_ROW * row;
@@ -426,32 +437,55 @@ __global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {
     } else {
         const int table = a.row ? a.row[row] : row;
         if (table < 0 || table >= a.p.rows) {
-            fill(out, a.group * HD, __builtin_nanf(""));
+            fill(out, heads * HD, __builtin_nanf(""));
             return;
         }
     }
-    for (int e4 = tid; e4 < a.group * (HD / 4); e4 += PT) {
-        const int g = e4 / (HD / 4);
+    const int n = min(on + sn, PM_PARTS);
+    for (int g = g0; g < g0 + heads; ++g) {
+        auto part = [&](int i) {
+            Sink p = i < on ? own_part(a, HD, o0 + i, kh) : shared_part(a, HD, s0 + (i - on) * step, kh);
+            const int at = g + (i < on ? 0 : col);
+            p.o += (size_t)at * HD, p.ml += at;
+            return p;
+        };
+        // The first parts' columns are on their way while the weights are formed.
+        floatx4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            x[u] = *reinterpret_cast<const floatx4*>(part(min(phase + u * R, n - 1)).o + 4 * c);
         float M = RG_NOREF, L = 0.0f;
-        floatx4 y = zero_f4();
-        for (int i = 0; i < on + sn; ++i) {
-            const Sink p = i < on ? own_part(a, HD, o0 + i, kh) : shared_part(a, HD, s0 + (i - on) * step, kh);
-            const int c = i < on ? 0 : col;
-            const float2 ml = p.ml[c + g];
-            const floatx4 x = *reinterpret_cast<const floatx4*>(p.o + (size_t)c * HD + 4 * (size_t)e4);
-            const float mn = fmaxf(M, ml.x), f = ex2(M - mn), h = ex2(ml.x - mn);
-            M = mn;
-            L = L * f + ml.y * h;
-            y = y * f + x * h;
+        for (int i = lane; i < n; i += 64) M = fmaxf(M, part(i).ml->x);
+        M = wave_max(M);
+        for (int i = lane; i < n; i += 64) {
+            const float2 ml = *part(i).ml;
+            const float f = ex2(ml.x - M);
+            L += ml.y * f;
+            if (tid < 64) wt[i] = f;
         }
-        *reinterpret_cast<floatx4*>(out + 4 * (size_t)e4) = y * (L > 0.0f || L != L ? 1.0f / L : 0.0f);
+        L = wave_sum(L);
+        __syncthreads();
+        floatx4 y = zero_f4();
+        for (int i = phase; i < n; i += U * R) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (i + u * R < n) y += x[u] * wt[i + u * R];
+                x[u] = *reinterpret_cast<const floatx4*>(part(min(i + (U + u) * R, n - 1)).o + 4 * c);
+            }
+        }
+        red[tid] = y;
+        __syncthreads();
+        if (phase == 0) {
+            for (int k = 1; k < R; ++k) y += red[tid + k * C];
+            *reinterpret_cast<floatx4*>(out + (g - g0) * HD + 4 * c) = y * (L > 0.0f || L != L ? 1.0f / L : 0.0f);
+        }
+        __syncthreads();
     }
 }
 
 hipError_t launch_paged(int hd, const PagedArgs& a, hipStream_t st) {
     const int mode = (a.softcap > 0.0f ? SM_CAP : 0) | (a.slopes ? SM_BIAS : 0);
-    const dim3 rows((unsigned)((size_t)a.nseq * a.kv_heads));
-    const dim3 grid((unsigned)((a.plan ? (size_t)a.max_shared + a.max_own : (size_t)a.nseq * a.runs) * a.kv_heads));
+    const dim3 grid((unsigned)((a.plan ? (size_t)a.items : (size_t)a.nseq * a.runs) * a.kv_heads));
     bool done = false;
 #define PK(HD, M, AUX)                                                                           \
     if (!done && hd == HD && mode == M && (a.stream ? AUX_STREAM : 0) == AUX) {                  \
@@ -465,9 +499,11 @@ hipError_t launch_paged(int hd, const PagedArgs& a, hipStream_t st) {
 #undef PK
     if (!done) return hipErrorInvalidValue;
     if (a.merge) {
+        const int heads = (size_t)a.nseq * a.kv_heads >= 1024 ? a.group : 1;
+        const dim3 rows((unsigned)((size_t)a.nseq * a.kv_heads * (a.group / heads)));
 #define MK(HD, P)                                                                                \
     if (hd == HD && (a.plan != nullptr) == P)                                                    \
-        hipLaunchKernelGGL((paged_merge_kernel<HD, P>), rows, dim3(PT), 0, st, a);
+        hipLaunchKernelGGL((paged_merge_kernel<HD, P>), rows, dim3(PT), 0, st, a, heads);
         MK(64, false) MK(64, true) MK(128, false) MK(128, true)
 #undef MK
     }

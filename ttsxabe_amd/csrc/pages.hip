@@ -14,7 +14,6 @@ namespace llmtie {
 
 // --------------------------------------------------------------------- plan
 
-constexpr int PP = 1024;
 constexpr int PG_SPAN = 4;  // blocks of an item at least: one a wave
 
 // What row r sees: the first f positions and those from lo to tk (f = lo = 0: all).
@@ -49,6 +48,7 @@ struct OwnBlocks {
 };
 
 // The sum of `v` over the threads before this one, and of all in `total`.
+template <int PP>
 __device__ __forceinline__ int scan_before(int v, int* waves, int tid, int& total) {
     int x = v;
 #pragma unroll
@@ -56,38 +56,50 @@ __device__ __forceinline__ int scan_before(int v, int* waves, int tid, int& tota
         const int y = __shfl_up(x, d);
         if ((tid & 63) >= d) x += y;
     }
-    __syncthreads();
     if ((tid & 63) == 63) waves[tid >> 6] = x;
     __syncthreads();
     int before = 0;
     total = 0;
+#pragma unroll
     for (int w = 0; w < PP / 64; ++w) {
         if (w < (tid >> 6)) before += waves[w];
         total += waves[w];
     }
+    __syncthreads();
     return before + x - v;
 }
+
+// A row's group (-1: none), what it sees and its own blocks.
+struct PlanRow {
+    RowSeen s;
+    int g;
+};
 
 // One workgroup. A shared tile is up to PG_COLS columns (rows of a group times a
 // kv head's query heads) over the blocks that all the group's rows see whole and
 // hold in the same pages; what else a row sees is its own tile's. Each tile is
 // cut into items of about the same cost, `target` of them a kv head in all.
+// Bound by its chain of loads and barriers: a row a thread, whose lengths are
+// read once, and few waves where there are few rows.
+template <int PP, bool ONE>
 __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __shared__ int gst[PG_GROUPS + 1], glo[PG_GROUPS], ghi[PG_GROUPS], gat[PG_GROUPS];
     __shared__ int waves[PP / 64];
     __shared__ unsigned long long work;
     const int tid = threadIdx.x;
     const int tile_rows = PG_TILE_ROWS(a.group);
+    const int per = ONE ? 1 : (a.nseq + PP - 1) / PP;
+    const int r0 = min(a.nseq, tid * per), r1 = min(a.nseq, r0 + per);
     int groups = a.starts ? a.groups : 0;
+    PlanRow held{RowSeen(a, min(tid, a.nseq - 1)), -1};
     for (int g = tid; g <= groups && groups; g += PP) gst[g] = max(0, min(a.starts[g], a.nseq));
-    for (int g = tid; g < groups; g += PP) ghi[g] = 0x7fffffff, glo[g] = 0;
+    for (int g = tid; g < groups; g += PP) ghi[g] = a.prefix[g], glo[g] = 0;
     if (tid == 0) work = 0;
     __syncthreads();
     // Starts that decrease: no groups (tiles would lie over one another, more than there is room for).
     int falls = 0;
     for (int g = tid; g < groups; g += PP) falls |= gst[g] > gst[g + 1];
-    if (__syncthreads_or(falls)) groups = 0;
-    // The group of row r, or -1.
+    if (groups && __syncthreads_or(falls)) groups = 0;
     auto group_of = [&](int r) {
         int lo = -1, hi = groups;
         while (hi - lo > 1) {
@@ -97,18 +109,22 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         }
         return lo >= 0 && r < gst[lo + 1] ? lo : -1;
     };
+    if constexpr (ONE) held.g = groups && tid < a.nseq ? group_of(tid) : -1;
+    auto row_of = [&](int r) {
+        if constexpr (ONE) return held;
+        return PlanRow{RowSeen(a, r), groups ? group_of(r) : -1};
+    };
     if (groups) {
-        for (int r = tid; r < a.nseq; r += PP) {
-            const int g = group_of(r);
-            if (g < 0) continue;
-            const RowSeen s(a, r);
-            atomicMin(&ghi[g], s.table < 0 ? 0 : s.tk);
-            atomicMax(&glo[g], s.lo);
+        for (int r = r0; r < r1; ++r) {
+            const PlanRow x = row_of(r);
+            if (x.g < 0) continue;
+            atomicMin(&ghi[x.g], x.s.table < 0 ? 0 : x.s.tk);
+            atomicMax(&glo[x.g], x.s.lo);
         }
         __syncthreads();
         for (int g = tid; g < groups; g += PP) {
             const int n = gst[g + 1] - gst[g];
-            const int lo = (glo[g] + 31) >> 5, hi = max(0, min(a.prefix[g], ghi[g])) >> 5;
+            const int lo = (glo[g] + 31) >> 5, hi = max(0, ghi[g]) >> 5;
             const bool share = !a.whole && n >= 2 && hi > lo;
             glo[g] = share ? lo : 0;
             ghi[g] = share ? hi : 0;
@@ -118,17 +134,9 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         }
         __syncthreads();
     }
-    // (Two binary searches a row: its group is not kept.)
-    auto own_of = [&](int r, RowSeen& s, int& g) {
-        g = groups ? group_of(r) : -1;
-        return OwnBlocks(s, g >= 0 ? glo[g] : 0, g >= 0 ? ghi[g] : 0);
-    };
+    auto own_of = [&](const PlanRow& x) { return OwnBlocks(x.s, x.g >= 0 ? glo[x.g] : 0, x.g >= 0 ? ghi[x.g] : 0); };
     unsigned long long mine = 0;
-    for (int r = tid; r < a.nseq; r += PP) {
-        RowSeen s(a, r);
-        int g;
-        mine += 4ull * (unsigned)own_of(r, s, g).n;
-    }
+    for (int r = r0; r < r1; ++r) mine += 4ull * (unsigned)own_of(row_of(r)).n;
     if (mine) atomicAdd(&work, mine);
     __syncthreads();
     // Cost of an item, four a block (seven of two column tiles).
@@ -136,89 +144,86 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     auto cut = [&](int blocks, int cost) {
         return a.whole ? 1 : (int)(((unsigned long long)blocks * cost + c - 1) / c);
     };
-    int* rows = a.plan + PG_HEAD;
-    int* items = rows + (size_t)PG_ROW * a.nseq + (PG_ROW * (size_t)a.nseq % 16);
+    int4* rows = reinterpret_cast<int4*>(a.plan + PG_HEAD);
+    int4* items = rows + (PG_ROW * (size_t)a.nseq + PG_ROW * (size_t)a.nseq % 16) / 4;
 
     // Shared tiles, a group's runs of blocks outermost, so that its tiles read a run at one time.
     int ns = 0;
-    {
-        const int per = (groups + PP - 1) / PP, g0 = min(groups, tid * per), g1 = min(groups, g0 + per);
-        auto items_of = [&](int g) {
-            if (ghi[g] <= glo[g]) return 0;
-            const int n = gst[g + 1] - gst[g];
-            return (n + tile_rows - 1) / tile_rows * cut(ghi[g] - glo[g], min(n, tile_rows) * a.group > 16 ? 7 : 4);
-        };
+    auto runs_of = [&](int g) {
+        return cut(ghi[g] - glo[g], min(gst[g + 1] - gst[g], tile_rows) * a.group > 16 ? 7 : 4);
+    };
+    auto tiles_of = [&](int g) { return (gst[g + 1] - gst[g] + tile_rows - 1) / tile_rows; };
+    if (groups) {
+        const int each = (groups + PP - 1) / PP, g0 = min(groups, tid * each), g1 = min(groups, g0 + each);
+        auto items_of = [&](int g) { return ghi[g] > glo[g] ? tiles_of(g) * runs_of(g) : 0; };
         int n = 0;
         for (int g = g0; g < g1; ++g) n += items_of(g);
-        int at = groups ? scan_before(n, waves, tid, ns) : 0;
+        int at = scan_before<PP>(n, waves, tid, ns);
         for (int g = g0; g < g1; ++g) gat[g] = at, at += items_of(g);
         __syncthreads();
         ns = min(ns, a.max_shared);
         for (int g = 0; g < groups; ++g) {
             if (ghi[g] <= glo[g]) continue;
-            const int n = gst[g + 1] - gst[g], tiles = (n + tile_rows - 1) / tile_rows;
-            const int nb = ghi[g] - glo[g], runs = cut(nb, min(n, tile_rows) * a.group > 16 ? 7 : 4);
-            const int share = (nb + runs - 1) / runs;
+            const int tiles = tiles_of(g), runs = runs_of(g), nb = ghi[g] - glo[g], share = (nb + runs - 1) / runs;
             for (int i = tid; i < tiles * runs; i += PP) {
                 if (gat[g] + i >= ns) break;
-                const int t = i % tiles, run = i / tiles, r0 = gst[g] + t * tile_rows;
-                const int b = run * share;
-                int* d = items + (size_t)PG_ITEM * (gat[g] + i);
-                d[0] = r0, d[1] = min(tile_rows, gst[g + 1] - r0), d[2] = RowSeen(a, r0).table, d[3] = 0;
-                d[4] = 0, d[5] = glo[g], d[6] = ghi[g], d[7] = ghi[g];
-                d[8] = b, d[9] = min(nb, b + share), d[10] = 0, d[11] = 0, d[12] = 0;
+                const int t = i % tiles, b = i / tiles * share, first = gst[g] + t * tile_rows;
+                const int row = a.row ? a.row[first] : first;
+                int4* d = items + PG_ITEM / 4 * (size_t)(gat[g] + i);
+                d[0] = make_int4(first, min(tile_rows, gst[g + 1] - first), row, 0);
+                d[1] = make_int4(0, glo[g], ghi[g], ghi[g]);
+                d[2] = make_int4(b, min(nb, b + share), 0, 0);
             }
         }
     }
     // Rows and their own items.
-    const int per = (a.nseq + PP - 1) / PP, r0 = min(a.nseq, tid * per), r1 = min(a.nseq, r0 + per);
-    auto items_of = [&](int n, int g) {
-        const bool shares = g >= 0 && ghi[g] > glo[g];
+    auto own_items = [&](const PlanRow& x, int n) {
+        const bool shares = x.g >= 0 && ghi[x.g] > glo[x.g];
         return n ? cut(n, 4) : shares ? 0 : 1;
     };
     int n = 0, no = 0;
     for (int r = r0; r < r1; ++r) {
-        RowSeen s(a, r);
-        int g;
-        const int nb = own_of(r, s, g).n;
-        n += items_of(nb, g);
+        const PlanRow x = row_of(r);
+        n += own_items(x, own_of(x).n);
     }
-    int at = scan_before(n, waves, tid, no);
+    int at = scan_before<PP>(n, waves, tid, no);
     for (int r = r0; r < r1; ++r) {
-        RowSeen s(a, r);
-        int g;
-        const OwnBlocks o = own_of(r, s, g);
-        const bool shares = g >= 0 && ghi[g] > glo[g];
-        const int runs = items_of(o.n, g), share = runs ? (o.n + runs - 1) / runs : 0;
-        int* d = rows + (size_t)PG_ROW * r;
-        d[0] = at, d[1] = runs;
-        d[2] = d[3] = d[4] = d[5] = 0;
+        const PlanRow x = row_of(r);
+        const OwnBlocks o = own_of(x);
+        const bool shares = x.g >= 0 && ghi[x.g] > glo[x.g];
+        const int runs = own_items(x, o.n), share = runs ? (o.n + runs - 1) / runs : 0;
+        int4 d = make_int4(at, runs, 0, 0), e = make_int4(0, 0, 0, 0);
         if (shares) {
-            const int in = r - gst[g], m = gst[g + 1] - gst[g], tiles = (m + tile_rows - 1) / tile_rows;
-            d[2] = gat[g] + in / tile_rows;
-            d[3] = cut(ghi[g] - glo[g], min(m, tile_rows) * a.group > 16 ? 7 : 4);
-            d[4] = tiles;
-            d[5] = in % tile_rows * a.group;
+            const int in = r - gst[x.g];
+            d.z = gat[x.g] + in / tile_rows;
+            d.w = runs_of(x.g);
+            e.x = tiles_of(x.g);
+            e.y = in % tile_rows * a.group;
         }
+        rows[PG_ROW / 4 * (size_t)r] = d;
+        rows[PG_ROW / 4 * (size_t)r + 1] = e;
         for (int i = 0; i < runs; ++i) {
             if (at + i >= a.max_own) break;
-            int* e = items + (size_t)PG_ITEM * (ns + at + i);
-            e[0] = r, e[1] = 1, e[2] = s.table, e[3] = runs == 1 && !shares;
-            e[4] = o.na, e[5] = o.b0, e[6] = o.c0, e[7] = o.d0;
-            e[8] = i * share, e[9] = min(o.n, (i + 1) * share), e[10] = s.f, e[11] = s.lo, e[12] = s.tk;
+            int4* t = items + PG_ITEM / 4 * (size_t)(ns + at + i);
+            t[0] = make_int4(r, 1, x.s.table, runs == 1 && !shares);
+            t[1] = make_int4(o.na, o.b0, o.c0, o.d0);
+            t[2] = make_int4(i * share, min(o.n, (i + 1) * share), x.s.f, x.s.lo);
+            t[3] = make_int4(x.s.tk, 0, 0, 0);
         }
         at += runs;
     }
     if (tid == 0) {
-        int* h = a.plan;
         no = min(no, a.max_own);
-        h[0] = ns + no, h[1] = ns, h[2] = a.nseq, h[3] = a.group, h[4] = a.kv_heads, h[5] = a.shift, h[6] = a.cols;
-        h[7] = a.rows, h[8] = a.max_shared, h[9] = a.max_own, h[10] = a.whole;
+        int4* h = reinterpret_cast<int4*>(a.plan);
+        h[0] = make_int4(ns + no, ns, a.nseq, a.group);
+        h[1] = make_int4(a.kv_heads, a.shift, a.cols, a.rows);
+        h[2] = make_int4(a.max_shared, a.max_own, a.whole, 0);
     }
 }
 
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(PP), 0, st, a);
+    if (a.nseq <= 256) hipLaunchKernelGGL((page_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((page_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, a);
     return hipGetLastError();
 }
 
