@@ -151,7 +151,7 @@ def test_select():
     assert select(bounds_len=8 * 2 * 2 * 128 - 1) == 4 and select(bounds=8) == 10
     assert select(q_len=1023) == 4 and select(q_stride=1) == 4 and select(chosen_len=29) == 4
     need = L.llmtie_select_pages_workspace(3, 1000, 64, 5, 2)
-    assert need == 3 * 2 * 16 and select(ws_len=need - 1) == 4 and select(ws=NULL) == 10
+    assert need >= 3 * 2 * 16 and select(ws_len=need - 1) == 4 and select(ws=NULL) == 10
     assert L.llmtie_select_pages_workspace(3, 1000, 64, 16, 2) == 0  # all are selected
     for name in ("q", "bounds", "tk", "chosen"):
         assert select(**{name: NULL}) == 10, name

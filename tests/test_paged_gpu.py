@@ -575,3 +575,44 @@ def test_streams(gpu):
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("n,units", [(100, 1), (300, 1), (700, 40), (9000, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_select_near_scores(gpu, n, units, hd):
+    """Pages a step of f16 apart in a dim or two: few near the border, many, more than are held, by one workgroup
+    and by several."""
+    heads, kv, page = 4, 2, 32
+    g = torch.Generator().manual_seed(n)
+    one = torch.randn(1, kv, 1, hd, generator=g)
+    bounds = torch.cat([one + 1.0, one - 1.0], 2).to(torch.float16).expand(n, -1, -1, -1).clone()
+    at = torch.randint(0, hd, (n, 2), generator=g)
+    bits = bounds.view(torch.int16)
+    p = torch.arange(n)
+    bits[p, 0, 0, at[:, 0]] += 1
+    bits[p, 1, 1, at[:, 1]] -= 1
+    if n == 700:  # and most of them far
+        bounds[: n // 2] *= 0.5
+    table = torch.randperm(n, generator=g)[None].expand(units, -1)
+    tk = [n * page - r for r in range(units)]
+    q = queries(7, units, heads, hd)
+    want = pr.select(q[:2], bounds, table[:2], list(range(units))[:2], tk, page, 20, 1, 1)
+    got = gpu.select_pages(q.cuda().view(-1), 0, heads * hd, bounds.cuda(), ints(table.tolist()), None, ints(tk),
+                           n * page, heads, page, 20, 1, 1)
+    assert torch.equal(got[:2].cpu(), want)
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1e-30, 1e30])
+def test_select_small_and_large_queries(gpu, scale):
+    heads, kv, hd, page, n = 6, 2, 128, 64, 200
+    g = torch.Generator().manual_seed(3)
+    mid, half = torch.randn(n, kv, 1, hd, generator=g), torch.randn(n, kv, 1, hd, generator=g).abs()
+    bounds = torch.cat([mid + half, mid - half], 2).to(torch.float16)
+    bounds[5] *= 1000.0
+    table = torch.arange(n)[None]
+    q = queries(7, 1, heads, hd) * scale
+    q[0, 1] *= 1e-6
+    want = pr.select(q, bounds, table, [0], [n * page], page, 30, 0, 1)
+    got = gpu.select_pages(q.cuda().view(-1), 0, heads * hd, bounds.cuda(), ints(table.tolist()), None, ints([n * page]),
+                           n * page, heads, page, 30, 0, 1)
+    assert torch.equal(got.cpu(), want)

@@ -1626,7 +1626,7 @@ int paged_checks(size_t nseq, size_t groups, size_t max_tk, const TableArg& t, s
     if (nseq > PG_MAX_ROWS) return overrun_slice(nseq, PG_MAX_ROWS);
     if (groups > (size_t)PG_GROUPS) return overrun_slice(groups, PG_GROUPS);
     const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
-    const size_t wgs = smul(sadd(z.max_shared, z.max_own), kv_heads);
+    const size_t wgs = std::max(smul(z.items, kv_heads), smul(smul(nseq, heads), head_dim / 4) / 256);
     if (wgs > MAX_WGS) return overrun_slice(wgs, MAX_WGS);
     return LLMTIE_OK;
 }
@@ -1641,6 +1641,15 @@ Pages pages_of(const uint16_t* cache, const TableArg& t, size_t pages, size_t pa
 // compute units once, of four blocks or more.
 size_t selected_runs(size_t units, size_t blocks) {
     return std::max<size_t>(1, std::min((blocks + 3) / 4, (size_t)compute_units() / std::max<size_t>(1, units)));
+}
+
+// Workgroups that score the pages of a (row, kv head): one (with its selection in
+// the same launch) where the launch has one for every second compute unit; else so many that
+// the compute units have one each, of 64 pages or more.
+size_t score_chunks(size_t units, size_t wide) {
+    const size_t cus = (size_t)compute_units();
+    if (units == 0 || 2 * units >= cus) return 1;
+    return std::max<size_t>(1, std::min(cus / units, wide / 64));
 }
 
 // Queries of nseq rows, a cache of pages, the context.
@@ -1854,8 +1863,11 @@ int llmtie_page_bounds(void* stream, const uint16_t* cache, size_t cache_len, si
 
 size_t llmtie_select_pages_workspace(size_t nseq, size_t max_tk, size_t page, size_t count, size_t kv_heads) {
     if (page == 0) return 0;
-    const size_t wide = max_tk / page + (max_tk % page != 0);
-    return wide > count ? smul(nseq, kv_heads, wide) : 0;
+    const size_t wide = max_tk / page + (max_tk % page != 0), units = smul(nseq, kv_heads);
+    if (wide <= count) return 0;
+    const size_t chunks = score_chunks(units, wide);
+    // Scores in f64, and where they are formed by several workgroups in f32 with each one's error.
+    return sadd(smul(units, wide), chunks > 1 ? smul(units, sadd(wide, chunks)) / 2 + 1 : 0);
 }
 
 int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
@@ -1883,6 +1895,7 @@ int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off
     if (nseq == 0) return ok();
     if (!q || !bounds || !table || !tk_dev || !chosen || (need && !ws)) return invalid("a buffer");
     if (off16(bounds) || off16(ws)) return refuse("bounds or a workspace off 16 bytes");
+    if (pages == 0) return refuse("no pages to select from");
     SelectArgs a{};
     a.q = q + q_off;
     a.bounds = bounds;
@@ -1890,7 +1903,11 @@ int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off
     a.row = row_dev;
     a.tk = tk_dev;
     a.chosen = chosen;
-    a.score = ws;
+    a.wide = (int)((max_tk + page - 1) / page);
+    a.chunks = (int)score_chunks(units, (size_t)a.wide);
+    a.exact = ws;
+    a.score = reinterpret_cast<float*>(ws + units * (size_t)a.wide);
+    a.worst = a.score + units * (size_t)a.wide;
     a.q_stride = nseq > 1 ? (long)q_stride : 0;
     a.nseq = (int)nseq;
     a.kv_heads = (int)kv_heads;
@@ -1902,7 +1919,6 @@ int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off
     a.count = (int)count;
     a.first = (int)first;
     a.last = (int)last;
-    a.wide = (int)((max_tk + page - 1) / page);
     return launched("select_pages", launch_select((int)head_dim, a, S(stream)));
 }
 

@@ -76,10 +76,13 @@ struct SelectArgs {
     const int* row;
     const int* tk;
     int* chosen;     // [nseq][kv_heads][count]
-    double* score;   // [nseq][kv_heads][cols]
+    double* exact;   // [nseq][kv_heads][wide]
+    float* score;    // [nseq][kv_heads][wide], where chunks > 1
+    float* worst;    // [nseq][kv_heads][chunks]
     long q_stride;
     int nseq, kv_heads, group, rows, cols, shift, pages, count, first, last;
     int wide;        // pages a row may have (of max_tk), at most cols
+    int chunks;      // workgroups that score a (row, kv head)'s pages
 };
 hipError_t launch_select(int hd, const SelectArgs& a, hipStream_t st);
 

@@ -409,77 +409,133 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     });
 }
 
-// The context of a row's query heads from its parts, in their order: M = max m,
-// O = sum 2^(m - M) O / sum 2^(m - M) l. A part in which a row sees no key has m =
-// RG_NOREF and l = 0. The threads are HD / 4 columns of four dims by phases of
-// the parts, whose loads go out together; a workgroup takes `heads` query heads of
-// a kv head, one where the launch is small (one sequence of 32 parts, all four
-// heads by one thread a column: 12.4 us).
+// The parts of a row's columns of kv head kh: `on` of its own, then `sn` of its
+// group's. None (n = 0): its item wrote the context.
+template <int HD, bool PLAN>
+struct Parts {
+    int o0, on, s0 = 0, n, step = 0, col = 0;
+    bool bad = false;  // no such table row
+    __device__ __forceinline__ Parts(const PagedArgs& a, int row) {
+        if constexpr (PLAN) {
+            const int* d = a.plan + PG_HEAD + (size_t)PG_ROW * row;
+            o0 = d[0], on = d[1], s0 = d[2], step = d[4], col = d[5];
+            n = on == 1 && d[3] == 0 ? 0 : on + d[3];
+        } else {
+            const int table = a.row ? a.row[row] : row;
+            bad = table < 0 || table >= a.p.rows;
+            o0 = row * a.runs, on = n = a.runs;
+        }
+    }
+    // The i-th part's O and (m, l) of query head g.
+    __device__ __forceinline__ Sink of(const PagedArgs& a, int i, int kh, int g) const {
+        Sink p = i < on ? own_part(a, HD, o0 + i, kh) : shared_part(a, HD, s0 + (i - on) * step, kh);
+        const int at = g + (i < on ? 0 : col);
+        p.o += (size_t)at * HD, p.ml += at;
+        return p;
+    }
+};
+
+// The context from its parts, in their order: M = max m, O = sum 2^(m - M) O / sum
+// 2^(m - M) l. A part in which a row sees no key has m = RG_NOREF and l = 0.
+//
+// Many rows, of few parts each: a thread takes four dims of a (row, head) (244
+// rows of 20 heads of 64, by a workgroup a (row, head) as below 13.8 us, so 7.3).
+template <int HD, bool PLAN>
+__global__ __launch_bounds__(PT) void paged_merge_rows_kernel(PagedArgs a) {
+    constexpr int C = HD / 4, U = 4;
+    const long i = (long)blockIdx.x * PT + threadIdx.x;
+    const int heads = a.kv_heads * a.group, c = (int)(i % C), h = (int)(i / C % heads);
+    const long row = i / C / heads;
+    if (row >= a.nseq || (PLAN && !plan_fits(a))) return;
+    const Parts<HD, PLAN> p(a, (int)row);
+    float* out = a.out + 4 * i;
+    const int kh = h / a.group, g = h % a.group;
+    if (p.bad) {
+        *reinterpret_cast<floatx4*>(out) = zero_f4() + __builtin_nanf("");
+        return;
+    }
+    if (p.n == 0) return;
+    float M = RG_NOREF, L = 0.0f;
+    floatx4 y = zero_f4();
+    for (int s0 = 0; s0 < p.n; s0 += U) {
+        float2 ml[U];
+        floatx4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const Sink s = p.of(a, min(s0 + u, p.n - 1), kh, g);
+            ml[u] = *s.ml;
+            x[u] = *reinterpret_cast<const floatx4*>(s.o + 4 * c);
+        }
+        float mn = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+        const float f = ex2(M - mn);
+        M = mn;
+        L *= f;
+        y *= f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (s0 + u >= p.n) break;
+            const float w = ex2(ml[u].x - M);
+            L += ml[u].y * w;
+            y += x[u] * w;
+        }
+    }
+    *reinterpret_cast<floatx4*>(out) = y * (L > 0.0f || L != L ? 1.0f / L : 0.0f);
+}
+
+// Few rows: a workgroup a (row, query head), the threads HD / 4 columns of four
+// dims by phases of the parts, whose loads go out together (one sequence of 32
+// parts, all four heads by one thread a column: 12.4 us, so 3.9).
 constexpr int PM_PARTS = 1088;  // parts of a row at most: each side's target and one
 
 template <int HD, bool PLAN>
-__global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a, int heads) {
+__global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {
     constexpr int C = HD / 4, R = PT / C, U = 4;
     __shared__ float wt[PM_PARTS];
     __shared__ floatx4 red[PT];
-    const int per = a.group / heads;
-    const int kh = (int)(blockIdx.x / (unsigned)per % (unsigned)a.kv_heads);
-    const int row = (int)(blockIdx.x / (unsigned)(per * a.kv_heads));
-    const int g0 = (int)(blockIdx.x % (unsigned)per) * heads;
+    const int heads = a.kv_heads * a.group, h = (int)(blockIdx.x % (unsigned)heads);
+    const int row = (int)(blockIdx.x / (unsigned)heads), kh = h / a.group;
     const int tid = threadIdx.x, c = tid % C, phase = tid / C, lane = tid & 63;
-    int o0 = row * a.runs, on = a.runs, s0 = 0, sn = 0, step = 0, col = 0;
-    float* out = a.out + (((size_t)row * a.kv_heads + kh) * a.group + g0) * HD;
-    if constexpr (PLAN) {
-        if (!plan_fits(a)) return;
-        const int* d = a.plan + PG_HEAD + (size_t)PG_ROW * row;
-        o0 = d[0], on = d[1], s0 = d[2], sn = d[3], step = d[4], col = d[5];
-        if (on == 1 && sn == 0) return;  // its item wrote it
-    } else {
-        const int table = a.row ? a.row[row] : row;
-        if (table < 0 || table >= a.p.rows) {
-            fill(out, heads * HD, __builtin_nanf(""));
-            return;
+    if (PLAN && !plan_fits(a)) return;
+    const Parts<HD, PLAN> p(a, row);
+    float* out = a.out + (size_t)blockIdx.x * HD;
+    if (p.bad) {
+        fill(out, HD, __builtin_nanf(""));
+        return;
+    }
+    const int n = min(p.n, PM_PARTS);
+    if (n == 0) return;
+    auto part = [&](int i) { return p.of(a, i, kh, h % a.group); };
+    // The first parts' columns are on their way while the weights are formed.
+    floatx4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        x[u] = *reinterpret_cast<const floatx4*>(part(min(phase + u * R, n - 1)).o + 4 * c);
+    float M = RG_NOREF, L = 0.0f;
+    for (int i = lane; i < n; i += 64) M = fmaxf(M, part(i).ml->x);
+    M = wave_max(M);
+    for (int i = lane; i < n; i += 64) {
+        const float2 ml = *part(i).ml;
+        const float f = ex2(ml.x - M);
+        L += ml.y * f;
+        if (tid < 64) wt[i] = f;
+    }
+    L = wave_sum(L);
+    __syncthreads();
+    floatx4 y = zero_f4();
+    for (int i = phase; i < n; i += U * R) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i + u * R < n) y += x[u] * wt[i + u * R];
+            x[u] = *reinterpret_cast<const floatx4*>(part(min(i + (U + u) * R, n - 1)).o + 4 * c);
         }
     }
-    const int n = min(on + sn, PM_PARTS);
-    for (int g = g0; g < g0 + heads; ++g) {
-        auto part = [&](int i) {
-            Sink p = i < on ? own_part(a, HD, o0 + i, kh) : shared_part(a, HD, s0 + (i - on) * step, kh);
-            const int at = g + (i < on ? 0 : col);
-            p.o += (size_t)at * HD, p.ml += at;
-            return p;
-        };
-        // The first parts' columns are on their way while the weights are formed.
-        floatx4 x[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-            x[u] = *reinterpret_cast<const floatx4*>(part(min(phase + u * R, n - 1)).o + 4 * c);
-        float M = RG_NOREF, L = 0.0f;
-        for (int i = lane; i < n; i += 64) M = fmaxf(M, part(i).ml->x);
-        M = wave_max(M);
-        for (int i = lane; i < n; i += 64) {
-            const float2 ml = *part(i).ml;
-            const float f = ex2(ml.x - M);
-            L += ml.y * f;
-            if (tid < 64) wt[i] = f;
-        }
-        L = wave_sum(L);
-        __syncthreads();
-        floatx4 y = zero_f4();
-        for (int i = phase; i < n; i += U * R) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (i + u * R < n) y += x[u] * wt[i + u * R];
-                x[u] = *reinterpret_cast<const floatx4*>(part(min(i + (U + u) * R, n - 1)).o + 4 * c);
-            }
-        }
-        red[tid] = y;
-        __syncthreads();
-        if (phase == 0) {
-            for (int k = 1; k < R; ++k) y += red[tid + k * C];
-            *reinterpret_cast<floatx4*>(out + (g - g0) * HD + 4 * c) = y * (L > 0.0f || L != L ? 1.0f / L : 0.0f);
-        }
-        __syncthreads();
+    red[tid] = y;
+    __syncthreads();
+    if (phase == 0) {
+        for (int k = 1; k < R; ++k) y += red[tid + k * C];
+        *reinterpret_cast<floatx4*>(out + 4 * c) = y * (L > 0.0f || L != L ? 1.0f / L : 0.0f);
     }
 }
 
@@ -499,11 +555,14 @@ hipError_t launch_paged(int hd, const PagedArgs& a, hipStream_t st) {
 #undef PK
     if (!done) return hipErrorInvalidValue;
     if (a.merge) {
-        const int heads = (size_t)a.nseq * a.kv_heads >= 1024 ? a.group : 1;
-        const dim3 rows((unsigned)((size_t)a.nseq * a.kv_heads * (a.group / heads)));
-#define MK(HD, P)                                                                                \
-    if (hd == HD && (a.plan != nullptr) == P)                                                    \
-        hipLaunchKernelGGL((paged_merge_kernel<HD, P>), rows, dim3(PT), 0, st, a, heads);
+        const size_t rows = (size_t)a.nseq * a.kv_heads * a.group;
+#define MK(HD, P)                                                                                              \
+    if (hd == HD && (a.plan != nullptr) == P) {                                                                \
+        if (rows >= 2048)                                                                                      \
+            hipLaunchKernelGGL((paged_merge_rows_kernel<HD, P>), dim3((unsigned)((rows * (HD / 4) + PT - 1) / PT)), \
+                               dim3(PT), 0, st, a);                                                            \
+        else hipLaunchKernelGGL((paged_merge_kernel<HD, P>), dim3((unsigned)rows), dim3(PT), 0, st, a);        \
+    }
         MK(64, false) MK(64, true) MK(128, false) MK(128, true)
 #undef MK
     }

@@ -291,154 +291,374 @@ hipError_t launch_page_bounds(int hd, const PageBoundsArgs& a, hipStream_t st) {
 
 // ---------------------------------------------------------------- selection
 //
-// Scores are formed in f64: a selection is whole numbers, and two pages' scores
-// differ by less than an f32 sum's rounding often enough (one selection in ten
-// thousand) that f32 would choose another page there than the definition does.
+// A selection is whole numbers, and two pages' scores lie within an f32 sum's
+// rounding of each other in one selection of ten thousand: the definition's sums
+// are f64's. But f64 decides at the border only. All scores s are formed by the
+// matrix units as s' from q as the sum of two f16 (scaled by a power of two so
+// that the largest |q| is in 2^14 to 2^15; the bounds are f16), with
+//   |s' - s| <= E = 2^-13 A + 1,   A = sum_d |q_d b_d| over the products of the sum:
+// q's two halves are 2^-22 of it off and 2^-25 more (256 times 65504 of these are
+// 0.5), the products are exact, and 4 HD additions to f32 lose at most 2^-23 of A
+// each, whatever order and rounding the matrix unit has: (512 + 2) 2^-23 A < 2^-13 A.
+// A itself is formed from the upper halves, 2^-11 off, within what is left of 2^-13.
+// With t the count-th largest s' and E the largest one, pages with s' > t + 2 E are
+// selected, those with s' < t - 2 E are not, and the few between (1 to 3 of 500
+// random ones) are ranked by sums in f64. (All sums in f64, 32 sequences of 2000-32768
+// positions, pages of 64: 59.5 us.)
 
-constexpr int SC = 256;
+constexpr int SE = 256;          // threads of a selection
+constexpr int DIGIT = 11;
+constexpr int PS_LDS = 8192;     // pages whose scores a workgroup holds
+constexpr int PS_NEAR = 256;     // pages near the border that it ranks
 
-// Sixteen lanes a page, eight dims each (of HD 64: eight lanes).
+struct SelectUnit {
+    int r, kh, table, live;
+    const float* q;
+    __device__ __forceinline__ SelectUnit(const SelectArgs& a, int unit) {
+        r = unit / a.kv_heads, kh = unit % a.kv_heads;
+        table = a.row ? a.row[r] : r;
+        const int tk = max(0, min(a.tk[r], a.wide << a.shift));
+        live = table < 0 || table >= a.rows ? 0 : (tk + (1 << a.shift) - 1) >> a.shift;
+        q = a.q + (size_t)r * a.q_stride;
+    }
+};
+
+// Scores s' of pages p0 .. p1 - 1 by the four waves, 16 pages a step: q's heads are
+// the rows of the tile, pages its columns. Returns this lane's largest E (infinite where a
+// page is not there or something is not finite).
 template <int HD>
-__global__ __launch_bounds__(SC) void page_score_kernel(SelectArgs a, int chunks) {
-    constexpr int LP = HD / 8, PPW = SC / LP;  // lanes of a page; pages of a workgroup's step
-    extern __shared__ double qs[];             // [group][2][HD]
-    const int tid = threadIdx.x;
-    const int unit = (int)(blockIdx.x / (unsigned)chunks), chunk = (int)(blockIdx.x % (unsigned)chunks);
-    const int r = unit / a.kv_heads, kh = unit % a.kv_heads;
-    const int t = a.row ? a.row[r] : r;
-    if (t < 0 || t >= a.rows) return;
-    const int tk = max(0, min(a.tk[r], a.wide << a.shift));
-    const int live = (tk + (1 << a.shift) - 1) >> a.shift;
-    const int share = (live + chunks - 1) / chunks, p0 = chunk * share, p1 = min(live, p0 + share);
-    if (p0 >= p1) return;
-    const float* q = a.q + (size_t)r * a.q_stride + (size_t)kh * a.group * HD;
-    for (int e = tid; e < a.group * HD; e += SC) {
-        const double x = (double)q[e];
-        qs[e / HD * 2 * HD + e % HD] = x < 0.0 ? 0.0 : x;  // (a NaN stays one)
-        qs[e / HD * 2 * HD + HD + e % HD] = x > 0.0 ? 0.0 : x;
-    }
-    __syncthreads();
-    const int l = tid % LP;
-    for (int p = p0 + tid / LP; p < p1; p += PPW) {
-        const int id = a.table[(size_t)t * a.cols + p];
-        const bool good = id >= 0 && id < a.pages;
-        const half_t* b = reinterpret_cast<const half_t*>(a.bounds) + ((size_t)(good ? id : 0) * a.kv_heads + kh) * 2 * HD + 8 * l;
-        const half8 mx = ld_h8(b), mn = ld_h8(b + HD);
-        double best = -__builtin_inf();
-        for (int g = 0; g < a.group; ++g) {
-            const double* w = qs + g * 2 * HD + 8 * l;
-            double s = 0.0;
+__device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUnit& x, int p0, int p1, float* out, int tid) {
+    constexpr int NS = HD / 32;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
+    const bool head = col < a.group;
+    const float* q = x.q + (size_t)(x.kh * a.group + (head ? col : 0)) * HD + 8 * grp;
+    const int* ids = a.table + (size_t)x.table * a.cols;
+    auto id_of = [&](int t) { return ids[min(p0 + 16 * t + col, p1 - 1)]; };
+    struct Step {
+        half8 mx[NS], mn[NS];
+        bool gone;
+    };
+    auto load = [&](Step& y, int id) __attribute__((always_inline)) {
+        y.gone = id < 0 || id >= a.pages;
+        const half_t* b = reinterpret_cast<const half_t*>(a.bounds) +
+                          ((size_t)(y.gone ? 0 : id) * a.kv_heads + x.kh) * 2 * HD + 8 * grp;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                s = __builtin_fma(w[j], (double)(float)mx[j], s);
-                s = __builtin_fma(w[HD + j], (double)(float)mn[j], s);
-            }
+        for (int s = 0; s < NS; ++s) y.mx[s] = ld_h8(b + 32 * s), y.mn[s] = ld_h8(b + HD + 32 * s);
+    };
+    constexpr int W = SE / 64;
+    const int steps = (p1 - p0 + 15) / 16;
+    Step cur, next;
+    int id = id_of(wave), ahead = id_of(wave + W);
+    load(cur, id);
+    // The power of two.
+    float v[NS][8], top = 0.0f;
 #pragma unroll
-            for (int d = 1; d < LP; d <<= 1) s += __shfl_xor(s, d);
-            best = fmax(best, s == s ? s : __builtin_inf());
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[s][j] = head ? q[32 * s + j] : 0.0f;
+            top = fmaxf(top, fabsf(v[s][j]));
         }
-        // A page that the cache does not have: its keys make the row NaN, as they would be attended.
-        if (!good) best = __builtin_inf();
-        if (l == 0) a.score[(size_t)unit * a.wide + p] = best;
+    top = wave_max(top);
+    int e = 0;
+    (void)frexpf(top, &e);  // top in 2^(e - 1) to 2^e
+    const int up = top > 0.0f && top < __builtin_inff() ? 15 - e : 0;
+    half8 ph[NS], pl[NS], nh[NS], nl[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            half_t hi, lo;
+            const float y = ldexpf(v[s][j], up);
+            split_h(y < 0.0f ? 0.0f : y, hi, lo);  // (a NaN stays one)
+            ph[s][j] = hi, pl[s][j] = lo;
+            split_h(y > 0.0f ? 0.0f : y, hi, lo);
+            nh[s][j] = hi, nl[s][j] = lo;
+        }
+    float worst = 0.0f;
+    for (int t = wave; t < steps; t += W) {
+        load(next, ahead);
+        ahead = id_of(t + 2 * W);
+        floatx4 sc = zero_f4(), ab = zero_f4();
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+            const half8 amx = __builtin_bit_cast(half8, __builtin_bit_cast(u4, cur.mx[s]) & 0x7fff7fffu);
+            const half8 amn = __builtin_bit_cast(half8, __builtin_bit_cast(u4, cur.mn[s]) | 0x80008000u);
+            ab = mfma16(ph[s], amx, ab);
+            ab = mfma16(nh[s], amn, ab);
+            sc = mfma16(pl[s], cur.mx[s], sc);
+            sc = mfma16(nl[s], cur.mn[s], sc);
+            sc = mfma16(ph[s], cur.mx[s], sc);
+            sc = mfma16(nh[s], cur.mn[s], sc);
+        }
+        float best = ninf(), most = 0.0f;
+        bool odd = cur.gone;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (4 * grp + r < a.group) {
+                best = fmaxf(best, sc[r]);
+                most = fmaxf(most, ab[r]);
+                odd = odd || !(ab[r] < 0x1p40f);  // (the most of finite ones is 2^39)
+            }
+        }
+        best = max4grp(best);
+        worst = fmaxf(worst, odd ? __builtin_inff() : most);
+        const int p = p0 + 16 * t + col;
+        if (grp == 0 && p < p1) out[p] = best;
+        cur = next;
     }
+    return worst < __builtin_inff() ? __builtin_fmaf(worst, 0x1p-13f, 1.0f) : worst;
 }
 
-// A score as bits that order as it does.
+// The definition: one page's score by a wave, in f64.
+template <int HD>
+__device__ __forceinline__ double score_exact(const SelectArgs& a, const SelectUnit& x, int p, int lane) {
+    constexpr int D = HD / 64;
+    const int id = a.table[(size_t)x.table * a.cols + p];
+    if (id < 0 || id >= a.pages) return __builtin_inf();  // as its keys make the row NaN
+    const half_t* b = reinterpret_cast<const half_t*>(a.bounds) + ((size_t)id * a.kv_heads + x.kh) * 2 * HD + D * lane;
+    double best = -__builtin_inf();
+    for (int g = 0; g < a.group; ++g) {
+        const float* q = x.q + (size_t)(x.kh * a.group + g) * HD + D * lane;
+        double s = 0.0;
+#pragma unroll
+        for (int j = 0; j < D; ++j) {
+            const double y = (double)q[j];
+            s = __builtin_fma(y < 0.0 ? 0.0 : y, (double)(float)b[j], s);
+            s = __builtin_fma(y > 0.0 ? 0.0 : y, (double)(float)b[HD + j], s);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        best = fmax(best, s == s ? s : __builtin_inf());
+    }
+    return best + 0.0;  // -0: 0
+}
+
+// Bits that order as the numbers do.
 __device__ __forceinline__ uint64_t order(double s) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, s + 0.0);  // -0: 0
+    const uint64_t u = __builtin_bit_cast(uint64_t, s);
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
+__device__ __forceinline__ uint32_t order(float s) {
+    const uint32_t u = __float_as_uint(s);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unorder(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
-constexpr int SE = 256, DIGIT = 11;
+struct SelectLds {
+    int hist[1 << DIGIT];
+    int waves[2][SE / 64];
+    int found[3];
+    int near, sure;
+    uint32_t worst;
+    int page[PS_NEAR];
+    double score[PS_NEAR];
+};
 
-// The `count` best pages of a (row, kv head): the border score by its digits
-// from the top, each a histogram of the pages that agree above it, until the
-// border's bin is taken whole; then the pages in order.
-__global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
-    __shared__ int hist[1 << DIGIT];
-    __shared__ int waves[2][SE / 64];
-    __shared__ int found[3];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, unit = (int)blockIdx.x;
-    const int r = unit / a.kv_heads;
-    const int t = a.row ? a.row[r] : r;
-    int* out = a.chosen + (size_t)unit * a.count;
-    const int tk = max(0, min(a.tk[r], a.wide << a.shift));
-    const int live = t < 0 || t >= a.rows ? 0 : (tk + (1 << a.shift) - 1) >> a.shift;
-    if (live <= a.count) {
-        for (int i = tid; i < a.count; i += SE) out[i] = i < live ? i : -1;
-        return;
-    }
-    const double* score = a.score + (size_t)unit * a.wide;
-    auto key = [&](int p) {
-        return p < a.first || p >= live - a.last ? ~0ull : order(score[p]);
-    };
-    uint64_t border = 0, mask = 0;
-    int need = a.count;  // of those that agree with the border above its digits so far
-    for (int top = 64; top > 0;) {
+// The digits, from the top, of the count-th largest of key(0 .. n - 1): each a
+// histogram of those that agree above it. `mask` holds the digits found when a
+// border's bin was taken whole (ALL: all of them), `need` how many of the border's
+// are taken.
+template <typename K, bool ALL, typename Key>
+__device__ __forceinline__ void border_of(SelectLds& w, int n, int count, int tid, Key&& key, K& border, K& mask, int& need) {
+    constexpr int B = (1 << DIGIT) / SE;
+    const int lane = tid & 63, wave = tid >> 6;
+    border = mask = 0, need = count;
+    for (int top = 8 * (int)sizeof(K); top > 0;) {
         const int bits = min(DIGIT, top), low = top - bits;
-        for (int i = tid; i < 1 << DIGIT; i += SE) hist[i] = 0;
-        __syncthreads();
-        for (int p = tid; p < live; p += SE) {
-            const uint64_t k = key(p);
-            if ((k & mask) == border) atomicAdd(&hist[(int)(k >> low) & ((1 << bits) - 1)], 1);
-        }
-        __syncthreads();
-        if (wave == 0) {
-            // From the top bin down: 64 lanes of 32 bins each.
-            constexpr int B = (1 << DIGIT) / 64;
-            int sum = 0;
-            for (int i = 0; i < B; ++i) sum += hist[(63 - lane) * B + i];
-            int upto = sum;
+        int4* h = reinterpret_cast<int4*>(w.hist);
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int y = __shfl_up(upto, d);
-                if (lane >= d) upto += y;
-            }
-            if (upto >= need && upto - sum < need) {
-                int left = need - (upto - sum), i = (63 - lane) * B + B - 1;
-                while (hist[i] < left) left -= hist[i--];
-                found[0] = i, found[1] = left, found[2] = hist[i];
+        for (int i = 0; i < B / 4; ++i) h[tid + SE * i] = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        for (int p = tid; p < n; p += SE) {
+            const K k = key(p);
+            if ((k & mask) == border) atomicAdd(&w.hist[(int)(k >> low) & ((1 << bits) - 1)], 1);
+        }
+        __syncthreads();
+        // From the top bin down, B bins a thread.
+        int bin[B], sum = 0;
+        const int first = (1 << DIGIT) - B * (tid + 1);
+#pragma unroll
+        for (int i = 0; i < B / 4; ++i) {
+            const int4 y = h[first / 4 + i];
+            bin[4 * i] = y.x, bin[4 * i + 1] = y.y, bin[4 * i + 2] = y.z, bin[4 * i + 3] = y.w;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) sum += bin[i];
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(upto, d);
+            if (lane >= d) upto += y;
+        }
+        if (lane == 63) w.waves[0][wave] = upto;
+        __syncthreads();
+        for (int k = 0; k < wave; ++k) upto += w.waves[0][k];
+        if (upto >= need && upto - sum < need) {
+            int left = need - (upto - sum);
+            bool done = false;
+#pragma unroll
+            for (int i = B - 1; i >= 0; --i) {
+                if (!done && bin[i] >= left) {
+                    w.found[0] = first + i, w.found[1] = left, w.found[2] = bin[i];
+                    done = true;
+                }
+                if (!done) left -= bin[i];
             }
         }
         __syncthreads();
-        border |= (uint64_t)found[0] << low;
-        mask |= (uint64_t)((1 << bits) - 1) << low;
-        need = found[1];
+        border |= (K)w.found[0] << low;
+        mask |= (K)((1 << bits) - 1) << low;
+        need = w.found[1];
         top = low;
-        const bool whole = found[2] == need;
-        __syncthreads();
-        if (whole) break;
+        if (!ALL && w.found[2] == need) break;
     }
-    // Pages above the border, and the first `need` at it.
-    int above = 0, at = 0;
-    for (int p0 = 0; p0 < live; p0 += SE) {
+}
+
+// Pages with above(p), and the first `need` with at(p), in order.
+template <typename Above, typename At>
+__device__ __forceinline__ void emit(SelectLds& w, int n, int need, int* out, int tid, Above&& above, At&& at) {
+    const int lane = tid & 63, wave = tid >> 6;
+    int na = 0, ne = 0;
+    for (int p0 = 0; p0 < n; p0 += SE) {
         const int p = p0 + tid;
-        const uint64_t k = p < live ? key(p) & mask : 0;
-        const bool gt = p < live && k > border, eq = p < live && k == border;
+        const bool gt = p < n && above(p), eq = p < n && !gt && at(p);
         const uint64_t mg = __ballot(gt), me = __ballot(eq), before = (1ull << lane) - 1;
-        if (lane == 0) waves[0][wave] = __popcll(mg), waves[1][wave] = __popcll(me);
         __syncthreads();
-        int g = above + __popcll(mg & before), e = at + __popcll(me & before);
-        for (int w = 0; w < SE / 64; ++w) {
-            if (w < wave) g += waves[0][w], e += waves[1][w];
-            above += waves[0][w], at += waves[1][w];
+        if (lane == 0) w.waves[0][wave] = __popcll(mg), w.waves[1][wave] = __popcll(me);
+        __syncthreads();
+        int g = na + __popcll(mg & before), e = ne + __popcll(me & before);
+        for (int k = 0; k < SE / 64; ++k) {
+            if (k < wave) g += w.waves[0][k], e += w.waves[1][k];
+            na += w.waves[0][k], ne += w.waves[1][k];
         }
         if (gt || (eq && e < need)) out[g + min(e, need)] = p;
+    }
+}
+
+// All sums in f64: pages past those that a workgroup holds, or something not finite.
+template <int HD>
+__device__ void select_exact(SelectLds& w, const SelectArgs& a, const SelectUnit& x, int unit, int* out, int tid) {
+    double* score = a.exact + (size_t)unit * a.wide;
+    for (int p = tid >> 6; p < x.live; p += SE / 64) {
+        const double s = score_exact<HD>(a, x, p, tid & 63);
+        if ((tid & 63) == 0) score[p] = s;
+    }
+    __syncthreads();
+    auto key = [&](int p) { return p < a.first || p >= x.live - a.last ? ~0ull : order(score[p]); };
+    uint64_t border, mask;
+    int need;
+    border_of<uint64_t, false>(w, x.live, a.count, tid, key, border, mask, need);
+    emit(w, x.live, need, out, tid, [&](int p) { return (key(p) & mask) > border; },
+         [&](int p) { return (key(p) & mask) == border; });
+}
+
+// A workgroup a (row, kv head). SCORED: its pages' scores are in the workspace.
+template <int HD, bool SCORED>
+__global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
+    extern __shared__ float sc[];
+    __shared__ SelectLds w;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, unit = (int)blockIdx.x;
+    const SelectUnit x(a, unit);
+    int* out = a.chosen + (size_t)unit * a.count;
+    if (x.live <= a.count) {
+        for (int i = tid; i < a.count; i += SE) out[i] = i < x.live ? i : -1;
+        return;
+    }
+    if (a.wide > PS_LDS) {
+        select_exact<HD>(w, a, x, unit, out, tid);
+        return;
+    }
+    if (tid == 0) w.worst = 0, w.near = 0, w.sure = 0;
+    __syncthreads();
+    float worst = 0.0f;
+    if constexpr (SCORED) {
+        const float* from = a.score + (size_t)unit * a.wide;
+        for (int p = tid; p < x.live; p += SE) sc[p] = from[p];
+        for (int i = tid; i < a.chunks; i += SE) worst = fmaxf(worst, a.worst[(size_t)unit * a.chunks + i]);
+    } else {
+        worst = score_pages<HD>(a, x, 0, x.live, sc, tid);
+    }
+    worst = wave_max(worst);
+    if (lane == 0) atomicMax(&w.worst, __float_as_uint(worst));  // (not below 0)
+    __syncthreads();
+    const float e2 = 2.0f * __uint_as_float(w.worst);
+    if (!(e2 < 0x1p40f)) {
+        select_exact<HD>(w, a, x, unit, out, tid);
+        return;
+    }
+    auto kept = [&](int p) { return p < a.first || p >= x.live - a.last; };
+    uint32_t border, mask;
+    int need;
+    border_of<uint32_t, true>(w, x.live, a.count, tid, [&](int p) { return kept(p) ? ~0u : order(sc[p]); }, border, mask, need);
+    if (border == ~0u) {  // no more than what is always kept
+        emit(w, x.live, 0, out, tid, kept, [](int) { return false; });
+        return;
+    }
+    const float t = unorder(border), high = t + e2, low = t - e2;
+    int sure = 0;
+    for (int p = tid; p < x.live; p += SE) {
+        if (kept(p) || sc[p] > high) {
+            ++sure;
+        } else if (sc[p] >= low) {
+            const int i = atomicAdd(&w.near, 1);
+            if (i < PS_NEAR) w.page[i] = p;
+        }
+    }
+    if (sure) atomicAdd(&w.sure, sure);
+    __syncthreads();
+    const int near = w.near, left = a.count - w.sure;
+    if (near > PS_NEAR) {
+        select_exact<HD>(w, a, x, unit, out, tid);
+        return;
+    }
+    if (near > left) {
+        for (int i = wave; i < near; i += SE / 64) {
+            const double s = score_exact<HD>(a, x, w.page[i], lane);
+            if (lane == 0) w.score[i] = s;
+        }
+        __syncthreads();
+        if (tid < near) {
+            int rank = 0;
+            for (int i = 0; i < near; ++i)
+                rank += w.score[i] > w.score[tid] || (w.score[i] == w.score[tid] && w.page[i] < w.page[tid]);
+            if (rank >= left) sc[w.page[tid]] = ninf();
+        }
         __syncthreads();
     }
+    emit(w, x.live, 0, out, tid, [&](int p) { return kept(p) || sc[p] >= low; }, [](int) { return false; });
+}
+
+// Few (row, kv head)s of many pages: their scores by `chunks` workgroups each.
+template <int HD>
+__global__ __launch_bounds__(SE) void page_score_kernel(SelectArgs a) {
+    __shared__ float top[SE / 64];
+    const int tid = threadIdx.x, unit = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks);
+    const SelectUnit x(a, unit);
+    const int share = (((x.live + 15) / 16 + a.chunks - 1) / a.chunks) * 16;
+    const int p0 = chunk * share, p1 = min(x.live, p0 + share);
+    float worst = 0.0f;
+    if (p0 < p1) worst = score_pages<HD>(a, x, p0, p1, a.score + (size_t)unit * a.wide, tid);
+    worst = wave_max(worst);
+    if ((tid & 63) == 0) top[tid >> 6] = worst;
+    __syncthreads();
+    if (tid == 0) a.worst[(size_t)unit * a.chunks + chunk] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 }
 
 hipError_t launch_select(int hd, const SelectArgs& a, hipStream_t st) {
-    const int units = a.nseq * a.kv_heads;
-    if (a.wide > a.count) {
-        // Workgroups of a (row, kv head) so that two a compute unit work, of 32 pages or more.
-        const int chunks = std::max(1, std::min((a.wide + 31) / 32, (512 + units - 1) / units));
-        const dim3 grid((unsigned)units * (unsigned)chunks);
-        const size_t lds = (size_t)a.group * 2 * hd * sizeof(double);
-        if (hd == 128) hipLaunchKernelGGL((page_score_kernel<128>), grid, dim3(SC), lds, st, a, chunks);
-        else hipLaunchKernelGGL((page_score_kernel<64>), grid, dim3(SC), lds, st, a, chunks);
+    const unsigned units = (unsigned)a.nseq * (unsigned)a.kv_heads;
+    const size_t lds = a.wide <= PS_LDS ? (size_t)a.wide * sizeof(float) : 0;
+    const bool scored = a.chunks > 1 && a.wide <= PS_LDS && a.wide > a.count;
+#define SL(HD)                                                                                                  \
+    if (hd == HD) {                                                                                             \
+        if (scored) {                                                                                           \
+            hipLaunchKernelGGL((page_score_kernel<HD>), dim3(units * (unsigned)a.chunks), dim3(SE), 0, st, a);  \
+            hipLaunchKernelGGL((page_select_kernel<HD, true>), dim3(units), dim3(SE), lds, st, a);              \
+        } else hipLaunchKernelGGL((page_select_kernel<HD, false>), dim3(units), dim3(SE), lds, st, a);          \
     }
-    hipLaunchKernelGGL(page_select_kernel, dim3((unsigned)units), dim3(SE), 0, st, a);
+    SL(64) SL(128)
+#undef SL
     return hipGetLastError();
 }
 
