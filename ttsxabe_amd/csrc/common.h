@@ -146,6 +146,15 @@ __device__ __forceinline__ float ld_coherent(const float* p) {
     return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// A barrier for what the waves stored in LDS themselves (lgkmcnt): a fence would
+// also wait for the next tile's direct loads.
+__device__ __forceinline__ void lds_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 // Wide reads of a workgroup-uniform region through a buffer resource: one
 // 8- or 16-byte load per lane, reads past `bytes` return zeros (so a ragged
 // tail needs no branch), and AUX is the cache policy: AUX_AGENT (sc1, the

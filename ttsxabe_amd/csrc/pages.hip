@@ -296,20 +296,23 @@ hipError_t launch_page_bounds(int hd, const PageBoundsArgs& a, hipStream_t st) {
 // are f64's. But f64 decides at the border only. All scores s are formed by the
 // matrix units as s' from q as the sum of two f16 (scaled by a power of two so
 // that the largest |q| is in 2^14 to 2^15; the bounds are f16), with
-//   |s' - s| <= E = 2^-13 A + 1,   A = sum_d |q_d b_d| over the products of the sum:
+//   |s' - s| <= E = 1.05 (4 HD + 2) 2^-23 A + 1,   A = sum_d |q_d b_d| over the products of the sum:
 // q's two halves are 2^-22 of it off and 2^-25 more (256 times 65504 of these are
 // 0.5), the products are exact, and 4 HD additions to f32 lose at most 2^-23 of A
-// each, whatever order and rounding the matrix unit has: (512 + 2) 2^-23 A < 2^-13 A.
-// A itself is formed from the upper halves, 2^-11 off, within what is left of 2^-13.
-// With t the count-th largest s' and E the largest one, pages with s' > t + 2 E are
-// selected, those with s' < t - 2 E are not, and the few between (1 to 3 of 500
-// random ones) are ranked by sums in f64. (All sums in f64, 32 sequences of 2000-32768
+// each, whatever order and rounding the matrix unit has. A itself is formed from
+// the upper halves, 2^-11 and its own additions off: within the 1.05, as the
+// roundings of t +- 2 E are.
+// With t the count-th largest s' (a bin of a histogram that it lies in) and E the largest
+// one, pages with s' > t + 2 E are selected, those with s' < t - 2 E are not, and the few
+// between (1 to 5 of 500 random ones) are ranked by sums in f64. (All sums in f64, 32 sequences of 2000-32768
 // positions, pages of 64: 59.5 us.)
 
-constexpr int SE = 256;          // threads of a selection
-constexpr int DIGIT = 11;
+constexpr int SE = 1024;         // threads of a selection
+constexpr int SC = 256;          // and of a part of its scores
+constexpr int DIGIT = 12;
 constexpr int PS_LDS = 8192;     // pages whose scores a workgroup holds
 constexpr int PS_NEAR = 256;     // pages near the border that it ranks
+constexpr int PS_BINS = 1024;
 
 struct SelectUnit {
     int r, kh, table, live;
@@ -323,15 +326,24 @@ struct SelectUnit {
     }
 };
 
-// Scores s' of pages p0 .. p1 - 1 by the four waves, 16 pages a step: q's heads are
-// the rows of the tile, pages its columns. Returns this lane's largest E (infinite where a
-// page is not there or something is not finite).
+// A kv head's queries as the matrix unit's operands: the upper and lower halves of
+// their positive and of their negative part, [4][HD / 32][64 lanes] of eight.
 template <int HD>
-__device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUnit& x, int p0, int p1, float* out, int tid) {
+struct QueryLds {
+    half_t part[4 * HD / 32 * 64 * 8];
+    float size[16];
+};
+
+// Scores s' of pages p0 .. p1 - 1 by W waves, 16 pages a step: q's heads are
+// the rows of the tile, pages its columns. Returns this lane's largest E (infinite where a
+// page is not there or something is not finite), and its largest and least s' of pages from k0 up to k1. Bound by reading the bounds: 16
+// waves a workgroup, each with a step's 8 KB on their way. (The operands formed by
+// each wave for itself took 16 waves 4.5 us, and eight waves were slower for it.)
+template <int HD, int W>
+__device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUnit& x, int p0, int p1, float* out,
+                                             QueryLds<HD>& ql, int tid, int k0, int k1, float& top, float& least) {
     constexpr int NS = HD / 32;
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, grp = lane >> 4;
-    const bool head = col < a.group;
-    const float* q = x.q + (size_t)(x.kh * a.group + (head ? col : 0)) * HD + 8 * grp;
     const int* ids = a.table + (size_t)x.table * a.cols;
     auto id_of = [&](int t) { return ids[min(p0 + 16 * t + col, p1 - 1)]; };
     struct Step {
@@ -345,40 +357,49 @@ __device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUn
 #pragma unroll
         for (int s = 0; s < NS; ++s) y.mx[s] = ld_h8(b + 32 * s), y.mn[s] = ld_h8(b + HD + 32 * s);
     };
-    constexpr int W = SE / 64;
     const int steps = (p1 - p0 + 15) / 16;
-    Step cur, next;
-    int id = id_of(wave), ahead = id_of(wave + W);
-    load(cur, id);
-    // The power of two.
-    float v[NS][8], top = 0.0f;
+    const int first = id_of(wave);
+    int ahead = id_of(wave + W);
+    constexpr int N = 16 * HD / (64 * W);  // values of a thread: heads past the group's are 0
+    const float* q = x.q + (size_t)x.kh * a.group * HD;
+    float v[N], size = 0.0f;
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+    for (int i = 0; i < N; ++i) {
+        const int e = tid + 64 * W * i;
+        v[i] = e < a.group * HD ? q[e] : 0.0f;
+        size = fmaxf(size, fabsf(v[i]));
+    }
+    Step cur;
+    load(cur, first);
+    size = wave_max(size);
+    if (lane == 0) ql.size[wave] = size;
+    lds_barrier();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[s][j] = head ? q[32 * s + j] : 0.0f;
-            top = fmaxf(top, fabsf(v[s][j]));
-        }
-    top = wave_max(top);
-    int e = 0;
-    (void)frexpf(top, &e);  // top in 2^(e - 1) to 2^e
-    const int up = top > 0.0f && top < __builtin_inff() ? 15 - e : 0;
+    for (int k = 0; k < W; ++k) size = fmaxf(size, ql.size[k]);
+    int e2 = 0;
+    (void)frexpf(size, &e2);  // in 2^(e2 - 1) to 2^e2
+    const int up = size > 0.0f && size < __builtin_inff() ? 15 - e2 : 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = tid + 64 * W * i, h = e / HD, d = e % HD;
+        half_t* at = ql.part + (d / 32 * 64 + h + 16 * (d / 8 % 4)) * 8 + d % 8;
+        half_t hi, lo;
+        const float y = ldexpf(v[i], up);
+        split_h(y < 0.0f ? 0.0f : y, hi, lo);  // (a NaN stays one)
+        at[0] = hi, at[NS * 512] = lo;
+        split_h(y > 0.0f ? 0.0f : y, hi, lo);
+        at[2 * NS * 512] = hi, at[3 * NS * 512] = lo;
+    }
+    lds_barrier();
     half8 ph[NS], pl[NS], nh[NS], nl[NS];
+    const half8* part = reinterpret_cast<const half8*>(ql.part);
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            half_t hi, lo;
-            const float y = ldexpf(v[s][j], up);
-            split_h(y < 0.0f ? 0.0f : y, hi, lo);  // (a NaN stays one)
-            ph[s][j] = hi, pl[s][j] = lo;
-            split_h(y > 0.0f ? 0.0f : y, hi, lo);
-            nh[s][j] = hi, nl[s][j] = lo;
-        }
+    for (int s = 0; s < NS; ++s) {
+        ph[s] = part[s * 64 + lane], pl[s] = part[(NS + s) * 64 + lane];
+        nh[s] = part[(2 * NS + s) * 64 + lane], nl[s] = part[(3 * NS + s) * 64 + lane];
+    }
     float worst = 0.0f;
     for (int t = wave; t < steps; t += W) {
-        load(next, ahead);
-        ahead = id_of(t + 2 * W);
         floatx4 sc = zero_f4(), ab = zero_f4();
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -392,8 +413,11 @@ __device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUn
             sc = mfma16(ph[s], cur.mx[s], sc);
             sc = mfma16(nh[s], cur.mn[s], sc);
         }
+        const bool gone = cur.gone;
+        load(cur, ahead);
+        ahead = id_of(t + 2 * W);
         float best = ninf(), most = 0.0f;
-        bool odd = cur.gone;
+        bool odd = gone;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (4 * grp + r < a.group) {
@@ -406,9 +430,9 @@ __device__ __forceinline__ float score_pages(const SelectArgs& a, const SelectUn
         worst = fmaxf(worst, odd ? __builtin_inff() : most);
         const int p = p0 + 16 * t + col;
         if (grp == 0 && p < p1) out[p] = best;
-        cur = next;
+        if (p >= k0 && p < min(p1, k1)) top = fmaxf(top, best), least = fminf(least, best);
     }
-    return worst < __builtin_inff() ? __builtin_fmaf(worst, 0x1p-13f, 1.0f) : worst;
+    return worst < __builtin_inff() ? __builtin_fmaf(worst, 1.05f * (4 * HD + 2) * 0x1p-23f, 1.0f) : worst;
 }
 
 // The definition: one page's score by a wave, in f64.
@@ -419,18 +443,26 @@ __device__ __forceinline__ double score_exact(const SelectArgs& a, const SelectU
     if (id < 0 || id >= a.pages) return __builtin_inf();  // as its keys make the row NaN
     const half_t* b = reinterpret_cast<const half_t*>(a.bounds) + ((size_t)id * a.kv_heads + x.kh) * 2 * HD + D * lane;
     double best = -__builtin_inf();
-    for (int g = 0; g < a.group; ++g) {
-        const float* q = x.q + (size_t)(x.kh * a.group + g) * HD + D * lane;
-        double s = 0.0;
+    constexpr int U = 4;  // heads side by side
+    for (int g0 = 0; g0 < a.group; g0 += U) {
+        double s[U];
 #pragma unroll
-        for (int j = 0; j < D; ++j) {
-            const double y = (double)q[j];
-            s = __builtin_fma(y < 0.0 ? 0.0 : y, (double)(float)b[j], s);
-            s = __builtin_fma(y > 0.0 ? 0.0 : y, (double)(float)b[HD + j], s);
+        for (int u = 0; u < U; ++u) {
+            const float* q = x.q + (size_t)(x.kh * a.group + min(g0 + u, a.group - 1)) * HD + D * lane;
+            s[u] = 0.0;
+#pragma unroll
+            for (int j = 0; j < D; ++j) {
+                const double y = (double)q[j];
+                s[u] = __builtin_fma(y < 0.0 ? 0.0 : y, (double)(float)b[j], s[u]);
+                s[u] = __builtin_fma(y > 0.0 ? 0.0 : y, (double)(float)b[HD + j], s[u]);
+            }
         }
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        best = fmax(best, s == s ? s : __builtin_inf());
+        for (int d = 1; d < 64; d <<= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) s[u] += __shfl_xor(s[u], d);
+#pragma unroll
+        for (int u = 0; u < U; ++u) best = fmax(best, s[u] == s[u] ? s[u] : __builtin_inf());
     }
     return best + 0.0;  // -0: 0
 }
@@ -440,27 +472,21 @@ __device__ __forceinline__ uint64_t order(double s) {
     const uint64_t u = __builtin_bit_cast(uint64_t, s);
     return u >> 63 ? ~u : u | 0x8000000000000000ull;
 }
-__device__ __forceinline__ uint32_t order(float s) {
-    const uint32_t u = __float_as_uint(s);
-    return u >> 31 ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float unorder(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
 struct SelectLds {
     int hist[1 << DIGIT];
-    int waves[2][SE / 64];
+    int waves[SE / 64], above[SE / 64], at[SE / 64];
     int found[3];
     int near, sure;
-    uint32_t worst;
+    float worst[SE / 64], top[SE / 64], least[SE / 64];
     int page[PS_NEAR];
     double score[PS_NEAR];
 };
 
 // The digits, from the top, of the count-th largest of key(0 .. n - 1): each a
-// histogram of those that agree above it. `mask` holds the digits found when a
-// border's bin was taken whole (ALL: all of them), `need` how many of the border's
-// are taken.
-template <typename K, bool ALL, typename Key>
+// histogram of those that agree above it. `mask` holds the digits found when the
+// border's bin is taken whole, `need` how many of the border's are taken.
+template <typename K, typename Key>
 __device__ __forceinline__ void border_of(SelectLds& w, int n, int count, int tid, Key&& key, K& border, K& mask, int& need) {
     constexpr int B = (1 << DIGIT) / SE;
     const int lane = tid & 63, wave = tid >> 6;
@@ -492,9 +518,9 @@ __device__ __forceinline__ void border_of(SelectLds& w, int n, int count, int ti
             const int y = __shfl_up(upto, d);
             if (lane >= d) upto += y;
         }
-        if (lane == 63) w.waves[0][wave] = upto;
+        if (lane == 63) w.waves[wave] = upto;
         __syncthreads();
-        for (int k = 0; k < wave; ++k) upto += w.waves[0][k];
+        for (int k = 0; k < wave; ++k) upto += w.waves[k];
         if (upto >= need && upto - sum < need) {
             int left = need - (upto - sum);
             bool done = false;
@@ -512,28 +538,33 @@ __device__ __forceinline__ void border_of(SelectLds& w, int n, int count, int ti
         mask |= (K)((1 << bits) - 1) << low;
         need = w.found[1];
         top = low;
-        if (!ALL && w.found[2] == need) break;
+        if (w.found[2] == need) break;
     }
 }
 
-// Pages with above(p), and the first `need` with at(p), in order.
+// Pages with above(p), and the first `need` with at(p), in order: a thread's pages lie together.
 template <typename Above, typename At>
 __device__ __forceinline__ void emit(SelectLds& w, int n, int need, int* out, int tid, Above&& above, At&& at) {
-    const int lane = tid & 63, wave = tid >> 6;
-    int na = 0, ne = 0;
-    for (int p0 = 0; p0 < n; p0 += SE) {
-        const int p = p0 + tid;
-        const bool gt = p < n && above(p), eq = p < n && !gt && at(p);
-        const uint64_t mg = __ballot(gt), me = __ballot(eq), before = (1ull << lane) - 1;
-        __syncthreads();
-        if (lane == 0) w.waves[0][wave] = __popcll(mg), w.waves[1][wave] = __popcll(me);
-        __syncthreads();
-        int g = na + __popcll(mg & before), e = ne + __popcll(me & before);
-        for (int k = 0; k < SE / 64; ++k) {
-            if (k < wave) g += w.waves[0][k], e += w.waves[1][k];
-            na += w.waves[0][k], ne += w.waves[1][k];
-        }
+    const int lane = tid & 63, wave = tid >> 6, per = (n + SE - 1) / SE, p0 = min(n, tid * per), p1 = min(n, p0 + per);
+    int ng = 0, ne = 0;
+    for (int p = p0; p < p1; ++p) {
+        const bool gt = above(p);
+        ng += gt, ne += !gt && at(p);
+    }
+    int g = ng, e = ne;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(g, d), z = __shfl_up(e, d);
+        if (lane >= d) g += y, e += z;
+    }
+    if (lane == 63) w.above[wave] = g, w.at[wave] = e;
+    __syncthreads();
+    for (int k = 0; k < wave; ++k) g += w.above[k], e += w.at[k];
+    g -= ng, e -= ne;
+    for (int p = p0; p < p1; ++p) {
+        const bool gt = above(p), eq = !gt && at(p);
         if (gt || (eq && e < need)) out[g + min(e, need)] = p;
+        g += gt, e += eq;
     }
 }
 
@@ -549,7 +580,7 @@ __device__ void select_exact(SelectLds& w, const SelectArgs& a, const SelectUnit
     auto key = [&](int p) { return p < a.first || p >= x.live - a.last ? ~0ull : order(score[p]); };
     uint64_t border, mask;
     int need;
-    border_of<uint64_t, false>(w, x.live, a.count, tid, key, border, mask, need);
+    border_of<uint64_t>(w, x.live, a.count, tid, key, border, mask, need);
     emit(w, x.live, need, out, tid, [&](int p) { return (key(p) & mask) > border; },
          [&](int p) { return (key(p) & mask) == border; });
 }
@@ -559,6 +590,7 @@ template <int HD, bool SCORED>
 __global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
     extern __shared__ float sc[];
     __shared__ SelectLds w;
+    __shared__ __attribute__((aligned(16))) QueryLds<HD> ql;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, unit = (int)blockIdx.x;
     const SelectUnit x(a, unit);
     int* out = a.chosen + (size_t)unit * a.count;
@@ -570,33 +602,73 @@ __global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
         select_exact<HD>(w, a, x, unit, out, tid);
         return;
     }
-    if (tid == 0) w.worst = 0, w.near = 0, w.sure = 0;
-    __syncthreads();
-    float worst = 0.0f;
+    auto kept = [&](int p) { return p < a.first || p >= x.live - a.last; };
+    const int keep = a.first + a.last;
+    if (keep == a.count) {
+        emit(w, x.live, 0, out, tid, kept, [](int) { return false; });
+        return;
+    }
+    for (int i = tid; i < PS_BINS; i += SE) w.hist[i] = 0;
+    if (tid == 0) w.near = 0, w.sure = 0;
+    float worst = 0.0f, top = ninf(), least = -ninf();
     if constexpr (SCORED) {
         const float* from = a.score + (size_t)unit * a.wide;
-        for (int p = tid; p < x.live; p += SE) sc[p] = from[p];
+        for (int p = tid; p < x.live; p += SE) {
+            const float s = from[p];
+            sc[p] = s;
+            if (!kept(p)) top = fmaxf(top, s), least = fminf(least, s);
+        }
         for (int i = tid; i < a.chunks; i += SE) worst = fmaxf(worst, a.worst[(size_t)unit * a.chunks + i]);
     } else {
-        worst = score_pages<HD>(a, x, 0, x.live, sc, tid);
+        worst = score_pages<HD, SE / 64>(a, x, 0, x.live, sc, ql, tid, a.first, x.live - a.last, top, least);
     }
-    worst = wave_max(worst);
-    if (lane == 0) atomicMax(&w.worst, __float_as_uint(worst));  // (not below 0)
+    worst = wave_max(worst), top = wave_max(top), least = -wave_max(-least);
+    if (lane == 0) w.worst[wave] = worst, w.top[wave] = top, w.least[wave] = least;
     __syncthreads();
-    const float e2 = 2.0f * __uint_as_float(w.worst);
+#pragma unroll
+    for (int k = 0; k < SE / 64; ++k)
+        worst = fmaxf(worst, w.worst[k]), top = fmaxf(top, w.top[k]), least = fminf(least, w.least[k]);
+    const float e2 = 2.0f * worst;
     if (!(e2 < 0x1p40f)) {
         select_exact<HD>(w, a, x, unit, out, tid);
         return;
     }
-    auto kept = [&](int p) { return p < a.first || p >= x.live - a.last; };
-    uint32_t border, mask;
-    int need;
-    border_of<uint32_t, true>(w, x.live, a.count, tid, [&](int p) { return kept(p) ? ~0u : order(sc[p]); }, border, mask, need);
-    if (border == ~0u) {  // no more than what is always kept
-        emit(w, x.live, 0, out, tid, kept, [](int) { return false; });
-        return;
+    // The bin of the border, of even ones between the least and the largest. (By
+    // digits as border_of has them, nearly all fall into a few bins of the first: 2048
+    // pages 20 us, so 10.)
+    const float wide = (top - least) / PS_BINS, mul = top > least ? PS_BINS / (top - least) : 0.0f;
+    for (int p = tid; p < x.live; p += SE)
+        if (!kept(p)) atomicAdd(&w.hist[min((int)((sc[p] - least) * mul), PS_BINS - 1)], 1);
+    __syncthreads();
+    if (wave == 0) {
+        constexpr int B = PS_BINS / 64;
+        const int4* h = reinterpret_cast<const int4*>(w.hist);
+        int bin[B], sum = 0;
+        const int first = PS_BINS - B * (lane + 1), need = a.count - keep;
+#pragma unroll
+        for (int i = 0; i < B / 4; ++i) {
+            const int4 y = h[first / 4 + i];
+            bin[4 * i] = y.x, bin[4 * i + 1] = y.y, bin[4 * i + 2] = y.z, bin[4 * i + 3] = y.w;
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) sum += bin[i];
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(upto, d);
+            if (lane >= d) upto += y;
+        }
+        if (upto >= need && upto - sum < need) {
+            int left = need - (upto - sum), at = first + B - 1;
+#pragma unroll
+            for (int i = B - 1; i > 0; --i)
+                if (at == first + i && bin[i] < left) left -= bin[i], --at;
+            w.found[0] = at;
+        }
     }
-    const float t = unorder(border), high = t + e2, low = t - e2;
+    __syncthreads();
+    // (The roundings of a bin's ends are a few 2^-24 of the largest score: within E's 1.05.)
+    const float low = least + (float)w.found[0] * wide - e2, high = least + (float)(w.found[0] + 1) * wide + e2;
     int sure = 0;
     for (int p = tid; p < x.live; p += SE) {
         if (kept(p) || sc[p] > high) {
@@ -606,7 +678,12 @@ __global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
             if (i < PS_NEAR) w.page[i] = p;
         }
     }
-    if (sure) atomicAdd(&w.sure, sure);
+    const uint64_t any = __ballot(sure != 0);
+    if (any) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) sure += __shfl_xor(sure, d);
+        if (lane == 0) atomicAdd(&w.sure, sure);
+    }
     __syncthreads();
     const int near = w.near, left = a.count - w.sure;
     if (near > PS_NEAR) {
@@ -632,14 +709,16 @@ __global__ __launch_bounds__(SE) void page_select_kernel(SelectArgs a) {
 
 // Few (row, kv head)s of many pages: their scores by `chunks` workgroups each.
 template <int HD>
-__global__ __launch_bounds__(SE) void page_score_kernel(SelectArgs a) {
-    __shared__ float top[SE / 64];
+__global__ __launch_bounds__(SC) void page_score_kernel(SelectArgs a) {
+    __shared__ float top[SC / 64];
+    __shared__ __attribute__((aligned(16))) QueryLds<HD> ql;
     const int tid = threadIdx.x, unit = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks);
     const SelectUnit x(a, unit);
     const int share = (((x.live + 15) / 16 + a.chunks - 1) / a.chunks) * 16;
     const int p0 = chunk * share, p1 = min(x.live, p0 + share);
     float worst = 0.0f;
-    if (p0 < p1) worst = score_pages<HD>(a, x, p0, p1, a.score + (size_t)unit * a.wide, tid);
+    float most = 0.0f, least = 0.0f;
+    if (p0 < p1) worst = score_pages<HD, SC / 64>(a, x, p0, p1, a.score + (size_t)unit * a.wide, ql, tid, 0, 0, most, least);
     worst = wave_max(worst);
     if ((tid & 63) == 0) top[tid >> 6] = worst;
     __syncthreads();
@@ -653,7 +732,7 @@ hipError_t launch_select(int hd, const SelectArgs& a, hipStream_t st) {
 #define SL(HD)                                                                                                  \
     if (hd == HD) {                                                                                             \
         if (scored) {                                                                                           \
-            hipLaunchKernelGGL((page_score_kernel<HD>), dim3(units * (unsigned)a.chunks), dim3(SE), 0, st, a);  \
+            hipLaunchKernelGGL((page_score_kernel<HD>), dim3(units * (unsigned)a.chunks), dim3(SC), 0, st, a);  \
             hipLaunchKernelGGL((page_select_kernel<HD, true>), dim3(units), dim3(SE), lds, st, a);              \
         } else hipLaunchKernelGGL((page_select_kernel<HD, false>), dim3(units), dim3(SE), lds, st, a);          \
     }

@@ -461,15 +461,6 @@ __device__ __forceinline__ bool odd_values(const half_t* vt, int tid) {
     return __any(x != 0);
 }
 
-// A barrier for what the waves stored in LDS themselves (lgkmcnt): a fence would
-// also wait for the next tile's direct loads.
-__device__ __forceinline__ void lds_barrier() {
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-    __builtin_amdgcn_s_barrier();
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-}
-
 // The bounds of all waves' rows (a barrier).
 __device__ __forceinline__ Bounds together(const Bounds& mine, int (*wb)[6], int wave, int lane) {
     if (lane == 0) {
