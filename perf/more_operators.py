@@ -266,7 +266,7 @@ def prepare(case, seed):
 
 def _plan(s):
     c = s["c"]
-    return s["gpu"].page_plan(s["tk"], s["row"], s["table"], c["heads"], s["paged"], max(_ends(c)[0]),
+    return s["gpu"].page_plan(s["tk"], s["row"], s["table"], c["heads"], s["paged"], s["table"].shape[1] * c["page"],
                               starts=s["starts"], prefix=s["prefix"], window=c["window"], shared=c["shared"])
 
 
@@ -408,8 +408,9 @@ def _kernels(s):
                            s["div"], n, heads, c["rot"], THETA, s["m"], c["pairs"] == "interleaved", s["paged"], q_out=q)
         return {"q": q, "cache": s["cache"]}
     if c["kind"] == "select":
-        return g.select_pages(s["q"], 0, heads * hd, s["bounds"], s["table"], s["row"], s["tk"], max(_ends(c)[0]), heads,
-                              c["page"], c["count"], first=c["first"], last=c["last"])
+        return g.select_pages(s["q"], 0, heads * hd, s["bounds"], s["table"], s["row"], s["tk"],
+                              s["table"].shape[1] * c["page"], heads, c["page"], c["count"], first=c["first"],
+                              last=c["last"])
     if c["kind"] == "decode":
         plan = s["plan"] if c["plan"] == "kept" else _plan(s)
         return g.attn_decode_paged(s["q"], 0, heads * hd, s["paged"], plan, heads, hd ** -0.5, softcap=c["softcap"],
