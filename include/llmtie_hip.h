@@ -484,9 +484,10 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
 
 /* The same over `count` pages of each (row, kv head): chosen[(r * kv_heads + h) *
  * count ..] are numbers of pages within the sequence (device int32, as
- * llmtie_select_pages leaves them, any order; ones below 0 or with no position that
- * the row has name nothing, a page named twice counts twice). Row r sees those of
- * their positions that are below tk_dev[r]. */
+ * llmtie_select_pages leaves them, any order, none twice; ones below 0 or with no
+ * position that the row has name nothing). Row r sees those of their positions that
+ * are below tk_dev[r]. Rows of one sequence that follow one another, as a prompt's do,
+ * are attended together, each page read once for those that selected it. */
 size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
                                       size_t head_dim);
 int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,

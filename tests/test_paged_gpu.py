@@ -72,8 +72,8 @@ def test_decode(gpu, c):
 def covered(plan, nseq, group):
     """For each row the blocks that its items walk, in the plan's words."""
     d = plan.data.cpu().tolist()
-    total, ns = d[0], d[1]
-    at = 16 + 8 * nseq + (8 * nseq % 16)
+    total, wide = d[0], d[1]
+    at = (16 + 12 * nseq + 15) // 16 * 16
     items = [d[at + 16 * i:at + 16 * i + 16] for i in range(total)]
     got = [[] for _ in range(nseq)]
     for i, e in enumerate(items):
@@ -81,14 +81,15 @@ def covered(plan, nseq, group):
         blocks = [b if b < na else b0 + b - na if b - na < c0 - b0 else d0 + b - na - (c0 - b0) for b in range(e[8], e[9])]
         for r in range(e[0], e[0] + e[1]):
             got[r] += blocks
-        assert e[1] * group <= 32 and (i < ns or e[1] == 1)
+        assert e[1] * group <= 32 and (i < wide or e[1] == 1)
     for r in range(nseq):
-        o0, on, s0, sn, step, col = d[16 + 8 * r:16 + 8 * r + 6]
+        o0, on, s0, sn, step, col, own = d[16 + 12 * r:16 + 12 * r + 7]
         for j in range(on):
-            assert items[ns + o0 + j][0] == r
+            e = items[o0 + j if own >= 0 else wide + o0 + j]
+            assert e[0] + max(own, 0) // group == r and e[3] & 2 == 0 and (own < 0 or o0 + j < wide)
         for j in range(sn):
             e = items[s0 + j * step]
-            assert s0 + j * step < ns and e[0] + col // group == r and col % group == 0
+            assert s0 + j * step < wide and e[3] & 2 and e[0] + col // group == r and col % group == 0
     return got
 
 
@@ -616,3 +617,91 @@ def test_select_small_and_large_queries(gpu, scale):
     got = gpu.select_pages(q.cuda().view(-1), 0, heads * hd, bounds.cuda(), ints(table.tolist()), None, ints([n * page]),
                            n * page, heads, page, 30, 0, 1)
     assert torch.equal(got.cpu(), want)
+
+
+def put(laid, t, j, dim, x):
+    """x into dim `dim` of the value of kv head 0 at position j of sequence t, in its page (which others may share)."""
+    p = int(laid.table[t, j // laid.page])
+    laid.pool[1, p, 0, j % laid.page, dim] = x
+    for s in range(len(laid.v)):
+        at = (laid.table[s] == p).nonzero()
+        if len(at):
+            i = int(at[0, 0]) * laid.page + j % laid.page
+            if i < laid.lengths[s]:
+                laid.v[s][0, i, dim] = x
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128), (4, 4, 64), (16, 1, 64)])
+def test_not_finite_shared_and_tiles(gpu, shape):
+    """Values that are not finite in a shared prefix, in one row's own part, and between the rows of a prompt."""
+    per = 11
+    laid = pr.Laid([768 + per, 900, 800], shape[1], shape[2], 64, [0, 3], [768], seed=8)
+    laid.pool[1][torch.isnan(laid.pool[1])] = math.inf  # what no row sees
+    put(laid, 0, 100, 3, math.inf)
+    put(laid, 0, 700, 4, math.nan)
+    put(laid, 0, 701, 5, -math.inf)
+    put(laid, 0, 101, 5, math.inf)  # and its opposite: NaN
+    put(laid, 0, 768 + 4, 6, -math.inf)  # seen from the prompt's fifth row on
+    put(laid, 1, 800, 7, math.inf)
+    tk = [768 + j + 1 for j in range(per)] + [900, 800]
+    row = [0] * per + [1, 2]
+    got, want, tol, _ = decode(gpu, laid, shape, tk, row, [0, per + 2], [768])
+    close(got, want, tol)
+    assert torch.isinf(want[5, 0, 6]) and torch.isfinite(want[3, 0, 6]) and torch.isnan(want[0, 0, 5])
+
+
+def test_not_finite_selected(gpu):
+    heads, kv, hd, page, per = 8, 2, 128, 32, 20
+    laid = pr.Laid([700], kv, hd, page, seed=8)
+    laid.pool[1][torch.isnan(laid.pool[1])] = math.nan
+    put(laid, 0, 5 * page + 3, 6, math.inf)
+    put(laid, 0, 690, 7, math.nan)
+    tk = [700 - per + 1 + j for j in range(per)]
+    r = random.Random(1)
+    chosen = torch.tensor([[sorted(r.sample(range(21), 5) + [21]) for _ in range(kv)] for _ in range(per)], dtype=torch.int32)
+    chosen[3, :, 0], chosen[4, :, 0] = 5, 6
+    chosen = chosen.sort(-1).values
+    for i in range(per):  # none twice
+        for h in range(kv):
+            ids = sorted(set(chosen[i, h].tolist()))
+            chosen[i, h] = torch.tensor(ids + [-1] * (6 - len(ids)))
+    q = queries(3, per, heads, hd)
+    got = gpu.attn_decode_selected(q.cuda().view(-1), 0, heads * hd, laid.cache(), ints(laid.table.tolist()), ints([0] * per),
+                                   ints(tk), chosen.cuda(), heads, hd ** -0.5)
+    want, tol = pr.attend(laid, q, tk, [0] * per, hd ** -0.5, chosen=chosen)
+    close(got, want, tol)
+    one = gpu.attn_decode_selected(q[3].cuda().view(-1), 0, heads * hd, laid.cache(), ints(laid.table.tolist()), None,
+                                   ints(tk[3:4]), chosen[3:4].cuda(), heads, hd ** -0.5)
+    close(one, want[3:4], tol[3:4])
+    assert torch.isinf(want[3, 0, 6])
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128), (2, 2, 64), (32, 2, 64), (5, 1, 128)])
+@pytest.mark.parametrize("window", [0, 90])
+def test_prompts_rows_masked(gpu, shape, window):
+    """Rows of prompts in no group, in tiles that are aligned to sequences and that are not, with windows, caps and
+    biases; some rows see nothing."""
+    lens = [300, 41, 700]
+    laid = pr.Laid(lens, shape[1], shape[2], 32, seed=3)
+    per = [37, 41, 64]
+    tk = [m - p + 1 + j for m, p in zip(lens, per) for j in range(p)]
+    row = [t for t, p in enumerate(per) for _ in range(p)]
+    tk[5] = tk[40] = 0
+    got, want, tol, plan = decode(gpu, laid, shape, tk, row, window=window, shared=3, softcap=20.0, bias=True, max_tk=700)
+    close(got, want, tol)
+    assert not got.view(want.shape)[5].any()
+    for t, blocks in enumerate(covered(plan, len(tk), shape[0] // shape[1])):
+        need = {int(j) // 32 for j in pr.seen_of(tk[t], 0, window, 3, tk[t]).nonzero()}
+        assert len(set(blocks)) == len(blocks) and need <= set(blocks)
+
+
+def test_many_prompt_rows(gpu):
+    """More rows than a thread each, of sequences that share a document and of some that do not."""
+    shape, per, n = (4, 1, 64), 100, 9
+    lens = [256 + per if t < 6 else 90 + per for t in range(n)]
+    laid = pr.Laid(lens, 1, 64, 32, [0, 6], [256], seed=3, cols=22)
+    tk = [m - per + 1 + j for m in lens for j in range(per)]
+    row = [t for t in range(n) for _ in range(per)]
+    got, want, tol, plan = decode(gpu, laid, shape, tk, row, [0, 6 * per], [256], max_tk=700)
+    close(got, want, tol)
+    covered(plan, len(tk), 4)

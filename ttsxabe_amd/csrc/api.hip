@@ -1599,20 +1599,21 @@ constexpr size_t PG_MAX_ROWS = (size_t)1 << 20;
 
 // How a step over pages is divided, from what the host knows of it.
 struct PagedSizes {
-    size_t target, max_shared, max_own, items;
+    size_t target, max_wide, max_own, items;
     bool whole;
 };
 // Items of a kv head: two workgroups a compute unit, fewer where the rows do not
-// hold four blocks for each. Rows that no group shares anything of and whose bound is
-// short are one item each.
+// hold four blocks for each. Few rows of a short bound are one item each, prefix and all.
 PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
     PagedSizes s;
     const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
+    const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads));
     s.target = std::max<size_t>(1, std::min(2 * (size_t)compute_units() / kv_heads, (nseq * blocks + 3) / 4));
-    s.whole = groups == 0 && blocks <= (size_t)RD_WHOLE;
-    const size_t tiles = groups ? nseq / (size_t)PG_TILE_ROWS((int)(heads / kv_heads)) + groups : 0;
+    s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * (size_t)compute_units());
+    // Shared tiles, and tiles of one sequence's rows.
+    const size_t tiles = (s.whole ? 0 : groups ? nseq / per + groups : 0) + (nseq + per - 1) / per;
     s.max_own = s.whole ? nseq : nseq + s.target;
-    s.max_shared = groups ? tiles + s.target : 0;
+    s.max_wide = s.whole ? nseq : tiles + s.target;
     s.items = s.whole ? nseq : nseq + tiles + s.target;
     return s;
 }
@@ -1631,16 +1632,27 @@ int paged_checks(size_t nseq, size_t groups, size_t max_tk, const TableArg& t, s
     return LLMTIE_OK;
 }
 size_t paged_floats(const PagedSizes& z, size_t heads, size_t kv_heads, size_t head_dim) {
-    return smul(sadd(smul(z.max_own, heads), smul(z.max_shared, PG_COLS, kv_heads)), head_dim + 2);
+    return smul(sadd(smul(z.max_own, heads), smul(z.max_wide, PG_COLS, kv_heads)), head_dim + 2);
 }
 Pages pages_of(const uint16_t* cache, const TableArg& t, size_t pages, size_t page) {
     return Pages{cache, t.ids, (int)t.rows, (int)t.cols, page_shift(page), (int)pages};
 }
 
 // Workgroups of a (row, kv head) over its selected pages: those that fill the
-// compute units once, of four blocks or more.
-size_t selected_runs(size_t units, size_t blocks) {
-    return std::max<size_t>(1, std::min((blocks + 3) / 4, (size_t)compute_units() / std::max<size_t>(1, units)));
+// compute units once, of four blocks or more. Of a tile of rows: two a compute unit, no
+// more than its rows have.
+struct SelectedSizes {
+    size_t runs, tile_runs, max_own, max_wide;
+};
+SelectedSizes selected_sizes(size_t nseq, size_t blocks, size_t heads, size_t kv_heads) {
+    SelectedSizes s;
+    const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads)), tiles = (nseq + per - 1) / per;
+    const size_t cus = (size_t)compute_units();
+    s.runs = std::max<size_t>(1, std::min((blocks + 3) / 4, cus / std::max<size_t>(1, smul(nseq, kv_heads))));
+    s.tile_runs = std::max<size_t>(1, std::min(std::min(nseq, per) * s.runs, 2 * cus / std::max<size_t>(1, smul(tiles, kv_heads))));
+    s.max_own = s.runs > 1 ? nseq * s.runs : 0;
+    s.max_wide = s.tile_runs > 1 && nseq > 1 ? tiles * s.tile_runs : 0;
+    return s;
 }
 
 // Workgroups that score the pages of a (row, kv head): one (with its selection in
@@ -1685,8 +1697,7 @@ int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q
 size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
     if (kv_heads == 0 || heads == 0 || heads % kv_heads != 0 || heads / kv_heads > 16 || nseq > PG_MAX_ROWS) return 0;
     const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
-    const size_t rows = smul(nseq, PG_ROW);
-    return sadd(sadd(PG_HEAD + rows, rows % 16), smul(sadd(z.max_shared, z.max_own), PG_ITEM));
+    return sadd(plan_items_at(nseq), smul(sadd(z.max_wide, z.max_own), PG_ITEM));
 }
 
 int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev, const int32_t* lo_dev, size_t nseq,
@@ -1718,7 +1729,7 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
     a.shift = page_shift(page);
     a.group = (int)(heads / kv_heads);
     a.kv_heads = (int)kv_heads;
-    a.max_shared = (int)z.max_shared;
+    a.max_wide = (int)z.max_wide;
     a.max_own = (int)z.max_own;
     a.target = (int)z.target;
     a.whole = z.whole ? 1 : 0;
@@ -1766,7 +1777,7 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
     a.nseq = (int)nseq;
     a.kv_heads = (int)kv_heads;
     a.group = (int)(heads / kv_heads);
-    a.max_shared = (int)z.max_shared;
+    a.max_wide = (int)z.max_wide;
     a.max_own = (int)z.max_own;
     a.items = (int)z.items;
     a.runs = 1;
@@ -1779,9 +1790,10 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
 
 size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
                                       size_t head_dim) {
-    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || nseq == 0) return 0;
-    const size_t runs = selected_runs(smul(nseq, kv_heads), smul(count, (page + 31) / 32));
-    return runs > 1 ? smul(smul(nseq, heads, runs), head_dim + 2) : 0;
+    if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16 || nseq == 0 || nseq > PG_MAX_ROWS)
+        return 0;
+    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), heads, kv_heads);
+    return smul(sadd(smul(z.max_own, heads), smul(z.max_wide, PG_COLS, kv_heads)), head_dim + 2);
 }
 
 int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
@@ -1801,8 +1813,8 @@ int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size
     if (chosen_len < smul(units, count)) return overrun_slice(smul(units, count), chosen_len);
     if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
     if (nseq == 0) return ok();
-    const size_t runs = selected_runs(units, smul(count, page / 32));
-    if (smul(units, runs) > MAX_WGS) return overrun_slice(smul(units, runs), MAX_WGS);
+    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), heads, kv_heads);
+    if (smul(units, z.runs) > MAX_WGS) return overrun_slice(smul(units, z.runs), MAX_WGS);
     const size_t floats = llmtie_attn_selected_workspace(nseq, count, page, heads, kv_heads, head_dim);
     if (ws_len < floats) return overrun_slice(floats, ws_len);
     if (!q || !cache || !table || !tk_dev || (count && !chosen) || !out || (floats && !ws)) return invalid("a buffer");
@@ -1820,10 +1832,12 @@ int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size
     a.nseq = (int)nseq;
     a.kv_heads = (int)kv_heads;
     a.group = (int)(heads / kv_heads);
-    a.max_own = (int)(nseq * runs);
+    a.max_own = (int)z.max_own;
+    a.max_wide = (int)z.max_wide;
     a.count = (int)count;
-    a.runs = (int)runs;
-    a.merge = runs > 1 ? 1 : 0;
+    a.runs = (int)z.runs;
+    a.tile_runs = (int)z.tile_runs;
+    a.merge = z.max_own || z.max_wide ? 1 : 0;
     a.scale = scale;
     a.softcap = softcap;
     return launched("attn_decode_selected", launch_paged((int)head_dim, a, S(stream)));

@@ -17,12 +17,17 @@ struct Pages {
 };
 
 constexpr int PG_GROUPS = 1024;  // groups of a plan at most
-constexpr int PG_COLS = 32;      // (row, query head) columns of a shared tile at most
+constexpr int PG_COLS = 32;      // (row, query head) columns of a tile at most
 
-// A plan's words: the header, PG_ROW a row, then PG_ITEM an item, the shared
-// tiles' items first.
-constexpr int PG_HEAD = 16, PG_ROW = 8, PG_ITEM = 16;
-constexpr int PG_TILE_ROWS(int group) { return PG_COLS / group; }
+// A plan's words: the header, PG_ROW a row, then PG_ITEM an item, the tiles' (the
+// wide ones) first.
+constexpr int PG_HEAD = 16, PG_ROW = 12, PG_ITEM = 16;
+__host__ __device__ constexpr int PG_TILE_ROWS(int group) { return PG_COLS / group; }
+__host__ __device__ inline size_t plan_items_at(size_t nseq) { return (PG_HEAD + PG_ROW * nseq + 15) / 16 * 16; }
+// What an item is: it writes its rows' context, it is of a shared tile.
+constexpr int PG_WHOLE = 1, PG_SHARED = 2;
+// Pages of a sequence up to which rows that selected pages of it are attended together.
+constexpr int PG_UNION = 4096;
 
 struct PagePlanArgs {
     const int* tk;      // [nseq] live positions
@@ -32,7 +37,7 @@ struct PagePlanArgs {
     const int* prefix;  // [groups] leading positions that a group's rows share
     int* plan;
     int nseq, groups, window, shared, rows, cols, shift, group, kv_heads;
-    int max_shared, max_own;  // items there is room for
+    int max_wide, max_own;    // items there is room for
     int target;               // items of a kv head that the work is divided into
     int whole;                // every row is one item (no group shares)
 };
@@ -47,12 +52,13 @@ struct PagedArgs {
     const int* chosen;   // selected pages only: [nseq][kv_heads][count]
     const float* slopes;
     const int* plan;     // null: selected pages
-    float* part;         // own items' O, then the shared ones', then their (m, l)
+    float* part;         // own items' O, then the wide ones', then their (m, l)
     long q_stride;
     int nseq, kv_heads, group;
-    int max_shared, max_own;
+    int max_wide, max_own;
     int items;           // of a kv head, at most
     int count, runs;     // selected pages: how many, and the workgroups of a (row, kv head)
+    int tile_runs;       // and of a tile of rows at most
     int stream;          // more bytes than are worth keeping in the Infinity Cache
     int merge;           // some row may have partials
     float scale, softcap;

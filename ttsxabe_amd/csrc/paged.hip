@@ -26,7 +26,11 @@ constexpr int PW = 4, PT = PW * LLMTIE_WAVE;
 template <int HD, int MODE, int NQT>
 struct Columns {
     static constexpr int NS = HD / 32, NT = HD / 16;
-    half8 qh[NQT][NS], ql[NQT][NS];
+    // q's lower halves: of two tiles in LDS, where one of the four waves (whose columns
+    // are the same) put them (in registers too, 210 of them spilled at HD 128).
+    static constexpr bool LOW_LDS = NQT > 1;
+    half8 qh[NQT][NS], ql[LOW_LDS ? 1 : NQT][LOW_LDS ? 1 : NS];
+    const half8* low;
     floatx4 o[NT][NQT];
     float m[NQT], l[NQT];
     float slope2[NQT];
@@ -37,9 +41,11 @@ struct Columns {
     int grp;
 
     // Columns of `rows` rows from r0 on, `group` heads of kv head kh each.
-    __device__ __forceinline__ void start(const PagedArgs& a, int r0, int rows, int kh, int lane, int tk) {
-        const int col = lane & 15, n = rows * a.group;
+    // (LOW_LDS: with a barrier.)
+    __device__ __forceinline__ void start(const PagedArgs& a, int r0, int rows, int kh, int lane, int tk, half8* mem = nullptr) {
+        const int col = lane & 15, n = rows * a.group, wave = (int)threadIdx.x >> 6;
         grp = lane >> 4;
+        low = mem;
         sl2 = a.scale * LLMTIE_LOG2E;
         c1 = (MODE & SM_CAP) != 0 ? a.scale / a.softcap : 0.0f;
         c2 = a.softcap * LLMTIE_LOG2E;
@@ -49,14 +55,18 @@ struct Columns {
             const bool has = 16 * u + col < n;
             const float* q = a.q + (size_t)(r0 + row) * a.q_stride + (size_t)(kh * a.group + g) * HD + 8 * grp;
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
+            for (int s = 0; s < NS; ++s) {
+                half8 lo;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     half_t x, y;
                     split_h(has ? q[32 * s + j] : 0.0f, x, y);
                     qh[u][s][j] = x;
-                    ql[u][s][j] = y;
+                    lo[j] = y;
                 }
+                if constexpr (!LOW_LDS) ql[u][s] = lo;
+                else if (wave == s) mem[(u * NS + s) * 64 + lane] = lo;
+            }
             if constexpr ((MODE & SM_BIAS) != 0) {
                 slope2[u] = a.slopes[kh * a.group + g] * LLMTIE_LOG2E;
                 at[u] = (tk >= 0 ? tk : min(a.tk[r0 + row], a.p.cols << a.p.shift)) - 1;
@@ -68,21 +78,30 @@ struct Columns {
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int u = 0; u < NQT; ++u) o[t][u] = zero_f4();
+        if constexpr (LOW_LDS) lds_barrier();
+    }
+    __device__ __forceinline__ half8 lower(int u, int s, int lane) const {
+        if constexpr (LOW_LDS) return low[(u * NS + s) * 64 + lane];
+        else return ql[u][s];
     }
     __device__ __forceinline__ void scores(const half8 (&k)[2 * NS]) {
 #pragma unroll
         for (int u = 0; u < NQT; ++u) sc[u][0] = sc[u][1] = zero_f4();
+        int lane = threadIdx.x & 63;
+        if constexpr (LOW_LDS) asm volatile("" : "+v"(lane));  // read each time, not held over the blocks
 #pragma unroll
         for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int T = 0; T < 2; ++T)
+            for (int u = 0; u < NQT; ++u) {
+                const half8 lo = lower(u, s, lane);
 #pragma unroll
-                for (int u = 0; u < NQT; ++u) {
-                    sc[u][T] = mfma16(k[T * NS + s], ql[u][s], sc[u][T]);
+                for (int T = 0; T < 2; ++T) {
+                    sc[u][T] = mfma16(k[T * NS + s], lo, sc[u][T]);
                     sc[u][T] = mfma16(k[T * NS + s], qh[u][s], sc[u][T]);
                 }
+            }
     }
-    // Keys k0 ..; see(key): whether they are seen, where not all are.
+    // Keys k0 ..; see(u, key): whether this lane's column of sixteen u sees them, where not all are.
     template <typename See>
     __device__ __forceinline__ void softmax(int k0, bool part, See&& see) {
 #pragma unroll
@@ -96,7 +115,7 @@ struct Columns {
                     const int key = k0 + 8 * grp + 4 * T + r;
                     float s = (MODE & SM_CAP) != 0 ? sc[u][T][r] : sc[u][T][r] * sl2;
                     if constexpr ((MODE & SM_BIAS) != 0) s = __builtin_fmaf(-slope2[u], (float)(at[u] - key), s);
-                    if (part) s = see(key) ? s : ninf();
+                    if (part) s = see(u, key) ? s : ninf();
                     sc[u][T][r] = s;
                     mx = fmaxf(mx, s);
                 }
@@ -133,51 +152,74 @@ struct Columns {
     }
 };
 
-// LDS of a workgroup: the four waves' O rows, padded, and their (m, l).
+// LDS of a workgroup: sixteen of the four waves' O rows, padded, and their (m, l).
 template <int HD>
 struct WaveParts {
     static constexpr int OP = HD + 4;
-    float o[PW * PG_COLS * OP];
-    float m[PW][PG_COLS], l[PW][PG_COLS];
+    float o[PW * 16 * OP];
+    float m[PW][16], l[PW][16];
+    half8 low[2 * (HD / 32) * 64];  // Columns::low
 };
 
-// Where a tile's columns go: the context itself, or partials.
+// Where a tile's columns go: the context itself (a row's heads together, rows
+// `stride` apart), or partials.
 struct Sink {
-    float* o;     // [columns][HD]
+    float* o;
     float2* ml;   // null: the context
+    long stride;  // elements from a row's columns to the next one's
 };
 
-// The four waves' columns joined.
-template <int HD, int MODE, int NQT>
-__device__ __forceinline__ void join(WaveParts<HD>& w, Columns<HD, MODE, NQT>& c, int cols, const Sink& to, int tid) {
+// The four waves' columns joined, sixteen at a time. CHECK: false, with nothing
+// written, where something is not finite.
+template <int HD, int MODE, int NQT, bool CHECK>
+__device__ __forceinline__ bool join(WaveParts<HD>& w, Columns<HD, MODE, NQT>& c, int group, int cols, const Sink& to,
+                                     int tid) {
     constexpr int NT = HD / 16, OP = WaveParts<HD>::OP;
     const int lane = tid & 63, wave = tid >> 6, col = lane & 15, grp = lane >> 4;
+    bool odd = false;
+    if constexpr (CHECK) {
+        float x = 0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int u = 0; u < NQT; ++u) x += (c.o[t][u][0] + c.o[t][u][1]) + (c.o[t][u][2] + c.o[t][u][3]);
+        odd = !(x - x == 0.0f);
+    }
 #pragma unroll
     for (int u = 0; u < NQT; ++u) {
+        if (16 * u >= cols) break;
+        const int n = min(16, cols - 16 * u);
         const float l = sum4grp(c.l[u]);
-        if (16 * u + col >= cols) continue;
-        const int at = wave * PG_COLS + 16 * u + col;
+        if (u) __syncthreads();
+        if (col < n) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) *reinterpret_cast<floatx4*>(&w.o[at * OP + 16 * t + 4 * grp]) = c.o[t][u];
-        if (grp == 0) w.m[wave][16 * u + col] = c.m[u], w.l[wave][16 * u + col] = l;
-    }
-    __syncthreads();
-    for (int e4 = tid; e4 < cols * (HD / 4); e4 += PT) {
-        const int g = e4 / (HD / 4), d = 4 * (e4 % (HD / 4));
-        float M = w.m[0][g], L = 0.0f;
-#pragma unroll
-        for (int k = 1; k < PW; ++k) M = fmaxf(M, w.m[k][g]);
-        floatx4 y = zero_f4();
-#pragma unroll
-        for (int k = 0; k < PW; ++k) {
-            const float f = ex2(w.m[k][g] - M);
-            L += w.l[k][g] * f;
-            y += *reinterpret_cast<const floatx4*>(&w.o[(k * PG_COLS + g) * OP + d]) * f;
+            for (int t = 0; t < NT; ++t)
+                *reinterpret_cast<floatx4*>(&w.o[(wave * 16 + col) * OP + 16 * t + 4 * grp]) = c.o[t][u];
+            if (grp == 0) w.m[wave][col] = c.m[u], w.l[wave][col] = l;
         }
-        if (!to.ml) y *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
-        *reinterpret_cast<floatx4*>(to.o + 4 * (size_t)e4) = y;
-        if (to.ml && d == 0) to.ml[g] = make_float2(M, L);
+        if (CHECK && u == 0) {
+            if (__syncthreads_or(odd)) return false;
+        } else {
+            __syncthreads();
+        }
+        for (int e4 = tid; e4 < n * (HD / 4); e4 += PT) {
+            const int g = e4 / (HD / 4), d = 4 * (e4 % (HD / 4)), at = 16 * u + g;
+            float M = w.m[0][g], L = 0.0f;
+#pragma unroll
+            for (int k = 1; k < PW; ++k) M = fmaxf(M, w.m[k][g]);
+            floatx4 y = zero_f4();
+#pragma unroll
+            for (int k = 0; k < PW; ++k) {
+                const float f = ex2(w.m[k][g] - M);
+                L += w.l[k][g] * f;
+                y += *reinterpret_cast<const floatx4*>(&w.o[(k * 16 + g) * OP + d]) * f;
+            }
+            if (!to.ml) y *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
+            *reinterpret_cast<floatx4*>(to.o + (size_t)(at / group) * to.stride + (at % group) * HD + d) = y;
+            if (to.ml && d == 0) to.ml[at] = make_float2(M, L);
+        }
     }
+    return true;
 }
 
 template <int HD, int AUX>
@@ -194,47 +236,58 @@ __device__ __forceinline__ void load_v(half8 (&v)[HD / 16], const Region& r, int
             half8, __builtin_amdgcn_raw_buffer_load_b128(r.r, 16 * lane + 1024 * (2 * (HD / 32) + j), 0, AUX));
 }
 
+// A wave's blocks of an item, every fourth from `base` on: lane k holds the
+// k-th's first position, its page (-1: nothing to read) and which of a tile's rows
+// see it, 64 looked up at a time.
+struct Blocks {
+    int pos, id;
+    uint32_t rows;
+    // place(i, rows): block i's first position, or -1. Returns whether a page that is needed is not there.
+    template <typename Place>
+    __device__ __forceinline__ bool look(const PagedArgs& a, int table, int i, int end, Place&& place) {
+        id = -1, pos = 0, rows = 0;
+        if (i >= end) return false;
+        pos = place(i, rows);
+        if (pos < 0) return false;
+        const int at = pos >> a.p.shift;
+        id = at < a.p.cols ? a.p.table[(size_t)table * a.p.cols + at] : -1;
+        if (id >= 0 && id < a.p.pages) return false;
+        id = -1;
+        return true;
+    }
+    template <int HD>
+    __device__ __forceinline__ Region block(const PagedArgs& a, int kh, int k) const {
+        const int i = __builtin_amdgcn_readlane(id, k), p = __builtin_amdgcn_readlane(pos, k), s = a.p.shift - 5;
+        const size_t b = (((size_t)max(i, 0) * a.kv_heads + kh) << s) + ((p >> 5) & ((1 << s) - 1));
+        return region(reinterpret_cast<const char*>(a.p.cache) + b * (128 * HD), i < 0 ? 0 : 128 * HD);
+    }
+    __device__ __forceinline__ bool has(int k) const { return __builtin_amdgcn_readlane(id, k) >= 0; }
+    __device__ __forceinline__ int key0(int k) const { return __builtin_amdgcn_readlane(pos, k); }
+};
+
 // One row's columns (a kv head's query heads), the waves taking every fourth
-// block of positions begin to end of its list; place(i) is block i's first
-// position, or -1. Bound by reading K and V: the next block's 16 loads a lane
-// are in flight while one is computed.
+// of blocks begin to end. Bound by reading K and V: the next block's 16 loads a lane
+// are in flight while one is computed. Returns false, with nothing written, where
+// something is not finite (see tile).
 template <int HD, int MODE, int AUX, typename Place>
-__device__ __forceinline__ void one_row(const PagedArgs& a, WaveParts<HD>& w, int row, int table, int kh, int begin, int end,
+__device__ __forceinline__ bool one_row(const PagedArgs& a, WaveParts<HD>& w, int row, int table, int kh, int begin, int end,
                                         int f, int lo, int tk, const Sink& to, Place&& place) {
     constexpr int NS = HD / 32, NT = HD / 16;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const size_t stride = (size_t)a.kv_heads << (a.p.shift - 5);  // blocks of a page
-    const int per = 1 << (a.p.shift - 5);
     Columns<HD, MODE, 1> c;
-    int id = -1, pos = 0;
-    bool bad = false;
-    auto look = [&](int base) {
-        const int i = base + wave + PW * lane;
-        id = -1, pos = 0;
-        if (i < end) {
-            pos = place(i);
-            if (pos >= 0) {
-                const int at = pos >> a.p.shift;
-                id = at < a.p.cols ? a.p.table[(size_t)table * a.p.cols + at] : -1;
-                if (id < 0 || id >= a.p.pages) id = -1, bad = true;
-            }
-        }
-    };
+    Blocks at;
     struct Block {
         half8 k[2 * NS], v[NT];
     };
     auto load = [&](Block& x, int k) __attribute__((always_inline)) {
-        const int i = __builtin_amdgcn_readlane(id, k), p = __builtin_amdgcn_readlane(pos, k);
-        const Region r = region(reinterpret_cast<const char*>(a.p.cache) +
-                                    ((size_t)max(i, 0) * stride + (size_t)kh * per + ((p >> 5) & (per - 1))) * (128 * HD),
-                                i < 0 ? 0 : 128 * HD);
+        const Region r = at.block<HD>(a, kh, k);
         load_k<HD, AUX>(x.k, r, lane);
         load_v<HD, AUX>(x.v, r, lane);
     };
     auto fold = [&](Block& x, int k) __attribute__((always_inline)) {
-        if (__builtin_amdgcn_readlane(id, k) < 0) return;
-        const int k0 = __builtin_amdgcn_readlane(pos, k);
-        auto see = [&](int key) { return key < f || (key >= lo && key < tk); };
+        if (!at.has(k)) return;
+        const int k0 = at.key0(k);
+        auto see = [&](int, int key) { return key < f || (key >= lo && key < tk); };
         const bool part = !(k0 + 32 <= f || (k0 >= lo && k0 + 32 <= tk));
         c.scores(x.k);
         c.softmax(k0, part, see);
@@ -243,22 +296,22 @@ __device__ __forceinline__ void one_row(const PagedArgs& a, WaveParts<HD>& w, in
             const int grp = lane >> 4;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool on = see(k0 + 8 * grp + j);
+                const bool on = see(0, k0 + 8 * grp + j);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) x.v[t][j] = on ? x.v[t][j] : (half_t)0.0f;
             }
         }
         c.values(x.v);
     };
-    bool any = false;
+    bool gone = false;
     Block x0, x1;
     for (int base = begin; base < end; base += PW * 64) {
-        look(base);
-        any = any || __any(bad);
+        const bool none = at.look(a, table, base + wave + PW * lane, end, place);
+        gone = gone || __any(none);
         const int n = min(64, (end - base - wave + PW - 1) / PW);  // the wave's blocks
         if (n <= 0) break;
         load(x0, 0);
-        load(x1, min(1, 63));
+        load(x1, 1);
         if (base == begin) c.start(a, row, 1, kh, lane, tk);
         for (int k = 0; k < n; k += 2) {
             fold(x0, k);
@@ -268,82 +321,140 @@ __device__ __forceinline__ void one_row(const PagedArgs& a, WaveParts<HD>& w, in
         }
     }
     if (begin + wave >= end) c.start(a, row, 1, kh, lane, tk);
-    if (any) c.l[0] = __builtin_nanf("");
-    join<HD, MODE, 1>(w, c, a.group, to, tid);
+    if (gone) c.l[0] = __builtin_nanf("");
+    return join<HD, MODE, 1, true>(w, c, a.group, a.group, to, tid);
 }
 
-// A shared tile: up to 32 columns of `rows` rows from r0 on, every key of its
-// blocks seen by all of them. The next block's keys are loaded once the scores
-// have this one's, and its values once the products have them.
-template <int HD, int MODE, int NQT>
-__device__ __forceinline__ void shared_tile(const PagedArgs& a, WaveParts<HD>& w, int r0, int rows, int table, int kh,
-                                            int first, int begin, int end, const Sink& to) {
+// What a column of a tile sees: the first f positions and those from lo to tk.
+struct ColumnSees {
+    int f, lo, tk;
+};
+
+// A tile: up to 32 columns of `rows` rows of one sequence or of one shared prefix, from r0
+// on. The next block's keys are loaded once the scores have this one's, and its
+// values once the products have them. See::ALL: its rows see all keys; OWN: each sees
+// keys of its own, sees(i) of the tile's i-th row.
+//
+// Returns false, with nothing written, where something is not finite. A value that a row
+// does not see, or whose weight's lower half is 0 or below, may then have made a NaN of an
+// infinity or of nothing; the rows are taken again one by one, as ONE: values that
+// the row does not see are cleared, and those that are not finite are added as they are.
+enum class See { ALL, OWN, ONE };
+template <int HD, int MODE, int NQT, See SEE, typename Place, typename Sees>
+__device__ __forceinline__ bool tile(const PagedArgs& a, WaveParts<HD>& w, int r0, int rows, int table, int kh, int begin,
+                                     int end, const Sink& to, Place&& place, Sees&& sees) {
     constexpr int NS = HD / 32, NT = HD / 16;
+    constexpr bool MASKED = SEE != See::ALL;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const size_t stride = (size_t)a.kv_heads << (a.p.shift - 5);
-    const int per = 1 << (a.p.shift - 5);
     Columns<HD, MODE, NQT> c;
-    int id = -1;
-    bool any = false;
+    Blocks at;
+    bool gone = false;
     half8 k[2 * NS], v[NT];
-    auto at = [&](int base, int i) __attribute__((always_inline)) {
-        const int p = __builtin_amdgcn_readlane(id, i), b = first + base + wave + PW * i;
-        return region(reinterpret_cast<const char*>(a.p.cache) +
-                          ((size_t)max(p, 0) * stride + (size_t)kh * per + (b & (per - 1))) * (128 * HD),
-                      p < 0 ? 0 : 128 * HD);
-    };
-    c.start(a, r0, rows, kh, lane, -1);
-    for (int base = begin; base < end; base += PW * 64) {
-        const int i = base + wave + PW * lane;
-        id = -1;
-        if (i < end) {
-            const int p = (first + i) >> (a.p.shift - 5);
-            id = p < a.p.cols ? a.p.table[(size_t)table * a.p.cols + p] : -1;
-            if (id < 0 || id >= a.p.pages) id = -1, any = true;
+    ColumnSees own[NQT];
+    int bit[NQT];
+    c.start(a, r0, rows, kh, lane, -1, w.low);
+    if constexpr (MASKED) {
+#pragma unroll
+        for (int u = 0; u < NQT; ++u) {
+            bit[u] = min(16 * u + (lane & 15), rows * a.group - 1) / a.group;
+            own[u] = sees(bit[u]);
         }
+    }
+    for (int base = begin; base < end; base += PW * 64) {
+        const bool none = at.look(a, table, base + wave + PW * lane, end, place);
+        gone = gone || __any(none);
         const int n = min(64, (end - base - wave + PW - 1) / PW);
         if (n <= 0) break;
-        Region r = at(base, 0);
+        Region r = at.block<HD>(a, kh, 0);
         load_k<HD, 0>(k, r, lane);
         load_v<HD, 0>(v, r, lane);
         for (int j = 0; j < n; ++j) {
-            const int k0 = 32 * (first + base + wave + PW * j);
-            const Region next = at(base, min(j + 1, 63));
+            const int k0 = at.key0(j);
+            const Region next = at.block<HD>(a, kh, min(j + 1, 63));
+            if (SEE == See::ONE && !at.has(j)) {  // not this row's
+                load_k<HD, 0>(k, next, lane);
+                load_v<HD, 0>(v, next, lane);
+                continue;
+            }
+            ColumnSees now[NQT];
+            bool part = false;
+            if constexpr (MASKED) {
+                const uint32_t on = SEE == See::ONE ? 1u : (uint32_t)__builtin_amdgcn_readlane((int)at.rows, j);
+                bool some = false;
+#pragma unroll
+                for (int u = 0; u < NQT; ++u) {
+                    now[u] = on >> bit[u] & 1 ? own[u] : ColumnSees{0, 0, 0};
+                    some = some || !(k0 + 32 <= now[u].f || (k0 >= now[u].lo && k0 + 32 <= now[u].tk));
+                }
+                part = __any(some);
+            }
             c.scores(k);
             load_k<HD, 0>(k, next, lane);
-            c.softmax(k0, false, [](int) { return true; });
+            c.softmax(k0, part, [&](int u, int key) {
+                return !MASKED || key < now[u].f || (key >= now[u].lo && key < now[u].tk);
+            });
+            if constexpr (SEE == See::ONE) {
+                half8 one;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + 8 * (lane >> 4) + i;
+                    one[i] = key < now[0].f || (key >= now[0].lo && key < now[0].tk) ? (half_t)1.0f : (half_t)0.0f;
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    half8 odd;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const half_t x = one[i] != (half_t)0.0f ? v[t][i] : (half_t)0.0f;
+                        const bool fine = x - x == (half_t)0.0f;
+                        v[t][i] = fine ? x : (half_t)0.0f;
+                        odd[i] = fine ? (half_t)0.0f : x;
+                    }
+                    c.o[t][0] = mfma16(odd, one, c.o[t][0]);
+                }
+            }
             c.values(v);
             load_v<HD, 0>(v, next, lane);
         }
     }
-    if (__any(any)) {
+    if (gone) {
 #pragma unroll
         for (int u = 0; u < NQT; ++u) c.l[u] = __builtin_nanf("");
     }
-    join<HD, MODE, NQT>(w, c, rows * a.group, to, tid);
+    return join<HD, MODE, NQT, SEE != See::ONE>(w, c, a.group, rows * a.group, to, tid);
 }
 
-// Partials: own items' O, [item][kv head][group][HD]; shared ones', [item][kv
+// Partials: own items' O, [item][kv head][group][HD]; wide ones' (tiles'), [item][kv
 // head][PG_COLS][HD]; then (m, l) of both in the same order.
-__device__ __forceinline__ Sink own_part(const PagedArgs& a, int hd, int item, int kh) {
-    const size_t at = ((size_t)item * a.kv_heads + kh) * a.group;
-    const size_t all = ((size_t)a.max_own * a.group + (size_t)a.max_shared * PG_COLS) * a.kv_heads;
-    return Sink{a.part + at * hd, reinterpret_cast<float2*>(a.part + all * hd) + at};
+__device__ __forceinline__ Sink part_at(const PagedArgs& a, int hd, size_t at) {
+    const size_t all = ((size_t)a.max_own * a.group + (size_t)a.max_wide * PG_COLS) * a.kv_heads;
+    return Sink{a.part + at * hd, reinterpret_cast<float2*>(a.part + all * hd) + at, (long)a.group * hd};
 }
-__device__ __forceinline__ Sink shared_part(const PagedArgs& a, int hd, int item, int kh) {
-    const size_t at = (size_t)a.max_own * a.group * a.kv_heads + ((size_t)item * a.kv_heads + kh) * PG_COLS;
-    const size_t all = ((size_t)a.max_own * a.group + (size_t)a.max_shared * PG_COLS) * a.kv_heads;
-    return Sink{a.part + at * hd, reinterpret_cast<float2*>(a.part + all * hd) + at};
+__device__ __forceinline__ Sink own_part(const PagedArgs& a, int hd, int item, int kh) {
+    return part_at(a, hd, ((size_t)item * a.kv_heads + kh) * a.group);
+}
+__device__ __forceinline__ Sink wide_part(const PagedArgs& a, int hd, int item, int kh) {
+    return part_at(a, hd, (size_t)a.max_own * a.group * a.kv_heads + ((size_t)item * a.kv_heads + kh) * PG_COLS);
+}
+__device__ __forceinline__ Sink context(const PagedArgs& a, int hd, int row, int kh) {
+    return Sink{a.out + ((size_t)row * a.kv_heads + kh) * a.group * hd, nullptr, (long)a.kv_heads * a.group * hd};
+}
+// The columns of a tile's row.
+__device__ __forceinline__ Sink row_of(const PagedArgs& a, int hd, const Sink& tile, int row) {
+    return Sink{tile.o + row * tile.stride, tile.ml ? tile.ml + row * a.group : nullptr, tile.stride};
 }
 
-__device__ __forceinline__ const int* plan_items(const PagedArgs& a) {
-    return a.plan + PG_HEAD + (size_t)PG_ROW * a.nseq + (PG_ROW * (size_t)a.nseq % 16);
+__device__ __forceinline__ const int* plan_row(const PagedArgs& a, int row) {
+    return a.plan + PG_HEAD + (size_t)PG_ROW * row;
+}
+__device__ __forceinline__ const int* plan_item(const PagedArgs& a, int item) {
+    return a.plan + plan_items_at(a.nseq) + (size_t)PG_ITEM * item;
 }
 // Whether the plan is one of this call's sizes (a step's own is).
 __device__ __forceinline__ bool plan_fits(const PagedArgs& a) {
     const int* h = a.plan;
     return h[2] == a.nseq && h[3] == a.group && h[4] == a.kv_heads && h[5] == a.p.shift && h[6] == a.p.cols &&
-           h[7] == a.p.rows && h[8] == a.max_shared && h[9] == a.max_own && h[10] == !a.merge;
+           h[7] == a.p.rows && h[8] == a.max_wide && h[9] == a.max_own && h[10] == !a.merge;
 }
 
 // Every element of a row's kv head.
@@ -356,80 +467,183 @@ __global__ __launch_bounds__(PT, 2) void paged_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) WaveParts<HD> w;
     const int kh = (int)(blockIdx.x % (unsigned)a.kv_heads), item = (int)(blockIdx.x / (unsigned)a.kv_heads);
     const int n = a.group * HD;
-    const int* d = plan_items(a) + (size_t)PG_ITEM * item;
+    const int* d = plan_item(a, item);
     if (!plan_fits(a)) {
-        for (int r = item; r < a.nseq; r += a.items)
-            fill(a.out + ((size_t)r * a.kv_heads + kh) * n, n, __builtin_nanf(""));
+        for (int r = item; r < a.nseq; r += a.items) fill(context(a, HD, r, kh).o, n, __builtin_nanf(""));
         return;
     }
     if (item >= a.plan[0]) return;
-    const int row = d[0], rows = d[1], table = d[2], begin = d[8], end = d[9], ns = a.plan[1];
-    if (item < ns) {
-        const Sink to = shared_part(a, HD, item, kh);
-        if (rows * a.group > 16) shared_tile<HD, MODE, 2>(a, w, row, rows, table, kh, d[5], begin, end, to);
-        else shared_tile<HD, MODE, 1>(a, w, row, rows, table, kh, d[5], begin, end, to);
-        return;
-    }
-    float* out = a.out + ((size_t)row * a.kv_heads + kh) * n;
-    const Sink to = d[3] ? Sink{out, nullptr} : own_part(a, HD, item - ns, kh);
-    if (table < 0) {
-        fill(out, n, __builtin_nanf(""));
-        return;
-    }
+    const int row = d[0], table = d[2], flags = d[3], begin = d[8], end = d[9], wide = a.plan[1];
+    int rows = d[1];
     const int na = d[4], b0 = d[5], c0 = d[6], d0 = d[7];
-    one_row<HD, MODE, AUX>(a, w, row, table, kh, begin, end, d[10], d[11], d[12], to, [&](int i) {
+    Sink to = flags & PG_WHOLE ? context(a, HD, row, kh)
+              : item < wide    ? wide_part(a, HD, item, kh)
+                               : own_part(a, HD, item - wide, kh);
+    if (table < 0) {
+        fill(to.o, n, __builtin_nanf(""));
+        return;
+    }
+    auto place = [&](int i, uint32_t& on) {
         const int j = i - na, x = c0 - b0;
+        on = ~0u;
         return 32 * (i < na ? i : j < x ? b0 + j : d0 + j - x);
-    });
+    };
+    const bool two = rows * a.group > 16, shared = (flags & PG_SHARED) != 0;
+    auto sees = [&](int i) {
+        const int* p = plan_row(a, row + i) + 8;
+        return shared ? ColumnSees{0, 0, 0x7fffffff} : ColumnSees{p[0], p[1], p[2]};
+    };
+    if (shared) {
+        if (two ? tile<HD, MODE, 2, See::ALL>(a, w, row, rows, table, kh, begin, end, to, place, sees)
+                : tile<HD, MODE, 1, See::ALL>(a, w, row, rows, table, kh, begin, end, to, place, sees))
+            return;
+    } else if (rows == 1) {
+        const ColumnSees s = sees(0);
+        if (one_row<HD, MODE, AUX>(a, w, row, table, kh, begin, end, s.f, s.lo, s.tk, to, place)) return;
+    } else if (two ? tile<HD, MODE, 2, See::OWN>(a, w, row, rows, table, kh, begin, end, to, place, sees)
+                   : tile<HD, MODE, 1, See::OWN>(a, w, row, rows, table, kh, begin, end, to, place, sees)) {
+        return;
+    }
+    for (int i = 0; i < rows; ++i) {
+        tile<HD, MODE, 1, See::ONE>(a, w, row + i, 1, table, kh, begin, end, row_of(a, HD, to, i), place,
+                                    [&](int) { return sees(i); });
+        __syncthreads();  // the join's arrays
+    }
 }
 
-// Over selected pages: workgroup (row, kv head, run) takes its share of `count` pages' blocks.
+// The rows of a selection that are attended together: an aligned tile of rows whose
+// sequence is one.
+struct Together {
+    int r0, rows, table;  // rows: 1 where they are taken one by one
+    __device__ __forceinline__ Together(const PagedArgs& a, int row) {
+        const int per = PG_TILE_ROWS(a.group);
+        r0 = row / per * per, rows = min(per, a.nseq - r0);
+        table = a.row ? a.row[row] : row;
+        bool one = rows > 1 && a.row && a.p.cols <= PG_UNION && table >= 0 && table < a.p.rows;
+        for (int i = 0; one && i < rows; ++i) one = a.row[r0 + i] == table;
+        if (!one) r0 = row, rows = 1;
+    }
+    __device__ __forceinline__ int runs(const PagedArgs& a) const {
+        return rows == 1 ? a.runs : min(a.tile_runs, rows * a.runs);
+    }
+};
+
+// Over selected pages: workgroup (row, kv head, run) takes its share of `count`
+// pages' blocks. Rows of one sequence mostly select the same pages (neighbours of a
+// prompt), so a tile of them walks the pages that any of them selected, each read once,
+// its workgroups being those of its rows (127 rows over 24 pages each of 32/8/128,
+// row by row 42.4 us).
 template <int HD, int MODE, int AUX>
 __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) WaveParts<HD> w;
+    __shared__ uint32_t mask[PG_UNION];   // rows that selected a page, a bit each
+    __shared__ uint16_t list[PG_UNION];   // the pages that some row selected
+    __shared__ int waves[PW];
     const int kh = (int)(blockIdx.x % (unsigned)a.kv_heads), item = (int)(blockIdx.x / (unsigned)a.kv_heads);
-    const int run = item % a.runs, row = item / a.runs, n = a.group * HD;
-    const int table = a.row ? a.row[row] : row;
-    const int tk = max(0, min(a.tk[row], a.p.cols << a.p.shift));
-    float* out = a.out + ((size_t)row * a.kv_heads + kh) * n;
-    const Sink to = a.runs == 1 ? Sink{out, nullptr} : own_part(a, HD, item, kh);
-    const bool live = table >= 0 && table < a.p.rows;
-    if (a.runs == 1 && !live) {
-        fill(out, n, __builtin_nanf(""));
+    const int run = item % a.runs, row = item / a.runs, tid = threadIdx.x, lane = tid & 63;
+    const int s = a.p.shift - 5;
+    auto length = [&](int r) { return max(0, min(a.tk[r], a.p.cols << a.p.shift)); };
+    const Together t(a, row);
+    const int runs = t.runs(a);
+    if (t.rows > 1) {
+        const int sub = (row - t.r0) * a.runs + run;
+        if (sub >= runs) return;
+        int top = 0;
+        for (int i = 0; i < t.rows; ++i) top = max(top, length(t.r0 + i));
+        const int live = (top + (1 << a.p.shift) - 1) >> a.p.shift;
+        for (int p = tid; p < live; p += PT) mask[p] = 0;
+        __syncthreads();
+        for (int e = tid; e < t.rows * a.count; e += PT) {
+            const int i = e / a.count, r = t.r0 + i;
+            const int p = a.chosen[((size_t)r * a.kv_heads + kh) * a.count + e % a.count];
+            if (p >= 0 && p < a.p.cols && p << a.p.shift < length(r)) atomicOr(&mask[p], 1u << i);
+        }
+        __syncthreads();
+        int n = 0;
+        for (int p0 = 0; p0 < live; p0 += PT) {
+            const int p = p0 + tid;
+            const bool on = p < live && mask[p] != 0;
+            const uint64_t m = __ballot(on);
+            if (lane == 0) waves[tid >> 6] = __popcll(m);
+            __syncthreads();
+            int at = n + __popcll(m & ((1ull << lane) - 1));
+            for (int k = 0; k < PW; ++k) {
+                if (k < tid >> 6) at += waves[k];
+                n += waves[k];
+            }
+            if (on) list[at] = (uint16_t)p;
+            __syncthreads();
+        }
+        const int blocks = n << s, share = (blocks + runs - 1) / runs, begin = sub * share, end = min(blocks, begin + share);
+        const Sink to = runs == 1 ? context(a, HD, t.r0, kh)
+                                  : wide_part(a, HD, t.r0 / PG_TILE_ROWS(a.group) * a.tile_runs + sub, kh);
+        auto place = [&](int i, uint32_t& on) {
+            const int p = list[i >> s];
+            on = mask[p];
+            return (p << a.p.shift) + 32 * (i & ((1 << s) - 1));
+        };
+        auto sees = [&](int i) { return ColumnSees{0, 0, length(t.r0 + i)}; };
+        if (t.rows * a.group > 16
+                ? tile<HD, MODE, 2, See::OWN>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees)
+                : tile<HD, MODE, 1, See::OWN>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees))
+            return;
+        for (int i = 0; i < t.rows; ++i) {
+            auto of_row = [&](int b, uint32_t& on) {
+                const int at = place(b, on);
+                return (on >> i & 1) && at < length(t.r0 + i) ? at : -1;
+            };
+            tile<HD, MODE, 1, See::ONE>(a, w, t.r0 + i, 1, t.table, kh, begin, end, row_of(a, HD, to, i), of_row,
+                                        [&](int) { return sees(i); });
+            __syncthreads();  // the join's arrays
+        }
         return;
     }
-    const int s = a.p.shift - 5, blocks = a.count << s;
-    const int share = (blocks + a.runs - 1) / a.runs, begin = run * share, end = live ? min(blocks, begin + share) : 0;
+    const int n = a.group * HD, tk = length(row);
+    const Sink to = runs == 1 ? context(a, HD, row, kh) : own_part(a, HD, item, kh);
+    const bool live = t.table >= 0 && t.table < a.p.rows;
+    if (runs == 1 && !live) {
+        fill(to.o, n, __builtin_nanf(""));
+        return;
+    }
+    const int blocks = a.count << s, share = (blocks + runs - 1) / runs, begin = run * share;
+    const int end = live ? min(blocks, begin + share) : 0;
     const int* chosen = a.chosen + ((size_t)row * a.kv_heads + kh) * a.count;
-    one_row<HD, MODE, AUX>(a, w, row, table, kh, begin, end, 0, 0, tk, to, [&](int i) {
+    auto place = [&](int i, uint32_t&) {
         const int p = chosen[i >> s];
         if (p < 0 || p >= a.p.cols) return -1;
         const int first = (p << a.p.shift) + 32 * (i & ((1 << s) - 1));
         return first < tk ? first : -1;
-    });
+    };
+    if (one_row<HD, MODE, AUX>(a, w, row, t.table, kh, begin, end, 0, 0, tk, to, place)) return;
+    tile<HD, MODE, 1, See::ONE>(a, w, row, 1, t.table, kh, begin, end, to, place, [&](int) { return ColumnSees{0, 0, tk}; });
 }
 
-// The parts of a row's columns of kv head kh: `on` of its own, then `sn` of its
-// group's. None (n = 0): its item wrote the context.
+// The parts of a row's columns of kv head kh: `on` of its own, then its group's.
+// None (n = 0): its item wrote the context.
 template <int HD, bool PLAN>
 struct Parts {
-    int o0, on, s0 = 0, n, step = 0, col = 0;
+    int o0, on, s0 = 0, n, step = 0, col = 0, own_col = -1;  // own_col: its own parts are a tile's
     bool bad = false;  // no such table row
     __device__ __forceinline__ Parts(const PagedArgs& a, int row) {
         if constexpr (PLAN) {
-            const int* d = a.plan + PG_HEAD + (size_t)PG_ROW * row;
-            o0 = d[0], on = d[1], s0 = d[2], step = d[4], col = d[5];
+            const int* d = plan_row(a, row);
+            o0 = d[0], on = d[1], s0 = d[2], step = d[4], col = d[5], own_col = d[6];
             n = on == 1 && d[3] == 0 ? 0 : on + d[3];
         } else {
-            const int table = a.row ? a.row[row] : row;
-            bad = table < 0 || table >= a.p.rows;
-            o0 = row * a.runs, on = n = a.runs;
+            const Together t(a, row);
+            bad = t.table < 0 || t.table >= a.p.rows;
+            on = t.runs(a);
+            n = on == 1 ? 0 : on;
+            o0 = row * a.runs;
+            if (t.rows > 1) o0 = t.r0 / PG_TILE_ROWS(a.group) * a.tile_runs, own_col = (row - t.r0) * a.group;
         }
     }
     // The i-th part's O and (m, l) of query head g.
     __device__ __forceinline__ Sink of(const PagedArgs& a, int i, int kh, int g) const {
-        Sink p = i < on ? own_part(a, HD, o0 + i, kh) : shared_part(a, HD, s0 + (i - on) * step, kh);
-        const int at = g + (i < on ? 0 : col);
+        Sink p = i >= on        ? wide_part(a, HD, s0 + (i - on) * step, kh)
+                 : own_col >= 0 ? wide_part(a, HD, o0 + i, kh)
+                                : own_part(a, HD, o0 + i, kh);
+        const int at = g + (i >= on ? col : own_col >= 0 ? own_col : 0);
         p.o += (size_t)at * HD, p.ml += at;
         return p;
     }

@@ -16,82 +16,88 @@ namespace llmtie {
 
 constexpr int PG_SPAN = 4;  // blocks of an item at least: one a wave
 
-// What row r sees: the first f positions and those from lo to tk (f = lo = 0: all).
-struct RowSeen {
-    int tk, lo, f, table;
-    __device__ __forceinline__ RowSeen(const PagePlanArgs& a, int r) {
-        table = a.row ? a.row[r] : r;
-        tk = max(0, min(a.tk[r], a.cols << a.shift));
-        if (table < 0 || table >= a.rows) table = -1;
-        lo = a.lo ? a.lo[r] : 0;
-        if (a.window) lo = max(lo, tk - a.window);
-        lo = max(0, min(lo, tk));
-        f = min(a.shared, tk);
-        if (f >= lo) f = lo = 0;
-    }
-};
+// What row r sees: the first f positions and those from lo to tk (f = lo = 0: all); its table row, or -1.
+__device__ __forceinline__ int4 row_sees(const PagePlanArgs& a, int r) {
+    const int tk = max(0, min(a.tk[r], a.cols << a.shift));
+    int table = a.row ? a.row[r] : r, lo = a.lo ? a.lo[r] : 0;
+    if (table < 0 || table >= a.rows) table = -1;
+    if (a.window) lo = max(lo, tk - a.window);
+    lo = max(0, min(lo, tk));
+    int f = min(a.shared, tk);
+    if (f >= lo) f = lo = 0;
+    return make_int4(f, lo, tk, table);
+}
 
-// The blocks of 32 positions that a row's own item walks: [0, na), [b0, c0) and
-// [d0, e), where the blocks from c0 to d0 are its group's.
+// The blocks of 32 positions that a row's own item walks, or those of a tile of
+// rows: [0, na), [b0, c0) and [d0, e), where the blocks from c0 to d0 are its group's.
 struct OwnBlocks {
-    int na, b0, c0, d0, n;
-    __device__ __forceinline__ OwnBlocks(const RowSeen& s, int glo, int ghi) {
-        const int e = (s.tk + 31) >> 5;
-        na = (s.f + 31) >> 5;
-        b0 = max(na, s.lo >> 5);
-        c0 = ghi > glo ? glo : e;
-        d0 = ghi > glo ? ghi : e;
-        c0 = max(b0, c0);
-        n = na + (s.lo < s.tk ? c0 - b0 + max(0, e - d0) : 0);
-        if (s.table < 0) n = 0;
+    int na = 0, b0 = 0x7fffffff, e = 0, c0, d0, n;
+    __device__ __forceinline__ void add(const int4& s) {
+        if (s.w < 0) return;
+        na = max(na, (s.x + 31) >> 5);
+        if (s.y < s.z) b0 = min(b0, s.y >> 5), e = max(e, (s.z + 31) >> 5);
+    }
+    __device__ __forceinline__ void close(int glo, int ghi) {
+        b0 = max(na, min(b0, e));
+        c0 = max(b0, ghi > glo ? glo : e);
+        d0 = ghi > glo ? ghi : c0;
+        n = na + (e ? c0 - b0 + max(0, e - d0) : 0);
     }
 };
 
-// The sum of `v` over the threads before this one, and of all in `total`.
+// The sums of `v` over the threads before this one, and of all in `total`.
 template <int PP>
-__device__ __forceinline__ int scan_before(int v, int* waves, int tid, int& total) {
-    int x = v;
+__device__ __forceinline__ int2 scan_before(int2 v, int2* waves, int tid, int2& total) {
+    int2 x = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if ((tid & 63) >= d) x += y;
+        const int y = __shfl_up(x.x, d), z = __shfl_up(x.y, d);
+        if ((tid & 63) >= d) x.x += y, x.y += z;
     }
     if ((tid & 63) == 63) waves[tid >> 6] = x;
     __syncthreads();
-    int before = 0;
-    total = 0;
+    int2 before = make_int2(x.x - v.x, x.y - v.y);
+    total = make_int2(0, 0);
 #pragma unroll
     for (int w = 0; w < PP / 64; ++w) {
-        if (w < (tid >> 6)) before += waves[w];
-        total += waves[w];
+        const int2 y = waves[w];
+        if (w < (tid >> 6)) before.x += y.x, before.y += y.y;
+        total.x += y.x, total.y += y.y;
     }
     __syncthreads();
-    return before + x - v;
+    return before;
 }
 
-// A row's group (-1: none), what it sees and its own blocks.
-struct PlanRow {
-    RowSeen s;
-    int g;
-};
-
-// One workgroup. A shared tile is up to PG_COLS columns (rows of a group times a
-// kv head's query heads) over the blocks that all the group's rows see whole and
-// hold in the same pages; what else a row sees is its own tile's. Each tile is
-// cut into items of about the same cost, `target` of them a kv head in all.
-// Bound by its chain of loads and barriers: a row a thread, whose lengths are
-// read once, and few waves where there are few rows.
+// One workgroup. Tiles are up to PG_COLS columns (rows times a kv head's query
+// heads): a group's rows over the blocks that all of them see whole and hold in the
+// same pages, and rows of one sequence that lie together (an aligned tile of them)
+// over what else they see, each key masked by row; what a row alone sees is its own
+// item's. All are cut into items of about the same cost, `target` of them a kv head in
+// all. Bound by its chain of loads and barriers: a row a thread, few waves where there
+// are few rows (ONE: what they see is held in LDS, else in the plan itself).
 template <int PP, bool ONE>
 __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __shared__ int gst[PG_GROUPS + 1], glo[PG_GROUPS], ghi[PG_GROUPS], gat[PG_GROUPS];
-    __shared__ int waves[PP / 64];
+    __shared__ int4 held[ONE ? PP : 1];
+    __shared__ int2 waves[PP / 64];
     __shared__ unsigned long long work;
     const int tid = threadIdx.x;
     const int tile_rows = PG_TILE_ROWS(a.group);
-    const int per = ONE ? 1 : (a.nseq + PP - 1) / PP;
+    // (Whole tiles a thread, or a row.)
+    const int per = ONE ? 1 : (a.nseq + PP * tile_rows - 1) / (PP * tile_rows) * tile_rows;
     const int r0 = min(a.nseq, tid * per), r1 = min(a.nseq, r0 + per);
     int groups = a.starts ? a.groups : 0;
-    PlanRow held{RowSeen(a, min(tid, a.nseq - 1)), -1};
+    int4* rows = reinterpret_cast<int4*>(a.plan + PG_HEAD);
+    int4* items = reinterpret_cast<int4*>(a.plan + plan_items_at(a.nseq));
+    for (int r = r0; r < r1; ++r) {
+        const int4 s = row_sees(a, r);
+        rows[PG_ROW / 4 * (size_t)r + 2] = s;
+        if constexpr (ONE) held[r] = s;
+    }
+    auto sees = [&](int r) {
+        if constexpr (ONE) return held[r];
+        else return rows[PG_ROW / 4 * (size_t)r + 2];
+    };
     for (int g = tid; g <= groups && groups; g += PP) gst[g] = max(0, min(a.starts[g], a.nseq));
     for (int g = tid; g < groups; g += PP) ghi[g] = a.prefix[g], glo[g] = 0;
     if (tid == 0) work = 0;
@@ -109,17 +115,14 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         }
         return lo >= 0 && r < gst[lo + 1] ? lo : -1;
     };
-    if constexpr (ONE) held.g = groups && tid < a.nseq ? group_of(tid) : -1;
-    auto row_of = [&](int r) {
-        if constexpr (ONE) return held;
-        return PlanRow{RowSeen(a, r), groups ? group_of(r) : -1};
-    };
+    auto wide_cost = [&](int n) { return min(n, tile_rows) * a.group > 16 ? 7 : 4; };
     if (groups) {
         for (int r = r0; r < r1; ++r) {
-            const PlanRow x = row_of(r);
-            if (x.g < 0) continue;
-            atomicMin(&ghi[x.g], x.s.table < 0 ? 0 : x.s.tk);
-            atomicMax(&glo[x.g], x.s.lo);
+            const int g = group_of(r);
+            if (g < 0) continue;
+            const int4 s = sees(r);
+            atomicMin(&ghi[g], s.w < 0 ? 0 : s.z);
+            atomicMax(&glo[g], s.y);
         }
         __syncthreads();
         for (int g = tid; g < groups; g += PP) {
@@ -129,70 +132,104 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
             glo[g] = share ? lo : 0;
             ghi[g] = share ? hi : 0;
             if (share)
-                atomicAdd(&work, (unsigned long long)((n + tile_rows - 1) / tile_rows) * (unsigned)(hi - lo) *
-                                     (min(n, tile_rows) * a.group > 16 ? 7u : 4u));
+                atomicAdd(&work, (unsigned long long)((n + tile_rows - 1) / tile_rows) * (unsigned)(hi - lo) * wide_cost(n));
         }
         __syncthreads();
     }
-    auto own_of = [&](const PlanRow& x) { return OwnBlocks(x.s, x.g >= 0 ? glo[x.g] : 0, x.g >= 0 ? ghi[x.g] : 0); };
-    unsigned long long mine = 0;
-    for (int r = r0; r < r1; ++r) mine += 4ull * (unsigned)own_of(row_of(r)).n;
-    if (mine) atomicAdd(&work, mine);
+    // A row's own part: with its tile's where that is of one sequence and one group.
+    struct Own {
+        OwnBlocks o;
+        int g, first, rows;  // rows: 1, or its tile's from `first` on
+    };
+    auto own_of = [&](int r) {
+        Own x;
+        x.g = groups ? group_of(r) : -1;
+        const int lo = x.g >= 0 ? glo[x.g] : 0, hi = x.g >= 0 ? ghi[x.g] : 0;
+        const int t0 = r / tile_rows * tile_rows, m = min(tile_rows, a.nseq - t0);
+        const int table = sees(r).w;
+        bool one = m > 1 && table >= 0 && a.row;
+        if (one && groups)
+            one = x.g >= 0 ? gst[x.g] <= t0 && t0 + m <= gst[x.g + 1] : t0 + m <= gst[0] || t0 >= gst[groups];
+        OwnBlocks all;
+        for (int i = 0; one && i < m; ++i) {
+            const int4 s = sees(t0 + i);
+            one = s.w == table;
+            all.add(s);
+        }
+        x.first = one ? t0 : r, x.rows = one ? m : 1;
+        if (!one) {
+            all = OwnBlocks();
+            all.add(sees(r));
+        }
+        all.close(lo, hi);
+        x.o = all;
+        return x;
+    };
+    Own mine;
+    if constexpr (ONE) mine = own_of(min(tid, a.nseq - 1));
+    auto own = [&](int r) {
+        if constexpr (ONE) return mine;
+        else return own_of(r);
+    };
+    unsigned long long cost = 0;
+    for (int r = r0; r < r1; ++r) {
+        const Own x = own(r);
+        if (x.first == r) cost += (unsigned long long)x.o.n * (x.rows > 1 ? wide_cost(x.rows) : 4);
+    }
+    if (cost) atomicAdd(&work, cost);
     __syncthreads();
     // Cost of an item, four a block (seven of two column tiles).
     const unsigned long long c = max((work + a.target - 1) / a.target, (unsigned long long)(4 * PG_SPAN));
     auto cut = [&](int blocks, int cost) {
         return a.whole ? 1 : (int)(((unsigned long long)blocks * cost + c - 1) / c);
     };
-    int4* rows = reinterpret_cast<int4*>(a.plan + PG_HEAD);
-    int4* items = rows + (PG_ROW * (size_t)a.nseq + PG_ROW * (size_t)a.nseq % 16) / 4;
 
     // Shared tiles, a group's runs of blocks outermost, so that its tiles read a run at one time.
     int ns = 0;
-    auto runs_of = [&](int g) {
-        return cut(ghi[g] - glo[g], min(gst[g + 1] - gst[g], tile_rows) * a.group > 16 ? 7 : 4);
-    };
+    auto runs_of = [&](int g) { return cut(ghi[g] - glo[g], wide_cost(gst[g + 1] - gst[g])); };
     auto tiles_of = [&](int g) { return (gst[g + 1] - gst[g] + tile_rows - 1) / tile_rows; };
     if (groups) {
         const int each = (groups + PP - 1) / PP, g0 = min(groups, tid * each), g1 = min(groups, g0 + each);
         auto items_of = [&](int g) { return ghi[g] > glo[g] ? tiles_of(g) * runs_of(g) : 0; };
-        int n = 0;
-        for (int g = g0; g < g1; ++g) n += items_of(g);
-        int at = scan_before<PP>(n, waves, tid, ns);
+        int2 n = make_int2(0, 0), total;
+        for (int g = g0; g < g1; ++g) n.x += items_of(g);
+        int at = scan_before<PP>(n, waves, tid, total).x;
         for (int g = g0; g < g1; ++g) gat[g] = at, at += items_of(g);
         __syncthreads();
-        ns = min(ns, a.max_shared);
+        ns = min(total.x, a.max_wide);
         for (int g = 0; g < groups; ++g) {
             if (ghi[g] <= glo[g]) continue;
             const int tiles = tiles_of(g), runs = runs_of(g), nb = ghi[g] - glo[g], share = (nb + runs - 1) / runs;
             for (int i = tid; i < tiles * runs; i += PP) {
                 if (gat[g] + i >= ns) break;
                 const int t = i % tiles, b = i / tiles * share, first = gst[g] + t * tile_rows;
-                const int row = a.row ? a.row[first] : first;
                 int4* d = items + PG_ITEM / 4 * (size_t)(gat[g] + i);
-                d[0] = make_int4(first, min(tile_rows, gst[g + 1] - first), row, 0);
+                d[0] = make_int4(first, min(tile_rows, gst[g + 1] - first), sees(first).w, PG_SHARED);
                 d[1] = make_int4(0, glo[g], ghi[g], ghi[g]);
                 d[2] = make_int4(b, min(nb, b + share), 0, 0);
             }
         }
     }
-    // Rows and their own items.
-    auto own_items = [&](const PlanRow& x, int n) {
+    // Tiles of one sequence's rows (x), and rows by themselves (y).
+    auto items_of = [&](const Own& x) {
         const bool shares = x.g >= 0 && ghi[x.g] > glo[x.g];
-        return n ? cut(n, 4) : shares ? 0 : 1;
+        return x.o.n ? cut(x.o.n, x.rows > 1 ? wide_cost(x.rows) : 4) : shares ? 0 : 1;
     };
-    int n = 0, no = 0;
+    int2 n = make_int2(0, 0), total;
     for (int r = r0; r < r1; ++r) {
-        const PlanRow x = row_of(r);
-        n += own_items(x, own_of(x).n);
+        const Own x = own(r);
+        if (x.rows == 1) n.y += items_of(x);
+        else if (x.first == r) n.x += items_of(x);
     }
-    int at = scan_before<PP>(n, waves, tid, no);
+    const int2 before = scan_before<PP>(n, waves, tid, total);
+    // (A tile's rows but its first: their tile's items are the first's, which a thread before them may hold.)
+    int wide = ns + before.x, alone = before.y, last = wide;
+    const int nw = min(ns + total.x, a.max_wide);
     for (int r = r0; r < r1; ++r) {
-        const PlanRow x = row_of(r);
-        const OwnBlocks o = own_of(x);
+        const Own x = own(r);
         const bool shares = x.g >= 0 && ghi[x.g] > glo[x.g];
-        const int runs = own_items(x, o.n), share = runs ? (o.n + runs - 1) / runs : 0;
-        int4 d = make_int4(at, runs, 0, 0), e = make_int4(0, 0, 0, 0);
+        const int runs = items_of(x), share = runs ? (x.o.n + runs - 1) / runs : 0;
+        int4 d = make_int4(alone, runs, 0, 0), e = make_int4(0, 0, -1, 0);
         if (shares) {
             const int in = r - gst[x.g];
             d.z = gat[x.g] + in / tile_rows;
@@ -200,24 +237,31 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
             e.x = tiles_of(x.g);
             e.y = in % tile_rows * a.group;
         }
+        if (x.rows > 1) {
+            // `wide` counts the tiles that begin up to here: this one's items end there, or begin.
+            if (x.first == r) last = wide;
+            d.x = x.first == r ? wide : (ONE ? wide - runs : last);
+            e.z = (r - x.first) * a.group;
+        }
         rows[PG_ROW / 4 * (size_t)r] = d;
         rows[PG_ROW / 4 * (size_t)r + 1] = e;
+        if (x.first != r) continue;
+        const int at = x.rows > 1 ? wide : nw + alone, end = x.rows > 1 ? nw : nw + a.max_own;
         for (int i = 0; i < runs; ++i) {
-            if (at + i >= a.max_own) break;
-            int4* t = items + PG_ITEM / 4 * (size_t)(ns + at + i);
-            t[0] = make_int4(r, 1, x.s.table, runs == 1 && !shares);
-            t[1] = make_int4(o.na, o.b0, o.c0, o.d0);
-            t[2] = make_int4(i * share, min(o.n, (i + 1) * share), x.s.f, x.s.lo);
-            t[3] = make_int4(x.s.tk, 0, 0, 0);
+            if (at + i >= end) break;
+            int4* t = items + PG_ITEM / 4 * (size_t)(at + i);
+            t[0] = make_int4(r, x.rows, sees(r).w, runs == 1 && !shares ? PG_WHOLE : 0);
+            t[1] = make_int4(x.o.na, x.o.b0, x.o.c0, x.o.d0);
+            t[2] = make_int4(i * share, min(x.o.n, (i + 1) * share), 0, 0);
         }
-        at += runs;
+        if (x.rows > 1) wide += runs;
+        else alone += runs;
     }
     if (tid == 0) {
-        no = min(no, a.max_own);
         int4* h = reinterpret_cast<int4*>(a.plan);
-        h[0] = make_int4(ns + no, ns, a.nseq, a.group);
+        h[0] = make_int4(nw + min(total.y, a.max_own), nw, a.nseq, a.group);
         h[1] = make_int4(a.kv_heads, a.shift, a.cols, a.rows);
-        h[2] = make_int4(a.max_shared, a.max_own, a.whole, 0);
+        h[2] = make_int4(a.max_wide, a.max_own, a.whole, 0);
     }
 }
 
