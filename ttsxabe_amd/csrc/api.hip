@@ -1611,7 +1611,7 @@ PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t heads, 
     s.target = std::max<size_t>(1, std::min(2 * (size_t)compute_units() / kv_heads, (nseq * blocks + 3) / 4));
     s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * (size_t)compute_units());
     // Shared tiles, and tiles of one sequence's rows.
-    const size_t tiles = (s.whole ? 0 : groups ? nseq / per + groups : 0) + (nseq + per - 1) / per;
+    const size_t tiles = (groups && !s.whole ? nseq / per + groups : 0) + std::min(nseq / 2, PG_RUNS * ((nseq + per - 1) / per));
     s.max_own = s.whole ? nseq : nseq + s.target;
     s.max_wide = s.whole ? nseq : tiles + s.target;
     s.items = s.whole ? nseq : nseq + tiles + s.target;
@@ -1793,7 +1793,9 @@ size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, si
     if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16 || nseq == 0 || nseq > PG_MAX_ROWS)
         return 0;
     const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), heads, kv_heads);
-    return smul(sadd(smul(z.max_own, heads), smul(z.max_wide, PG_COLS, kv_heads)), head_dim + 2);
+    if (!z.max_own && !z.max_wide) return 0;
+    // Parts, and a word a row.
+    return sadd(smul(sadd(smul(z.max_own, heads), smul(z.max_wide, PG_COLS, kv_heads)), head_dim + 2), nseq);
 }
 
 int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,

@@ -26,8 +26,8 @@ constexpr int PW = 4, PT = PW * LLMTIE_WAVE;
 template <int HD, int MODE, int NQT>
 struct Columns {
     static constexpr int NS = HD / 32, NT = HD / 16;
-    // q's lower halves: of two tiles in LDS, where one of the four waves (whose columns
-    // are the same) put them (in registers too, 210 of them spilled at HD 128).
+    // q goes through LDS, as the four waves' columns are the same. Its lower halves, of two
+    // tiles, stay there (in registers too, 210 of them spilled at HD 128).
     static constexpr bool LOW_LDS = NQT > 1;
     half8 qh[NQT][NS], ql[LOW_LDS ? 1 : NQT][LOW_LDS ? 1 : NS];
     const half8* low;
@@ -40,45 +40,69 @@ struct Columns {
     float sl2, c1, c2;
     int grp;
 
-    // Columns of `rows` rows from r0 on, `group` heads of kv head kh each.
-    // (LOW_LDS: with a barrier.)
-    __device__ __forceinline__ void start(const PagedArgs& a, int r0, int rows, int kh, int lane, int tk, half8* mem = nullptr) {
-        const int col = lane & 15, n = rows * a.group, wave = (int)threadIdx.x >> 6;
+    // Columns of `rows` rows from r0 on, `group` heads of kv head kh each (past the last
+    // one: that one again, which nobody keeps): their queries on the way, a quarter a
+    // wave. tk: the row's length where it has one row.
+    static constexpr int QP = (NQT * NS + PW - 1) / PW;  // (tile, 32 dims) pairs of a wave
+    floatx4 raw[QP][2];
+    __device__ __forceinline__ void fetch(const PagedArgs& a, int r0, int rows, int kh, int lane, int wave, int tk) {
+        const int col = lane & 15, n = rows * a.group;
         grp = lane >> 4;
-        low = mem;
-        sl2 = a.scale * LLMTIE_LOG2E;
-        c1 = (MODE & SM_CAP) != 0 ? a.scale / a.softcap : 0.0f;
-        c2 = a.softcap * LLMTIE_LOG2E;
+        auto column = [&](int u, int& row, int& g) {
+            const int c = min(16 * u + col, n - 1);
+            row = rows == 1 ? 0 : c / a.group, g = c - row * a.group;
+        };
 #pragma unroll
-        for (int u = 0; u < NQT; ++u) {
-            const int c = min(16 * u + col, n - 1), row = c / a.group, g = c % a.group;
-            const bool has = 16 * u + col < n;
-            const float* q = a.q + (size_t)(r0 + row) * a.q_stride + (size_t)(kh * a.group + g) * HD + 8 * grp;
+        for (int i = 0; i < QP; ++i) {
+            const int p = min(wave + PW * i, NQT * NS - 1);
+            int row, g;
+            column(p / NS, row, g);
+            const float* q = a.q + (size_t)(r0 + row) * a.q_stride + (size_t)(kh * a.group + g) * HD + 8 * grp + 32 * (p % NS);
+            __builtin_memcpy(&raw[i][0], q, 16);  // (4-byte aligned)
+            __builtin_memcpy(&raw[i][1], q + 4, 16);
+        }
+        if constexpr ((MODE & SM_BIAS) != 0) {
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                half8 lo;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    half_t x, y;
-                    split_h(has ? q[32 * s + j] : 0.0f, x, y);
-                    qh[u][s][j] = x;
-                    lo[j] = y;
-                }
-                if constexpr (!LOW_LDS) ql[u][s] = lo;
-                else if (wave == s) mem[(u * NS + s) * 64 + lane] = lo;
-            }
-            if constexpr ((MODE & SM_BIAS) != 0) {
+            for (int u = 0; u < NQT; ++u) {
+                int row, g;
+                column(u, row, g);
                 slope2[u] = a.slopes[kh * a.group + g] * LLMTIE_LOG2E;
                 at[u] = (tk >= 0 ? tk : min(a.tk[r0 + row], a.p.cols << a.p.shift)) - 1;
             }
-            m[u] = RG_NOREF;
-            l[u] = 0.0f;
         }
+    }
+    // (With a barrier.)
+    __device__ __forceinline__ void start(const PagedArgs& a, int lane, int wave, half8* mem) {
+        sl2 = a.scale * LLMTIE_LOG2E;
+        c1 = (MODE & SM_CAP) != 0 ? a.scale / a.softcap : 0.0f;
+        c2 = a.softcap * LLMTIE_LOG2E;
+        low = mem + NQT * NS * 64;
+#pragma unroll
+        for (int i = 0; i < QP; ++i) {
+            const int p = min(wave + PW * i, NQT * NS - 1);
+            half8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                half_t x, y;
+                split_h(raw[i][j / 4][j % 4], x, y);
+                hi[j] = x, lo[j] = y;
+            }
+            mem[p * 64 + lane] = hi, mem[(NQT * NS + p) * 64 + lane] = lo;
+        }
+#pragma unroll
+        for (int u = 0; u < NQT; ++u) m[u] = RG_NOREF, l[u] = 0.0f;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int u = 0; u < NQT; ++u) o[t][u] = zero_f4();
-        if constexpr (LOW_LDS) lds_barrier();
+        lds_barrier();
+#pragma unroll
+        for (int u = 0; u < NQT; ++u)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                qh[u][s] = mem[(u * NS + s) * 64 + lane];
+                if constexpr (!LOW_LDS) ql[u][s] = low[(u * NS + s) * 64 + lane];
+            }
     }
     __device__ __forceinline__ half8 lower(int u, int s, int lane) const {
         if constexpr (LOW_LDS) return low[(u * NS + s) * 64 + lane];
@@ -158,7 +182,7 @@ struct WaveParts {
     static constexpr int OP = HD + 4;
     float o[PW * 16 * OP];
     float m[PW][16], l[PW][16];
-    half8 low[2 * (HD / 32) * 64];  // Columns::low
+    half8 q[2 * 2 * (HD / 32) * 64];  // Columns::start
 };
 
 // Where a tile's columns go: the context itself (a row's heads together, rows
@@ -303,16 +327,21 @@ __device__ __forceinline__ bool one_row(const PagedArgs& a, WaveParts<HD>& w, in
         }
         c.values(x.v);
     };
-    bool gone = false;
     Block x0, x1;
+    c.fetch(a, row, 1, kh, lane, wave, tk);
+    bool none = at.look(a, table, begin + wave + PW * lane, end, place), gone = __any(none);
+    load(x0, 0);
+    c.start(a, lane, wave, w.q);
+    load(x1, 1);
     for (int base = begin; base < end; base += PW * 64) {
-        const bool none = at.look(a, table, base + wave + PW * lane, end, place);
-        gone = gone || __any(none);
         const int n = min(64, (end - base - wave + PW - 1) / PW);  // the wave's blocks
         if (n <= 0) break;
-        load(x0, 0);
-        load(x1, 1);
-        if (base == begin) c.start(a, row, 1, kh, lane, tk);
+        if (base != begin) {
+            none = at.look(a, table, base + wave + PW * lane, end, place);
+            gone = gone || __any(none);
+            load(x0, 0);
+            load(x1, 1);
+        }
         for (int k = 0; k < n; k += 2) {
             fold(x0, k);
             load(x0, min(k + 2, 63));
@@ -320,7 +349,6 @@ __device__ __forceinline__ bool one_row(const PagedArgs& a, WaveParts<HD>& w, in
             load(x1, min(k + 3, 63));
         }
     }
-    if (begin + wave >= end) c.start(a, row, 1, kh, lane, tk);
     if (gone) c.l[0] = __builtin_nanf("");
     return join<HD, MODE, 1, true>(w, c, a.group, a.group, to, tid);
 }
@@ -332,68 +360,66 @@ struct ColumnSees {
 
 // A tile: up to 32 columns of `rows` rows of one sequence or of one shared prefix, from r0
 // on. The next block's keys are loaded once the scores have this one's, and its
-// values once the products have them. See::ALL: its rows see all keys; OWN: each sees
-// keys of its own, sees(i) of the tile's i-th row.
+// values once the products have them. Each row sees keys of its own, sees(i) of the
+// tile's i-th one (of a shared prefix, all; one function for both, whose pieces the compiler
+// else merges at the price of 100 spilled registers).
 //
 // Returns false, with nothing written, where something is not finite. A value that a row
 // does not see, or whose weight's lower half is 0 or below, may then have made a NaN of an
-// infinity or of nothing; the rows are taken again one by one, as ONE: values that
+// infinity or of nothing; the rows are taken again one by one (ONE): values that
 // the row does not see are cleared, and those that are not finite are added as they are.
-enum class See { ALL, OWN, ONE };
-template <int HD, int MODE, int NQT, See SEE, typename Place, typename Sees>
+template <int HD, int MODE, int NQT, bool ONE, typename Place, typename Sees>
 __device__ __forceinline__ bool tile(const PagedArgs& a, WaveParts<HD>& w, int r0, int rows, int table, int kh, int begin,
                                      int end, const Sink& to, Place&& place, Sees&& sees) {
     constexpr int NS = HD / 32, NT = HD / 16;
-    constexpr bool MASKED = SEE != See::ALL;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Columns<HD, MODE, NQT> c;
     Blocks at;
-    bool gone = false;
     half8 k[2 * NS], v[NT];
     ColumnSees own[NQT];
     int bit[NQT];
-    c.start(a, r0, rows, kh, lane, -1, w.low);
-    if constexpr (MASKED) {
+    c.fetch(a, r0, rows, kh, lane, wave, -1);
 #pragma unroll
-        for (int u = 0; u < NQT; ++u) {
-            bit[u] = min(16 * u + (lane & 15), rows * a.group - 1) / a.group;
-            own[u] = sees(bit[u]);
-        }
+    for (int u = 0; u < NQT; ++u) {
+        bit[u] = rows == 1 ? 0 : min(16 * u + (lane & 15), rows * a.group - 1) / a.group;
+        own[u] = sees(bit[u]);
     }
+    bool none = at.look(a, table, begin + wave + PW * lane, end, place), gone = __any(none);
+    Region r = at.block<HD>(a, kh, 0);
+    load_k<HD, 0>(k, r, lane);
+    load_v<HD, 0>(v, r, lane);
+    c.start(a, lane, wave, w.q);
     for (int base = begin; base < end; base += PW * 64) {
-        const bool none = at.look(a, table, base + wave + PW * lane, end, place);
-        gone = gone || __any(none);
         const int n = min(64, (end - base - wave + PW - 1) / PW);
         if (n <= 0) break;
-        Region r = at.block<HD>(a, kh, 0);
-        load_k<HD, 0>(k, r, lane);
-        load_v<HD, 0>(v, r, lane);
+        if (base != begin) {
+            none = at.look(a, table, base + wave + PW * lane, end, place);
+            gone = gone || __any(none);
+            r = at.block<HD>(a, kh, 0);
+            load_k<HD, 0>(k, r, lane);
+            load_v<HD, 0>(v, r, lane);
+        }
         for (int j = 0; j < n; ++j) {
             const int k0 = at.key0(j);
             const Region next = at.block<HD>(a, kh, min(j + 1, 63));
-            if (SEE == See::ONE && !at.has(j)) {  // not this row's
+            if (ONE && !at.has(j)) {  // not this row's
                 load_k<HD, 0>(k, next, lane);
                 load_v<HD, 0>(v, next, lane);
                 continue;
             }
             ColumnSees now[NQT];
-            bool part = false;
-            if constexpr (MASKED) {
-                const uint32_t on = SEE == See::ONE ? 1u : (uint32_t)__builtin_amdgcn_readlane((int)at.rows, j);
-                bool some = false;
+            const uint32_t on = ONE ? 1u : (uint32_t)__builtin_amdgcn_readlane((int)at.rows, j);
+            bool some = false;
 #pragma unroll
-                for (int u = 0; u < NQT; ++u) {
-                    now[u] = on >> bit[u] & 1 ? own[u] : ColumnSees{0, 0, 0};
-                    some = some || !(k0 + 32 <= now[u].f || (k0 >= now[u].lo && k0 + 32 <= now[u].tk));
-                }
-                part = __any(some);
+            for (int u = 0; u < NQT; ++u) {
+                now[u] = on >> bit[u] & 1 ? own[u] : ColumnSees{0, 0, 0};
+                some = some || !(k0 + 32 <= now[u].f || (k0 >= now[u].lo && k0 + 32 <= now[u].tk));
             }
             c.scores(k);
             load_k<HD, 0>(k, next, lane);
-            c.softmax(k0, part, [&](int u, int key) {
-                return !MASKED || key < now[u].f || (key >= now[u].lo && key < now[u].tk);
-            });
-            if constexpr (SEE == See::ONE) {
+            c.softmax(k0, __any(some),
+                      [&](int u, int key) { return key < now[u].f || (key >= now[u].lo && key < now[u].tk); });
+            if constexpr (ONE) {
                 half8 one;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -421,7 +447,7 @@ __device__ __forceinline__ bool tile(const PagedArgs& a, WaveParts<HD>& w, int r
 #pragma unroll
         for (int u = 0; u < NQT; ++u) c.l[u] = __builtin_nanf("");
     }
-    return join<HD, MODE, NQT, SEE != See::ONE>(w, c, a.group, rows * a.group, to, tid);
+    return join<HD, MODE, NQT, !ONE>(w, c, a.group, rows * a.group, to, tid);
 }
 
 // Partials: own items' O, [item][kv head][group][HD]; wide ones' (tiles'), [item][kv
@@ -493,40 +519,47 @@ __global__ __launch_bounds__(PT, 2) void paged_kernel(PagedArgs a) {
         const int* p = plan_row(a, row + i) + 8;
         return shared ? ColumnSees{0, 0, 0x7fffffff} : ColumnSees{p[0], p[1], p[2]};
     };
-    if (shared) {
-        if (two ? tile<HD, MODE, 2, See::ALL>(a, w, row, rows, table, kh, begin, end, to, place, sees)
-                : tile<HD, MODE, 1, See::ALL>(a, w, row, rows, table, kh, begin, end, to, place, sees))
-            return;
-    } else if (rows == 1) {
+    if (rows == 1) {
         const ColumnSees s = sees(0);
         if (one_row<HD, MODE, AUX>(a, w, row, table, kh, begin, end, s.f, s.lo, s.tk, to, place)) return;
-    } else if (two ? tile<HD, MODE, 2, See::OWN>(a, w, row, rows, table, kh, begin, end, to, place, sees)
-                   : tile<HD, MODE, 1, See::OWN>(a, w, row, rows, table, kh, begin, end, to, place, sees)) {
+    } else if (two ? tile<HD, MODE, 2, false>(a, w, row, rows, table, kh, begin, end, to, place, sees)
+                   : tile<HD, MODE, 1, false>(a, w, row, rows, table, kh, begin, end, to, place, sees)) {
         return;
     }
     for (int i = 0; i < rows; ++i) {
-        tile<HD, MODE, 1, See::ONE>(a, w, row + i, 1, table, kh, begin, end, row_of(a, HD, to, i), place,
+        tile<HD, MODE, 1, true>(a, w, row + i, 1, table, kh, begin, end, row_of(a, HD, to, i), place,
                                     [&](int) { return sees(i); });
         __syncthreads();  // the join's arrays
     }
 }
 
-// The rows of a selection that are attended together: an aligned tile of rows whose
-// sequence is one.
+// The rows of a selection that are attended together: those of an aligned tile of
+// rows that follow one another and whose sequence is one. (By a whole wave.)
 struct Together {
-    int r0, rows, table;  // rows: 1 where they are taken one by one
+    int tile, r0, rows, table;  // rows: 1 where they are taken one by one
     __device__ __forceinline__ Together(const PagedArgs& a, int row) {
-        const int per = PG_TILE_ROWS(a.group);
-        r0 = row / per * per, rows = min(per, a.nseq - r0);
-        table = a.row ? a.row[row] : row;
-        bool one = rows > 1 && a.row && a.p.cols <= PG_UNION && table >= 0 && table < a.p.rows;
-        for (int i = 0; one && i < rows; ++i) one = a.row[r0 + i] == table;
-        if (!one) r0 = row, rows = 1;
+        const int per = PG_TILE_ROWS(a.group), lane = threadIdx.x & 63;
+        tile = row / per, r0 = tile * per;
+        const int n = min(per, a.nseq - r0), at = row - r0;
+        const int t = a.row ? a.row[r0 + min(lane, n - 1)] : r0 + lane;
+        table = __builtin_amdgcn_readlane(t, at);
+        // Bits of the rows that differ: the nearest on each side of this one.
+        const uint64_t other = ~__ballot(lane < n && t == table);
+        const uint64_t below = other & ((1ull << at) - 1), above = other >> at;
+        const int first = below ? 64 - __clzll(below) : 0, last = at + __ffsll((long long)above) - 1;
+        r0 += first, rows = last - first;
+        if (a.p.cols > PG_UNION || table < 0 || table >= a.p.rows) r0 = row, rows = 1;
     }
     __device__ __forceinline__ int runs(const PagedArgs& a) const {
         return rows == 1 ? a.runs : min(a.tile_runs, rows * a.runs);
     }
 };
+// What the join has to know of a row: its place in its tile's rows and their count;
+// whether its table row is missing.
+__device__ __forceinline__ int* row_note(const PagedArgs& a, int hd, int row) {
+    const size_t all = ((size_t)a.max_own * a.group + (size_t)a.max_wide * PG_COLS) * a.kv_heads;
+    return reinterpret_cast<int*>(a.part + all * (hd + 2)) + row;
+}
 
 // Over selected pages: workgroup (row, kv head, run) takes its share of `count`
 // pages' blocks. Rows of one sequence mostly select the same pages (neighbours of a
@@ -545,6 +578,8 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     auto length = [&](int r) { return max(0, min(a.tk[r], a.p.cols << a.p.shift)); };
     const Together t(a, row);
     const int runs = t.runs(a);
+    const bool live = t.table >= 0 && t.table < a.p.rows;
+    if (a.merge && run == 0 && kh == 0 && tid == 0) *row_note(a, HD, row) = (row - t.r0) | t.rows << 8 | (live ? 0 : 1 << 16);
     if (t.rows > 1) {
         const int sub = (row - t.r0) * a.runs + run;
         if (sub >= runs) return;
@@ -576,7 +611,8 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
         }
         const int blocks = n << s, share = (blocks + runs - 1) / runs, begin = sub * share, end = min(blocks, begin + share);
         const Sink to = runs == 1 ? context(a, HD, t.r0, kh)
-                                  : wide_part(a, HD, t.r0 / PG_TILE_ROWS(a.group) * a.tile_runs + sub, kh);
+                                  : row_of(a, HD, wide_part(a, HD, t.tile * a.tile_runs + sub, kh),
+                                           t.r0 - t.tile * PG_TILE_ROWS(a.group));
         auto place = [&](int i, uint32_t& on) {
             const int p = list[i >> s];
             on = mask[p];
@@ -584,15 +620,15 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
         };
         auto sees = [&](int i) { return ColumnSees{0, 0, length(t.r0 + i)}; };
         if (t.rows * a.group > 16
-                ? tile<HD, MODE, 2, See::OWN>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees)
-                : tile<HD, MODE, 1, See::OWN>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees))
+                ? tile<HD, MODE, 2, false>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees)
+                : tile<HD, MODE, 1, false>(a, w, t.r0, t.rows, t.table, kh, begin, end, to, place, sees))
             return;
         for (int i = 0; i < t.rows; ++i) {
             auto of_row = [&](int b, uint32_t& on) {
                 const int at = place(b, on);
                 return (on >> i & 1) && at < length(t.r0 + i) ? at : -1;
             };
-            tile<HD, MODE, 1, See::ONE>(a, w, t.r0 + i, 1, t.table, kh, begin, end, row_of(a, HD, to, i), of_row,
+            tile<HD, MODE, 1, true>(a, w, t.r0 + i, 1, t.table, kh, begin, end, row_of(a, HD, to, i), of_row,
                                         [&](int) { return sees(i); });
             __syncthreads();  // the join's arrays
         }
@@ -600,7 +636,6 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     }
     const int n = a.group * HD, tk = length(row);
     const Sink to = runs == 1 ? context(a, HD, row, kh) : own_part(a, HD, item, kh);
-    const bool live = t.table >= 0 && t.table < a.p.rows;
     if (runs == 1 && !live) {
         fill(to.o, n, __builtin_nanf(""));
         return;
@@ -615,7 +650,7 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
         return first < tk ? first : -1;
     };
     if (one_row<HD, MODE, AUX>(a, w, row, t.table, kh, begin, end, 0, 0, tk, to, place)) return;
-    tile<HD, MODE, 1, See::ONE>(a, w, row, 1, t.table, kh, begin, end, to, place, [&](int) { return ColumnSees{0, 0, tk}; });
+    tile<HD, MODE, 1, true>(a, w, row, 1, t.table, kh, begin, end, to, place, [&](int) { return ColumnSees{0, 0, tk}; });
 }
 
 // The parts of a row's columns of kv head kh: `on` of its own, then its group's.
@@ -630,12 +665,12 @@ struct Parts {
             o0 = d[0], on = d[1], s0 = d[2], step = d[4], col = d[5], own_col = d[6];
             n = on == 1 && d[3] == 0 ? 0 : on + d[3];
         } else {
-            const Together t(a, row);
-            bad = t.table < 0 || t.table >= a.p.rows;
-            on = t.runs(a);
+            const int note = *row_note(a, HD, row), rows = note >> 8 & 255, per = PG_TILE_ROWS(a.group);
+            bad = note >> 16 != 0;
+            on = rows == 1 ? a.runs : min(a.tile_runs, rows * a.runs);
             n = on == 1 ? 0 : on;
             o0 = row * a.runs;
-            if (t.rows > 1) o0 = t.r0 / PG_TILE_ROWS(a.group) * a.tile_runs, own_col = (row - t.r0) * a.group;
+            if (rows > 1) o0 = row / per * a.tile_runs, own_col = row % per * a.group;
         }
     }
     // The i-th part's O and (m, l) of query head g.

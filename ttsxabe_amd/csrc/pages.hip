@@ -70,8 +70,8 @@ __device__ __forceinline__ int2 scan_before(int2 v, int2* waves, int tid, int2& 
 
 // One workgroup. Tiles are up to PG_COLS columns (rows times a kv head's query
 // heads): a group's rows over the blocks that all of them see whole and hold in the
-// same pages, and rows of one sequence that lie together (an aligned tile of them)
-// over what else they see, each key masked by row; what a row alone sees is its own
+// same pages, and rows of one sequence that follow one another (within an aligned
+// tile of rows) over what else they see, each key masked by row; what a row alone sees is its own
 // item's. All are cut into items of about the same cost, `target` of them a kv head in
 // all. Bound by its chain of loads and barriers: a row a thread, few waves where there
 // are few rows (ONE: what they see is held in LDS, else in the plan itself).
@@ -83,8 +83,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __shared__ unsigned long long work;
     const int tid = threadIdx.x;
     const int tile_rows = PG_TILE_ROWS(a.group);
-    // (Whole tiles a thread, or a row.)
-    const int per = ONE ? 1 : (a.nseq + PP * tile_rows - 1) / (PP * tile_rows) * tile_rows;
+    const int per = ONE ? 1 : (a.nseq + PP - 1) / PP;
     const int r0 = min(a.nseq, tid * per), r1 = min(a.nseq, r0 + per);
     int groups = a.starts ? a.groups : 0;
     int4* rows = reinterpret_cast<int4*>(a.plan + PG_HEAD);
@@ -136,40 +135,58 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         }
         __syncthreads();
     }
-    // A row's own part: with its tile's where that is of one sequence and one group.
+    // A row's own part: with those of the rows of its aligned tile that follow one another
+    // and are of one sequence and group.
     struct Own {
         OwnBlocks o;
-        int g, first, rows;  // rows: 1, or its tile's from `first` on
+        int g, first, rows;
     };
     auto own_of = [&](int r) {
         Own x;
         x.g = groups ? group_of(r) : -1;
-        const int lo = x.g >= 0 ? glo[x.g] : 0, hi = x.g >= 0 ? ghi[x.g] : 0;
-        const int t0 = r / tile_rows * tile_rows, m = min(tile_rows, a.nseq - t0);
-        const int table = sees(r).w;
-        bool one = m > 1 && table >= 0 && a.row;
-        if (one && groups)
-            one = x.g >= 0 ? gst[x.g] <= t0 && t0 + m <= gst[x.g + 1] : t0 + m <= gst[0] || t0 >= gst[groups];
-        OwnBlocks all;
-        for (int i = 0; one && i < m; ++i) {
-            const int4 s = sees(t0 + i);
-            one = s.w == table;
-            all.add(s);
+        const int table = sees(r).w, t0 = r / tile_rows * tile_rows;
+        int from = t0, to = min(t0 + tile_rows, a.nseq);
+        if (x.g >= 0) from = max(from, gst[x.g]), to = min(to, gst[x.g + 1]);
+        else if (groups && r < gst[0]) to = min(to, gst[0]);
+        else if (groups) from = max(from, gst[groups]);
+        if (table < 0 || !a.row) from = r, to = r + 1;
+        x.first = r;
+        while (x.first > from && sees(x.first - 1).w == table) --x.first;
+        int end = x.first;
+        for (; end < to; ++end) {
+            const int4 s = sees(end);
+            if (end > r && s.w != table) break;
+            x.o.add(s);
         }
-        x.first = one ? t0 : r, x.rows = one ? m : 1;
-        if (!one) {
-            all = OwnBlocks();
-            all.add(sees(r));
+        x.rows = end - x.first;
+        if (x.rows < max(2, tile_rows / PG_RUNS)) {  // (so many tiles there is room for)
+            x.first = r, x.rows = 1;
+            x.o = OwnBlocks();
+            x.o.add(sees(r));
         }
-        all.close(lo, hi);
-        x.o = all;
+        x.o.close(x.g >= 0 ? glo[x.g] : 0, x.g >= 0 ? ghi[x.g] : 0);
         return x;
     };
     Own mine;
-    if constexpr (ONE) mine = own_of(min(tid, a.nseq - 1));
+    if constexpr (ONE) {
+        mine = own_of(min(tid, a.nseq - 1));
+    } else {  // kept where the row's words will be
+        for (int r = r0; r < r1; ++r) {
+            const Own x = own_of(r);
+            rows[PG_ROW / 4 * (size_t)r] = make_int4(x.o.na, x.o.b0, x.o.c0, x.o.d0);
+            rows[PG_ROW / 4 * (size_t)r + 1] = make_int4(x.o.n, x.g, x.first, x.rows);
+        }
+    }
     auto own = [&](int r) {
-        if constexpr (ONE) return mine;
-        else return own_of(r);
+        if constexpr (ONE) {
+            return mine;
+        } else {
+            const int4 d = rows[PG_ROW / 4 * (size_t)r], e = rows[PG_ROW / 4 * (size_t)r + 1];
+            Own x;
+            x.o.na = d.x, x.o.b0 = d.y, x.o.c0 = d.z, x.o.d0 = d.w, x.o.n = e.x;
+            x.g = e.y, x.first = e.z, x.rows = e.w;
+            return x;
+        }
     };
     unsigned long long cost = 0;
     for (int r = r0; r < r1; ++r) {
@@ -222,8 +239,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         else if (x.first == r) n.x += items_of(x);
     }
     const int2 before = scan_before<PP>(n, waves, tid, total);
-    // (A tile's rows but its first: their tile's items are the first's, which a thread before them may hold.)
-    int wide = ns + before.x, alone = before.y, last = wide;
+    int wide = ns + before.x, alone = before.y;
     const int nw = min(ns + total.x, a.max_wide);
     for (int r = r0; r < r1; ++r) {
         const Own x = own(r);
@@ -238,9 +254,8 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
             e.y = in % tile_rows * a.group;
         }
         if (x.rows > 1) {
-            // `wide` counts the tiles that begin up to here: this one's items end there, or begin.
-            if (x.first == r) last = wide;
-            d.x = x.first == r ? wide : (ONE ? wide - runs : last);
+            // `wide` counts the items of the tiles that begin before this row: its own tile's are the last, but for its first row.
+            d.x = x.first == r ? wide : wide - runs;
             e.z = (r - x.first) * a.group;
         }
         rows[PG_ROW / 4 * (size_t)r] = d;
@@ -267,6 +282,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
 
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t st) {
     if (a.nseq <= 256) hipLaunchKernelGGL((page_plan_kernel<256, true>), dim3(1), dim3(256), 0, st, a);
+    else if (a.nseq <= 1024) hipLaunchKernelGGL((page_plan_kernel<1024, true>), dim3(1), dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((page_plan_kernel<1024, false>), dim3(1), dim3(1024), 0, st, a);
     return hipGetLastError();
 }
