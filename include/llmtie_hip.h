@@ -461,7 +461,8 @@ int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q
  * whole blocks of 32 positions and no further than the shortest row's length. max_tk is the
  * longest length or near it (it says which launch is made; longer rows are attended too).
  * GQA groups up to 16, at most 1024 groups and 2^20 rows. */
-size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads);
+size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads,
+                            size_t kv_heads);
 int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev, const int32_t* lo_dev, size_t nseq,
                      const int32_t* starts, const int32_t* prefix, size_t groups, size_t max_tk, size_t window,
                      size_t shared, size_t table_rows, size_t table_cols, size_t page, size_t heads, size_t kv_heads,
@@ -472,8 +473,8 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
  * it was made with (rows are NaN under a plan of other sizes). ws: a workspace of
  * llmtie_attn_paged_workspace floats, 16-byte aligned, written and read on `stream` by this
  * call alone. out = [nseq, heads*head_dim] f32, 16-byte aligned as the cache is. */
-size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads,
-                                   size_t head_dim);
+size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads,
+                                   size_t kv_heads, size_t head_dim);
 int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
                              const uint16_t* cache, size_t cache_len, size_t pages, size_t page, const int32_t* table,
                              size_t table_len, size_t table_rows, size_t table_cols, const int32_t* tk_dev,
@@ -487,9 +488,10 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
  * llmtie_select_pages leaves them, any order, none twice; ones below 0 or with no
  * position that the row has name nothing). Row r sees those of their positions that
  * are below tk_dev[r]. Rows of one sequence that follow one another, as a prompt's do,
- * are attended together, each page read once for those that selected it. */
-size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
-                                      size_t head_dim);
+ * are attended together, each page read once for those that selected it, where there are more
+ * rows than the table has. */
+size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t table_rows, size_t heads,
+                                      size_t kv_heads, size_t head_dim);
 int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride,
                                 const uint16_t* cache, size_t cache_len, size_t pages, size_t page,
                                 const int32_t* table, size_t table_len, size_t table_rows, size_t table_cols,

@@ -114,18 +114,18 @@ def test_attention(call):
 
 def test_plan():
     L = _lib.lib()
-    need = L.llmtie_page_plan_len(3, 1, 1000, 8, 2)
+    need = L.llmtie_page_plan_len(3, 1, 1000, 4, 8, 2)
     assert plan(plan_len=need - 1) == 4 and list(last().field)[:2] == [need, need - 1]
     assert attn(plan_len=need - 1) == 4
     assert plan(groups=1025) == 4 and plan(nseq=2**20 + 1, row=P) == 4
     for name in ("tk", "plan", "starts", "prefix"):
         assert plan(**{name: NULL}) == 10, name
     assert plan(nseq=0) == 0
-    assert L.llmtie_page_plan_len(2**64 - 1, 1, 1000, 8, 2) == 0 and L.llmtie_page_plan_len(3, 1, 1000, 9, 2) == 0
-    floats = L.llmtie_attn_paged_workspace(3, 1, 1000, 8, 2, 128)
+    assert L.llmtie_page_plan_len(2**64 - 1, 1, 1000, 4, 8, 2) == 0 and L.llmtie_page_plan_len(3, 1, 1000, 4, 9, 2) == 0
+    floats = L.llmtie_attn_paged_workspace(3, 1, 1000, 4, 8, 2, 128)
     assert attn(ws_len=floats - 1) == 4 and attn(ws=NULL) == 10 and attn(ws=8) == 10
     # Short rows that share nothing need none.
-    assert L.llmtie_attn_paged_workspace(3, 0, 500, 8, 2, 128) == 0
+    assert L.llmtie_attn_paged_workspace(3, 0, 500, 4, 8, 2, 128) == 0
 
 
 def test_selected():
@@ -133,7 +133,7 @@ def test_selected():
     assert selected(chosen_len=29) == 4 and list(last().field)[:2] == [30, 29]
     assert selected(chosen=NULL) == 10
     assert selected(count=2**30) == 4
-    floats = L.llmtie_attn_selected_workspace(3, 5, 64, 8, 2, 128)
+    floats = L.llmtie_attn_selected_workspace(3, 5, 64, 4, 8, 2, 128)
     assert floats and selected(ws_len=floats - 1) == 4 and selected(ws=NULL) == 10 and selected(ws=8) == 10
 
 

@@ -74,12 +74,12 @@ SIGNATURES = {
                                   SZ, SZ, SZ, SZ, SZ, F, F, I, P, SZ, SZ, SZ]),
     "llmtie_paged_rope_store": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, I, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, P, P, SZ, P,
                                     SZ, SZ, SZ, P, SZ, SZ, SZ, SZ, SZ, SZ, F, F, I, P, SZ, SZ, SZ]),
-    "llmtie_page_plan_len": (SZ, [SZ, SZ, SZ, SZ, SZ]),
+    "llmtie_page_plan_len": (SZ, [SZ, SZ, SZ, SZ, SZ, SZ]),
     "llmtie_page_plan": (I, [P, P, P, P, SZ, P, P, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, SZ, P, SZ]),
-    "llmtie_attn_paged_workspace": (SZ, [SZ, SZ, SZ, SZ, SZ, SZ]),
+    "llmtie_attn_paged_workspace": (SZ, [SZ, SZ, SZ, SZ, SZ, SZ, SZ]),
     "llmtie_attn_decode_paged": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, P, SZ, SZ, SZ, SZ, SZ, SZ, SZ,
                                      F, F, P, SZ, P, SZ, P, SZ]),
-    "llmtie_attn_selected_workspace": (SZ, [SZ, SZ, SZ, SZ, SZ, SZ]),
+    "llmtie_attn_selected_workspace": (SZ, [SZ, SZ, SZ, SZ, SZ, SZ, SZ]),
     "llmtie_attn_decode_selected": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, P, P, SZ, SZ, SZ, SZ, SZ, SZ,
                                         F, F, P, SZ, P, SZ, P, SZ]),
     "llmtie_page_bounds": (I, [P, P, SZ, SZ, SZ, P, SZ, SZ, SZ, P, P, P, SZ, SZ, SZ, SZ, P, SZ]),

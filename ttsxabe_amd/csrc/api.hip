@@ -1600,20 +1600,25 @@ constexpr size_t PG_MAX_ROWS = (size_t)1 << 20;
 // How a step over pages is divided, from what the host knows of it.
 struct PagedSizes {
     size_t target, max_wide, max_own, items;
-    bool whole;
+    bool whole, together;
 };
 // Items of a kv head: two workgroups a compute unit, fewer where the rows do not
 // hold four blocks for each. Few rows of a short bound are one item each, prefix and all.
-PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
+// Rows of one sequence are looked for, to be attended together, where there are more
+// rows than sequences in the table (tokens of a batch have none, and do without the search
+// and a join's launch: 23 rows of 32/8/64 over 6 pages each 12.8 -> 10 us).
+PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads, size_t kv_heads) {
     PagedSizes s;
+    s.together = nseq > table_rows;
     const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
     const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads));
     s.target = std::max<size_t>(1, std::min(2 * (size_t)compute_units() / kv_heads, (nseq * blocks + 3) / 4));
     s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * (size_t)compute_units());
     // Shared tiles, and tiles of one sequence's rows.
-    const size_t tiles = (groups && !s.whole ? nseq / per + groups : 0) + std::min(nseq / 2, PG_RUNS * ((nseq + per - 1) / per));
+    const size_t tiles = (groups && !s.whole ? nseq / per + groups : 0) +
+                         (s.together ? std::min(nseq / 2, PG_RUNS * ((nseq + per - 1) / per)) : 0);
     s.max_own = s.whole ? nseq : nseq + s.target;
-    s.max_wide = s.whole ? nseq : tiles + s.target;
+    s.max_wide = s.whole ? nseq : tiles ? tiles + s.target : 0;
     s.items = s.whole ? nseq : nseq + tiles + s.target;
     return s;
 }
@@ -1626,7 +1631,7 @@ int paged_checks(size_t nseq, size_t groups, size_t max_tk, const TableArg& t, s
     if (max_tk == 0 || max_tk > smul(t.cols, page)) return overrun_cache(max_tk, smul(t.cols, page));
     if (nseq > PG_MAX_ROWS) return overrun_slice(nseq, PG_MAX_ROWS);
     if (groups > (size_t)PG_GROUPS) return overrun_slice(groups, PG_GROUPS);
-    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, t.rows, heads, kv_heads);
     const size_t wgs = std::max(smul(z.items, kv_heads), smul(smul(nseq, heads), head_dim / 4) / 256);
     if (wgs > MAX_WGS) return overrun_slice(wgs, MAX_WGS);
     return LLMTIE_OK;
@@ -1643,15 +1648,17 @@ Pages pages_of(const uint16_t* cache, const TableArg& t, size_t pages, size_t pa
 // more than its rows have.
 struct SelectedSizes {
     size_t runs, tile_runs, max_own, max_wide;
+    bool together;
 };
-SelectedSizes selected_sizes(size_t nseq, size_t blocks, size_t heads, size_t kv_heads) {
+SelectedSizes selected_sizes(size_t nseq, size_t blocks, size_t table_rows, size_t heads, size_t kv_heads) {
     SelectedSizes s;
     const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads)), tiles = (nseq + per - 1) / per;
     const size_t cus = (size_t)compute_units();
     s.runs = std::max<size_t>(1, std::min((blocks + 3) / 4, cus / std::max<size_t>(1, smul(nseq, kv_heads))));
     s.tile_runs = std::max<size_t>(1, std::min(std::min(nseq, per) * s.runs, 2 * cus / std::max<size_t>(1, smul(tiles, kv_heads))));
     s.max_own = s.runs > 1 ? nseq * s.runs : 0;
-    s.max_wide = s.tile_runs > 1 && nseq > 1 ? tiles * s.tile_runs : 0;
+    s.together = nseq > table_rows;
+    s.max_wide = s.together && s.tile_runs > 1 ? tiles * s.tile_runs : 0;
     return s;
 }
 
@@ -1694,9 +1701,10 @@ int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q
                       TableArg{table, table_len, table_rows, table_cols, true});
 }
 
-size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads) {
+size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads,
+                            size_t kv_heads) {
     if (kv_heads == 0 || heads == 0 || heads % kv_heads != 0 || heads / kv_heads > 16 || nseq > PG_MAX_ROWS) return 0;
-    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, table_rows, heads, kv_heads);
     return sadd(plan_items_at(nseq), smul(sadd(z.max_wide, z.max_own), PG_ITEM));
 }
 
@@ -1707,12 +1715,12 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
     const TableArg t{nullptr, SIZE_MAX, table_rows, table_cols, true};
     if (int r = paged_checks(nseq, groups, max_tk, t, page, heads, kv_heads, head_dim)) return r;
     if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
-    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, heads, kv_heads);
+    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, table_rows, heads, kv_heads);
     if (plan_len < need) return overrun_slice(need, plan_len);
     if (nseq == 0) return ok();
     if (!tk_dev || !plan || (groups && (!starts || !prefix))) return invalid("a buffer");
     if (off16(plan)) return refuse("a plan off 16 bytes");
-    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, table_rows, heads, kv_heads);
     PagePlanArgs a{};
     a.tk = tk_dev;
     a.row = row_dev;
@@ -1733,14 +1741,15 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
     a.max_own = (int)z.max_own;
     a.target = (int)z.target;
     a.whole = z.whole ? 1 : 0;
+    a.together = z.together && row_dev ? 1 : 0;
     return launched("page_plan", launch_page_plan(a, S(stream)));
 }
 
-size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t heads, size_t kv_heads,
-                                   size_t head_dim) {
+size_t llmtie_attn_paged_workspace(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads,
+                                   size_t kv_heads, size_t head_dim) {
     if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16 || nseq == 0 || nseq > PG_MAX_ROWS)
         return 0;
-    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, table_rows, heads, kv_heads);
     return z.whole ? 0 : paged_floats(z, heads, kv_heads, head_dim);
 }
 
@@ -1757,8 +1766,8 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
     const size_t n = smul(heads, head_dim);
     if (int r = query_checks(q, q_len, q_off, q_stride, nseq, n, out_len, cache_len, pages, page, kv_heads, head_dim))
         return r;
-    const PagedSizes z = paged_sizes(nseq, groups, max_tk, heads, kv_heads);
-    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, heads, kv_heads);
+    const PagedSizes z = paged_sizes(nseq, groups, max_tk, table_rows, heads, kv_heads);
+    const size_t need = llmtie_page_plan_len(nseq, groups, max_tk, table_rows, heads, kv_heads);
     if (plan_len < need) return overrun_slice(need, plan_len);
     const size_t floats = z.whole ? 0 : paged_floats(z, heads, kv_heads, head_dim);
     if (nseq == 0) return ok();
@@ -1788,11 +1797,11 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
     return launched("attn_decode_paged", launch_paged((int)head_dim, a, S(stream)));
 }
 
-size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t heads, size_t kv_heads,
-                                      size_t head_dim) {
+size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t table_rows, size_t heads,
+                                      size_t kv_heads, size_t head_dim) {
     if (!llmtie_supports_flash(head_dim, heads, kv_heads) || heads / kv_heads > 16 || nseq == 0 || nseq > PG_MAX_ROWS)
         return 0;
-    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), heads, kv_heads);
+    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), table_rows, heads, kv_heads);
     if (!z.max_own && !z.max_wide) return 0;
     // Parts, and a word a row.
     return sadd(smul(sadd(smul(z.max_own, heads), smul(z.max_wide, PG_COLS, kv_heads)), head_dim + 2), nseq);
@@ -1815,9 +1824,9 @@ int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size
     if (chosen_len < smul(units, count)) return overrun_slice(smul(units, count), chosen_len);
     if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
     if (nseq == 0) return ok();
-    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), heads, kv_heads);
+    const SelectedSizes z = selected_sizes(nseq, smul(count, page / 32), table_rows, heads, kv_heads);
     if (smul(units, z.runs) > MAX_WGS) return overrun_slice(smul(units, z.runs), MAX_WGS);
-    const size_t floats = llmtie_attn_selected_workspace(nseq, count, page, heads, kv_heads, head_dim);
+    const size_t floats = llmtie_attn_selected_workspace(nseq, count, page, table_rows, heads, kv_heads, head_dim);
     if (ws_len < floats) return overrun_slice(floats, ws_len);
     if (!q || !cache || !table || !tk_dev || (count && !chosen) || !out || (floats && !ws)) return invalid("a buffer");
     if (off16(cache) || off16(out) || off16(ws)) return refuse("a cache, a context or a workspace off 16 bytes");
@@ -1839,6 +1848,7 @@ int llmtie_attn_decode_selected(void* stream, const float* q, size_t q_len, size
     a.count = (int)count;
     a.runs = (int)z.runs;
     a.tile_runs = (int)z.tile_runs;
+    a.together = z.together && row_dev ? 1 : 0;
     a.merge = z.max_own || z.max_wide ? 1 : 0;
     a.scale = scale;
     a.softcap = softcap;

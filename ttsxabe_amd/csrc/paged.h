@@ -41,6 +41,7 @@ struct PagePlanArgs {
     int max_wide, max_own;    // items there is room for
     int target;               // items of a kv head that the work is divided into
     int whole;                // every row is one item (no group shares)
+    int together;             // rows of one sequence may follow one another
 };
 hipError_t launch_page_plan(const PagePlanArgs& a, hipStream_t st);
 
@@ -60,6 +61,7 @@ struct PagedArgs {
     int items;           // of a kv head, at most
     int count, runs;     // selected pages: how many, and the workgroups of a (row, kv head)
     int tile_runs;       // and of a tile of rows at most
+    int together;        // rows of one sequence may follow one another
     int stream;          // more bytes than are worth keeping in the Infinity Cache
     int merge;           // some row may have partials
     float scale, softcap;

@@ -540,6 +540,10 @@ struct Together {
     __device__ __forceinline__ Together(const PagedArgs& a, int row) {
         const int per = PG_TILE_ROWS(a.group), lane = threadIdx.x & 63;
         tile = row / per, r0 = tile * per;
+        if (!a.together) {
+            r0 = row, rows = 1, table = a.row ? a.row[row] : row;
+            return;
+        }
         const int n = min(per, a.nseq - r0), at = row - r0;
         const int t = a.row ? a.row[r0 + min(lane, n - 1)] : r0 + lane;
         table = __builtin_amdgcn_readlane(t, at);

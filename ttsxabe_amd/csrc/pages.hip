@@ -149,7 +149,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         if (x.g >= 0) from = max(from, gst[x.g]), to = min(to, gst[x.g + 1]);
         else if (groups && r < gst[0]) to = min(to, gst[0]);
         else if (groups) from = max(from, gst[groups]);
-        if (table < 0 || !a.row) from = r, to = r + 1;
+        if (table < 0 || !a.together) from = r, to = r + 1;
         x.first = r;
         while (x.first > from && sees(x.first - 1).w == table) --x.first;
         int end = x.first;

@@ -191,6 +191,47 @@ __device__ __forceinline__ void row(const RotaryArgs& a, int r, int h0, int h1, 
     }
 }
 
+// The values of n rows (1 to 8) from r on that lie together within eight positions, heads
+// v0 .. h1 - 1 of k's and v's: eight of them in whole 16-byte chunks.
+template <int V>
+__device__ __forceinline__ void store_run(const RotaryArgs& a, int r, int n, int v0, int h1, int tid) {
+    const int quads = a.hd / 4;
+    for (int e = tid; e < (h1 - v0) * quads; e += RO) {
+        const int h = v0 - a.kv + e / quads, d = 4 * (e % quads);
+        float x[8][4];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const float* src = a.v + (size_t)(r + min(p, n - 1)) * a.v_stride + (size_t)h * a.hd + d;
+#pragma unroll
+            for (int i = 0; i < 4; i += V) {
+                const Vec<V> y = ld_vec<V>(src + i);
+#pragma unroll
+                for (int c = 0; c < V; ++c) x[p][i + c] = y.x[c];
+            }
+        }
+        int kk;
+        half_t* b = home<true>(a, r, h, kk);
+        if (!b) continue;
+        b += 32 * a.hd;
+        if (n == 8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                half8 y;
+#pragma unroll
+                for (int p = 0; p < 8; ++p) y[p] = to_h(x[p][i]);
+                *reinterpret_cast<half8*>(b + t16_v_off(kk, d + i)) = y;
+            }
+            continue;
+        }
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            if (p >= n) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[t16_v_off(kk + p, d + i)] = to_h(x[p][i]);
+        }
+    }
+}
+
 // Eight rows a workgroup, heads h0 .. h1 - 1 of k's and v's, for prompts: rows
 // that fill a run of eight cache positions store v in whole 16-byte chunks, and
 // k's 16-byte chunks of the rows lie together. r0 is a multiple of eight behind
@@ -214,12 +255,26 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
     }
     const int v0 = max(h0, a.kv);
     if (v0 >= h1) return;
+    if constexpr (PAGED) {
+        // Packed prompts begin at any place of their sequences: the workgroup takes the runs
+        // within eight positions that begin at one of its rows, whole or not (three prompts
+        // of 701 rows of 32/8/128, by the first row's alignment 22.6 us, so 18.5).
+        const int lane = tid & 63, r = r0 + lane;
+        const bool in = r < a.rows;
+        const int s = in ? a.slot[r] : -1, i = in ? a.index[r] : 0;
+        const bool first = !in || (i & 7) == 0 || r == 0 || a.slot[r - 1] != s || a.index[r - 1] != i - 1;
+        const uint64_t begins = __ballot(first);
+        for (int j = 0; j < 8 && r0 + j < a.rows; ++j) {
+            if (!(begins >> j & 1)) continue;
+            const int n = __ffsll((long long)(begins >> (j + 1)));  // rows of the run
+            store_run<V>(a, r0 + j, n, v0, h1, tid);
+        }
+        return;
+    }
     bool run = r0 >= 0 && r0 + 8 <= a.rows;
     if (run) {
         const int s = a.slot[r0], i = a.index[r0];
-        int kk;  // (a run of eight lies in one page)
-        run = (i & 7) == 0 && (PAGED ? home<PAGED>(a, r0, 0, kk) != nullptr
-                                     : s >= 0 && s < a.slots && i >= 0 && i < a.cap - 7);
+        run = (i & 7) == 0 && s >= 0 && s < a.slots && i >= 0 && i < a.cap - 7;
         for (int p = 1; p < 8 && run; ++p) run = a.slot[r0 + p] == s && a.index[r0 + p] == i + p;
     }
     const int quads = a.hd / 4;
@@ -239,7 +294,7 @@ __device__ __forceinline__ void rows8(const RotaryArgs& a, int r0, int h0, int h
         }
         int kk;
         if (run) {
-            half_t* b = home<PAGED>(a, r0, h, kk) + 32 * a.hd;
+            half_t* b = home<false>(a, r0, h, kk) + 32 * a.hd;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 half8 y;
@@ -271,7 +326,7 @@ __global__ __launch_bounds__(RO) void rotary_kernel(RotaryArgs a, int g8, int hp
     if constexpr (GROUPS) {
         if ((int)blockIdx.x < g8) {
             const int per = (2 * a.kv + hpb8 - 1) / hpb8, g = (int)blockIdx.x / per, h0 = (int)blockIdx.x % per * hpb8;
-            const int shift = a.index[0] & 7;
+            const int shift = PAGED ? 0 : a.index[0] & 7;
             rows8<V, PAGED>(a, 8 * g - shift, h0, min(2 * a.kv, h0 + hpb8), cs, tid);
             return;
         }

@@ -820,11 +820,11 @@ class Gpu:
         if min(max_tk, heads, window, shared) < 0:
             raise InvalidArgument("a negative count")
         kv, hd = cache.kv_heads, cache.head_dim
-        size = self._L.llmtie_page_plan_len(n, groups, max_tk, heads, kv)
+        size = self._L.llmtie_page_plan_len(n, groups, max_tk, rows, heads, kv)
         plan = torch.empty(size, dtype=torch.int32, device=self.device)
         self._run(self._L.llmtie_page_plan, tk_dev.data_ptr(), _p(row_dev), _p(lo_dev), n, _p(starts), _p(prefix), groups,
                   max_tk, window, shared, rows, cols, cache.page, heads, kv, hd, plan.data_ptr(), size)
-        floats = self._L.llmtie_attn_paged_workspace(n, groups, max_tk, heads, kv, hd)
+        floats = self._L.llmtie_attn_paged_workspace(n, groups, max_tk, rows, heads, kv, hd)
         return PagePlan(plan, tk_dev, table, heads, kv, hd, cache.page, groups, max_tk, floats)
 
     def attn_decode_paged(self, q, q_off, q_stride, cache: PagedCache16, plan: PagePlan, heads, scale, softcap=0.0,
@@ -873,10 +873,11 @@ class Gpu:
             out = torch.empty(n, dtype=torch.float32, device=self.device)
         else:
             self._on(out, _F32, "out")
-        floats = self._L.llmtie_attn_selected_workspace(nseq, count, cache.page, heads, kv, hd)
+        pages = self._table(table)
+        floats = self._L.llmtie_attn_selected_workspace(nseq, count, cache.page, pages[2], heads, kv, hd)
         ws = self._room(floats)
         self._run(self._L.llmtie_attn_decode_selected, q.data_ptr(), q.numel(), q_off, q_stride, data.data_ptr(),
-                  data.numel(), cache.pages, cache.page, *self._table(table), tk_dev.data_ptr(), _p(row_dev),
+                  data.numel(), cache.pages, cache.page, *pages, tk_dev.data_ptr(), _p(row_dev),
                   chosen.data_ptr(), chosen.numel(), count, nseq, heads, kv, hd, scale, softcap, _p(slopes), _n(slopes),
                   _p(ws), floats, out.data_ptr(), out.numel())
         return out if out.numel() == n else out[:n]
