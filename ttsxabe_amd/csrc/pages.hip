@@ -77,9 +77,10 @@ __device__ __forceinline__ int2 scan_before(int2 v, int2* waves, int tid, int2& 
 // are few rows (ONE: what they see is held in LDS, else in the plan itself).
 template <int PP, bool ONE>
 __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
-    __shared__ int gst[PG_GROUPS + 1], glo[PG_GROUPS], ghi[PG_GROUPS], gat[PG_GROUPS];
+    __shared__ int gst[PG_GROUPS + 1], glo[PG_GROUPS], ghi[PG_GROUPS], gat[PG_GROUPS], gruns[PG_GROUPS];
     __shared__ int4 held[ONE ? PP : 1];
     __shared__ int2 waves[PP / 64];
+    __shared__ uint64_t links[PP / 64 + 1];
     __shared__ unsigned long long work;
     const int tid = threadIdx.x;
     const int tile_rows = PG_TILE_ROWS(a.group);
@@ -88,23 +89,26 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     int groups = a.starts ? a.groups : 0;
     int4* rows = reinterpret_cast<int4*>(a.plan + PG_HEAD);
     int4* items = reinterpret_cast<int4*>(a.plan + plan_items_at(a.nseq));
+    auto sees = [&](int r) {
+        if constexpr (ONE) return held[r];
+        else return rows[PG_ROW / 4 * (size_t)r + 2];
+    };
+    // (The groups' loads before the first row's are waited for.)
+    int falls = 0;
+    for (int g = tid; g < groups; g += PP) {
+        const int x = max(0, min(a.starts[g], a.nseq)), y = max(0, min(a.starts[g + 1], a.nseq)), p = a.prefix[g];
+        gst[g] = x, ghi[g] = p, glo[g] = 0;
+        if (g == groups - 1) gst[groups] = y;
+        falls |= x > y;
+    }
     for (int r = r0; r < r1; ++r) {
         const int4 s = row_sees(a, r);
         rows[PG_ROW / 4 * (size_t)r + 2] = s;
         if constexpr (ONE) held[r] = s;
     }
-    auto sees = [&](int r) {
-        if constexpr (ONE) return held[r];
-        else return rows[PG_ROW / 4 * (size_t)r + 2];
-    };
-    for (int g = tid; g <= groups && groups; g += PP) gst[g] = max(0, min(a.starts[g], a.nseq));
-    for (int g = tid; g < groups; g += PP) ghi[g] = a.prefix[g], glo[g] = 0;
     if (tid == 0) work = 0;
-    __syncthreads();
     // Starts that decrease: no groups (tiles would lie over one another, more than there is room for).
-    int falls = 0;
-    for (int g = tid; g < groups; g += PP) falls |= gst[g] > gst[g + 1];
-    if (groups && __syncthreads_or(falls)) groups = 0;
+    if (__syncthreads_or(falls)) groups = 0;
     auto group_of = [&](int r) {
         int lo = -1, hi = groups;
         while (hi - lo > 1) {
@@ -141,29 +145,40 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         OwnBlocks o;
         int g, first, rows;
     };
+    // Whether row r goes on with the sequence and the group of the one before.
+    auto goes_on = [&](int r) {
+        if (!a.together || r <= 0 || r >= a.nseq) return false;
+        const int t = sees(r).w;
+        return t >= 0 && t == sees(r - 1).w && (!groups || group_of(r) == group_of(r - 1));
+    };
+    if constexpr (ONE) {
+        const uint64_t on = __ballot(goes_on(tid));
+        if ((tid & 63) == 0) links[tid >> 6] = on;
+        if (tid == 0) links[PP / 64] = 0;
+        __syncthreads();
+    }
     auto own_of = [&](int r) {
         Own x;
         x.g = groups ? group_of(r) : -1;
-        const int table = sees(r).w, t0 = r / tile_rows * tile_rows;
-        int from = t0, to = min(t0 + tile_rows, a.nseq);
-        if (x.g >= 0) from = max(from, gst[x.g]), to = min(to, gst[x.g + 1]);
-        else if (groups && r < gst[0]) to = min(to, gst[0]);
-        else if (groups) from = max(from, gst[groups]);
-        if (table < 0 || !a.together) from = r, to = r + 1;
+        const int t0 = r / tile_rows * tile_rows, to = min(t0 + tile_rows, a.nseq);
         x.first = r;
-        while (x.first > from && sees(x.first - 1).w == table) --x.first;
-        int end = x.first;
-        for (; end < to; ++end) {
-            const int4 s = sees(end);
-            if (end > r && s.w != table) break;
-            x.o.add(s);
+        int end = r + 1;
+        if constexpr (ONE) {
+            // The links of rows t0 up to t0 + 63: bits up to r back to the last that is not set, and on from there.
+            const int w = t0 >> 6, sh = t0 & 63;
+            const uint64_t on = (links[w] >> sh | (sh ? links[w + 1] << (64 - sh) : 0)) & ~1ull;
+            const int at = r - t0;
+            const uint64_t begins = ~on & ((2ull << at) - 1);  // (bit 0 is one)
+            x.first = t0 + 63 - __clzll((long long)begins);
+            const uint64_t breaks = ~on >> (at + 1);
+            end = breaks ? min(to, r + __ffsll((long long)breaks)) : to;
+        } else if (a.together) {
+            while (x.first > t0 && goes_on(x.first)) --x.first;
+            while (end < to && goes_on(end)) ++end;
         }
         x.rows = end - x.first;
-        if (x.rows < max(2, tile_rows / PG_RUNS)) {  // (so many tiles there is room for)
-            x.first = r, x.rows = 1;
-            x.o = OwnBlocks();
-            x.o.add(sees(r));
-        }
+        if (x.rows < max(2, tile_rows / PG_RUNS)) x.first = r, x.rows = 1;  // (so many tiles there is room for)
+        for (int i = 0; i < x.rows; ++i) x.o.add(sees(x.first + i));
         x.o.close(x.g >= 0 ? glo[x.g] : 0, x.g >= 0 ? ghi[x.g] : 0);
         return x;
     };
@@ -193,38 +208,45 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         const Own x = own(r);
         if (x.first == r) cost += (unsigned long long)x.o.n * (x.rows > 1 ? wide_cost(x.rows) : 4);
     }
-    if (cost) atomicAdd(&work, cost);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) cost += __shfl_xor(cost, d);
+    if ((tid & 63) == 0) atomicAdd(&work, cost);
     __syncthreads();
-    // Cost of an item, four a block (seven of two column tiles).
-    const unsigned long long c = max((work + a.target - 1) / a.target, (unsigned long long)(4 * PG_SPAN));
-    auto cut = [&](int blocks, int cost) {
-        return a.whole ? 1 : (int)(((unsigned long long)blocks * cost + c - 1) / c);
-    };
+    // Cost of an item, four a block (seven of two column tiles). (A sequence costs up to
+    // 7 * 2^25: 32 bits, as divisions of 64 take half a microsecond each, 9 us of 14.)
+    const unsigned long long each = (work + a.target - 1) / a.target;
+    const unsigned c = (unsigned)max(min(each, 0x7fffffffull), (unsigned long long)(4 * PG_SPAN));
+    auto cut = [&](int blocks, int cost) { return a.whole ? 1 : (int)(((unsigned)blocks * cost + c - 1) / c); };
 
     // Shared tiles, a group's runs of blocks outermost, so that its tiles read a run at one time.
     int ns = 0;
-    auto runs_of = [&](int g) { return cut(ghi[g] - glo[g], wide_cost(gst[g + 1] - gst[g])); };
+    auto runs_of = [&](int g) { return gruns[g]; };
     auto tiles_of = [&](int g) { return (gst[g + 1] - gst[g] + tile_rows - 1) / tile_rows; };
     if (groups) {
         const int each = (groups + PP - 1) / PP, g0 = min(groups, tid * each), g1 = min(groups, g0 + each);
-        auto items_of = [&](int g) { return ghi[g] > glo[g] ? tiles_of(g) * runs_of(g) : 0; };
         int2 n = make_int2(0, 0), total;
-        for (int g = g0; g < g1; ++g) n.x += items_of(g);
+        for (int g = g0; g < g1; ++g) {
+            gruns[g] = ghi[g] > glo[g] ? cut(ghi[g] - glo[g], wide_cost(gst[g + 1] - gst[g])) : 0;
+            n.x += tiles_of(g) * gruns[g];
+        }
         int at = scan_before<PP>(n, waves, tid, total).x;
-        for (int g = g0; g < g1; ++g) gat[g] = at, at += items_of(g);
+        for (int g = g0; g < g1; ++g) gat[g] = at, at += tiles_of(g) * gruns[g];
         __syncthreads();
         ns = min(total.x, a.max_wide);
-        for (int g = 0; g < groups; ++g) {
-            if (ghi[g] <= glo[g]) continue;
-            const int tiles = tiles_of(g), runs = runs_of(g), nb = ghi[g] - glo[g], share = (nb + runs - 1) / runs;
-            for (int i = tid; i < tiles * runs; i += PP) {
-                if (gat[g] + i >= ns) break;
-                const int t = i % tiles, b = i / tiles * share, first = gst[g] + t * tile_rows;
-                int4* d = items + PG_ITEM / 4 * (size_t)(gat[g] + i);
-                d[0] = make_int4(first, min(tile_rows, gst[g + 1] - first), sees(first).w, PG_SHARED);
-                d[1] = make_int4(0, glo[g], ghi[g], ghi[g]);
-                d[2] = make_int4(b, min(nb, b + share), 0, 0);
+        for (int i = tid; i < ns; i += PP) {
+            // Its group: the last one that begins at or before it and has items.
+            int lo = 0, hi = groups;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (gat[mid] <= i) lo = mid;
+                else hi = mid;
             }
+            const int g = lo, tiles = tiles_of(g), nb = ghi[g] - glo[g], share = (nb + gruns[g] - 1) / gruns[g];
+            const int in = i - gat[g], t = in % tiles, b = in / tiles * share, first = gst[g] + t * tile_rows;
+            int4* d = items + PG_ITEM / 4 * (size_t)i;
+            d[0] = make_int4(first, min(tile_rows, gst[g + 1] - first), sees(first).w, PG_SHARED);
+            d[1] = make_int4(0, glo[g], ghi[g], ghi[g]);
+            d[2] = make_int4(b, min(nb, b + share), 0, 0);
         }
     }
     // Tiles of one sequence's rows (x), and rows by themselves (y).
