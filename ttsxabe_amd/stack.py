@@ -15,14 +15,20 @@ needed, at least 256 positions (model.rs:703-721), copying the live prefix.
 `LlamaBatch` (no counterpart in the reference, which steps its sequences one
 by one) runs several sequences of the same stack at once: prompts packed into
 one pass, each a document of its own, and one token of all of them a step, over
-the slots of tiled caches.
+the slots of tiled caches. `LlamaPages` does so over pages, which sequences that
+begin alike share.
 """
 from __future__ import annotations
 
 import numpy as np
 import torch
 
-from .gpu import CacheOverrun, DecodeScratch, Gpu, InvalidArgument, TiledCache16, rope_scaling
+from .gpu import CacheOverrun, DecodeScratch, Gpu, InvalidArgument, PagedCache16, TiledCache16, rope_scaling
+
+
+def _no_selection(cfg):
+    if getattr(cfg, "select", None) is not None:
+        raise ValueError("a configuration that selects pages, which LlamaPages attends")
 
 
 class LlamaStack:
@@ -43,6 +49,7 @@ class LlamaStack:
                           ("scaled rotary positions", kind != "none" and factor != 1.0)):
             if has:
                 raise ValueError(f"a configuration with {what}, which LlamaBatch computes")
+        _no_selection(cfg)
         self.g, self.cfg, self.layout = gpu, cfg, layout
         dev = gpu.device
         self.w = {k: torch.from_numpy(np.ascontiguousarray(v)).to(dev) for k, v in weights.items()}
@@ -127,13 +134,8 @@ class LlamaStack:
         return (self._norm(h[-1:], w["norm"]) @ w["lm_head"].T)[0]
 
 
-class LlamaBatch:
-    """Up to `slots` sequences of `cap` positions side by side. Beside the
-    geometry `cfg` may hold `rope_interleaved` (weights for pairs (2i, 2i + 1), as
-    a GGUF stores them), `rope_dim` (rotated dims of a head, 0: all),
-    `rope_scaling` ((kind, factor, original positions), see gpu.rope_scaling),
-    `softcap`, `window` with `shared` leading positions kept, and `slopes` (a
-    distance bias a head)."""
+class _Sequences:
+    """What several sequences of one stack at once have in common, wherever their keys lie."""
 
     def __init__(self, gpu: Gpu, cfg, weights: dict, slots: int, cap: int):
         self.g, self.cfg, self.slots, self.cap = gpu, cfg, slots, cap
@@ -142,9 +144,7 @@ class LlamaBatch:
         for l in range(cfg.layers):  # q, k and v in one product, rows the rotation and the stores read as they are
             w[f"{l}.wqkv"] = torch.cat([w.pop(f"{l}.wq"), w.pop(f"{l}.wk"), w.pop(f"{l}.wv")])
         self.w = w
-        self.cache = [TiledCache16(cfg.kv_heads, cfg.head_dim, cap, device=dev, slots=slots) for _ in range(cfg.layers)]
         self.packed = None  # the keys of the prompts being packed, one layer at a time
-        self.scratch = DecodeScratch()
         self.length = [0] * slots
         self.rot = getattr(cfg, "rope_dim", 0) or cfg.head_dim
         kind, factor, original = getattr(cfg, "rope_scaling", None) or ("none", 1.0, 8192)
@@ -161,8 +161,9 @@ class LlamaBatch:
     def _ints(self, v):
         return torch.tensor(v, dtype=torch.int32, device=self.g.device)
 
-    def _check(self, slots, new, ids):
+    def _check(self, slots, new, ids, length=None):
         # (An id past the embedding ends the process from the device.)
+        length = self.length if length is None else length
         vocab = len(self.w["embed"])
         if ids and not (min(ids) >= 0 and max(ids) < vocab):
             raise InvalidArgument(f"a token that is not one of {vocab}")
@@ -171,9 +172,9 @@ class LlamaBatch:
         for s, n in zip(slots, new):
             if n < 1:
                 raise InvalidArgument("a sequence without tokens")
-            if self.length[s] + n > self.cap:
-                raise CacheOverrun(f"appending at {self.length[s] + n} to a cache with room for {self.cap}",
-                                   (self.length[s] + n, self.cap))
+            if length[s] + n > self.cap:
+                raise CacheOverrun(f"appending at {length[s] + n} to a cache with room for {self.cap}",
+                                   (length[s] + n, self.cap))
 
     def _norm(self, x, w):
         return x * torch.rsqrt((x * x).mean(dim=-1, keepdim=True) + self.cfg.eps) * w
@@ -189,58 +190,86 @@ class LlamaBatch:
             h = h + (torch.nn.functional.silu(x @ w[f"{l}.wg"].T) * (x @ w[f"{l}.wu"].T)) @ w[f"{l}.wd"].T
         return h
 
-    def _store(self, qkv, q, pos, slot, index, cache, q_out):
-        c = self.cfg
-        qd, kd = c.heads * c.head_dim, c.kv_heads * c.head_dim
-        self.g.t16_rope_store(qkv if q else None, 0, qkv, qd, qkv, qd + kd, qd + 2 * kd, pos, slot, index, self.div,
-                              len(pos), c.heads, self.rot, self.theta, self.mscale, self.inter, cache, q_out=q_out)
+    def _logits(self, h):
+        return self._norm(h, self.w["norm"]) @ self.w["lm_head"].T
 
-    def prefill(self, prompts, slots) -> torch.Tensor:
-        """Logits [len(prompts), vocab] of the prompts' last tokens; prompt i begins a sequence in slots[i] (what was
-        there is dropped)."""
-        c, g = self.cfg, self.g
-        lens = [len(p) for p in prompts]
-        if len(slots) != len(prompts) or not prompts:
-            raise InvalidArgument("a slot for each prompt")
-        tokens = [int(t) for p in prompts for t in p]
-        before = self.length
-        self.length = [0 if s in set(slots) else n for s, n in enumerate(before)]
-        try:
-            self._check(slots, lens, tokens)
-        except Exception:
-            self.length = before
-            raise
-        n = sum(lens)
-        starts = np.concatenate([[0], np.cumsum(lens)]).tolist()
-        r = g.key_ranges(n, 0, self._ints(starts), None, True, self.window, 0)
+    def _parts(self, qkv, q):
+        """A stacked projection as the stores' first arguments (q: whether it is rotated too)."""
+        qd, kd = self.cfg.heads * self.cfg.head_dim, self.cfg.kv_heads * self.cfg.head_dim
+        return qkv if q else None, 0, qkv, qd, qkv, qd + kd, qd + 2 * kd
+
+    def _store(self, qkv, q, pos, slot, index, cache, q_out):
+        self.g.t16_rope_store(*self._parts(qkv, q), pos, slot, index, self.div, len(pos), self.cfg.heads, self.rot,
+                              self.theta, self.mscale, self.inter, cache, q_out=q_out)
+
+    def _ranges(self, lens):
+        """Which keys the rows of packed prompts see; None where they go one by one."""
+        g, n = self.g, sum(lens)
+        starts = self._ints(np.concatenate([[0], np.cumsum(lens)]).tolist())
         if self.shared and self.window:
             # Each document's own leading positions stay seen: a range of keys
             # holds one run of them only, so documents longer than the window
             # and these go one by one.
             if max(lens) > self.window + self.shared:
-                if len(prompts) > 1:
-                    return torch.cat([self.prefill([p], [s]) for p, s in zip(prompts, slots)])
-                r = g.key_ranges(n, 0, None, None, True, self.window, self.shared)
-            else:
-                r = g.key_ranges(n, 0, self._ints(starts), None, True, 0, 0)
+                return None if len(lens) > 1 else g.key_ranges(n, 0, None, None, True, self.window, self.shared)
+            return g.key_ranges(n, 0, starts, None, True, 0, 0)
+        return g.key_ranges(n, 0, starts, None, True, self.window, 0)
+
+    def _pack(self, tokens, lens, r, keep):
+        """Logits of packed prompts' last tokens, attended in a cache of their own; keep(l, qkv) stores a layer's keys
+        where they stay."""
+        c, g, n = self.cfg, self.g, len(tokens)
         if self.packed is None or self.packed.cap < n:
             self.packed = TiledCache16(c.kv_heads, c.head_dim, max(256, 1 << (n - 1).bit_length()), device=g.device,
                                        zero=False)
         row = torch.arange(n, dtype=torch.int32, device=g.device)
         zero = torch.zeros_like(row)
-        slot = self._ints(np.repeat(slots, lens).tolist())
         q = torch.empty(n * c.heads * c.head_dim, dtype=torch.float16, device=g.device)
 
         def attend(l, qkv):
             self._store(qkv, True, r.pos, zero, row, self.packed, q)
-            self._store(qkv, False, r.pos, slot, r.pos, self.cache[l], None)
+            keep(l, qkv)
             return g.flash_attn_ranges(q, 0, c.heads * c.head_dim, self.packed, 0, r, n, 0, c.heads, self.scale,
                                        **self.scores)
 
-        h = self._layers(torch.tensor(tokens, device=g.device), attend)[torch.tensor(starts[1:], device=g.device) - 1]
+        last = torch.tensor(np.cumsum(lens) - 1, device=g.device)
+        return self._logits(self._layers(torch.tensor(tokens, device=g.device), attend)[last])
+
+
+class LlamaBatch(_Sequences):
+    """Up to `slots` sequences of `cap` positions side by side. Beside the
+    geometry `cfg` may hold `rope_interleaved` (weights for pairs (2i, 2i + 1), as
+    a GGUF stores them), `rope_dim` (rotated dims of a head, 0: all),
+    `rope_scaling` ((kind, factor, original positions), see gpu.rope_scaling),
+    `softcap`, `window` with `shared` leading positions kept, and `slopes` (a
+    distance bias a head)."""
+
+    def __init__(self, gpu: Gpu, cfg, weights: dict, slots: int, cap: int):
+        _no_selection(cfg)
+        super().__init__(gpu, cfg, weights, slots, cap)
+        self.cache = [TiledCache16(cfg.kv_heads, cfg.head_dim, cap, device=gpu.device, slots=slots)
+                      for _ in range(cfg.layers)]
+        self.scratch = DecodeScratch()
+
+    def prefill(self, prompts, slots) -> torch.Tensor:
+        """Logits [len(prompts), vocab] of the prompts' last tokens; prompt i begins a sequence in slots[i] (what was
+        there is dropped)."""
+        lens = [len(p) for p in prompts]
+        if len(slots) != len(prompts) or not prompts:
+            raise InvalidArgument("a slot for each prompt")
+        tokens = [int(t) for p in prompts for t in p]
+        begun = [0 if s in set(slots) else n for s, n in enumerate(self.length)]
+        self._check(slots, lens, tokens, begun)
+        self.length = begun
+        r = self._ranges(lens)
+        if r is None:
+            return torch.cat([self.prefill([p], [s]) for p, s in zip(prompts, slots)])
+        slot = self._ints(np.repeat(slots, lens).tolist())
+        out = self._pack(tokens, lens, r,
+                         lambda l, qkv: self._store(qkv, False, r.pos, slot, r.pos, self.cache[l], None))
         for s, m in zip(slots, lens):
             self.length[s] = m
-        return self._norm(h, self.w["norm"]) @ self.w["lm_head"].T
+        return out
 
     def step(self, ids, slots) -> torch.Tensor:
         """Logits [len(ids), vocab] after one more token of each of the sequences in `slots`."""
@@ -261,4 +290,192 @@ class LlamaBatch:
         h = self._layers(torch.tensor(ids, device=g.device), attend)
         for s in slots:
             self.length[s] += 1
-        return self._norm(h, self.w["norm"]) @ self.w["lm_head"].T
+        return self._logits(h)
+
+
+class LlamaPages(_Sequences):
+    """Up to `slots` sequences of up to `cap` positions over one pool of `pages` pages of `page` positions a layer
+    (a power of two from 32): each holds the pages of its length, and sequences begun behind another share its full
+    pages, which a step attends once for all of them. `cfg` as LlamaBatch's; its `select` ((count, first, last), no
+    window beside it) has a step's sequences of more pages than `count` attend so many of them, the first and last
+    ones and those whose keys' bounds allow the largest products."""
+
+    def __init__(self, gpu: Gpu, cfg, weights: dict, slots: int, cap: int, pages: int, page: int = 64):
+        self.select = getattr(cfg, "select", None)
+        if self.select is not None and getattr(cfg, "window", 0):
+            raise ValueError("a configuration that selects pages behind a window")
+        super().__init__(gpu, cfg, weights, slots, cap)
+        dev = gpu.device
+        self.page, self.cache = page, [PagedCache16(cfg.kv_heads, cfg.head_dim, pages, page, device=dev)
+                                       for _ in range(cfg.layers)]
+        self.bounds = None
+        if self.select is not None:
+            self.bounds = [torch.zeros(pages, cfg.kv_heads, 2, cfg.head_dim, dtype=torch.float16, device=dev)
+                           for _ in range(cfg.layers)]
+        self.spare = list(range(pages - 1, -1, -1))  # pages that nobody holds
+        self.held = [0] * pages                      # sequences that hold a page
+        self.own = [[] for _ in range(slots)]        # pages of each sequence, in order
+        self.table = torch.full((slots, (cap + page - 1) // page), -1, dtype=torch.int32, device=dev)
+
+    def free(self, slots):
+        """Ends the sequences in `slots`."""
+        self._check(slots, [], [])
+        for s in slots:
+            for p in self.own[s]:
+                self.held[p] -= 1
+                if not self.held[p]:
+                    self.spare.append(p)
+            self.own[s], self.length[s] = [], 0
+
+    def _take(self, need):
+        """Pages for need[s] more positions of each slot s (all of them, or none)."""
+        more = {s: (self.length[s] + n + self.page - 1) // self.page - len(self.own[s]) for s, n in need.items()}
+        if sum(more.values()) > len(self.spare):
+            raise CacheOverrun(f"{sum(more.values())} pages of {len(self.spare)}", (sum(more.values()), len(self.spare)))
+        for s, n in more.items():
+            for _ in range(n):
+                p = self.spare.pop()
+                self.held[p] = 1
+                self.own[s].append(p)
+
+    def _show(self, slots):
+        """The slots' rows of the table on the device."""
+        wide = self.table.shape[1]
+        self.table[torch.tensor(list(slots), device=self.g.device)] = self._ints(
+            [self.own[s] + [-1] * (wide - len(self.own[s])) for s in slots])
+
+    def _keep(self, l, qkv, q, pos, row, q_out=None):
+        c = self.cfg
+        self.g.paged_rope_store(*self._parts(qkv, q), pos, row, pos, self.table, self.div, len(pos), c.heads, self.rot,
+                                self.theta, self.mscale, self.inter, self.cache[l], q_out=q_out)
+
+    def _bound(self, l, row, low, tk, new):
+        if self.bounds is not None:
+            self.g.page_bounds(self.cache[l], self.table, row, low, tk, new, self.bounds[l])
+
+    def prefill(self, prompts, slots, behind=None) -> torch.Tensor:
+        """Logits [len(prompts), vocab] of the prompts' last tokens; prompt i begins a sequence in slots[i] (what was
+        there is dropped), behind all positions of the sequence in slot `behind` if that is given."""
+        lens = [len(p) for p in prompts]
+        if len(slots) != len(prompts) or not prompts:
+            raise InvalidArgument("a slot for each prompt")
+        if behind is not None and (not 0 <= behind < self.slots or behind in slots or not self.length[behind]):
+            raise InvalidArgument(f"sequences behind slot {behind}")
+        tokens = [int(t) for p in prompts for t in p]
+        past = 0 if behind is None else self.length[behind]
+        self._check(slots, lens, tokens, [past] * self.slots)
+        lead = [] if behind is None else self.own[behind][:past // self.page]
+        freed = sum(1 for p in {p for s in slots for p in self.own[s]}
+                    if self.held[p] == sum(p in self.own[s] for s in slots))
+        need = sum((past + n + self.page - 1) // self.page - len(lead) for n in lens)
+        if need > len(self.spare) + freed:
+            raise CacheOverrun(f"{need} pages of {len(self.spare) + freed}", (need, len(self.spare) + freed))
+        self.free(slots)
+        for s in slots:
+            self.own[s] = list(lead)
+            for p in lead:
+                self.held[p] += 1
+            self.length[s] = len(lead) * self.page
+        self._take({s: past + n - self.length[s] for s, n in zip(slots, lens)})
+        self._show(slots)
+        if past % self.page:  # the page that is not full is each one's own
+            old = self.own[behind][len(lead)]
+            new = torch.tensor([self.own[s][len(lead)] for s in slots], device=self.g.device)
+            for c in self.cache:
+                c.data.view(c.pages, -1)[new] = c.data.view(c.pages, -1)[old].clone()
+        for s, n in zip(slots, lens):
+            self.length[s] = past + n
+        if behind is None:
+            return self._begin(prompts, lens, slots, tokens)
+        c, g, n = self.cfg, self.g, len(tokens)
+        at = [past + j for m in lens for j in range(m)]
+        pos, row = self._ints(at), self._ints(np.repeat(slots, lens).tolist())
+        ends, first = self._ints([past + m for m in lens]), self._ints([past] * len(lens))
+        rows = self._ints(list(slots))
+        tk = pos + 1
+        # (As rows of a table of these sequences alone: there are then more rows than sequences.)
+        few, which = self.table[rows.long()], self._ints(np.repeat(np.arange(len(slots)), lens).tolist())
+        plan = g.page_plan(tk, which, few, c.heads, self.cache[0], past + max(lens), starts=self._ints([0, n]),
+                           prefix=self._ints([len(lead) * self.page]), window=self.window, shared=self.shared)
+        q = torch.empty(n * c.heads * c.head_dim, dtype=torch.float32, device=g.device)
+
+        def attend(l, qkv):
+            self._keep(l, qkv, True, pos, row, q)
+            self._bound(l, rows, first, ends, max(lens))
+            return g.attn_decode_paged(q, 0, c.heads * c.head_dim, self.cache[l], plan, c.heads, self.scale, **self.scores)
+
+        last = torch.tensor(np.cumsum(lens) - 1, device=g.device)
+        return self._logits(self._layers(torch.tensor(tokens, device=g.device), attend)[last])
+
+    def _begin(self, prompts, lens, slots, tokens):
+        r = self._ranges(lens)
+        if r is None:
+            return torch.cat([self._begin([p], [len(p)], [s], [int(t) for t in p]) for p, s in zip(prompts, slots)])
+        row, rows, ends = self._ints(np.repeat(slots, lens).tolist()), self._ints(list(slots)), self._ints(lens)
+
+        def keep(l, qkv):
+            self._keep(l, qkv, False, r.pos, row)
+            self._bound(l, rows, None, ends, max(lens))
+
+        return self._pack(tokens, lens, r, keep)
+
+    def _groups(self, slots):
+        """`slots` in an order in which sequences that share pages follow one another: the order, each group's
+        first row and the one behind the last, and the positions that its rows share."""
+        order = sorted(range(len(slots)), key=lambda i: self.own[slots[i]])
+        starts, prefix = [], []
+        for i, x in enumerate(order):
+            own = self.own[slots[x]]
+            if starts:
+                head = self.own[slots[order[starts[-1]]]]
+                n = next((k for k, (a, b) in enumerate(zip(head, own)) if a != b), min(len(head), len(own)))
+                had = prefix[-1] // self.page if i - starts[-1] > 1 else n
+                if n and 2 * n >= had:  # (else it would take more than half of what the others share)
+                    prefix[-1] = min(had, n) * self.page
+                    continue
+            starts.append(i)
+            prefix.append(0)
+        return order, starts + [len(slots)], prefix
+
+    def step(self, ids, slots) -> torch.Tensor:
+        """Logits [len(ids), vocab] after one more token of each of the sequences in `slots`."""
+        c, g = self.cfg, self.g
+        if len(ids) != len(slots) or not slots:
+            raise InvalidArgument("a token for each slot")
+        ids = [int(t) for t in ids]
+        self._check(slots, [1] * len(slots), ids)
+        if any(not self.length[s] for s in slots):
+            raise InvalidArgument("a step of a sequence that is not begun")
+        more = [s for s in slots if self.length[s] == len(self.own[s]) * self.page]
+        self._take({s: 1 for s in more})
+        if more:
+            self._show(more)
+        order, starts, prefix = self._groups(slots)
+        to = [slots[i] for i in order]
+        at = [self.length[s] for s in to]
+        pos, row, tk = self._ints(at), self._ints(to), self._ints([p + 1 for p in at])
+        q = torch.empty(len(ids) * c.heads * c.head_dim, dtype=torch.float32, device=g.device)
+        width, most = c.heads * c.head_dim, max(at) + 1
+        few = self.select is not None and (most + self.page - 1) // self.page > self.select[0]
+        if not few:
+            sharing = any(prefix)
+            plan = g.page_plan(tk, row, self.table, c.heads, self.cache[0], most,
+                               starts=self._ints(starts) if sharing else None,
+                               prefix=self._ints(prefix) if sharing else None, window=self.window, shared=self.shared)
+
+        def attend(l, qkv):
+            self._keep(l, qkv, True, pos, row, q)
+            self._bound(l, row, pos, tk, 1)
+            if not few:
+                return g.attn_decode_paged(q, 0, width, self.cache[l], plan, c.heads, self.scale, **self.scores)
+            chosen = g.select_pages(q, 0, width, self.bounds[l], self.table, row, tk, most, c.heads, self.page,
+                                    *self.select)
+            return g.attn_decode_selected(q, 0, width, self.cache[l], self.table, row, tk, chosen, c.heads, self.scale,
+                                          **self.scores)
+
+        h = self._layers(torch.tensor([ids[i] for i in order], device=g.device), attend)
+        for s in slots:
+            self.length[s] += 1
+        back = torch.empty(len(order), dtype=torch.long)
+        back[torch.tensor(order)] = torch.arange(len(order))
+        return self._logits(h)[back.to(g.device)]
