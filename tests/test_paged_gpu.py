@@ -705,3 +705,141 @@ def test_many_prompt_rows(gpu):
     got, want, tol, plan = decode(gpu, laid, shape, tk, row, [0, 6 * per], [256], max_tk=700)
     close(got, want, tol)
     covered(plan, len(tk), 4)
+
+
+@pytest.mark.parametrize("shape", [(8, 2, 128), (2, 2, 64), (16, 1, 64)])
+@pytest.mark.parametrize("shared", [0, 40])
+def test_page_that_later_rows_lack(gpu, shape, shared):
+    """Rows of one sequence attended together, of which some need a page that is not there: the others do without it."""
+    heads, kv, hd = shape
+    page, lens, per = 32, [300, 200], [40, 30]
+    laid = pr.Laid(lens, kv, hd, page, seed=3)
+    tk = [m - p + 1 + j for m, p in zip(lens, per) for j in range(p)]
+    row = [t for t, p in enumerate(per) for _ in range(p)]
+    q = queries(5, len(tk), heads, hd)
+    table = laid.table.clone()
+    table[0, 9] = -1              # positions from 288 on
+    table[1, 3] = laid.pages + 7  # from 96 to 127: within a window of some rows
+    window = 90
+    cache, dt = laid.cache(), ints(table.tolist())
+    plan = gpu.page_plan(ints(tk), ints(row), dt, heads, cache, 300, window=window, shared=shared)
+    got = gpu.attn_decode_paged(q.cuda().view(-1), 0, heads * hd, cache, plan, heads, hd ** -0.5).view(q.shape).cpu()
+    want, tol = pr.attend(laid, q, tk, row, hd ** -0.5, window=window, shared=shared)
+    bad = torch.tensor([any(int(j) // page == (9, 3)[t] for j in pr.seen_of(m, 0, window, shared, m).nonzero())
+                        for m, t in zip(tk, row)])
+    assert 0 < bad.sum() < len(tk)
+    assert torch.isnan(got[bad]).all()
+    close(got[~bad].contiguous(), want[~bad], tol[~bad])
+    # Selected: the even rows choose the pages that are not there.
+    chosen = torch.full((len(tk), kv, 4), -1, dtype=torch.int32)
+    for r, t in enumerate(row):
+        chosen[r] = torch.tensor([0, 2, 4, (9, 3)[t] if r % 2 == 0 else 5], dtype=torch.int32)
+    got = gpu.attn_decode_selected(q.cuda().view(-1), 0, heads * hd, cache, dt, ints(row), ints(tk), chosen.cuda(), heads,
+                                   hd ** -0.5).view(q.shape).cpu()
+    want, tol = pr.attend(laid, q, tk, row, hd ** -0.5, chosen=chosen)
+    bad = torch.tensor([r % 2 == 0 and tk[r] > 32 * (9, 3)[t] for r, t in enumerate(row)])
+    assert 0 < bad.sum() < len(tk)
+    assert torch.isnan(got[bad]).all()
+    close(got[~bad].contiguous(), want[~bad], tol[~bad])
+
+
+def test_more_prompt_rows_than_threads(gpu):
+    """Rows of prompts of which a plan's thread takes several, behind shared documents and not."""
+    shape, per, n = (4, 2, 64), 130, 9
+    lens = [256 + per if t < 3 else 96 + per if t < 5 else 20 + per for t in range(n)]
+    laid = pr.Laid(lens, 2, 64, 32, [0, 3, 5], [256, 64], seed=3, cols=13)
+    tk = [m - per + 1 + j for m in lens for j in range(per)]
+    row = [t for t in range(n) for _ in range(per)]
+    got, want, tol, plan = decode(gpu, laid, shape, tk, row, [0, 3 * per, 5 * per], [256, 64], max_tk=400)
+    close(got, want, tol)
+    covered(plan, len(tk), 2)
+
+
+@pytest.mark.parametrize("n", [7400, 8192])
+def test_select_of_most_held_pages(gpu, n):
+    """As many pages as one workgroup holds the scores of."""
+    heads, kv, hd, page, units, count = 4, 2, 128, 32, 64, 40
+    g = torch.Generator().manual_seed(n)
+    mid, half = torch.randn(n, kv, 1, hd, generator=g), 1.0 + torch.randn(n, kv, 1, hd, generator=g).abs()
+    bounds = torch.cat([mid + half, mid - half], 2).to(torch.float16)
+    table = torch.randperm(n, generator=g)[None].expand(units, -1)
+    tk = [n * page - r for r in range(units)]
+    q = queries(7, units, heads, hd)
+    want = pr.select(q[:1], bounds, table[:1], [0], tk, page, count, 1, 1)
+    got = gpu.select_pages(q.cuda().view(-1), 0, heads * hd, bounds.cuda(), ints(table.tolist()), None, ints(tk),
+                           n * page, heads, page, count, 1, 1)
+    assert torch.equal(got[:1].cpu(), want)
+
+
+def test_prompt_rows_from_a_graph(gpu):
+    """Rows of prompts, planned and attended together, over all and over selected pages, replayed as lengths change."""
+    heads, kv, hd, page, cols = 8, 2, 128, 64, 20
+    laid = pr.Laid([1200, 1100], kv, hd, page, seed=3, cols=cols)
+    cache, table = laid.cache(), ints(laid.table.tolist())
+    n = 50
+    row, tk = ints([0] * n), ints([1] * n)
+    q = queries(5, n, heads, hd)
+    dq = q.cuda().view(-1)
+    chosen = torch.zeros(n, kv, 3, dtype=torch.int32).cuda()
+
+    def step():
+        plan = gpu.page_plan(tk, row, table, heads, cache, cols * page, window=500)
+        full = gpu.attn_decode_paged(dq, 0, heads * hd, cache, plan, heads, 0.09)
+        some = gpu.attn_decode_selected(dq, 0, heads * hd, cache, table, row, tk, chosen, heads, 0.09)
+        return full, some
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    r = random.Random(3)
+    for i, split in enumerate([50, 0, 23, 1, 40]):
+        lengths = [r.randint(0, 1000) + j % 32 if i != 3 else j for j in range(n)]
+        rows = [0] * split + [1] * (n - split)
+        pages = torch.tensor([[sorted(r.sample(range(max(3, m // page)), 3)) for _ in range(kv)] for m in lengths],
+                             dtype=torch.int32)
+        tk.copy_(torch.tensor(lengths, dtype=torch.int32))
+        row.copy_(torch.tensor(rows, dtype=torch.int32))
+        chosen.copy_(pages)
+        graph.replay()
+        torch.cuda.synchronize()
+        close(held[0], *pr.attend(laid, q, lengths, rows, 0.09, window=500))
+        close(held[1], *pr.attend(laid, q, lengths, rows, 0.09, chosen=pages))
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("shape,page", [((6, 2, 64), 4096), ((7, 1, 128), 2048), ((33, 11, 64), 32), ((13, 1, 64), 512)])
+def test_queries_out_of_step(gpu, shape, page):
+    """Queries four bytes off any larger unit, rows far apart, a context in a buffer that the caller holds."""
+    heads, kv, hd = shape
+    lens = [4500, 37, 4097]
+    laid = pr.Laid(lens, kv, hd, page, seed=2)
+    cache, table = laid.cache(), ints(laid.table.tolist())
+    per = 5
+    tk = [max(1, m - per + 1 + j) for m in lens for j in range(per)]
+    row = [t for t in range(3) for _ in range(per)]
+    q = queries(4, len(tk), heads, hd)
+    stride, off = heads * hd + 3, 5
+    flat = torch.full((off + stride * len(tk),), math.nan)
+    flat[off:].view(len(tk), stride)[:, :heads * hd] = q.view(len(tk), -1)
+    flat = flat.cuda()
+    n = len(tk) * heads * hd
+    out = torch.full((n + 64,), 7.0, device="cuda")
+    plan = gpu.page_plan(ints(tk), ints(row), table, heads, cache, 4500)
+    got = gpu.attn_decode_paged(flat, off, stride, cache, plan, heads, hd ** -0.5, out=out)
+    want, tol = pr.attend(laid, q, tk, row, hd ** -0.5)
+    close(got, want, tol)
+    assert (out[n:] == 7.0).all()
+    live = max((m + page - 1) // page for m in lens)
+    chosen = torch.arange(live, dtype=torch.int32).expand(len(tk), kv, -1).contiguous().cuda()
+    out.fill_(7.0)
+    got = gpu.attn_decode_selected(flat, off, stride, cache, table, ints(row), ints(tk), chosen, heads, hd ** -0.5, out=out)
+    close(got, want, tol)
+    assert (out[n:] == 7.0).all()
+    if live > 1:
+        bounds = torch.zeros(laid.pages, kv, 2, hd, dtype=torch.float16).cuda()
+        gpu.page_bounds(cache, table, None, None, ints(lens), max(lens), bounds)
+        sel = gpu.select_pages(flat, off, stride, bounds, table, ints(row), ints(tk), 4500, heads, page, live - 1, 0, 1)
+        want = pr.select(q, bounds.float().cpu(), laid.table, row, tk, page, live - 1, 0, 1)
+        assert torch.equal(sel.cpu(), want)

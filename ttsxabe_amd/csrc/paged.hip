@@ -443,9 +443,10 @@ __device__ __forceinline__ bool tile(const PagedArgs& a, WaveParts<HD>& w, int r
             load_v<HD, 0>(v, next, lane);
         }
     }
+    // (Of a tile, not finite: other rows may do without that page.)
     if (gone) {
-#pragma unroll
-        for (int u = 0; u < NQT; ++u) c.l[u] = __builtin_nanf("");
+        if constexpr (ONE) c.l[0] = __builtin_nanf("");
+        else c.o[0][0][0] = __builtin_nanf("");
     }
     return join<HD, MODE, NQT, !ONE>(w, c, a.group, rows * a.group, to, tid);
 }
@@ -527,8 +528,13 @@ __global__ __launch_bounds__(PT, 2) void paged_kernel(PagedArgs a) {
         return;
     }
     for (int i = 0; i < rows; ++i) {
-        tile<HD, MODE, 1, true>(a, w, row + i, 1, table, kh, begin, end, row_of(a, HD, to, i), place,
-                                    [&](int) { return sees(i); });
+        const ColumnSees of = sees(i);
+        auto of_row = [&](int b, uint32_t& on) {
+            const int p = place(b, on);
+            return p < of.f || (p + 32 > of.lo && p < of.tk) ? p : -1;
+        };
+        tile<HD, MODE, 1, true>(a, w, row + i, 1, table, kh, begin, end, row_of(a, HD, to, i), of_row,
+                                [&](int) { return of; });
         __syncthreads();  // the join's arrays
     }
 }
