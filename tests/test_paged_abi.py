@@ -164,3 +164,17 @@ def test_store():
     assert store(rot=127) == 7 and store(hd=96) == 1
     assert store(rows=0) == 0
     assert store(q_out=1 << 41) == 10  # over k's rows
+
+
+def test_groups_of_a_step():
+    """Which sequences a step of LlamaPages attends together, and no more groups of them than a plan takes."""
+    from ttsxabe_amd.stack import LlamaPages
+    x = LlamaPages.__new__(LlamaPages)
+    x.page, x.own = 32, [[5], [1, 2, 9], [7, 8], [1, 2, 3], [6], [1, 2, 4, 10]]
+    order, starts, prefix = x._groups([0, 1, 2, 3, 4, 5])
+    assert order == [3, 5, 1, 0, 4, 2] and starts == [0, 3, 6] and prefix == [64, 0]
+    x.own = [[2 * t + 10**6, t + 10**7] for t in range(3000)]
+    assert x._groups(list(range(3000)))[1:] == ([0, 3000], [0])
+    x.own = [[t // 2, t + 10**7] for t in range(3000)]
+    order, starts, prefix = x._groups(list(range(3000)))
+    assert len(prefix) == 1024 and starts[-2:] == [2046, 3000] and prefix == [32] * 1023 + [0]

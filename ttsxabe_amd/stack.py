@@ -25,6 +25,8 @@ import torch
 
 from .gpu import CacheOverrun, DecodeScratch, Gpu, InvalidArgument, PagedCache16, TiledCache16, rope_scaling
 
+PLAN_GROUPS = 1024  # that Gpu.page_plan takes
+
 
 def _no_selection(cfg):
     if getattr(cfg, "select", None) is not None:
@@ -435,6 +437,11 @@ class LlamaPages(_Sequences):
                     continue
             starts.append(i)
             prefix.append(0)
+        # Sequences that share nothing side by side as one group, and no more groups than a plan takes.
+        kept = [i for i in range(len(starts)) if prefix[i] or not i or prefix[i - 1]][:PLAN_GROUPS]
+        starts, prefix = [starts[i] for i in kept], [prefix[i] for i in kept]
+        if len(kept) == PLAN_GROUPS:
+            prefix[-1] = 0
         return order, starts + [len(slots)], prefix
 
     def step(self, ids, slots) -> torch.Tensor:
