@@ -1603,10 +1603,11 @@ struct PagedSizes {
     bool whole, together;
 };
 // Items of a kv head: two workgroups a compute unit, fewer where the rows do not
-// hold four blocks for each. Few rows of a short bound are one item each, prefix and all.
+// hold four blocks for each (three: 32 rows behind 8192 positions 23.9 -> 26.5 us, 244 behind
+// 4096 29.4 -> 33.0, 40 of up to 2000 of their own in five groups 48.7 -> 45.9). Few rows of a short bound are one item each, prefix and all.
 // Rows of one sequence are looked for, to be attended together, where there are more
 // rows than sequences in the table (tokens of a batch have none, and do without the search
-// and a join's launch: 23 rows of 32/8/64 over 6 pages each 12.8 -> 10 us).
+// and, over few selected pages, without a join's launch, 4 us).
 PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads, size_t kv_heads) {
     PagedSizes s;
     s.together = nseq > table_rows;

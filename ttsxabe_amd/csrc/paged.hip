@@ -575,7 +575,7 @@ __device__ __forceinline__ int* row_note(const PagedArgs& a, int hd, int row) {
 // pages' blocks. Rows of one sequence mostly select the same pages (neighbours of a
 // prompt), so a tile of them walks the pages that any of them selected, each read once,
 // its workgroups being those of its rows (127 rows over 24 pages each of 32/8/128,
-// row by row 42.4 us).
+// row by row 42.5 us, so 35.0).
 template <int HD, int MODE, int AUX>
 __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) WaveParts<HD> w;
@@ -698,7 +698,8 @@ struct Parts {
 // 2^(m - M) l. A part in which a row sees no key has m = RG_NOREF and l = 0.
 //
 // Many rows, of few parts each: a thread takes four dims of a (row, head) (244
-// rows of 20 heads of 64, by a workgroup a (row, head) as below 13.8 us, so 7.3).
+// rows of 20 heads of 64, by a workgroup a (row, head) as below 12.4 us, so 5.2; 127
+// of 32 of 128 10.6, so 4.8).
 template <int HD, bool PLAN>
 __global__ __launch_bounds__(PT) void paged_merge_rows_kernel(PagedArgs a) {
     constexpr int C = HD / 4, U = 4;
@@ -745,7 +746,7 @@ __global__ __launch_bounds__(PT) void paged_merge_rows_kernel(PagedArgs a) {
 
 // Few rows: a workgroup a (row, query head), the threads HD / 4 columns of four
 // dims by phases of the parts, whose loads go out together (one sequence of 32
-// parts, all four heads by one thread a column: 12.4 us, so 3.9).
+// parts, all four heads by one thread a column: 12.4 us, so 4.0).
 constexpr int PM_PARTS = 1088;  // parts of a row at most: each side's target and one
 
 template <int HD, bool PLAN>

@@ -74,7 +74,8 @@ __device__ __forceinline__ int2 scan_before(int2 v, int2* waves, int tid, int2& 
 // tile of rows) over what else they see, each key masked by row; what a row alone sees is its own
 // item's. All are cut into items of about the same cost, `target` of them a kv head in
 // all. Bound by its chain of loads and barriers: a row a thread, few waves where there
-// are few rows (ONE: what they see is held in LDS, else in the plan itself).
+// are few rows (ONE: what they see is held in LDS, else in the plan itself). 40 rows in
+// five groups 6.4 us, 244 rows of four prompts 10.2.
 template <int PP, bool ONE>
 __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __shared__ int gst[PG_GROUPS + 1], glo[PG_GROUPS], ghi[PG_GROUPS], gat[PG_GROUPS], gruns[PG_GROUPS];
@@ -213,7 +214,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     if ((tid & 63) == 0) atomicAdd(&work, cost);
     __syncthreads();
     // Cost of an item, four a block (seven of two column tiles). (A sequence costs up to
-    // 7 * 2^25: 32 bits, as divisions of 64 take half a microsecond each, 9 us of 14.)
+    // 7 * 2^25: 32 bits, as divisions of 64 take half a microsecond each.)
     const unsigned long long each = (work + a.target - 1) / a.target;
     const unsigned c = (unsigned)max(min(each, 0x7fffffffull), (unsigned long long)(4 * PG_SPAN));
     auto cut = [&](int blocks, int cost) { return a.whole ? 1 : (int)(((unsigned)blocks * cost + c - 1) / c); };
