@@ -843,3 +843,54 @@ def test_queries_out_of_step(gpu, shape, page):
         sel = gpu.select_pages(flat, off, stride, bounds, table, ints(row), ints(tk), 4500, heads, page, live - 1, 0, 1)
         want = pr.select(q, bounds.float().cpu(), laid.table, row, tk, page, live - 1, 0, 1)
         assert torch.equal(sel.cpu(), want)
+
+
+def test_queries_not_finite(gpu):
+    """A NaN or an infinity in one row's queries, among rows attended together: that row's heads alone."""
+    heads, kv, hd, page = 8, 2, 128, 32
+    lens, per = [300, 333], 24
+    laid = pr.Laid(lens, kv, hd, page, [0, 2], [256], seed=3)
+    cache, table = laid.cache(), ints(laid.table.tolist())
+    tk = [m - per + 1 + j for m in lens for j in range(per)]
+    row = [t for t in range(2) for _ in range(per)]
+    q = queries(5, len(tk), heads, hd)
+    odd = q.clone()
+    odd[5, 2, 7], odd[30, 6, 0] = math.nan, math.inf
+    chosen = torch.arange(8, dtype=torch.int32).expand(len(tk), kv, -1).contiguous()
+    rest = torch.ones(len(tk), heads, dtype=torch.bool)
+    rest[5, 2] = rest[30, 6] = False
+    plan = gpu.page_plan(ints(tk), ints(row), table, heads, cache, 333, starts=ints([0, 48]), prefix=ints([256]))
+    a = gpu.attn_decode_paged(odd.cuda().view(-1), 0, heads * hd, cache, plan, heads, 0.09).view(q.shape).cpu()
+    b = gpu.attn_decode_selected(odd.cuda().view(-1), 0, heads * hd, cache, table, ints(row), ints(tk), chosen.cuda(), heads,
+                                 0.09).view(q.shape).cpu()
+    for got, (want, tol) in ((a, pr.attend(laid, q, tk, row, 0.09)), (b, pr.attend(laid, q, tk, row, 0.09, chosen=chosen))):
+        assert got[~rest].isnan().all()
+        close(got[rest], want[rest], tol[rest])
+
+
+def test_nothing(gpu):
+    """No rows, no pages chosen, no live positions."""
+    heads, kv, hd, page = 8, 2, 128, 32
+    laid = pr.Laid([100, 64], kv, hd, page, seed=3)
+    cache, table = laid.cache(), ints(laid.table.tolist())
+    none, q = ints([]), torch.empty(0, device="cuda")
+    plan = gpu.page_plan(none, none, table, heads, cache, 100)
+    assert gpu.attn_decode_paged(q, 0, heads * hd, cache, plan, heads, 0.09).numel() == 0
+    bounds = torch.full((laid.pages, kv, 2, hd), 3.0, dtype=torch.float16, device="cuda")
+    gpu.page_bounds(cache, table, none, None, none, 0, bounds)
+    gpu.page_bounds(cache, table, None, None, ints([0, 0]), 5, bounds)
+    gpu.page_bounds(cache, table, None, ints([100, 64]), ints([100, 64]), 5, bounds)
+    assert (bounds == 3.0).all()
+    chosen = gpu.select_pages(q, 0, heads * hd, bounds, table, none, none, 100, heads, page, 2)
+    assert chosen.shape == (0, kv, 2)
+    assert gpu.attn_decode_selected(q, 0, heads * hd, cache, table, none, none, chosen, heads, 0.09).numel() == 0
+    q = queries(3, 2, heads, hd).cuda().view(-1)
+    chosen = gpu.select_pages(q, 0, heads * hd, bounds, table, None, ints([0, 0]), 100, heads, page, 2)
+    assert (chosen == -1).all()
+    got = gpu.attn_decode_selected(q, 0, heads * hd, cache, table, None, ints([100, 64]), chosen, heads, 0.09)
+    assert not got.any()
+    got = gpu.attn_decode_selected(q, 0, heads * hd, cache, table, None, ints([100, 64]), chosen[:, :, :0].contiguous(), heads,
+                                   0.09)
+    assert not got.any()
+    plan = gpu.page_plan(ints([0, 0]), None, table, heads, cache, 100, starts=ints([0, 2]), prefix=ints([64]))
+    assert not gpu.attn_decode_paged(q, 0, heads * hd, cache, plan, heads, 0.09).any()
