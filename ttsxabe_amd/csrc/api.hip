@@ -1599,12 +1599,14 @@ constexpr size_t PG_MAX_ROWS = (size_t)1 << 20;
 
 // How a step over pages is divided, from what the host knows of it.
 struct PagedSizes {
-    size_t target, max_wide, max_own, items;
+    size_t target, tile_target, max_wide, max_own, items;
     bool whole, together;
 };
 // Items of a kv head: two workgroups a compute unit, fewer where the rows do not
-// hold four blocks for each (three: 32 rows behind 8192 positions 23.9 -> 26.5 us, 244 behind
-// 4096 29.4 -> 33.0, 40 of up to 2000 of their own in five groups 48.7 -> 45.9). Few rows of a short bound are one item each, prefix and all.
+// hold four blocks for each. Three for 16 rows or more whose work is not mostly tiles'
+// (rows of 32/8/128 by themselves: 32 of 256 to 8192 107.6 -> 103.3 us, 100 of 20 to 3000
+// 58.7 -> 55.6, 40 in five groups 48.7 -> 45.9, but one of 60000 43.6 -> 46.1, 8 of 4000
+// 28.0 -> 28.9; tiles: 32 rows behind 8192 positions 23.9 -> 26.5, 244 behind 4096 29.4 -> 33.0). Few rows of a short bound are one item each, prefix and all.
 // Rows of one sequence are looked for, to be attended together, where there are more
 // rows than sequences in the table (tokens of a batch have none, and do without the search
 // and, over few selected pages, without a join's launch, 4 us).
@@ -1613,8 +1615,10 @@ PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t table_r
     s.together = nseq > table_rows;
     const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
     const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads));
-    s.target = std::max<size_t>(1, std::min(2 * (size_t)compute_units() / kv_heads, (nseq * blocks + 3) / 4));
-    s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * (size_t)compute_units());
+    const size_t cus = (size_t)compute_units(), most = (nseq * blocks + 3) / 4;
+    s.target = std::max<size_t>(1, std::min((nseq < 16 ? 2 : 3) * cus / kv_heads, most));
+    s.tile_target = std::max<size_t>(1, std::min(2 * cus / kv_heads, most));
+    s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * cus);
     // Shared tiles, and tiles of one sequence's rows.
     const size_t tiles = (groups && !s.whole ? nseq / per + groups : 0) +
                          (s.together ? std::min(nseq / 2, PG_RUNS * ((nseq + per - 1) / per)) : 0);
@@ -1741,6 +1745,7 @@ int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev
     a.max_wide = (int)z.max_wide;
     a.max_own = (int)z.max_own;
     a.target = (int)z.target;
+    a.tile_target = (int)z.tile_target;
     a.whole = z.whole ? 1 : 0;
     a.together = z.together && row_dev ? 1 : 0;
     return launched("page_plan", launch_page_plan(a, S(stream)));

@@ -40,6 +40,7 @@ struct PagePlanArgs {
     int nseq, groups, window, shared, rows, cols, shift, group, kv_heads;
     int max_wide, max_own;    // items there is room for
     int target;               // items of a kv head that the work is divided into
+    int tile_target;          // and where the most of it is tiles'
     int whole;                // every row is one item (no group shares)
     int together;             // rows of one sequence may follow one another
 };

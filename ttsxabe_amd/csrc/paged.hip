@@ -747,7 +747,7 @@ __global__ __launch_bounds__(PT) void paged_merge_rows_kernel(PagedArgs a) {
 // Few rows: a workgroup a (row, query head), the threads HD / 4 columns of four
 // dims by phases of the parts, whose loads go out together (one sequence of 32
 // parts, all four heads by one thread a column: 12.4 us, so 4.0).
-constexpr int PM_PARTS = 1088;  // parts of a row at most: each side's target and one
+constexpr int PM_PARTS = 1088;  // parts of a row at most: three workgroups a compute unit, and two
 
 template <int HD, bool PLAN>
 __global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {

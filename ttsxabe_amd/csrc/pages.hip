@@ -82,7 +82,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __shared__ int4 held[ONE ? PP : 1];
     __shared__ int2 waves[PP / 64];
     __shared__ uint64_t links[PP / 64 + 1];
-    __shared__ unsigned long long work;
+    __shared__ unsigned long long work, tiled;
     const int tid = threadIdx.x;
     const int tile_rows = PG_TILE_ROWS(a.group);
     const int per = ONE ? 1 : (a.nseq + PP - 1) / PP;
@@ -107,7 +107,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
         rows[PG_ROW / 4 * (size_t)r + 2] = s;
         if constexpr (ONE) held[r] = s;
     }
-    if (tid == 0) work = 0;
+    if (tid == 0) work = tiled = 0;
     // Starts that decrease: no groups (tiles would lie over one another, more than there is room for).
     if (__syncthreads_or(falls)) groups = 0;
     auto group_of = [&](int r) {
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
             glo[g] = share ? lo : 0;
             ghi[g] = share ? hi : 0;
             if (share)
-                atomicAdd(&work, (unsigned long long)((n + tile_rows - 1) / tile_rows) * (unsigned)(hi - lo) * wide_cost(n));
+                atomicAdd(&tiled, (unsigned long long)((n + tile_rows - 1) / tile_rows) * (unsigned)(hi - lo) * wide_cost(n));
         }
         __syncthreads();
     }
@@ -207,7 +207,8 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     unsigned long long cost = 0;
     for (int r = r0; r < r1; ++r) {
         const Own x = own(r);
-        if (x.first == r) cost += (unsigned long long)x.o.n * (x.rows > 1 ? wide_cost(x.rows) : 4);
+        if (x.rows == 1) cost += (unsigned long long)x.o.n * 4;
+        else if (x.first == r) atomicAdd(&tiled, (unsigned long long)x.o.n * wide_cost(x.rows));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) cost += __shfl_xor(cost, d);
@@ -215,7 +216,8 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
     __syncthreads();
     // Cost of an item, four a block (seven of two column tiles). (A sequence costs up to
     // 7 * 2^25: 32 bits, as divisions of 64 take half a microsecond each.)
-    const unsigned long long each = (work + a.target - 1) / a.target;
+    const unsigned target = (unsigned)(tiled > work ? a.tile_target : a.target);
+    const unsigned long long each = (work + tiled + target - 1) / target;
     const unsigned c = (unsigned)max(min(each, 0x7fffffffull), (unsigned long long)(4 * PG_SPAN));
     auto cut = [&](int blocks, int cost) { return a.whole ? 1 : (int)(((unsigned)blocks * cost + c - 1) / c); };
 
