@@ -894,3 +894,49 @@ def test_nothing(gpu):
     assert not got.any()
     plan = gpu.page_plan(ints([0, 0]), None, table, heads, cache, 100, starts=ints([0, 2]), prefix=ints([64]))
     assert not gpu.attn_decode_paged(q, 0, heads * hd, cache, plan, heads, 0.09).any()
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_rows_random(gpu, seed):
+    """Rows of prompts and single tokens of several sequences, in order or not, some behind a document in groups of any
+    bounds: attended, their pages selected, and attended over selected pages."""
+    r = random.Random(seed)
+    kv, group, hd = r.choice([1, 2, 3, 5]), r.choice([1, 2, 3, 4, 5, 7, 8, 16]), r.choice([64, 128])
+    page, n = r.choice([32, 64, 128, 512]), r.choice([1, 2, 3, 6])
+    heads, doc = kv * group, r.choice([0, 0, page, 3 * page, 10 * page])
+    lens = [doc + r.choice([1, 5, 33, 100, 400, 900]) for _ in range(n)]
+    laid = pr.Laid(lens, kv, hd, page, [0, n], [doc], seed=seed, behind=r.choice([-1, 10**6]))
+    rows = []
+    for t in range(n):
+        m = r.choice([1, 1, 3, 8, 20, 50])
+        rows += [(t, max(0, lens[t] - m + 1 + j) if r.random() < 0.9 else r.randint(0, lens[t])) for j in range(m)]
+    if r.random() < 0.3:
+        r.shuffle(rows)
+    row, tk = [t for t, _ in rows], [m for _, m in rows]
+    starts = prefix = None
+    if doc and r.random() < 0.7:
+        starts, prefix = [0, len(row)], [r.choice([doc, doc - 1, max(doc - 33, 0)])]
+    if doc and r.random() < 0.3 and len(row) > 4:
+        starts, prefix = [1, len(row) // 2, len(row) - 1], [doc, doc // 2]
+    window, shared = r.choice([0, 0, 40, 300]), r.choice([0, 0, 4, 70])
+    lo = [r.randint(0, 200) for _ in row] if r.random() < 0.3 else None
+    cap, bias = r.choice([0.0, 30.0]), r.random() < 0.4
+    got, want, tol, plan = decode(gpu, laid, (heads, kv, hd), tk, row, starts, prefix, window, shared, lo, cap, bias,
+                                  max_tk=max(lens), seed=seed)
+    close(got, want, tol)
+    covered(plan, len(row), group)
+    q = queries(seed, len(row), heads, hd)
+    dq, table, cache = q.cuda().view(-1), ints(laid.table.tolist()), laid.cache()
+    bounds = torch.zeros(laid.pages, kv, 2, hd, dtype=torch.float16).cuda()
+    gpu.page_bounds(cache, table, None, None, ints(lens), max(lens), bounds)
+    count = r.randint(1, max((m + page - 1) // page for m in lens))
+    first = r.randint(0, count)
+    last = r.randint(0, count - first)
+    chosen = gpu.select_pages(dq, 0, heads * hd, bounds, table, ints(row), ints(tk), max(lens), heads, page, count, first,
+                              last)
+    want = pr.select(q[:8], bounds.cpu(), laid.table, row[:8], tk[:8], page, count, first, last)
+    assert torch.equal(chosen[:8].cpu(), want)
+    sl = slopes_of(heads) if bias else None
+    got = gpu.attn_decode_selected(dq, 0, heads * hd, cache, table, ints(row), ints(tk), chosen, heads, hd ** -0.5, cap,
+                                   None if sl is None else sl.cuda())
+    close(got, *pr.attend(laid, q, tk, row, hd ** -0.5, cap, sl, chosen=chosen.cpu()))
