@@ -132,13 +132,14 @@ struct Columns {
         for (int u = 0; u < NQT; ++u) {
             if constexpr ((MODE & SM_CAP) != 0) cap_scores(sc[u], c1, sl2, c2);
             float mx = ninf();
+            const float far = (MODE & SM_BIAS) != 0 ? (float)(at[u] - k0 - 8 * grp) : 0.0f;
 #pragma unroll
             for (int T = 0; T < 2; ++T)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int key = k0 + 8 * grp + 4 * T + r;
                     float s = (MODE & SM_CAP) != 0 ? sc[u][T][r] : sc[u][T][r] * sl2;
-                    if constexpr ((MODE & SM_BIAS) != 0) s = __builtin_fmaf(-slope2[u], (float)(at[u] - key), s);
+                    if constexpr ((MODE & SM_BIAS) != 0) s = __builtin_fmaf(-slope2[u], far - (float)(4 * T + r), s);
                     if (part) s = see(u, key) ? s : ninf();
                     sc[u][T][r] = s;
                     mx = fmaxf(mx, s);
