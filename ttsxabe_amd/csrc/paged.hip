@@ -22,6 +22,9 @@ namespace llmtie {
 
 constexpr int PW = 4, PT = PW * LLMTIE_WAVE;
 
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+
 // What a wave does with 32 keys for NQT * 16 columns.
 template <int HD, int MODE, int NQT>
 struct Columns {
@@ -32,6 +35,8 @@ struct Columns {
     half8 qh[NQT][NS], ql[LOW_LDS ? 1 : NQT][LOW_LDS ? 1 : NS];
     const half8* low;
     floatx4 o[NT][NQT];
+    // Weights are 2^(s - m), up to 2^RD_LIFT, and l their sum. The reference m is the
+    // largest score less RD_LIFT, or as it is past 2^23, where that is not exact.
     float m[NQT], l[NQT];
     float slope2[NQT];
     int at[NQT];  // SM_BIAS: the column's own position
@@ -145,24 +150,28 @@ struct Columns {
                     mx = fmaxf(mx, s);
                 }
             mx = max4grp(mx);
-            if (__any(mx > m[u])) {
-                const float mn = fmaxf(m[u], mx), fac = ex2(m[u] - mn);
-                m[u] = mn;
+            const bool more = mx - m[u] > RD_LIFT;
+            if (__any(more)) {
+                const float to = !more ? m[u] : fabsf(mx) < 0x1p23f ? mx - RD_LIFT : mx, fac = ex2(m[u] - to);
+                m[u] = to;
                 l[u] *= fac;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) o[t][u] *= fac;
             }
+            // Upper halves two at a time, and what is left of each in one instruction.
 #pragma unroll
             for (int T = 0; T < 2; ++T)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    // (The difference first: the key m is has 0, however large m is.)
-                    const float p = ex2((sc[u][T][r] - m[u]) + RD_LIFT);
-                    l[u] += p;
-                    half_t x, y;
-                    split_h(p, x, y);
-                    ph[u][4 * T + r] = x;
-                    pl[u][4 * T + r] = y;
+                for (int r = 0; r < 4; r += 2) {
+                    floatx2 p = {ex2(sc[u][T][r] - m[u]), ex2(sc[u][T][r + 1] - m[u])};
+                    l[u] += p[0];
+                    l[u] += p[1];
+                    const halfx2 x = __builtin_convertvector(p, halfx2);
+                    p[0] = __builtin_fmaf(-(float)x[0], 1.0f, p[0]);
+                    p[1] = __builtin_fmaf(-(float)x[1], 1.0f, p[1]);
+                    const halfx2 y = __builtin_convertvector(p, halfx2);
+                    ph[u][4 * T + r] = x[0], ph[u][4 * T + r + 1] = x[1];
+                    pl[u][4 * T + r] = y[0], pl[u][4 * T + r + 1] = y[1];
                 }
         }
     }
