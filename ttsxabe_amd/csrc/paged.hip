@@ -585,7 +585,7 @@ __device__ __forceinline__ int* row_note(const PagedArgs& a, int hd, int row) {
 // pages' blocks. Rows of one sequence mostly select the same pages (neighbours of a
 // prompt), so a tile of them walks the pages that any of them selected, each read once,
 // its workgroups being those of its rows (127 rows over 24 pages each of 32/8/128,
-// row by row 42.5 us, so 35.0).
+// row by row 42.5 us, so 34.5).
 template <int HD, int MODE, int AUX>
 __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) WaveParts<HD> w;
