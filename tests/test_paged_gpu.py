@@ -940,3 +940,38 @@ def test_rows_random(gpu, seed):
     got = gpu.attn_decode_selected(dq, 0, heads * hd, cache, table, ints(row), ints(tk), chosen, heads, hd ** -0.5, cap,
                                    None if sl is None else sl.cuda())
     close(got, *pr.attend(laid, q, tk, row, hd ** -0.5, cap, sl, chosen=chosen.cpu()))
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0**14, 2.0**20, 2.0**23, 2.0**28])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_large_equal_scores(gpu, size, sign):
+    """Scores of `size` (or less it) at some positions and twice it below at the others: the mean of the values there
+    (each weight is the same number, whatever the reference is; f32 sums of up to 700 values lose 700 * 2^-24 of the
+    largest, 4.2)."""
+    heads, kv, hd, page, n, per = 8, 2, 128, 32, 700, 6
+    laid = pr.Laid([n], kv, hd, page, seed=3)
+    laid.k[0].zero_()
+    laid.k[0][:, :, 0] = sign * 64.0 - 128.0  # far below
+    laid.k[0][:, 40::3, 0] = sign * 64.0      # the equal ones
+    laid.pool[0].zero_()
+    for i in range(laid.table.shape[1]):
+        m = min(page, n - i * page)
+        laid.pool[0, int(laid.table[0, i]), :, :m] = laid.k[0][:, i * page:i * page + m]
+    q = torch.zeros(per, heads, hd)
+    q[:, :, 0] = 2.0
+    cache, table = laid.cache(), ints(laid.table.tolist())
+    tk, row = [n - per + 1 + j for j in range(per)], [0] * per
+    chosen = torch.arange(22, dtype=torch.int32).expand(per, kv, -1).contiguous().cuda()
+    plan = gpu.page_plan(ints(tk), ints(row), table, heads, cache, n)
+    scale = size / 128.0 * math.log(2.0)
+    a = gpu.attn_decode_paged(q.cuda().view(-1), 0, heads * hd, cache, plan, heads, scale)
+    b = gpu.attn_decode_selected(q.cuda().view(-1), 0, heads * hd, cache, table, ints(row), ints(tk), chosen, heads, scale)
+    for got in (a, b):
+        got = got.view(per, heads, hd).double().cpu()
+        for r in range(per):
+            for h in range(heads):
+                v = laid.v[0][h // 4, :tk[r]].double()
+                w = torch.full((tk[r],), 2.0 ** (-2.0 * min(size, 500.0)), dtype=torch.float64)
+                w[40::3] = 1.0
+                want = (w[:, None] * v).sum(0) / w.sum()
+                assert (got[r, h] - want).abs().max() < 700 * 2.0**-24 * 4.2 + (2e-6 if size == 1.0 else 0.0)

@@ -137,6 +137,7 @@ struct Columns {
         for (int u = 0; u < NQT; ++u) {
             if constexpr ((MODE & SM_CAP) != 0) cap_scores(sc[u], c1, sl2, c2);
             float mx = ninf();
+            // The distance of the lane's first key (below 2^24 exact, as those of its others are).
             const float far = (MODE & SM_BIAS) != 0 ? (float)(at[u] - k0 - 8 * grp) : 0.0f;
 #pragma unroll
             for (int T = 0; T < 2; ++T)

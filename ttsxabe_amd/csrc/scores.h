@@ -16,6 +16,7 @@ constexpr float RG_NOREF = -1e30f;
 // (unlifted, keys 25 below a dominant one were in l and not in O). O and l
 // carry the same factor, and 2^15 is within f16. Its addition is not seen in
 // the time (32 sequences of 256-8192 96.2 us with and without it, one of 4001 9.6).
+// The kernels over pages have it in the reference, a weight's one subtraction.
 constexpr float RD_LIFT = 15.0f;
 
 // c2 tanh(c1 s) of a lane's eight scores, c1 c2 = sl2. For |x| up to 0.45 the
