@@ -47,10 +47,11 @@ struct Columns {
 
     // Columns of `rows` rows from r0 on, `group` heads of kv head kh each (past the last
     // one: that one again, which nobody keeps): their queries on the way, a quarter a
-    // wave. tk: the row's length where it has one row.
+    // wave. A row's position is that of its length, also where it is alone in a shared tile
+    // (whose ColumnSees has no end).
     static constexpr int QP = (NQT * NS + PW - 1) / PW;  // (tile, 32 dims) pairs of a wave
     floatx4 raw[QP][2];
-    __device__ __forceinline__ void fetch(const PagedArgs& a, int r0, int rows, int kh, int lane, int wave, int tk) {
+    __device__ __forceinline__ void fetch(const PagedArgs& a, int r0, int rows, int kh, int lane, int wave) {
         const int col = lane & 15, n = rows * a.group;
         grp = lane >> 4;
         auto column = [&](int u, int& row, int& g) {
@@ -72,7 +73,7 @@ struct Columns {
                 int row, g;
                 column(u, row, g);
                 slope2[u] = a.slopes[kh * a.group + g] * LLMTIE_LOG2E;
-                at[u] = (tk >= 0 ? tk : min(a.tk[r0 + row], a.p.cols << a.p.shift)) - 1;
+                at[u] = min(a.tk[r0 + row], a.p.cols << a.p.shift) - 1;
             }
         }
     }
@@ -339,7 +340,7 @@ __device__ __forceinline__ bool one_row(const PagedArgs& a, WaveParts<HD>& w, in
         c.values(x.v);
     };
     Block x0, x1;
-    c.fetch(a, row, 1, kh, lane, wave, tk);
+    c.fetch(a, row, 1, kh, lane, wave);
     bool none = at.look(a, table, begin + wave + PW * lane, end, place), gone = __any(none);
     load(x0, 0);
     c.start(a, lane, wave, w.q);
@@ -389,7 +390,7 @@ __device__ __forceinline__ bool tile(const PagedArgs& a, WaveParts<HD>& w, int r
     half8 k[2 * NS], v[NT];
     ColumnSees own[NQT];
     int bit[NQT];
-    c.fetch(a, r0, rows, kh, lane, wave, -1);
+    c.fetch(a, r0, rows, kh, lane, wave);
 #pragma unroll
     for (int u = 0; u < NQT; ++u) {
         bit[u] = rows == 1 ? 0 : min(16 * u + (lane & 15), rows * a.group - 1) / a.group;
