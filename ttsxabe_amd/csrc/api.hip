@@ -1614,14 +1614,14 @@ PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t table_r
     PagedSizes s;
     s.together = nseq > table_rows;
     const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
-    const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads));
+    const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads)), runs = (size_t)PG_TILE_RUNS((int)(heads / kv_heads));
     const size_t cus = (size_t)compute_units(), most = (nseq * blocks + 3) / 4;
     s.target = std::max<size_t>(1, std::min((nseq < 16 ? 2 : 3) * cus / kv_heads, most));
     s.tile_target = std::max<size_t>(1, std::min(2 * cus / kv_heads, most));
     s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * cus);
     // Shared tiles, and tiles of one sequence's rows.
     const size_t tiles = (groups && !s.whole ? nseq / per + groups : 0) +
-                         (s.together ? std::min(nseq / 2, PG_RUNS * ((nseq + per - 1) / per)) : 0);
+                         (s.together ? std::min(nseq / 2, runs * ((nseq + per - 1) / per)) : 0);
     s.max_own = s.whole ? nseq : nseq + s.target;
     s.max_wide = s.whole ? nseq : tiles ? tiles + s.target : 0;
     s.items = s.whole ? nseq : nseq + tiles + s.target;

@@ -22,8 +22,14 @@ constexpr int PG_COLS = 32;      // (row, query head) columns of a tile at most
 // A plan's words: the header, PG_ROW a row, then PG_ITEM an item, the tiles' (the
 // wide ones) first.
 constexpr int PG_HEAD = 16, PG_ROW = 12, PG_ITEM = 16;
-constexpr int PG_RUNS = 4;       // tiles of one sequence's rows that an aligned tile of rows may hold
 __host__ __device__ constexpr int PG_TILE_ROWS(int group) { return PG_COLS / group; }
+// Rows of one sequence that are a tile at least, a quarter of one; and the tiles of such
+// rows that an aligned tile of rows can hold, which a plan has room for: four, five of two
+// rows where a tile has ten, fewer of fewer rows.
+__host__ __device__ constexpr int PG_RUN_ROWS(int group) {
+    return PG_TILE_ROWS(group) / 4 > 2 ? PG_TILE_ROWS(group) / 4 : 2;
+}
+__host__ __device__ constexpr int PG_TILE_RUNS(int group) { return PG_TILE_ROWS(group) / PG_RUN_ROWS(group); }
 __host__ __device__ inline size_t plan_items_at(size_t nseq) { return (PG_HEAD + PG_ROW * nseq + 15) / 16 * 16; }
 // What an item is: it writes its rows' context, it is of a shared tile.
 constexpr int PG_WHOLE = 1, PG_SHARED = 2;

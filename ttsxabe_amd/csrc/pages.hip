@@ -178,7 +178,7 @@ __global__ __launch_bounds__(PP) void page_plan_kernel(PagePlanArgs a) {
             while (end < to && goes_on(end)) ++end;
         }
         x.rows = end - x.first;
-        if (x.rows < max(2, tile_rows / PG_RUNS)) x.first = r, x.rows = 1;  // (so many tiles there is room for)
+        if (x.rows < PG_RUN_ROWS(a.group)) x.first = r, x.rows = 1;  // (so many tiles there is room for)
         for (int i = 0; i < x.rows; ++i) x.o.add(sees(x.first + i));
         x.o.close(x.g >= 0 ? glo[x.g] : 0, x.g >= 0 ? ghi[x.g] : 0);
         return x;
