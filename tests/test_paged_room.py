@@ -1,6 +1,8 @@
 """The room that a plan of a step over pages is given, against the items that its rows come to, by the plan's
 arithmetic one row at a time. Both are the host's: no launch is made."""
 import random
+import re
+from pathlib import Path
 
 import pytest
 
@@ -94,3 +96,21 @@ def test_room_of_random_rows(seed):
         has = room(len(row), len(prefix), limit, n, group * kv, kv)
         asks = need(tk, row, starts, prefix, limit, group, kv)
         assert asks[0] <= max(0, has[0]) and asks[1] <= has[1], (group, kv, len(row), prefix, asks, has)
+
+
+def test_parts_of_a_row():
+    """A row's parts are no more than its join takes, however long it and the positions that it shares are."""
+    text = (Path(_lib.__file__).parent / "csrc" / "paged.h").read_text()
+    most = int(re.search(r"PG_PARTS = (\d+);", text).group(1))
+    L = _lib.lib()
+    for nseq in (1, 2, 15, 16, 40):
+        for groups in (0, 1):
+            words = L.llmtie_page_plan_len(nseq, groups, 2**30, nseq, 1, 1)
+            items = (words - (16 + 12 * nseq + 15) // 16 * 16) // 16
+            # (Room for `target` items beside one a row, or one a tile: twice where rows share.)
+            target = (items - nseq) if not groups else (items - nseq - nseq // 32 - 1) // 2
+            assert target == targets(nseq, 2**30, 1)[0] and target + 2 <= most
+        floats = L.llmtie_attn_selected_workspace(nseq, 2**18, 4096, nseq, 1, 1, 64)
+        assert floats <= nseq * (most * 66 + 1)
+        floats = L.llmtie_attn_selected_workspace(nseq, 2**18, 4096, 1, 1, 1, 64)
+        assert floats <= nseq * (most * 66 + 1) + -(-nseq // 32) * most * 32 * 66

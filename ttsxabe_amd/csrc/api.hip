@@ -1615,7 +1615,9 @@ PagedSizes paged_sizes(size_t nseq, size_t groups, size_t max_tk, size_t table_r
     s.together = nseq > table_rows;
     const size_t blocks = (std::min<size_t>(max_tk, (size_t)1 << 30) + 31) / 32;
     const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads)), runs = (size_t)PG_TILE_RUNS((int)(heads / kv_heads));
-    const size_t cus = (size_t)compute_units(), most = (nseq * blocks + 3) / 4;
+    const size_t cus = (size_t)compute_units();
+    // (A row's own work and its group's are of the whole, each rounded up: target + 2 parts at most. 770 of 256 compute units.)
+    const size_t most = std::min<size_t>((nseq * blocks + 3) / 4, PG_PARTS - 2);
     s.target = std::max<size_t>(1, std::min((nseq < 16 ? 2 : 3) * cus / kv_heads, most));
     s.tile_target = std::max<size_t>(1, std::min(2 * cus / kv_heads, most));
     s.whole = blocks <= (size_t)RD_WHOLE && (groups == 0 || nseq * kv_heads <= 2 * cus);
@@ -1659,8 +1661,10 @@ SelectedSizes selected_sizes(size_t nseq, size_t blocks, size_t table_rows, size
     SelectedSizes s;
     const size_t per = (size_t)PG_TILE_ROWS((int)(heads / kv_heads)), tiles = (nseq + per - 1) / per;
     const size_t cus = (size_t)compute_units();
-    s.runs = std::max<size_t>(1, std::min((blocks + 3) / 4, cus / std::max<size_t>(1, smul(nseq, kv_heads))));
-    s.tile_runs = std::max<size_t>(1, std::min(std::min(nseq, per) * s.runs, 2 * cus / std::max<size_t>(1, smul(tiles, kv_heads))));
+    const size_t most = std::min<size_t>((blocks + 3) / 4, PG_PARTS);
+    s.runs = std::max<size_t>(1, std::min(most, cus / std::max<size_t>(1, smul(nseq, kv_heads))));
+    const size_t tiled = std::min<size_t>(std::min(nseq, per) * s.runs, PG_PARTS);
+    s.tile_runs = std::max<size_t>(1, std::min(tiled, 2 * cus / std::max<size_t>(1, smul(tiles, kv_heads))));
     s.max_own = s.runs > 1 ? nseq * s.runs : 0;
     s.together = nseq > table_rows;
     s.max_wide = s.together && s.tile_runs > 1 ? tiles * s.tile_runs : 0;

@@ -33,6 +33,8 @@ __host__ __device__ constexpr int PG_TILE_RUNS(int group) { return PG_TILE_ROWS(
 __host__ __device__ inline size_t plan_items_at(size_t nseq) { return (PG_HEAD + PG_ROW * nseq + 15) / 16 * 16; }
 // What an item is: it writes its rows' context, it is of a shared tile.
 constexpr int PG_WHOLE = 1, PG_SHARED = 2;
+// Parts that a row's context is joined from at most, its own and its group's: the sizes keep to it.
+constexpr int PG_PARTS = 1088;
 // Pages of a sequence up to which rows that selected pages of it are attended together.
 constexpr int PG_UNION = 4096;
 

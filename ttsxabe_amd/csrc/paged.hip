@@ -759,12 +759,10 @@ __global__ __launch_bounds__(PT) void paged_merge_rows_kernel(PagedArgs a) {
 // Few rows: a workgroup a (row, query head), the threads HD / 4 columns of four
 // dims by phases of the parts, whose loads go out together (one sequence of 32
 // parts, all four heads by one thread a column: 12.4 us, so 4.0).
-constexpr int PM_PARTS = 1088;  // parts of a row at most: three workgroups a compute unit, and two
-
 template <int HD, bool PLAN>
 __global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {
     constexpr int C = HD / 4, R = PT / C, U = 4;
-    __shared__ float wt[PM_PARTS];
+    __shared__ float wt[PG_PARTS];
     __shared__ floatx4 red[PT];
     const int heads = a.kv_heads * a.group, h = (int)(blockIdx.x % (unsigned)heads);
     const int row = (int)(blockIdx.x / (unsigned)heads), kh = h / a.group;
@@ -776,7 +774,7 @@ __global__ __launch_bounds__(PT) void paged_merge_kernel(PagedArgs a) {
         fill(out, HD, __builtin_nanf(""));
         return;
     }
-    const int n = min(p.n, PM_PARTS);
+    const int n = min(p.n, PG_PARTS);  // (all of them: paged_sizes, selected_sizes)
     if (n == 0) return;
     auto part = [&](int i) { return p.of(a, i, kh, h % a.group); };
     // The first parts' columns are on their way while the weights are formed.
