@@ -588,7 +588,7 @@ __device__ __forceinline__ int* row_note(const PagedArgs& a, int hd, int row) {
 // prompt), so a tile of them walks the pages that any of them selected, each read once,
 // its workgroups being those of its rows (127 rows over 24 pages each of 32/8/128,
 // row by row 42.5 us, so 34.5).
-template <int HD, int MODE, int AUX>
+template <int HD, int MODE>
 __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
     __shared__ __attribute__((aligned(16))) WaveParts<HD> w;
     __shared__ uint32_t mask[PG_UNION];   // rows that selected a page, a bit each
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(PT, 2) void selected_kernel(PagedArgs a) {
         const int first = (p << a.p.shift) + 32 * (i & ((1 << s) - 1));
         return first < tk ? first : -1;
     };
-    if (one_row<HD, MODE, AUX>(a, w, row, t.table, kh, begin, end, 0, 0, tk, to, place)) return;
+    if (one_row<HD, MODE, 0>(a, w, row, t.table, kh, begin, end, 0, 0, tk, to, place)) return;
     tile<HD, MODE, 1, true>(a, w, row, 1, t.table, kh, begin, end, to, place, [&](int) { return ColumnSees{0, 0, tk}; });
 }
 
@@ -813,16 +813,15 @@ hipError_t launch_paged(int hd, const PagedArgs& a, hipStream_t st) {
     const int mode = (a.softcap > 0.0f ? SM_CAP : 0) | (a.slopes ? SM_BIAS : 0);
     const dim3 grid((unsigned)((a.plan ? (size_t)a.items : (size_t)a.nseq * a.runs) * a.kv_heads));
     bool done = false;
-#define PK(HD, M, AUX)                                                                           \
-    if (!done && hd == HD && mode == M && (a.stream ? AUX_STREAM : 0) == AUX) {                  \
-        if (a.plan) hipLaunchKernelGGL((paged_kernel<HD, M, AUX>), grid, dim3(PT), 0, st, a);    \
-        else hipLaunchKernelGGL((selected_kernel<HD, M, AUX>), grid, dim3(PT), 0, st, a);        \
-        done = true;                                                                             \
+#define PM(HD, M)                                                                                       \
+    if (!done && hd == HD && mode == M) {                                                               \
+        if (!a.plan) hipLaunchKernelGGL((selected_kernel<HD, M>), grid, dim3(PT), 0, st, a);            \
+        else if (a.stream) hipLaunchKernelGGL((paged_kernel<HD, M, AUX_STREAM>), grid, dim3(PT), 0, st, a); \
+        else hipLaunchKernelGGL((paged_kernel<HD, M, 0>), grid, dim3(PT), 0, st, a);                    \
+        done = true;                                                                                    \
     }
-#define PM(HD, M) PK(HD, M, 0) PK(HD, M, AUX_STREAM)
     PM(64, 0) PM(64, 1) PM(64, 2) PM(64, 3) PM(128, 0) PM(128, 1) PM(128, 2) PM(128, 3)
 #undef PM
-#undef PK
     if (!done) return hipErrorInvalidValue;
     if (a.merge) {
         const size_t rows = (size_t)a.nseq * a.kv_heads * a.group;
