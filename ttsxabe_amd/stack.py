@@ -20,6 +20,8 @@ begin alike share.
 """
 from __future__ import annotations
 
+from collections import Counter
+
 import numpy as np
 import torch
 
@@ -367,8 +369,8 @@ class LlamaPages(_Sequences):
         past = 0 if behind is None else self.length[behind]
         self._check(slots, lens, tokens, [past] * self.slots)
         lead = [] if behind is None else self.own[behind][:past // self.page]
-        freed = sum(1 for p in {p for s in slots for p in self.own[s]}
-                    if self.held[p] == sum(p in self.own[s] for s in slots))
+        ending = Counter(p for s in slots for p in self.own[s])
+        freed = sum(self.held[p] == n for p, n in ending.items())
         need = sum((past + n + self.page - 1) // self.page - len(lead) for n in lens)
         if need > len(self.spare) + freed:
             raise CacheOverrun(f"{need} pages of {len(self.spare) + freed}", (need, len(self.spare) + freed))
