@@ -226,3 +226,34 @@ def test_groups_from_a_graph(gpu):
         close(held, *pr.attend(laid, q, lengths, list(range(n)), 0.09, 20.0, slopes_of(heads), window=900, shared=8), what=(s, p))
         again, eager = step()
         assert torch.equal(held, eager) and torch.equal(data[:11], again[:11])  # (a plan's header is 11 words)
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_shared_random(gpu, seed):
+    """Rows of sequences behind documents, in groups of any bounds, with the scores, windows and first positions of any
+    kind: every block that a row needs is in one item of its own, and its context is the plain form's."""
+    r = random.Random(100 + seed)
+    kv, group, hd = r.choice([1, 2, 3]), r.choice([1, 2, 3, 4, 5, 6, 8, 10, 12, 16]), r.choice([64, 128])
+    page, per = r.choice([32, 64, 128]), 32 // group
+    cuts, prefix, lens = [0], [], []
+    for _ in range(r.randint(1, 3)):
+        doc = page * r.randint(-(-700 // page), 1200 // page)
+        lens += [doc + r.choice([0, 1, 31, 32, 33, r.randint(0, 300)]) for _ in range(r.choice([1, 2, per, per + 1]))]
+        cuts.append(len(lens))
+        prefix.append(doc)
+    laid = pr.Laid(lens, kv, hd, page, cuts, prefix, seed=seed)
+    row, tk, starts = [], [], [0]
+    for a, b in zip(cuts, cuts[1:]):
+        for t in range(a, b):
+            m = r.choice([1, 1, 1, 2, 3, per])
+            row += [t] * m
+            tk += [max(0, lens[t] - m + 1 + j) for j in range(m)]
+        starts.append(len(row))
+    window, shared = r.choice([0, 0, 0, r.randint(1, 1200)]), r.choice([0, 5, 100])
+    lo = [r.randint(0, 600) for _ in row] if r.random() < 0.3 else None
+    got, want, tol, plan = decode(gpu, laid, (kv * group, kv, hd), tk, row, starts, prefix, window, shared, lo,
+                                  r.choice([0.0, 20.0]), r.random() < 0.6, seed=seed)
+    for t, blocks in enumerate(covered(plan, len(row), group)):
+        need = {int(j) // 32 for j in pr.seen_of(tk[t], lo[t] if lo else 0, window, shared, tk[t]).nonzero()}
+        assert len(set(blocks)) == len(blocks) and need <= set(blocks), t
+    close(got, want, tol)
