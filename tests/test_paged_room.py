@@ -6,6 +6,8 @@ from pathlib import Path
 
 import pytest
 
+from test_abi import last
+from test_paged_abi import P, select
 from ttsxabe_amd import _lib
 
 WIDE, RUNS, SPAN = 32, 4, 4  # columns of a tile, what part of its rows makes one, blocks of an item at least
@@ -96,6 +98,13 @@ def test_room_of_random_rows(seed):
         has = room(len(row), len(prefix), limit, n, group * kv, kv)
         asks = need(tk, row, starts, prefix, limit, group, kv)
         assert asks[0] <= max(0, has[0]) and asks[1] <= has[1], (group, kv, len(row), prefix, asks, has)
+
+
+def test_rows_of_a_selection():
+    """More workgroups of 1024 threads than a launch (fewer than 2^32 threads) holds are refused by name."""
+    room = dict(row=P, heads=1, kv=1, hd=64, q_len=2**62, ws_len=2**62, chosen_len=2**62)
+    for n in (2**22, 2**24 - 600):
+        assert select(nseq=n, **room) == 4 and list(last().field)[:2] == [n, 2**22 - 1]
 
 
 def test_parts_of_a_row():

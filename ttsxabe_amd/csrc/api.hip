@@ -1925,7 +1925,7 @@ int llmtie_select_pages(void* stream, const float* q, size_t q_len, size_t q_off
     if (reach(q_off, nseq, q_stride, n) > q_len) return overrun_slice(reach(q_off, nseq, q_stride, n), q_len);
     if (chosen_len < smul(units, count)) return overrun_slice(smul(units, count), chosen_len);
     if (!row_dev && nseq > table_rows) return overrun_slice(nseq, table_rows);
-    if (sadd(units, 512) > MAX_WGS) return overrun_slice(units, MAX_WGS - 512);
+    if (units > MAX_WGS / 4) return overrun_slice(units, MAX_WGS / 4);  // (workgroups of 1024 threads)
     const size_t need = llmtie_select_pages_workspace(nseq, max_tk, page, count, kv_heads);
     if (ws_len < need) return overrun_slice(need, ws_len);
     if (nseq == 0) return ok();
