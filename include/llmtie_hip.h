@@ -435,12 +435,15 @@ int llmtie_t16_rope_store(void* stream, const float* q, size_t q_len, size_t q_o
  * prompts: row r is at position tk_dev[r] - 1 of table row row_dev[r] (row_dev NULL:
  * row r) and sees some of the tk_dev[r] first positions. A row that sees no key gets
  * zeros; one whose table row does not exist, or that needs a page the cache does not
- * have, NaN. Keys that a row does not see contribute nothing, whatever they hold.
- * Lengths, tables and rows may change between replays of captured calls. Scores
- * are those of the key ranges above, with the same bounds of their arguments. */
+ * have, NaN. Keys that a row does not see contribute nothing, whatever they hold;
+ * a value that it does see and that is not finite leaves that element of its context
+ * not finite (an infinity or NaN), whatever its weight. Lengths, tables and rows
+ * may change between replays of captured calls. Scores are those of the key ranges
+ * above, with the same bounds of their arguments. */
 
 /* llmtie_t16_rope_store into pages: row r to position index[r] of table row
- * seq[r]. Rows whose table row, position or page does not exist store nothing. */
+ * seq[r]. Rows whose table row, position or page does not exist store nothing; no two
+ * rows of a call may name the same place, nor one by two sequences that share a page. */
 int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q_off, size_t q_stride, void* q_out,
                             size_t q_out_len, size_t q_out_off, size_t q_out_stride, int q_out_f16, const float* k,
                             size_t k_len, size_t k_off, size_t k_stride, const float* v, size_t v_len, size_t v_off,
@@ -460,7 +463,9 @@ int llmtie_paged_rope_store(void* stream, const float* q, size_t q_len, size_t q
  * attended once for up to 32 / (heads / kv_heads) rows together. A prefix counts in
  * whole blocks of 32 positions and no further than the shortest row's length. max_tk is the
  * longest length or near it (it says which launch is made; longer rows are attended too).
- * GQA groups up to 16, at most 1024 groups and 2^20 rows. */
+ * Rows of one sequence that follow one another in row_dev, as a prompt's do, are attended together,
+ * their keys read once, where nseq > table_rows; in a table of as many rows or more each
+ * reads its own, and only prefixes are shared. GQA groups up to 16, at most 1024 groups and 2^20 rows. */
 size_t llmtie_page_plan_len(size_t nseq, size_t groups, size_t max_tk, size_t table_rows, size_t heads,
                             size_t kv_heads);
 int llmtie_page_plan(void* stream, const int32_t* tk_dev, const int32_t* row_dev, const int32_t* lo_dev, size_t nseq,
@@ -485,9 +490,9 @@ int llmtie_attn_decode_paged(void* stream, const float* q, size_t q_len, size_t 
 
 /* The same over `count` pages of each (row, kv head): chosen[(r * kv_heads + h) *
  * count ..] are numbers of pages within the sequence (device int32, as
- * llmtie_select_pages leaves them, any order, none twice; ones below 0 or with no
- * position that the row has name nothing). Row r sees those of their positions that
- * are below tk_dev[r]. Rows of one sequence that follow one another, as a prompt's do,
+ * llmtie_select_pages leaves them, in any order; none may be there twice, it would count
+ * once or twice; ones below 0 or with no position that the row has name nothing). Row r
+ * sees those of their positions that are below tk_dev[r]. Rows of one sequence that follow one another, as a prompt's do,
  * are attended together, each page read once for those that selected it, where there are more
  * rows than the table has. */
 size_t llmtie_attn_selected_workspace(size_t nseq, size_t count, size_t page, size_t table_rows, size_t heads,
