@@ -2,6 +2,7 @@
 import random
 
 import pytest
+import torch
 
 from ttsxabe_amd.gpu import CacheOverrun
 from ttsxabe_amd.stack import LlamaPages
@@ -52,3 +53,26 @@ def test_pages_that_new_prompts_find(seed):
         assert e.value.fields == (room + 1, room)
         assert Pages.looked <= 2 * sum(map(len, own))
         assert x.own == own and x.length == [32 * len(s) for s in own]
+
+
+@pytest.mark.parametrize("behind", [None, 3])
+def test_prompts_that_fail(behind):
+    """A pass that ends in an error begins nothing: its slots are empty, their pages are back, others are as they were."""
+    x = held([[0, 1], [2], [], [3, 4, 5]], 20)
+    x.length[3] = 70  # its third page is not full
+
+    class Device:
+        device = "cpu"
+
+        def __getattr__(self, name):
+            raise MemoryError(name)
+
+    x.g, x.cache, x.window, x.shared = Device(), [], 0, 0
+    x.table = torch.full((4, 10), -1, dtype=torch.int32)
+    x.cfg = type("Cfg", (), {"heads": 4, "head_dim": 64, "kv_heads": 4})
+    x.cache = [type("Cache", (), {"pages": 20, "data": torch.zeros(20, 8)})]
+    with pytest.raises(MemoryError):
+        x.prefill([[1] * 40, [2] * 5], [0, 2], behind=behind)
+    assert x.length == [0, 32, 0, 70] and [list(s) for s in x.own] == [[], [2], [], [3, 4, 5]]
+    assert sorted(x.spare) == [0, 1] + list(range(6, 20)) and [p for p in range(20) if x.held[p]] == [2, 3, 4, 5]
+    assert all(x.held[p] == 1 for p in (2, 3, 4, 5))

@@ -375,6 +375,14 @@ class LlamaPages(_Sequences):
         if need > len(self.spare) + freed:
             raise CacheOverrun(f"{need} pages of {len(self.spare) + freed}", (need, len(self.spare) + freed))
         self.free(slots)
+        try:
+            return self._fill(prompts, lens, slots, tokens, behind, past, lead)
+        except Exception:  # (of keys that were not all stored there is nothing to go on from)
+            self.free(slots)
+            raise
+
+    def _fill(self, prompts, lens, slots, tokens, behind, past, lead):
+        """The prompts' pages (`lead` ones of the `past` positions that they follow before them) and their pass."""
         for s in slots:
             self.own[s] = list(lead)
             for p in lead:
